@@ -1,0 +1,383 @@
+"""Activations kept in 8 bits for the backward pass, and the backward operators that read them
+(``csrc/act8.cu``, ``csrc/act8.cuh``).
+
+What a training step keeps of every transformer block is most of its memory.  ``store8`` writes
+activations as one signed byte a channel and one step byte for each 32 channels of a row; the value
+is code * 2^(step - 127), at most half a step (1/127.5 of the group's largest magnitude) off.  The
+step is a power of two, so the values are exact in bf16 and the tensor cores multiply what was
+stored.  A group that holds a NaN or an infinity reads as NaN throughout.
+
+    packed = store8([x, y, z])                # one launch, one allocation
+    x, y, z = restore8(packed)                # back to their types
+    gemm_wgrad8(dy, packed[0])                # weight gradient dY^T X
+    situ_bwd8(gu8, gout, beta, lbeta)         # gated activation, backward (and forward again)
+    attn_bwd8(q8, k8, v8, o8, lse, go)        # dense attention, probabilities recomputed
+
+``model.act_store = "int8"`` keeps the activations of the fused blocks this way
+(``ops/block.py``).  CPU tensors take the formulas of ``ops/reference.py``.  All launches go to the
+current stream of the tensors' device; workspaces belong to the call.  There is no counterpart in
+the reference, which recomputes blocks instead (reference ``models/imf_dit_video.py:909-972``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+import math
+import struct
+from typing import List, Optional, Sequence, Tuple, Union
+
+import torch
+
+from . import cuda as _cuda
+from . import reference as ref
+
+Tensor = torch.Tensor
+BF16, F32 = torch.bfloat16, torch.float32
+GROUP = 32
+_MAX_RECS = 16                 # tensors a launch takes
+_REC = struct.Struct("<3Q8q")  # x, codes, steps, n0, n1, n2, s0, s1, s2, cols, fp32
+_KERNELS = None
+
+
+def _kernels():
+    """``ops.kernels`` with the argument types of this module's launchers set (loads the library)."""
+    global _KERNELS
+    if _KERNELS is None:
+        if not _cuda.available():
+            raise RuntimeError("8-bit activations on a GPU need the kernel library")
+        from . import kernels as K
+
+        vp, ci, cl, i64, cf = (ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_int64,
+                               ctypes.c_float)
+        for name in ("imf_store8", "imf_restore8"):
+            getattr(K._lib, name).restype = ci
+            getattr(K._lib, name).argtypes = [vp, ci, vp]
+        K._lib.imf_situ_bwd8.restype = ci
+        K._lib.imf_situ_bwd8.argtypes = [vp] * 5 + [cl, ci] + [i64] * 3 + [cf, cf, ci, vp]
+        _KERNELS = K
+    return _KERNELS
+
+
+def _pitches(cols: int) -> Tuple[int, int]:
+    groups = -(-cols // GROUP)
+    return groups * GROUP, (groups + 3) // 4 * 4
+
+
+class Packed8:
+    """A tensor of ``shape`` in 8 bits: ``codes`` int8 (rows, channels rounded up to 32) and ``steps``
+    uint8 (rows, groups rounded up to 4), rows being all leading dimensions; ``dtype`` is what
+    ``restore8`` returns (bf16, or fp32 for a tensor that was fp32).  Of one ``store8`` call all
+    share one buffer, which lives until the last of them is gone."""
+
+    __slots__ = ("shape", "dtype", "rows", "cols", "device", "_codes", "_steps", "_arena", "_at")
+
+    def __init__(self, codes: Tensor, steps: Tensor, shape: Sequence[int], dtype: torch.dtype = BF16):
+        self._geometry(shape, dtype, codes.device)
+        pitch, spitch = _pitches(self.cols)
+        if codes.dtype != torch.int8 or tuple(codes.shape) != (self.rows, pitch) or not codes.is_contiguous():
+            raise ValueError(f"codes of {tuple(shape)}: contiguous int8 ({self.rows}, {pitch}) expected, got "
+                             f"{codes.dtype} {tuple(codes.shape)}")
+        if steps.dtype != torch.uint8 or tuple(steps.shape) != (self.rows, spitch) or not steps.is_contiguous():
+            raise ValueError(f"steps of {tuple(shape)}: contiguous uint8 ({self.rows}, {spitch}) expected, got "
+                             f"{steps.dtype} {tuple(steps.shape)}")
+        if codes.device != steps.device:
+            raise ValueError("codes and steps are on different devices")
+        if codes.data_ptr() % 16 or steps.data_ptr() % 4:
+            raise ValueError("codes need a 16-byte, steps a 4-byte aligned address")
+        self._codes, self._steps, self._arena, self._at = codes, steps, None, None
+
+    def _geometry(self, shape, dtype, device) -> None:
+        if dtype not in (BF16, F32):
+            raise ValueError(f"8-bit activations are bf16 or fp32, not {dtype}")
+        self.shape = torch.Size(shape)
+        if len(self.shape) < 1 or min(self.shape, default=1) < 0:
+            raise ValueError(f"not the shape of an activation: {tuple(shape)}")
+        self.dtype, self.device = dtype, device
+        self.cols = self.shape[-1]
+        self.rows = math.prod(self.shape[:-1])
+
+    @classmethod
+    def _in(cls, arena: Tensor, at: Tuple[int, int], shape, dtype) -> "Packed8":
+        """In the buffer ``arena`` at byte offsets ``at`` of codes and steps."""
+        p = cls.__new__(cls)
+        p._geometry(shape, dtype, arena.device)
+        p._codes = p._steps = None
+        p._arena, p._at = arena, at
+        return p
+
+    @property
+    def codes(self) -> Tensor:
+        if self._codes is None:
+            pitch, o = _pitches(self.cols)[0], self._at[0]
+            self._codes = self._arena[o:o + self.rows * pitch].view(torch.int8).view(self.rows, pitch)
+        return self._codes
+
+    @property
+    def steps(self) -> Tensor:
+        if self._steps is None:
+            spitch, o = _pitches(self.cols)[1], self._at[1]
+            self._steps = self._arena[o:o + self.rows * spitch].view(self.rows, spitch)
+        return self._steps
+
+    def _ptrs(self) -> Tuple[int, int]:
+        if self._arena is not None:
+            base = self._arena.data_ptr()
+            return base + self._at[0], base + self._at[1]
+        return self._codes.data_ptr(), self._steps.data_ptr()
+
+    @property
+    def nbytes(self) -> int:
+        return self.rows * sum(_pitches(self.cols))
+
+    def view(self, *shape: int) -> "Packed8":
+        """The same rows under other leading dimensions."""
+        if shape[-1] != self.cols or math.prod(shape[:-1]) != self.rows:
+            raise ValueError(f"{tuple(self.shape)} cannot be seen as {tuple(shape)}")
+        p = Packed8.__new__(Packed8)
+        p._geometry(shape, self.dtype, self.device)
+        p._codes, p._steps, p._arena, p._at = self._codes, self._steps, self._arena, self._at
+        return p
+
+    def restore(self) -> Tensor:
+        return restore8(self)
+
+    def __repr__(self) -> str:
+        return f"Packed8({tuple(self.shape)}, {self.dtype}, {self.nbytes} bytes, {self.device})"
+
+
+def _row_dims(t: Tensor) -> Optional[List[int]]:
+    """[n0, n1, n2, s0, s1, s2] of a tensor's rows (all dimensions but the last, merged where the
+    strides allow it), or None where more than three remain or the channels are not adjacent."""
+    if t.dim() > 1 and t.shape[-1] > 1 and t.stride(-1) != 1 or t.dim() == 1 and t.stride(0) != 1 < t.shape[0]:
+        return None
+    dims: List[List[int]] = []
+    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+        if n == 1:
+            continue
+        if dims and dims[-1][1] == n * s:
+            dims[-1] = [dims[-1][0] * n, s]
+        else:
+            dims.append([n, s])
+    if len(dims) > 3:
+        return None
+    dims = [[1, 0]] * (3 - len(dims)) + dims
+    return [d[0] for d in dims] + [d[1] for d in dims]
+
+
+def _on(device: torch.device):
+    """Makes the tensors' device the current one for the launches inside."""
+    return torch.cuda.device(device)
+
+
+def _launch(fn_name: str, recs: List[bytes]) -> None:
+    K = _kernels()
+    fn = getattr(K._lib, fn_name)
+    for i in range(0, len(recs), _MAX_RECS):
+        part = recs[i:i + _MAX_RECS]
+        K._check(fn(b"".join(part), len(part), K._stream()), fn_name)
+        K.LAUNCHES.count += 1
+
+
+def _current(device: torch.device) -> bool:
+    return device.index == torch._C._cuda_getDevice()
+
+
+def _same_device(what: str, *ts) -> torch.device:
+    dev = ts[0].device
+    if any(t.device != dev for t in ts):
+        raise ValueError(f"{what}: tensors on different devices")
+    return dev
+
+
+def store8(xs: Union[Tensor, Sequence[Tensor]]) -> Union[Packed8, List[Packed8]]:
+    """8-bit form of one tensor or of several (bf16 or fp32, one device; last dimension = channels,
+    any number of leading ones, rows at any strides).  Several share one launch and one buffer."""
+    if isinstance(xs, Tensor):
+        return store8([xs])[0]
+    xs = [x.detach() for x in xs]
+    if not xs:
+        return []
+    for x in xs:
+        if x.dtype not in (BF16, F32) or x.dim() < 1:
+            raise ValueError(f"store8 takes bf16 or fp32 activations, not {x.dtype} of {x.dim()} dimensions")
+    dev = _same_device("store8", *xs)
+    if not xs[0].is_cuda:
+        out = []
+        for x in xs:
+            codes, steps = ref.store8(x.reshape(math.prod(x.shape[:-1]), x.shape[-1]))
+            out.append(Packed8(codes, steps, x.shape, x.dtype))
+        return out
+    if not _current(dev):
+        with _on(dev):
+            return store8(xs)
+    at, total = [], 0
+    for x in xs:
+        pitch, spitch = _pitches(x.shape[-1])
+        rows = math.prod(x.shape[:-1])
+        o1 = total + (rows * pitch + 127) // 128 * 128
+        at.append((total, o1))
+        total = o1 + (rows * spitch + 127) // 128 * 128
+    arena = torch.empty(total, dtype=torch.uint8, device=dev)
+    base = arena.data_ptr()
+    out, recs, hold = [], [], []
+    for x, (oc, os_) in zip(xs, at):
+        out.append(Packed8._in(arena, (oc, os_), x.shape, x.dtype))
+        if x.numel() == 0:
+            continue
+        dims = _row_dims(x)
+        if dims is None:                       # channels apart, or rows that are no three strides
+            x = x.contiguous()
+            hold.append(x)
+            dims = _row_dims(x)
+        recs.append(_REC.pack(x.data_ptr(), base + oc, base + os_, *dims, x.shape[-1], int(x.dtype == F32)))
+    if recs:
+        _launch("imf_store8", recs)
+    return out
+
+
+def restore8(ps: Union[Packed8, Sequence[Packed8]], outs=None) -> Union[Tensor, List[Tensor]]:
+    """The values of one packed tensor or of several, in one launch; ``outs``: where they go (one
+    tensor, or a list with None for a new one), of the packed shape and type, rows at any three
+    strides, channels adjacent."""
+    if isinstance(ps, Packed8):
+        return restore8([ps], None if outs is None else [outs])[0]
+    ps = list(ps)
+    if not ps:
+        return []
+    outs = [None] * len(ps) if outs is None else list(outs)
+    if len(outs) != len(ps):
+        raise ValueError(f"{len(ps)} packed tensors and {len(outs)} outputs")
+    dev = _same_device("restore8", *ps, *[o for o in outs if o is not None])
+    for p, o in zip(ps, outs):
+        if o is not None and (o.shape != p.shape or o.dtype != p.dtype):
+            raise ValueError(f"output {o.dtype} {tuple(o.shape)} for packed {p.dtype} {tuple(p.shape)}")
+    if dev.type != "cuda":
+        for i, p in enumerate(ps):
+            v = ref.values8(p.codes, p.steps, p.cols).to(p.dtype).view(p.shape)
+            outs[i] = v if outs[i] is None else outs[i].copy_(v)
+        return outs
+    if not _current(dev):
+        with _on(dev):
+            return restore8(ps, outs)
+    recs = []
+    for i, p in enumerate(ps):
+        if outs[i] is None:
+            outs[i] = torch.empty(p.shape, dtype=p.dtype, device=dev)
+        o = outs[i]
+        if o.numel() == 0:
+            continue
+        dims = _row_dims(o)
+        if dims is None:
+            raise ValueError("restore8 output: the channels have to be adjacent and the rows at three strides at most")
+        recs.append(_REC.pack(o.data_ptr(), *p._ptrs(), *dims, p.cols, int(p.dtype == F32)))
+    if recs:
+        _launch("imf_restore8", recs)
+    return outs
+
+
+def gemm_wgrad8(dy: Tensor, x8: Packed8, out: Optional[Tensor] = None, accumulate: bool = False) -> Tensor:
+    """Weight gradient ``out[n_out, n_in] (+)= dy^T x`` of a linear layer whose input (rows, n_in) is
+    kept in 8 bits; ``dy`` (rows, n_out) bf16 with 16-byte aligned rows, fp32 result, slices of
+    the rows summed in a fixed order (see ``kernels.gemm_wgrad``)."""
+    if not isinstance(x8, Packed8) or x8.dtype != BF16:
+        raise ValueError("gemm_wgrad8 takes a bf16 activation packed by store8")
+    if dy.dtype != BF16 or dy.dim() != 2 or dy.shape[0] != x8.rows:
+        raise ValueError(f"dy {dy.dtype} {tuple(dy.shape)} does not go with packed rows {x8.rows}")
+    N, C = dy.shape[1], x8.cols
+    if out is None:
+        accumulate = False
+    elif out.dtype != F32 or tuple(out.shape) != (N, C) or (C > 1 and out.stride(1) != 1):
+        raise ValueError(f"out has to be fp32 ({N}, {C}) with adjacent columns")
+    dev = _same_device("gemm_wgrad8", dy, x8, *([] if out is None else [out]))
+    if out is None:
+        out = torch.empty(N, C, dtype=F32, device=dev)
+    if dy.numel() == 0 or C == 0:
+        return out if accumulate else out.zero_()
+    if dev.type != "cuda":
+        g = dy.float().t() @ ref.values8(x8.codes, x8.steps, C)
+        return out.add_(g) if accumulate else out.copy_(g)
+    if not _current(dev):
+        with _on(dev):
+            return gemm_wgrad8(dy, x8, out, accumulate)
+    if dy.stride(1) != 1 and N > 1 or dy.stride(0) % 8 or dy.data_ptr() % 16:
+        raise ValueError("dy needs adjacent columns and 16-byte aligned rows")
+    K = _kernels()
+    x = torch.empty(x8.rows, _pitches(C)[0], dtype=BF16, device=dev)[:, :C]
+    restore8(x8.view(x8.rows, C), x)
+    return K.gemm_wgrad(dy, x, out, accumulate)
+
+
+def situ_bwd8(gu8: Packed8, gout: Tensor, beta: float, lbeta: Optional[float]) -> Tuple[Tensor, Tensor]:
+    """Reverse mode of y = situ(gate) up' from the packed [gate | up] (rows, 2F): returns (its
+    gradient (rows, 2F), y (rows, F)), bf16 -- y is what the next layer's weight gradient multiplies, so
+    it need not be kept.  ``gout`` (rows, F) bf16, adjacent columns."""
+    if not isinstance(gu8, Packed8) or gu8.dtype != BF16 or gu8.cols % 2:
+        raise ValueError("situ_bwd8 takes a bf16 [gate | up] packed by store8")
+    rows, F = gu8.rows, gu8.cols // 2
+    if gout.dtype != BF16 or gout.dim() != 2 or tuple(gout.shape) != (rows, F):
+        raise ValueError(f"gout {gout.dtype} {tuple(gout.shape)}: bf16 ({rows}, {F}) expected")
+    if not beta > 0 or (lbeta is not None and not lbeta > 0):
+        raise ValueError(f"beta {beta} and linear beta {lbeta} have to be positive")
+    dev = _same_device("situ_bwd8", gu8, gout)
+    g_gu = torch.empty(rows, 2 * F, dtype=BF16, device=dev)
+    act = torch.empty(rows, F, dtype=BF16, device=dev)
+    if rows == 0 or F == 0:
+        return g_gu, act
+    if dev.type != "cuda":
+        gu = ref.values8(gu8.codes, gu8.steps, 2 * F)
+        a, b, y = ref.situ_mul_grad(gu[:, :F], gu[:, F:], gout, beta, lbeta)
+        return g_gu.copy_(torch.cat([a, b], 1)), act.copy_(y)
+    if not _current(dev):
+        with _on(dev):
+            return situ_bwd8(gu8, gout, beta, lbeta)
+    if F > 1 and gout.stride(1) != 1:
+        raise ValueError("gout needs adjacent columns")
+    K = _kernels()
+    codes, steps = gu8._ptrs()
+    K._check(K._lib.imf_situ_bwd8(codes, steps, gout.data_ptr(), g_gu.data_ptr(), act.data_ptr(), rows, F,
+                                  gout.stride(0), 2 * F, F, float(beta), float(lbeta or 0.0),
+                                  int(lbeta is not None), K._stream()), "imf_situ_bwd8")
+    K.LAUNCHES.count += 1
+    return g_gu, act
+
+
+def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Packed8, Tensor], lse: Tensor,
+              go: Tensor, scale: Optional[float] = None, gv_out: Optional[Tensor] = None
+              ) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dq, dk, dv) of dense attention on (B, L, H, head_dim 64 or 128) from checkpoints of q, k, v and
+    the output o, the forward's log-sum-exp (B, H, L) and the output gradient ``go`` (bf16):
+
+        P = exp(scale q k^T - lse),  dV = P^T go,  dS = P * (go v^T - rowsum(go * o)),
+        dQ = scale dS k,  dK = scale dS^T q
+
+    v and o may also be bf16 tensors (a band of a wider buffer that is restored anyway).  ``gv_out``
+    takes dv, as in ``kernels.attn_bwd``, whose fixed-order mode holds here too."""
+    for name, t in (("q", q8), ("k", k8)):
+        if not isinstance(t, Packed8):
+            raise ValueError(f"attn_bwd8: {name} has to be packed by store8")
+    shape = q8.shape
+    if len(shape) != 4 or shape[3] not in (64, 128):
+        raise ValueError(f"attn_bwd8 takes (B, L, H, 64 or 128), not {tuple(shape)}")
+    B, L, H, hd = shape
+    for name, t in (("q", q8), ("k", k8), ("v", v8), ("o", o8), ("go", go), ("gv_out", gv_out)):
+        if t is not None and (t.shape != shape or t.dtype != BF16):
+            raise ValueError(f"attn_bwd8: {name} is {t.dtype} {tuple(t.shape)}, q is bf16 {tuple(shape)}")
+    if lse.dtype != F32 or tuple(lse.shape) != (B, H, L) or not lse.is_contiguous():
+        raise ValueError(f"attn_bwd8: lse has to be contiguous fp32 {(B, H, L)}")
+    dev = _same_device("attn_bwd8", q8, k8, v8, o8, lse, go, *([] if gv_out is None else [gv_out]))
+    if 0 in shape:
+        new = lambda: torch.empty(shape, dtype=BF16, device=dev)
+        return new(), new(), new() if gv_out is None else gv_out
+    plain = lambda t: t.restore() if isinstance(t, Packed8) else t
+    if dev.type != "cuda":
+        dq, dk, dv = ref.attention_grad(*(plain(t) for t in (q8, k8, v8, o8)), lse, go, scale)
+        dv = dv.to(BF16) if gv_out is None else gv_out.copy_(dv)
+        return dq.to(BF16), dk.to(BF16), dv
+    if not _current(dev):
+        with _on(dev):
+            return attn_bwd8(q8, k8, v8, o8, lse, go, scale, gv_out)
+    K = _kernels()
+    packed = [t for t in (q8, k8, v8, o8) if isinstance(t, Packed8)]
+    got = iter(restore8(packed))
+    q, k, v, o = (next(got) if isinstance(t, Packed8) else t for t in (q8, k8, v8, o8))
+    return K.attn_bwd(q, k, v, o, lse, go, scale=scale, gv_out=gv_out)

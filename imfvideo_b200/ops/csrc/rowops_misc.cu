@@ -9,6 +9,7 @@
 // `_gate_add_kernel` (reference models/triton_mla_block_jvp.py:237-521) and
 // add the backward halves the reference leaves to autograd.
 #include "rowops_common.cuh"
+#include "situ.cuh"
 
 namespace imf {
 
@@ -602,31 +603,6 @@ __global__ void __launch_bounds__(ROW_THREADS) outgate_bwd_kernel(const EwArgs a
     const float4 one = make_float4(1.f - s.x, 1.f - s.y, 1.f - s.z, 1.f - s.w);
     st4(a.ga + (size_t)row * a.ld_ga + c, g * s);
     st4(a.gb + (size_t)row * a.ld_gb + c, g * o * s * one);
-  }
-}
-
-// situ(g) = beta tanh(g/beta) sigmoid(g); up' = lbeta tanh(up/lbeta).  The hyperbolic
-// tangent is the hardware approximation (one MUFU op, error below bf16 resolution) and the
-// sigmoid is written through it, sigmoid(x) = 0.5 tanh(x / 2) + 0.5: three special-function
-// ops per element, so the kernels below stay memory-bound.
-__device__ __forceinline__ float tanh_fast(float x) {
-  float y;
-  asm("tanh.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void situ1(float g, float u, float beta, float inv_beta, float lbeta,
-                                      float inv_lbeta, int has_lb, float& a, float& da_dg,
-                                      float& up, float& dup_du) {
-  const float th = tanh_fast(g * inv_beta), sg = fmaf(0.5f, tanh_fast(0.5f * g), 0.5f);
-  a = beta * th * sg;
-  da_dg = (1.f - th * th) * sg + beta * th * sg * (1.f - sg);
-  if (has_lb) {
-    const float tu = tanh_fast(u * inv_lbeta);
-    up = lbeta * tu;
-    dup_du = 1.f - tu * tu;
-  } else {
-    up = u;
-    dup_du = 1.f;
   }
 }
 

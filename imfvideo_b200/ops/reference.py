@@ -189,3 +189,62 @@ def newton_schulz(G: Tensor, coeffs: Tuple[float, float, float], steps: int = 5,
         B = b * A + c * (A @ A)
         X = a * X + B @ X
     return X.T if tr else X
+
+
+# --------------------------------------------------------------------------
+# Activations in 8 bits (``ops/act8.py``, ``csrc/act8.cuh``)
+# --------------------------------------------------------------------------
+def store8(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """(codes (rows, pitch) int8, steps (rows, spitch) uint8) of a (rows, C) tensor: for each 32
+    channels a power of two 2^(s-127) so that the largest of them is 64 to 127 steps (s = 255:
+    a NaN or an infinity among them); pitches rounded up to 32 channels and 4 groups."""
+    rows, C = x.shape
+    G = -(-C // 32)
+    g = x.new_zeros(rows, G * 32, dtype=torch.float32)
+    g[:, :C] = x
+    g = g.view(rows, G, 32)
+    amax = g.abs().amax(-1)
+    s = ((amax.view(torch.int32) + 0x10000) >> 23) - 6
+    s = s.clamp(0, 248)
+    inv = ((254 - s) << 23).view(torch.float32)
+    bad = ~torch.isfinite(amax)
+    codes = torch.round(g * inv[..., None]).clamp(-127, 127).masked_fill(bad[..., None], 0)
+    steps = torch.zeros(rows, (G + 3) // 4 * 4, dtype=torch.uint8, device=x.device)
+    steps[:, :G] = s.masked_fill(bad, 255).to(torch.uint8)
+    return codes.to(torch.int8).view(rows, G * 32), steps
+
+
+def values8(codes: Tensor, steps: Tensor, C: int) -> Tensor:
+    """fp32 (rows, C) values code * 2^(s-127) of ``store8``'s outputs (s = 255: NaN)."""
+    rows, pitch = codes.shape
+    s = steps[:, :pitch // 32].to(torch.int32)
+    bits = torch.where(s == 0, 0x00400000, torch.where(s == 255, 0x7fc00000, s << 23)).to(torch.int32)
+    step = bits.view(torch.float32)
+    return (codes.view(rows, pitch // 32, 32).float() * step[..., None]).view(rows, pitch)[:, :C]
+
+
+def situ_mul_grad(gate: Tensor, up: Tensor, gout: Tensor, beta: float, linear_beta: Optional[float]
+                  ) -> Tuple[Tensor, Tensor, Tensor]:
+    """(d gate, d up, y) of y = situ_mul(gate, up) for the output gradient ``gout``, in fp32."""
+    g, u, go = gate.float(), up.float(), gout.float()
+    th, sg = torch.tanh(g / beta), torch.sigmoid(g)
+    a = beta * th * sg
+    da = (1 - th * th) * sg + a * (1 - sg)
+    if linear_beta is None:
+        up_, dup = u, torch.ones_like(u)
+    else:
+        tu = torch.tanh(u / linear_beta)
+        up_, dup = linear_beta * tu, 1 - tu * tu
+    return go * da * up_, go * a * dup, a * up_
+
+
+def attention_grad(q: Tensor, k: Tensor, v: Tensor, o: Tensor, lse: Tensor, go: Tensor,
+                   scale: Optional[float] = None) -> Tuple[Tensor, Tensor, Tensor]:
+    """(dq, dk, dv) in fp32 of softmax attention on (B, L, H, d) tensors; the probabilities are
+    recomputed from the scores and ``lse`` (B, H, L)."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    q, k, v, o, go = (t.float().transpose(1, 2) for t in (q, k, v, o, go))
+    p = torch.exp(q @ k.transpose(-1, -2) * scale - lse[..., None])
+    ds = p * (go @ v.transpose(-1, -2) - (go * o).sum(-1, keepdim=True))
+    out = (ds @ k * scale, ds.transpose(-1, -2) @ q * scale, p.transpose(-1, -2) @ go)
+    return tuple(t.transpose(1, 2) for t in out)

@@ -1,0 +1,404 @@
+"""GPU: activations in 8 bits and the backward operators on them, against the formulas in 64 bits."""
+import math
+
+import pytest
+import torch
+
+from imfvideo_b200.ops import reference as ref
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32 = torch.bfloat16, torch.float32
+TANH = 2.0 ** -10.9          # relative error of the hardware's hyperbolic tangent (PTX ISA: 2^-11)
+
+
+@pytest.fixture(scope="module")
+def A():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from imfvideo_b200.ops import cuda as cu
+
+    assert cu.available(), "kernel library must load on a GPU box"
+    from imfvideo_b200.ops import act8
+
+    return act8
+
+
+@pytest.fixture(scope="module")
+def K(A):
+    from imfvideo_b200.ops import kernels
+
+    return kernels
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def _randn(g, *shape, s=1.0, dtype=BF16):
+    return (torch.randn(*shape, device="cuda", generator=g) * s).to(dtype)
+
+
+def _activations(g, rows, C, dtype=BF16):
+    """Channels of different size, some of them far above the rest."""
+    s = torch.exp(torch.randn(C, device="cuda", generator=g))
+    return (torch.randn(rows, C, device="cuda", generator=g) * s).to(dtype)
+
+
+def _same(a, b):
+    return torch.equal(torch.isnan(a), torch.isnan(b)) and torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0))
+
+
+def _check_store(A, x, p=None):
+    p = A.store8(x) if p is None else p
+    flat = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    codes, steps = ref.store8(flat)
+    assert torch.equal(p.codes, codes) and torch.equal(p.steps, steps)
+    v = A.restore8(p)
+    want = ref.values8(codes, steps, x.shape[-1]).to(x.dtype).view(x.shape)
+    assert v.dtype == x.dtype and v.shape == x.shape and _same(v, want)
+    return p
+
+
+# ------------------------------------------------------------- store, restore ---
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("rows,C", [(1, 1), (1, 32), (3, 7), (5, 33), (2, 64), (77, 48), (130, 528), (31, 1021),
+                                    (2068, 682), (4099, 1376), (9000, 2064)])
+def test_store_and_restore(A, dtype, rows, C):
+    _check_store(A, _activations(_gen(rows + C), rows, C, dtype))
+
+
+def test_edges_of_the_format(A):
+    from test_act8 import edge_rows
+
+    for dtype in (BF16, F32):
+        _check_store(A, edge_rows().cuda().to(dtype))
+    top = torch.full((2, 64), torch.finfo(F32).max, device="cuda")
+    top[1] = -top[1]
+    _check_store(A, top)
+    every = torch.arange(-127, 128, device="cuda").to(F32)              # every code, at every step
+    x = torch.zeros(249, 9, 32, device="cuda")
+    x.view(249, -1)[:, :255] = every
+    x[:, :, 31] = 127.0                                                 # so that the step is one
+    x = x * torch.exp2(torch.arange(249, device="cuda").double() - 127).to(F32)[:, None, None]
+    p = _check_store(A, x.view(249, -1))
+    assert torch.equal(p.steps[:, :8].long(), torch.arange(249, device="cuda")[:, None].expand(249, 8))
+    assert torch.equal(A.restore8(p), x.view(249, -1))
+
+
+def test_strides_alignment_and_many_tensors(A):
+    g = _gen(5)
+    wide = _randn(g, 2, 50, 3, 112)
+    odd = _randn(g, 40, 203)
+    f = _randn(g, 6, 5, 4, 3, 40, dtype=F32)
+    xs = [wide[..., 48:], wide.transpose(1, 2), wide[:, ::3], odd[:, 3:], odd[:, 1:70], odd.t()[:, :33],
+          wide[:, :, 1], f[..., 4:], f.permute(0, 2, 1, 3, 4), f.permute(3, 1, 0, 2, 4)[::2, :, :, ::3], odd[7],
+          odd[:, 5], torch.empty(0, 40, device="cuda"), _randn(g, 9, 1, 8).expand(9, 4, 8)]
+    xs += [_randn(g, 3 + i, 40 + i) for i in range(25)]                 # more than one launch takes
+    ps = A.store8(xs)
+    for x, p in zip(xs, ps):
+        _check_store(A, x, p)
+    for p, v in zip(ps, A.restore8(ps)):
+        assert _same(v, p.restore())
+
+
+def test_restore_into_views_leaves_the_rest(A):
+    g = _gen(6)
+    p, q = A.store8([_randn(g, 2, 33, 3, 45), _randn(g, 66, 77, dtype=F32)])
+    a = torch.full((2, 33, 3, 64), -7.75, dtype=BF16, device="cuda")
+    b = torch.full((66, 100), -7.75, device="cuda")
+    out = A.restore8([p, q], [a[..., 11:56], b[:, 23:]])
+    assert _same(a[..., 11:56], p.restore()) and _same(b[:, 23:], q.restore())
+    assert (a[..., :11] == -7.75).all() and (a[..., 56:] == -7.75).all() and (b[:, :23] == -7.75).all()
+    assert out[0].data_ptr() == a[..., 11:56].data_ptr()
+    with pytest.raises(ValueError):
+        A.restore8(q, torch.empty(77, 66, device="cuda").t())
+    with pytest.raises(ValueError):
+        A.restore8([p], [torch.empty(2, 33, 3, 45, dtype=BF16)])         # on the CPU
+
+
+def test_offsets_beyond_32_bits(A):
+    """Rows 2^30 elements apart, and a tensor of more than 2^32 bytes of codes."""
+    buf = torch.zeros(2 * 2 ** 30 + 128, dtype=BF16, device="cuda")
+    x = buf.as_strided((3, 80), (2 ** 30, 1))
+    x.copy_(_randn(_gen(7), 3, 80))
+    _check_store(A, x)
+    y = torch.zeros_like(buf).as_strided((3, 80), (2 ** 30, 1))
+    A.restore8(A.store8(x), y)
+    assert _same(y, A.store8(x).restore())
+    del buf, x, y
+    rows = 2 ** 32 // 4096 + 3
+    big = torch.ones(rows, 4096, dtype=BF16, device="cuda")
+    big[-1] = torch.arange(4096, device="cuda") % 61
+    p = A.store8(big)
+    v = A.restore8(p)
+    assert torch.equal(v[-2:], A.store8(big[-2:]).restore()) and bool((v[:-1] == 1).all())
+    del big, p, v
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------- weight gradient ---
+def _wgrad_check(got, dy, p, base=None):
+    x = ref.values8(p.codes, p.steps, p.cols)
+    want = dy.double().t() @ x.double()
+    size = dy.double().abs().t() @ x.double().abs()
+    if base is not None:
+        want, size = want + base.double(), size + base.double().abs()
+    # every addition may drop 2^-23 of a running sum that is at most `size`
+    assert ((got.double() - want).abs() <= (dy.shape[0] + 4) * 2.0 ** -23 * size).all()
+    assert (got.double() - want).norm() <= 1e-5 * want.norm()
+
+
+@pytest.mark.parametrize("rows,N,C", [(1, 8, 1), (1, 136, 300), (7, 16, 31), (63, 128, 128), (64, 8, 64),
+                                      (65, 264, 77), (130, 528, 256), (532, 528, 257), (1000, 144, 512),
+                                      (4099, 40, 1021), (2068, 1376, 256), (29140, 256, 128), (16500, 72, 40)])
+def test_weight_gradient(A, K, rows, N, C):
+    g = _gen(rows)
+    dy, p = _randn(g, rows, N), A.store8(_activations(g, rows, C))
+    got = A.gemm_wgrad8(dy, p)
+    assert got.dtype == F32 and got.shape == (N, C)
+    _wgrad_check(got, dy, p)
+    assert torch.equal(A.gemm_wgrad8(dy, p), got)                        # fixed order
+    base = torch.randn(N, C, device="cuda", generator=g)
+    acc = base.clone()
+    assert A.gemm_wgrad8(dy, p, out=acc, accumulate=True) is acc
+    _wgrad_check(acc, dy, p, base)
+    K.check_status()
+
+
+def test_weight_gradient_views(A, K):
+    """A band of a wider dY, a result inside a guarded wider buffer at aligned and at odd pitches."""
+    g = _gen(11)
+    dy = _randn(g, 777, 400)[:, 8:8 + 203]
+    p = A.store8(_randn(g, 3, 259, 100))                                 # rows from two dimensions
+    for ld, c0 in ((160, 32), (163, 5)):
+        for accumulate in (False, True):
+            buf = torch.full((203, ld), 3.5, device="cuda")
+            out = buf[:, c0:c0 + 100]
+            A.gemm_wgrad8(dy, p, out=out, accumulate=accumulate)
+            _wgrad_check(out, dy, p, torch.full((203, 100), 3.5, device="cuda") if accumulate else None)
+            assert (buf[:, :c0] == 3.5).all() and (buf[:, c0 + 100:] == 3.5).all()
+    assert torch.equal(A.gemm_wgrad8(dy[:0], A.store8(_randn(g, 0, 100))), torch.zeros(203, 100, device="cuda"))
+    with pytest.raises(ValueError):
+        A.gemm_wgrad8(_randn(g, 777, 203), p)                            # rows 406 bytes apart
+    with pytest.raises(ValueError):
+        A.gemm_wgrad8(_randn(g, 777, 208)[:, 1:], p)
+    with pytest.raises(ValueError):
+        A.gemm_wgrad8(_randn(g, 208, 777).t(), p)
+    K.check_status()
+
+
+def test_weight_gradient_bad_values(A, K):
+    """A group with an infinity makes NaN of its own 32 columns, an infinity of dY of its own row."""
+    g = _gen(12)
+    x, dy = _randn(g, 300, 96), _randn(g, 300, 64)
+    x[17, 40] = float("inf")
+    bad = torch.isnan(A.gemm_wgrad8(dy, A.store8(x)))
+    assert bad[:, 32:64].all() and not bad[:, :32].any() and not bad[:, 64:].any()
+    x[17, 40], dy[5, 9] = 1.0, float("nan")
+    bad = torch.isnan(A.gemm_wgrad8(dy, A.store8(x)))
+    assert bad[9].all() and bad.sum() == 96
+    K.check_status()
+
+
+# ------------------------------------------------------------- gated activation ---
+@pytest.mark.parametrize("lbeta", [25.0, None])
+@pytest.mark.parametrize("rows,F", [(1, 1), (1, 8), (3, 21), (77, 688), (130, 24), (2068, 682), (5000, 1000)])
+def test_gated_activation(A, rows, F, lbeta):
+    g = _gen(rows + F)
+    gu, gout = _randn(g, rows, 2 * F, s=2.0), _randn(g, rows, F)
+    p = A.store8(gu)
+    grad, y = A.situ_bwd8(p, gout, 4.0, lbeta)
+    v = ref.values8(p.codes, p.steps, 2 * F).double()
+    gate, up, go = v[:, :F], v[:, F:], gout.double()
+    dg, du, want_y = (t.double() for t in ref.situ_mul_grad(gate, up, gout, 4.0, lbeta))
+    up_ = up.abs() if lbeta is None else (lbeta * torch.tanh(up / lbeta)).abs()
+    # a = beta th sg with sg = (1 + tanh(gate / 2)) / 2: TANH |th| on th, TANH / 2 on sg (both below 1), so
+    # 1.5 beta TANH on a; (1 - th^2) sg is 2.5 TANH off, beta th sg (1 - sg) at most 2 beta TANH; up' and
+    # its derivative 1 - tu^2 TANH and 2 TANH; then one rounding to bf16
+    a_err, da_err, u_err = 6.0 * TANH, (2.5 + 8.0) * TANH, TANH if lbeta else 0.0
+    half = 2.0 ** -8
+    assert ((y.double() - want_y).abs() <= half * want_y.abs() + 1.01 * (a_err + 4 * u_err) * up_ + 1e-30).all()
+    assert ((grad[:, :F].double() - dg).abs() <= half * dg.abs() + 1.01 * go.abs() * up_ * (da_err + 2 * u_err)
+            + 1e-30).all()
+    assert ((grad[:, F:].double() - du).abs() <= half * du.abs() + 1.01 * go.abs() * (a_err + 8 * u_err) + 1e-30).all()
+    wide = torch.full((rows, F + 24), 1e4, dtype=BF16, device="cuda")    # a band of a wider gradient
+    wide[:, 8:8 + F] = gout
+    again, y2 = A.situ_bwd8(p, wide[:, 8:8 + F], 4.0, lbeta)
+    assert torch.equal(again, grad) and torch.equal(y2, y)
+
+
+def test_gated_activation_refuses_scattered_columns(A):
+    p = A.store8(torch.zeros(4, 64, dtype=BF16, device="cuda"))
+    with pytest.raises(ValueError):
+        A.situ_bwd8(p, torch.zeros(32, 4, dtype=BF16, device="cuda").t(), 4.0, 25.0)
+
+
+# ------------------------------------------------------------- attention ---
+def _attention(A, K, B, L, H, hd, seed, s=1.0):
+    g = _gen(seed)
+    q, k, v, go = (_randn(g, B, L, H, hd, s=x) for x in (s, 1.0, 1.0, 1.0))
+    o, _, lse = K.attn_fwd(q, k, v)
+    return A.store8([q, k, v, o]), lse, go, o
+
+
+def _oracle(ps, lse, go, scale=None):
+    v = [p.restore().double() for p in ps]
+    q, k, v, o, go = (t.transpose(1, 2) for t in (*v, go.double()))
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    P = torch.exp(q @ k.transpose(-1, -2) * scale - lse.double()[..., None])
+    ds = P * (go @ v.transpose(-1, -2) - (go * o).sum(-1, keepdim=True))
+    out = (ds @ k * scale, ds.transpose(-1, -2) @ q * scale, P.transpose(-1, -2) @ go)
+    return [t.transpose(1, 2) for t in out]
+
+
+def _near(got, want, what):
+    # q times a constant, the probabilities, dS and the result are each rounded to bf16, 2^-8 at most and
+    # unrelated from element to element: 4 roundings of 2^-8 / sqrt(3) each add up to 2 2^-8 / sqrt(3) = 4.6e-3
+    # of the norm at the very most of their range; twice that
+    for a, b, name in zip(got, want, ("dq", "dk", "dv")):
+        rel = ((a.double() - b).norm() / b.norm()).item()
+        assert rel < 1e-2, (what, name, rel)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("B,L,H", [(1, 2, 1), (2, 65, 3), (1, 128, 4), (3, 333, 2), (1, 1025, 5), (1, 2049, 1)])
+def test_attention(A, K, B, L, H, hd):
+    ps, lse, go, o = _attention(A, K, B, L, H, hd, L + H)
+    got = A.attn_bwd8(*ps, lse, go)
+    _near(got, _oracle(ps, lse, go), (B, L, H, hd))
+    # a bf16 v and o in the place of packed ones, dv into a band
+    v, o_ = ps[2].restore(), ps[3].restore()
+    wide = torch.full((B, L, H, hd + 48), 3.0, dtype=BF16, device="cuda")
+    dq, dk, dv = A.attn_bwd8(ps[0], ps[1], v, o_, lse, go, gv_out=wide[..., 48:])
+    assert dv.data_ptr() == wide[..., 48:].data_ptr() and (wide[..., :48] == 3).all()
+    _near((dq, dk, dv), [t.double() for t in got], "mixed")
+    K.check_status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_one_token(A, K, hd):
+    """dQ and dK of a single token are zero but for the rounding of delta (2^-17 of |go| |o|)."""
+    ps, lse, go, o = _attention(A, K, 2, 1, 3, hd, 3)
+    dq, dk, dv = A.attn_bwd8(*ps, lse, go)
+    _, _, want = _oracle(ps, lse, go)
+    q, k, v, _ = (p.restore().double() for p in ps)
+    # dv = P go: the kernel rounds q times a constant to bf16 before the score product, each factor off by
+    # 2^-8 at most, so the exponent is off by 2^-8 scale sum |q k| at most and P by expm1 of that (the
+    # score's own fp32 rounding is in the 1e-5); then P and dv are rounded to bf16, 2^-8 each
+    exponent = 2.0 ** -8 * hd ** -0.5 * (q * k).abs().sum(-1, keepdim=True) + 1e-5
+    rel = (1 + torch.expm1(exponent)) * (1 + 2.0 ** -8) ** 2 - 1
+    assert ((dv.double() - want).abs() <= rel * want.abs() + 1e-30).all()
+    size = (go.double().norm(dim=-1) * v.norm(dim=-1))[..., None] * 2.0 ** -15 * hd ** -0.5
+    assert (dq.double().abs() <= size * k.abs() * 1.2 + 1e-12).all()
+    assert (dk.double().abs() <= size * q.abs() * 1.2 + 1e-12).all()
+
+
+def test_attention_fixed_order_and_views(A, K):
+    ps, lse, go, o = _attention(A, K, 1, 1500, 3, 64, 21)
+    wide = torch.empty(1, 1500, 3, 96, dtype=BF16, device="cuda")
+    wide[..., 32:] = go
+    was = K.DETERMINISTIC
+    try:
+        K.set_deterministic(True)
+        a = A.attn_bwd8(*ps, lse, wide[..., 32:])
+        b = A.attn_bwd8(*ps, lse, go)
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+    finally:
+        K.set_deterministic(was)
+    got = A.attn_bwd8(*ps, lse, go.transpose(1, 2).contiguous().transpose(1, 2))
+    _near(got, [t.double() for t in a], "order of go")
+    _near(A.attn_bwd8(*ps, lse, go, scale=0.05), _oracle(ps, lse, go, 0.05), "scale")
+    none = torch.empty(0, 5, 2, 64, dtype=BF16, device="cuda")
+    assert A.attn_bwd8(*A.store8([none] * 4), torch.empty(0, 2, 5, device="cuda"), none)[0].shape == none.shape
+    with pytest.raises(ValueError):
+        A.attn_bwd8(*ps, lse.transpose(1, 2).contiguous().transpose(1, 2), go)
+    K.check_status()
+
+
+def test_attention_gradient_is_a_difference_quotient(A, K):
+    """Along a random direction of q, k and v the loss changes as the gradients say (64-bit differences)."""
+    B, L, H, hd = 1, 40, 2, 64
+    g = _gen(30)
+    q, k, v, go = (_randn(g, B, L, H, hd, s=0.5) for _ in range(4))
+    ps = A.store8([q, k, v])
+    z = [p.restore().double() for p in ps]
+
+    def fwd(q, k, v):
+        s = torch.einsum("blhd,bmhd->bhlm", q, k) / math.sqrt(hd)
+        return torch.einsum("bhlm,bmhd->blhd", torch.softmax(s, -1), v), torch.logsumexp(s, -1)
+
+    o, lse = fwd(*z)
+    grads = A.attn_bwd8(*ps, o.bfloat16(), lse.float(), go)
+    for i in range(3):
+        d = torch.randn(z[i].shape, device="cuda", generator=g, dtype=torch.float64)
+        up, down = list(z), list(z)
+        up[i], down[i] = z[i] + 1e-4 * d, z[i] - 1e-4 * d
+        want = ((fwd(*up)[0] - fwd(*down)[0]) * go.double()).sum() / 2e-4
+        got = (grads[i].double() * d).sum()
+        # 2-norm of the roundings of one gradient (see _near) against a unit direction
+        assert (got - want).abs() <= 1e-2 * grads[i].double().norm() * 3
+
+
+# ------------------------------------------------------------- streams, graphs, together ---
+def _linear_step(A, x, gu, dy, gout):
+    """What a block does: keep, then gradients from what was kept."""
+    x8, gu8 = A.store8([x, gu])
+    grad, act = A.situ_bwd8(gu8, gout, 4.0, 25.0)
+    return A.gemm_wgrad8(dy, x8), grad, act, A.restore8(x8)
+
+
+def test_another_stream_and_two_graphs(A, K):
+    g = _gen(40)
+    mk = lambda: (_randn(g, 600, 256), _randn(g, 600, 2 * 344), _randn(g, 600, 528), _randn(g, 600, 344))
+    a, b = mk(), mk()
+    want = [_linear_step(A, *t) for t in (a, b)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = _linear_step(A, *a)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(x, y) for x, y in zip(got, want[0]))
+    graphs, outs = [], []
+    for t in (a, b):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(_linear_step(A, *t))
+        graphs.append(graph)
+    for t, s in zip(a + b, mk() + mk()):
+        t.copy_(s)
+    want = [_linear_step(A, *t) for t in (a, b)]
+    for _ in range(2):
+        for graph in graphs:
+            graph.replay()
+    torch.cuda.synchronize()
+    for got, w in zip(outs, want):
+        assert all(torch.equal(x, y) for x, y in zip(got, w))
+    K.check_status()
+
+
+def test_attention_in_a_graph(A, K):
+    g = _gen(41)
+    q, k, v, go = (_randn(g, 1, 700, 2, 64) for _ in range(4))
+
+    def step():
+        o, _, lse = K.attn_fwd(q, k, v)
+        return A.attn_bwd8(*A.store8([q, k, v, o]), lse, go)
+
+    was = K.DETERMINISTIC
+    try:
+        K.set_deterministic(True)
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = step()
+        for t in (q, k, v, go):
+            t.copy_(_randn(g, *t.shape))
+        want = step()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out, want))
+    finally:
+        K.set_deterministic(was)
+    K.check_status()
