@@ -52,6 +52,10 @@ def _kernels():
         for name in ("imf_store8", "imf_restore8"):
             getattr(K._lib, name).restype = ci
             getattr(K._lib, name).argtypes = [vp, ci, vp]
+        K._lib.imf_wgrad8_work.restype = i64
+        K._lib.imf_wgrad8_work.argtypes = [ci] * 4
+        K._lib.imf_wgrad8.restype = ci
+        K._lib.imf_wgrad8.argtypes = [vp, i64, vp, vp, ci, ci, ci, vp, i64, ci, vp, i64, vp, vp]
         K._lib.imf_situ_bwd8.restype = ci
         K._lib.imf_situ_bwd8.argtypes = [vp] * 5 + [cl, ci] + [i64] * 3 + [cf, cf, ci, vp]
         _KERNELS = K
@@ -299,12 +303,20 @@ def gemm_wgrad8(dy: Tensor, x8: Packed8, out: Optional[Tensor] = None, accumulat
     if not _current(dev):
         with _on(dev):
             return gemm_wgrad8(dy, x8, out, accumulate)
-    if dy.stride(1) != 1 and N > 1 or dy.stride(0) % 8 or dy.data_ptr() % 16:
+    rows = x8.rows
+    ld = dy.stride(0) if rows > 1 else (N + 7) // 8 * 8
+    if dy.stride(1) != 1 and N > 1 or ld % 8 or dy.data_ptr() % 16:
         raise ValueError("dy needs adjacent columns and 16-byte aligned rows")
     K = _kernels()
-    x = torch.empty(x8.rows, _pitches(C)[0], dtype=BF16, device=dev)[:, :C]
-    restore8(x8.view(x8.rows, C), x)
-    return K.gemm_wgrad(dy, x, out, accumulate)
+    ldo = out.stride(0) if N > 1 else (C + 3) // 4 * 4
+    floats = K._lib.imf_wgrad8_work(rows, N, C, int(ldo % 4 == 0 and out.data_ptr() % 16 == 0))
+    work = torch.empty(floats, dtype=F32, device=dev) if floats else None
+    codes, steps = x8._ptrs()
+    K._check(K._lib.imf_wgrad8(dy.data_ptr(), ld, codes, steps, rows, N, C, out.data_ptr(), ldo, int(accumulate),
+                               None if work is None else work.data_ptr(), floats,
+                               K.status_word(dev).data_ptr(), K._stream()), "imf_wgrad8")
+    K.LAUNCHES.count += 2 if floats else 1
+    return out
 
 
 def situ_bwd8(gu8: Packed8, gout: Tensor, beta: float, lbeta: Optional[float]) -> Tuple[Tensor, Tensor]:

@@ -45,10 +45,11 @@ __device__ __forceinline__ uint32_t a8_encode4_top(const float* v, float inv) {
   return a8_encode4(c, 1.f);
 }
 
-// the step in both halves, as bf16 (2^-127 is half the smallest normal number)
+// the step in both halves, as bf16: the byte is the exponent.  2^-127 is half the smallest normal number
+// and 255 a NaN, both of which the upper mantissa bit makes
 __device__ __forceinline__ __nv_bfloat162 a8_step2(uint32_t s) {
-  const uint32_t h = s == A8_BAD ? 0x7fc0u : s == 0u ? 0x0040u : s << 7;
-  const uint32_t w = h | (h << 16);
+  uint32_t w = s * 0x00800080u;
+  if (s - 1u >= 254u) w |= 0x00400040u;
   return *reinterpret_cast<const __nv_bfloat162*>(&w);
 }
 // two codes (low bytes of the halves of x) times the step, exact.  The low seven bits of a code are the

@@ -1,0 +1,491 @@
+// Weight gradient of a linear layer whose input was kept in 8 bits (format: act8.cuh):
+//
+//   dW[N, C] (+)= dY^T X,   dY [R, N] bf16,  X [R, C] = codes * 2^(step - 127),  fp32 result
+//
+// on tcgen05 with the accumulator in TMEM.  Both operands are consumed MN-major as they lie in memory
+// (the contraction runs over the rows).  The step belongs to 32 channels of ONE row, so it cannot be taken
+// out of the sum; the codes are converted on their way from shared memory to shared memory instead,
+// and exactly (bf16 holds code * 2^k), so the product is that of the stored values.
+//
+// Two CTAs (a cluster) share a 256 (N) x BN (C) tile and its products (cta_group::2): each holds 128 of the
+// rows of dY^T and half of X's columns, so each converts half a tile for 256 rows of products.  k-blocks are
+// 64 rows of R.  Warps 0-3: epilogue; warp 4: loads (dY and codes by TMA, the steps by cp.async: their rows
+// are no 16-byte multiples); warp 5 of the first CTA: tcgen05.mma; then CONV groups of warps that convert a
+// k-block each.  R is cut into slices (split-K) where that fills the SMs; a second kernel adds their planes up
+// in a fixed order, so results repeat bit for bit.
+//
+// The tensor core's fp32 accumulator drops bits with every k-step, 1.2e-5 of the result's norm after 32,780
+// rows; so a chain ends after CHUNK_KB k-blocks, and the TMA unit adds the next one's sum to the stored one
+// (one CTA owns the place, and waits for one addition before the next: the order is fixed).
+//
+// What bounds it: the way into shared memory.  TMA takes about three clocks for a box row of 128 bytes, so a
+// k-block of 128 rows of dY^T and 128 columns of codes (BN 256) takes 600 clocks alone and 820 with all SMs reading,
+// against 512 of tcgen05.mma; with BN 512 (two accumulators share the rows of dY^T) 1,570 against 1,024.
+// 32,780 rows x 5,472 x 1,024: 315 us (1,166 TFLOP/s) with BN 512, 381 with 256; one CTA per tile 372 (256 x
+// 256) to 620 us (128 x 256), conversion included; restoring X to bf16 first and the bf16 kernel of gemm.cu 428.
+// 29,140 x 1,376 x 256: 39 us, the bf16 kernel alone 45.  Tried and slower: codes loaded into registers by the
+// converting warps (594 us at 5,472 x 1,024: the proxy fence waits for the loads), remote arrivals and
+// waits with cluster scope (627 us: the release waits for everything the thread has in flight), the k-blocks of
+// all tiles dealt to the pairs in equal runs (356 us: pairs at different rows share nothing in L2).
+#include "act8.cuh"
+#include "common.cuh"
+#include "host_util.h"
+
+namespace imf {
+namespace w8 {
+
+constexpr int BM = 128, BK = 64;           // rows of dY^T per CTA; rows of a k-block
+constexpr int CHUNK_KB = 128;              // k-blocks that one chain of accumulations runs over
+
+template <int BN>
+struct Smem {
+  static constexpr int BNL = BN / 2;                 // columns of this CTA
+  static constexpr int NH = BN == 512 ? 2 : 1;       // products of 256 columns
+  static constexpr int ACCS = NH == 2 ? 1 : 2;       // accumulators that TMEM holds
+  static constexpr int STAGES = BN == 512 ? 4 : BN == 256 ? 6 : 8;
+  static constexpr int CONV = BN == 512 ? 2 : 3;     // converted tiles in flight, one group of warps each
+  static constexpr int GROUP_WARPS = BN == 512 ? 8 : 4;
+  static constexpr int THREADS = (6 + CONV * GROUP_WARPS) * 32;
+  static constexpr int OUT = BN == 512 ? 1 : 2;      // staging buffers of an epilogue warp
+  static constexpr int WORDS = BNL > 128 ? 2 : 1;    // 4-byte words of steps per row
+  alignas(1024) uint8_t a[STAGES][BM * BK * 2];      // dY: two panels [64 rows][128 bytes], swizzled
+  alignas(1024) uint8_t b[CONV][BNL * BK * 2];       // X as bf16: BNL / 64 such panels
+  alignas(1024) uint8_t c[4][OUT][32 * 128];         // per epilogue warp: 32 rows x 32 fp32, swizzled
+  alignas(1024) uint8_t b8[STAGES][BK * BNL];        // codes [64 rows][BNL]
+  alignas(16) uint8_t st[STAGES][BK * 4 * WORDS];    // step bytes [64 rows][4 WORDS]
+  uint64_t full[STAGES], empty[STAGES], conv_full[CONV], conv_empty[CONV], acc_full[2], acc_empty[2];
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+struct Params {
+  const uint8_t* steps;
+  int64_t spitch;
+  int R, N, C;
+  int n_c, tiles, num_kb, splits, kb_per;
+  int accumulate;          // what is stored is added to what the result holds
+  int* status;
+};
+
+// k-blocks [kb0, kb1) of a tile, whose sum goes to a plane
+struct Piece {
+  int tile, plane, kb0, kb1;
+};
+// the pieces of a pair of CTAs: all tiles of a slice before the next one's, so that pairs read the same rows
+struct Walk {
+  const Params& p;
+  int64_t pos;
+  int pairs;
+  IMF_DEVICE Walk(const Params& prm, int pair, int n) : p(prm), pos(pair), pairs(n) {}
+  IMF_DEVICE bool next(Piece& w) {
+    if (pos >= (int64_t)p.tiles * p.splits) return false;
+    w.plane = (int)(pos / p.tiles);
+    w.tile = (int)(pos - (int64_t)w.plane * p.tiles);
+    w.kb0 = w.plane * p.kb_per;
+    w.kb1 = min(w.kb0 + p.kb_per, p.num_kb);
+    pos += pairs;
+    return true;
+  }
+};
+
+IMF_DEVICE void cp_async4(void* dst, const void* src, bool in) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(in ? 4 : 0)
+               : "memory");
+}
+IMF_DEVICE void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+IMF_DEVICE void tma_reduce_add_3d(const CUtensorMap* m, const void* src, int c0, int c1, int c2) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(m)), "r"(smem_u32(src)), "r"(c0), "r"(c1), "r"(c2)
+               : "memory");
+}
+// all but the newest bulk store have read their source
+IMF_DEVICE void tma_store_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
+
+// ---- the pair of CTAs
+IMF_DEVICE uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+IMF_DEVICE void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// arrive on the first CTA's barrier
+IMF_DEVICE void arrive_first(uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .b32 ra;\n\t"
+      "mapa.shared::cluster.u32 ra, %0, 0;\n\t"
+      "mbarrier.arrive.shared::cluster.b64 _, [ra];\n\t}" ::"r"(smem_u32(bar))
+      : "memory");
+}
+// the arrival, in both CTAs, of this thread's products so far
+IMF_DEVICE void commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
+      : "memory");
+}
+IMF_DEVICE void mma_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+template <int BN>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Smem<BN>::THREADS, 1)
+wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ CUtensorMap tm_b,
+              const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  using S = Smem<BN>;
+  constexpr int STAGES = S::STAGES, BNL = S::BNL, CONV = S::CONV, GROUP_WARPS = S::GROUP_WARPS, ACCS = S::ACCS,
+                NH = S::NH, WORDS = S::WORDS, PN = BN / NH;      // PN: columns of a product
+  // the same offset in both CTAs, whose windows start alike: the products address them by one descriptor
+  auto& s = *reinterpret_cast<S*>(smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&s.full[i], 1 + 32);                 // the bytes' announcement, and each lane's step bytes
+      mbar_init(&s.empty[i], 1);
+    }
+    for (int i = 0; i < CONV; ++i) {
+      mbar_init(&s.conv_full[i], 2 * GROUP_WARPS);   // one arrival per warp of the group, from both CTAs
+      mbar_init(&s.conv_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.acc_full[i], 1);
+      mbar_init(&s.acc_empty[i], 2 * 4);
+    }
+    s.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 5) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem_base)),
+                 "r"(512u)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* abort_flag = &s.abort_flag;
+  Walk walk(p, pair, pairs);
+  Piece w;
+  const auto m_of = [&](int tile) { return tile / p.n_c * (2 * BM) + rank * BM; };     // first row of this CTA
+  const auto n_of = [&](int tile) { return tile % p.n_c * BN; };
+
+  if (warp == 4) {
+    // ------------------------------------------------------------- loads --
+    if (lane == 0) {
+      prefetch_tmap(&tm_a);
+      prefetch_tmap(&tm_b);
+      prefetch_tmap(&tm_c);
+    }
+    constexpr uint32_t bytes = BM * BK * 2 + BK * BNL;
+    uint32_t it = 0;
+    bool ok = true;
+    while (ok && walk.next(w)) {
+      const int m0 = m_of(w.tile), n0 = n_of(w.tile) + rank * BNL;
+      const int64_t g = n0 / 128 * 4;                // the word with the steps of these columns
+      for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
+        const int st = it % STAGES;
+        if (it >= STAGES)
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.empty[st], ((it / STAGES) & 1) ^ 1, abort_flag, p.status,
+                                                    STATUS_TIMEOUT_EMPTY));
+        if (!ok) break;
+        const int k0 = kb * BK;
+        if (lane == 0) {
+          mbar_arrive_expect_tx(&s.full[st], bytes);
+          tma_load_2d(s.b8[st], &tm_b, &s.full[st], n0, k0);
+          tma_load_2d(s.a[st], &tm_a, &s.full[st], m0, k0);
+          tma_load_2d(s.a[st] + BK * 128, &tm_a, &s.full[st], m0 + 64, k0);
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * WORDS; ++i) {        // rows and words past the end: zeros, nothing is read
+          const int r = i / WORDS * 32 + lane, w4 = i % WORDS;
+          const bool in = k0 + r < p.R && g + 4 * w4 < p.spitch;
+          cp_async4(s.st[st] + (r * WORDS + w4) * 4, in ? p.steps + (int64_t)(k0 + r) * p.spitch + g + 4 * w4 : p.steps,
+                    in);
+        }
+        cp_async_arrive(&s.full[st]);
+      }
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    if (!ok)                                         // given up: see the copies in flight land (bounded)
+      for (uint32_t j = it < STAGES ? 0 : it - STAGES; j < it; ++j)
+        for (int spin = 0; spin < 100000 && !mbar_test(&s.full[j % STAGES], (j / STAGES) & 1); ++spin) {
+        }
+  } else if (warp == 5) {
+    // --------------------------------------------------------------- MMA --
+    if (rank == 0 && elect_one()) {
+      constexpr uint32_t idesc = idesc_bf16(2 * BM, PN, 1, 1);
+      uint32_t it = 0, ch = 0;                       // k-blocks and chains so far
+      bool ok = true;
+      while (ok && walk.next(w)) {
+        for (int c0 = w.kb0; c0 < w.kb1 && ok; c0 += CHUNK_KB, ++ch) {
+          const int c1 = min(c0 + CHUNK_KB, w.kb1);
+          const uint32_t buf = ch % ACCS, acc = tmem + buf * BN;
+          if (ch >= ACCS)
+            ok = mbar_wait(&s.acc_empty[buf], (ch / ACCS - 1) & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
+          if (!ok) break;
+          tc_fence_after();
+          for (int kb = c0; kb < c1; ++kb, ++it) {
+            // a group's arrival says that its CTA's dY is there too
+            const int st = it % STAGES, cs = it % CONV;
+            ok = mbar_wait(&s.conv_full[cs], (it / CONV) & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t a_base = smem_u32(s.a[st]), b_base = smem_u32(s.b[cs]);
+#pragma unroll
+            for (int ks = 0; ks < BK / 16; ++ks)
+#pragma unroll
+              for (int h = 0; h < NH; ++h)
+                mma_pair(acc + h * PN, sdesc_mnmajor(a_base + ks * 2048, BK * 128),
+                         sdesc_mnmajor(b_base + h * (PN / 2 * BK * 2) + ks * 2048, BK * 128), idesc,
+                         kb != c0 || ks != 0);
+            commit_both(&s.conv_empty[cs]);
+            commit_both(&s.empty[st]);               // the codes were read before conv_full
+          }
+          if (ok) commit_both(&s.acc_full[buf]);
+        }
+      }
+    }
+  } else if (warp >= 6) {
+    // -------------------------------------------------------- conversion --
+    // a lane owns eight codes of a row: a warp reads whole rows, and eight lanes write the eight 16-byte
+    // chunks of a panel's line, no bank twice.  Its rows are a multiple of eight apart, so its place in a
+    // line, and every address but for a constant, stays the same
+    constexpr int LANES = BNL / 8, ROWS = 32 / LANES;    // lanes of a row, rows a warp takes at a time
+    constexpr int STEP = GROUP_WARPS * ROWS, UNITS = BK / STEP;
+    static_assert(STEP % 8 == 0, "rows of a lane keep their place in the swizzle");
+    const int grp = (warp - 6) / GROUP_WARPS, col = lane % LANES;
+    const int r0 = ((warp - 6) % GROUP_WARPS) * ROWS + lane / LANES;
+    uint8_t* const dst = s.b[grp] + (col / 8) * (BK * 128) + r0 * 128 + (((col & 7) ^ (r0 & 7)) << 4);
+    uint32_t it = 0;
+    bool ok = true;
+    while (ok && walk.next(w)) {
+      const int st0 = r0 * 4 * WORDS + ((n_of(w.tile) + rank * BNL) / 32 & 3) + col / 4;
+      for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
+        if ((int)(it % CONV) != grp) continue;
+        const int st = it % STAGES;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.full[st], (it / STAGES) & 1, abort_flag, p.status,
+                                               STATUS_TIMEOUT_TMA));
+        if (!ok) break;
+        // converted into registers while products still read the tile; what is left between their end
+        // and the next ones are the stores
+        const uint8_t *src = s.b8[st] + r0 * BNL + col * 8, *steps = s.st[st] + st0;
+        uint2 codes[UNITS];
+        uint32_t step[UNITS];
+        uint4 v[UNITS];
+#pragma unroll
+        for (int j = 0; j < UNITS; ++j) {
+          codes[j] = *reinterpret_cast<const uint2*>(src + j * STEP * BNL);
+          step[j] = steps[j * STEP * 4 * WORDS];
+        }
+#pragma unroll
+        for (int j = 0; j < UNITS; ++j) {
+          v[j] = a8_decode8(codes[j], a8_step2(step[j]));
+          asm volatile("" : "+r"(v[j].x), "+r"(v[j].y), "+r"(v[j].z), "+r"(v[j].w));   // here, not behind the wait
+        }
+        if (it >= CONV)
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.conv_empty[grp], ((it / CONV) & 1) ^ 1, abort_flag, p.status,
+                                                    STATUS_TIMEOUT_MMA));
+        if (!ok) break;
+#pragma unroll
+        for (int j = 0; j < UNITS; ++j) *reinterpret_cast<uint4*>(dst + j * STEP * 128) = v[j];
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) arrive_first(&s.conv_full[grp]);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------- epilogue --
+    uint32_t ch = 0, step = 0;
+    bool ok = true;
+    while (ok && walk.next(w)) {
+      const int row0 = m_of(w.tile) + warp * 32, n0 = n_of(w.tile);
+      for (int c0 = w.kb0; c0 < w.kb1; c0 += CHUNK_KB, ++ch) {
+        const uint32_t buf = ch % ACCS;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_full[buf], (ch / ACCS) & 1, abort_flag, p.status,
+                                                  STATUS_TIMEOUT_MMA));
+        if (!ok) break;
+        tc_fence_after();
+        const bool add = p.accumulate || c0 != w.kb0;
+        if (c0 != w.kb0 && lane == 0) tma_store_wait_all();          // the chain before is in memory
+        if (row0 < p.N) {
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 32) {
+            // column of the accumulator -> of the tile: a product's first half is the first CTA's
+            const int n = NH == 1 ? n0 + c : n0 + (c & 128) * 2 + (c >> 8) * 128 + (c & 127);
+            if (n >= p.C) continue;
+            uint32_t r[32];
+            tmem_ld32(tmem_addr(tmem + buf * BN, warp * 32, c), r);
+            if (lane == 0) {
+              if (S::OUT == 2) tma_store_wait_read1();
+              else tma_store_wait_read();
+            }
+            __syncwarp();
+            tc_wait_ld();
+            uint8_t *stage = s.c[warp][step++ % S::OUT], *line = stage + lane * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              *reinterpret_cast<uint4*>(line + ((i ^ (lane & 7)) << 4)) =
+                  make_uint4(r[4 * i], r[4 * i + 1], r[4 * i + 2], r[4 * i + 3]);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (add) tma_reduce_add_3d(&tm_c, stage, n, row0, w.plane);
+              else tma_store_3d(&tm_c, stage, n, row0, w.plane);
+              tma_store_commit();
+            }
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_first(&s.acc_empty[buf]);
+      }
+    }
+    if (lane == 0) tma_store_wait_all();
+    tc_fence_before();
+  }
+  __syncthreads();
+  cluster_sync();            // the other CTA's products have read this one's tiles
+  if (warp == 5) {
+    __syncwarp();
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+  }
+}
+
+static int sm_count() {
+  static int sms_of[HOST_MAX_DEVICES] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  int sms = (dev >= 0 && dev < HOST_MAX_DEVICES) ? sms_of[dev] : 0;
+  if (!sms) {
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || sms <= 0) sms = 148;
+    if (dev >= 0 && dev < HOST_MAX_DEVICES) sms_of[dev] = sms;
+  }
+  return sms;
+}
+
+struct Plan {
+  int bn, splits, kb_per, pairs;
+};
+
+// Tile width and slices: the least time among the counts that fill one, two or three rounds of pairs (and one
+// slice).  In us, measured on full clips and short ones: a k-block, what a tile costs besides (the
+// store of its accumulator above all), and 5 + 0.22 a MB for planes and the kernel that adds them up.  Widths against
+// each other: 32,780 x 2,064 x 1,024 141 us (512) and 162 (256); 32,780 x 1,024 x 512 53 and 49; 2,068 x 1,376
+// x 256 20.5 (256) and 18.4 (128).
+static Plan plan(int R, int N, int C, int sms) {
+  const int num_kb = (R + BK - 1) / BK, most = sms > 1 ? sms / 2 : 1;
+  Plan best{128, 1, num_kb, 1};
+  double least = 1e30;
+  for (int bn = 128; bn <= 512; bn *= 2) {
+    const double kb_us = bn == 512 ? 0.82 : bn == 256 ? 0.50 : 0.45, tile_us = bn == 512 ? 6 : bn == 256 ? 3.5 : 2.5;
+    const int64_t tiles = (int64_t)((N + 2 * BM - 1) / (2 * BM)) * ((C + bn - 1) / bn);
+    for (int rounds = 0; rounds <= 3; ++rounds) {
+      int64_t want = rounds ? rounds * most / tiles : 1;
+      if (want > num_kb / 2) want = num_kb / 2;        // two k-blocks a slice at least
+      if (want < 1) want = 1;
+      const int per = (int)((num_kb + want - 1) / want), sp = (num_kb + per - 1) / per;
+      const double lines = (double)((tiles * sp + most - 1) / most);
+      double cost = lines * (per * kb_us + tile_us);
+      if (sp > 1) cost += 5.0 + 0.22 * (sp * (4e-6 * N * C));
+      if (cost < least) {
+        least = cost;
+        best = Plan{bn, sp, per, (int)(tiles * sp < most ? tiles * sp : most)};
+      }
+    }
+  }
+  return best;
+}
+
+template <int BN>
+static int launch(const void* dy, int64_t ld_dy, const void* codes, const void* steps, int R, int N, int C,
+                  float* dst, int64_t ld_dst, int64_t plane, int accumulate, const Plan& pl, int* status, cudaStream_t st) {
+  CUtensorMap ta, tb, tc;
+  int rc;
+  {
+    uint64_t dims[2] = {(uint64_t)N, (uint64_t)R}, str[2] = {2, (uint64_t)ld_dy * 2};
+    uint32_t box[2] = {64, BK};
+    if ((rc = make_tmap(&ta, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(dy), dims, str, box))) return rc;
+  }
+  const uint64_t pitch = ((uint64_t)C + 31) / 32 * 32;
+  {
+    uint64_t dims[2] = {pitch, (uint64_t)R}, str[2] = {1, pitch};
+    uint32_t box[2] = {BN / 2, BK};
+    if ((rc = make_tmap(&tb, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(codes), dims, str, box,
+                        CU_TENSOR_MAP_SWIZZLE_NONE)))
+      return rc;
+  }
+  {
+    uint64_t dims[3] = {(uint64_t)C, (uint64_t)N, (uint64_t)pl.splits};
+    uint64_t str[3] = {4, (uint64_t)ld_dst * 4, (uint64_t)plane * 4};
+    uint32_t box[3] = {32, 32, 1};
+    if ((rc = make_tmap(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, dst, dims, str, box))) return rc;
+  }
+  Params p;
+  p.steps = static_cast<const uint8_t*>(steps);
+  p.spitch = (int64_t)(pitch / 32 + 3) / 4 * 4;
+  p.R = R; p.N = N; p.C = C;
+  p.n_c = (C + BN - 1) / BN;
+  p.tiles = (N + 2 * BM - 1) / (2 * BM) * p.n_c;
+  p.num_kb = (R + BK - 1) / BK;
+  p.splits = pl.splits;
+  p.kb_per = pl.kb_per;
+  p.accumulate = accumulate;
+  p.status = status;
+  const size_t smem = sizeof(Smem<BN>) + 1024;
+  static bool allowed[HOST_MAX_DEVICES] = {false};
+  if (!allow_smem((const void*)wgrad8_kernel<BN>, smem, allowed)) return IMF_ERR_LAUNCH;
+  wgrad8_kernel<BN><<<(unsigned)pl.pairs * 2, Smem<BN>::THREADS, smem, st>>>(ta, tb, tc, p);
+  return cudaGetLastError() == cudaSuccess ? IMF_OK : IMF_ERR_LAUNCH;
+}
+
+static int64_t plane_floats(int N, int C) { return (int64_t)N * (((int64_t)C + 3) & ~int64_t(3)); }
+
+}  // namespace w8
+}  // namespace imf
+
+// Floats of workspace that imf_wgrad8 wants.  `direct`: the result's address and row pitch are 16-byte multiples.
+extern "C" int64_t imf_wgrad8_work(int R, int N, int C, int direct) {
+  using namespace imf;
+  if (R <= 0 || N <= 0 || C <= 0) return 0;
+  const w8::Plan pl = w8::plan(R, N, C, w8::sm_count());
+  return pl.splits > 1 || !direct ? pl.splits * w8::plane_floats(N, C) : 0;
+}
+
+extern "C" int imf_splitk_reduce_ld(const float* partial, int splits, int M, int N, int64_t ldp, int64_t plane, float* out,
+                                    int64_t ldo, float alpha, int accumulate, void* stream);
+
+// dy [R, N] bf16 (row pitch ld_dy), codes / steps: checkpoint of X [R, C]; out [N, C] fp32 (row pitch ldo).
+extern "C" int imf_wgrad8(const void* dy, int64_t ld_dy, const void* codes, const void* steps, int R, int N, int C,
+                          float* out, int64_t ldo, int accumulate, float* work, int64_t work_floats, int* status,
+                          void* stream) {
+  using namespace imf;
+  if (R <= 0 || N <= 0 || C <= 0 || !dy || !codes || !steps || !out || (ld_dy & 7)) return IMF_ERR_ARG;
+  if (R > 0x7fffff00 || N > 0x7fffff00 || C > 0x7ffffe00) return IMF_ERR_TOO_LARGE;
+  if ((reinterpret_cast<uintptr_t>(codes) & 15u) || (reinterpret_cast<uintptr_t>(steps) & 3u)) return IMF_ERR_ARG;
+  const w8::Plan pl = w8::plan(R, N, C, w8::sm_count());
+  if ((int64_t)((N + 255) / 256) * ((C + pl.bn - 1) / pl.bn) * pl.splits > 0x7fffffff) return IMF_ERR_TOO_LARGE;
+  const bool direct = pl.splits == 1 && (ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  const int64_t plane = w8::plane_floats(N, C), cp = plane / N;
+  if (!direct && (!work || work_floats < pl.splits * plane || (reinterpret_cast<uintptr_t>(work) & 15u)))
+    return IMF_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = pl.bn == 512 ? w8::launch<512> : pl.bn == 256 ? w8::launch<256> : w8::launch<128>;
+  const int rc = direct ? go(dy, ld_dy, codes, steps, R, N, C, out, ldo, (int64_t)N * ldo, accumulate, pl, status, st)
+                        : go(dy, ld_dy, codes, steps, R, N, C, work, cp, plane, 0, pl, status, st);
+  if (rc || direct) return rc;
+  return imf_splitk_reduce_ld(work, pl.splits, N, C, cp, plane, out, ldo, 1.f, accumulate, stream);
+}

@@ -635,7 +635,7 @@ namespace imf {
 constexpr int REDUCE_GROUPS = 4, REDUCE_LANES = 64;
 template <int VEC>
 __global__ void __launch_bounds__(REDUCE_GROUPS * REDUCE_LANES)
-splitk_reduce_kernel(const float* __restrict__ partial, int splits, long plane, int N,
+splitk_reduce_kernel(const float* __restrict__ partial, int splits, long count, int N, int64_t ldp, int64_t plane,
                      float* __restrict__ out, int64_t ldo, float alpha, int accumulate) {
   __shared__ float sums[REDUCE_GROUPS][REDUCE_LANES * VEC];
   const int lane = threadIdx.x % REDUCE_LANES, grp = threadIdx.x / REDUCE_LANES;
@@ -643,22 +643,23 @@ splitk_reduce_kernel(const float* __restrict__ partial, int splits, long plane, 
   float acc[VEC];
 #pragma unroll
   for (int j = 0; j < VEC; ++j) acc[j] = 0.f;
-  if (i < plane) {
+  if (i < count) {
+    const float* src = partial + (ldp == N ? i : (i / N) * ldp + (i % N));
     const int z0 = grp * splits / REDUCE_GROUPS, z1 = (grp + 1) * splits / REDUCE_GROUPS;
 #pragma unroll 4
     for (int z = z0; z < z1; ++z) {
       if constexpr (VEC == 4) {
-        const float4 v = *reinterpret_cast<const float4*>(partial + z * plane + i);
+        const float4 v = *reinterpret_cast<const float4*>(src + z * plane);
         acc[0] += v.x; acc[1] += v.y; acc[2] += v.z; acc[3] += v.w;
       } else {
-        acc[0] += partial[z * plane + i];
+        acc[0] += src[z * plane];
       }
     }
   }
 #pragma unroll
   for (int j = 0; j < VEC; ++j) sums[grp][j * REDUCE_LANES + lane] = acc[j];
   __syncthreads();
-  if (grp != 0 || i >= plane) return;
+  if (grp != 0 || i >= count) return;
   float* dst = out + (i / N) * ldo + (i % N);
 #pragma unroll
   for (int j = 0; j < VEC; ++j) {
@@ -670,22 +671,24 @@ splitk_reduce_kernel(const float* __restrict__ partial, int splits, long plane, 
 }
 }  // namespace imf
 
-// out[M, N] (row pitch ldo) (+)= alpha * sum_z partial[z]
-extern "C" int imf_splitk_reduce(const float* partial, int splits, int M, int N, float* out,
-                                 int64_t ldo, float alpha, int accumulate, void* stream) {
-  if (splits < 1 || M <= 0 || N <= 0) return imf::IMF_ERR_ARG;
-  const long plane = (long)M * N;
+// out[M, N] (row pitch ldo) (+)= alpha * sum_z partial[z], planes of M rows at pitch ldp
+extern "C" int imf_splitk_reduce_ld(const float* partial, int splits, int M, int N, int64_t ldp, int64_t plane, float* out,
+                                    int64_t ldo, float alpha, int accumulate, void* stream) {
+  if (splits < 1 || M <= 0 || N <= 0 || ldp < N) return imf::IMF_ERR_ARG;
+  const long count = (long)M * N;
   cudaStream_t st = (cudaStream_t)stream;
-  const bool vec = N % 4 == 0 && ldo % 4 == 0 &&
+  const bool vec = N % 4 == 0 && ldo % 4 == 0 && ldp % 4 == 0 && plane % 4 == 0 &&
                    ((reinterpret_cast<uintptr_t>(partial) | reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-  const long threads = vec ? plane / 4 : plane;
+  const long threads = vec ? count / 4 : count;
   const unsigned blocks = (unsigned)((threads + imf::REDUCE_LANES - 1) / imf::REDUCE_LANES);
   constexpr int T = imf::REDUCE_GROUPS * imf::REDUCE_LANES;
-  if (vec)
-    imf::splitk_reduce_kernel<4><<<blocks, T, 0, st>>>(partial, splits, plane, N, out, ldo, alpha, accumulate);
-  else
-    imf::splitk_reduce_kernel<1><<<blocks, T, 0, st>>>(partial, splits, plane, N, out, ldo, alpha, accumulate);
+  auto kern = vec ? imf::splitk_reduce_kernel<4> : imf::splitk_reduce_kernel<1>;
+  kern<<<blocks, T, 0, st>>>(partial, splits, count, N, ldp, plane, out, ldo, alpha, accumulate);
   return cudaGetLastError() == cudaSuccess ? imf::IMF_OK : imf::IMF_ERR_LAUNCH;
+}
+extern "C" int imf_splitk_reduce(const float* partial, int splits, int M, int N, float* out,
+                                 int64_t ldo, float alpha, int accumulate, void* stream) {
+  return imf_splitk_reduce_ld(partial, splits, M, N, N, (long)M * N, out, ldo, alpha, accumulate, stream);
 }
 
 namespace imf {

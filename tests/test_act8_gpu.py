@@ -151,7 +151,8 @@ def _wgrad_check(got, dy, p, base=None):
 
 @pytest.mark.parametrize("rows,N,C", [(1, 8, 1), (1, 136, 300), (7, 16, 31), (63, 128, 128), (64, 8, 64),
                                       (65, 264, 77), (130, 528, 256), (532, 528, 257), (1000, 144, 512),
-                                      (4099, 40, 1021), (2068, 1376, 256), (29140, 256, 128), (16500, 72, 40)])
+                                      (4099, 40, 1021), (2068, 1376, 256), (29140, 256, 128), (16500, 72, 40),
+                                      (70, 5400, 1000), (8300, 10000, 500), (300, 20000, 130)])
 def test_weight_gradient(A, K, rows, N, C):
     g = _gen(rows)
     dy, p = _randn(g, rows, N), A.store8(_activations(g, rows, C))
