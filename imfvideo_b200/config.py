@@ -56,6 +56,9 @@ class ModelConfig:
     rope_theta: float = 10000.0
     attn_res_block_size: int = 4
     grad_checkpoint: bool = True
+    # not in the reference: how the fused blocks keep their activations for the backward pass, "bf16" or
+    # "int8" (one byte a channel with a power-of-two step for each 32; about a third of the memory)
+    act_store: str = "bf16"
     eval_mode: bool = False
     max_params: int = 300_000_000
 

@@ -285,8 +285,11 @@ class TransformerBlock(nn.Module):
                  qk_nope_head_dim, qk_rope_head_dim, v_head_dim, mlp_ratio=8 / 3,
                  weight_init_constant=1.0, norm_eps=1e-6, attn_impl=sdpa_math_attention,
                  use_attn_res=False, situ_beta=4.0, situ_linear_beta=25.0,
-                 mla_use_output_gate=True):
+                 mla_use_output_gate=True, act_store="bf16"):
         super().__init__()
+        if act_store not in ("bf16", "int8"):
+            raise ValueError(f"act_store is 'bf16' or 'int8', not {act_store!r}")
+        self.act_store = act_store        # how the fused path keeps activations for the backward pass
         self.norm1 = RMSNorm(hidden_size, eps=norm_eps)
         self.attn = MLAAttention(hidden_size, num_heads, q_lora_rank, kv_lora_rank,
                                  qk_nope_head_dim, qk_rope_head_dim, v_head_dim,
@@ -312,7 +315,8 @@ class TransformerBlock(nn.Module):
             from ..ops.block import BlockGeom
 
             f = self.mlp.w1.out_features
-            g = self._geom = BlockGeom(self.attn, self.norm1.weight.shape[0], f + (-f) % 8)
+            g = self._geom = BlockGeom(self.attn, self.norm1.weight.shape[0], f + (-f) % 8,
+                                       act8=self.act_store == "int8")
         return g
 
     def fused_ok(self, x: Tensor, compute_dtype) -> bool:
@@ -544,7 +548,8 @@ class IMFDiTVideo(nn.Module):
                  weight_init_constant=0.32, rmsnorm_eps=1e-6, rope_theta=10000.0,
                  attn_impl=sdpa_math_attention, eval_mode=False, attn_res_block_size=0,
                  situ_beta=4.0, situ_linear_beta=25.0, mla_use_output_gate=True,
-                 grad_checkpoint=False, compute_dtype: Optional[torch.dtype] = None):
+                 grad_checkpoint=False, compute_dtype: Optional[torch.dtype] = None,
+                 act_store="bf16"):
         super().__init__()
         self.head_dim = hidden_size // num_heads
         self.attn_res_block_size = attn_res_block_size
@@ -617,7 +622,8 @@ class IMFDiTVideo(nn.Module):
                   mlp_ratio=mlp_ratio, weight_init_constant=weight_init_constant,
                   norm_eps=rmsnorm_eps, attn_impl=attn_impl,
                   use_attn_res=attn_res_block_size > 0, situ_beta=situ_beta,
-                  situ_linear_beta=situ_linear_beta, mla_use_output_gate=mla_use_output_gate)
+                  situ_linear_beta=situ_linear_beta, mla_use_output_gate=mla_use_output_gate,
+                  act_store=act_store)
         shared_depth = depth - aux_head_depth
         self.shared_blocks = nn.ModuleList(TransformerBlock(**kw) for _ in range(shared_depth))
         self.u_heads = nn.ModuleList(TransformerBlock(**kw) for _ in range(aux_head_depth))

@@ -14,7 +14,7 @@ stored.  A group that holds a NaN or an infinity reads as NaN throughout.
     attn_bwd8(q8, k8, v8, o8, lse, go)        # dense attention, probabilities recomputed
 
 ``model.act_store = "int8"`` keeps the activations of the fused blocks this way
-(``ops/block.py``).  CPU tensors take the formulas of ``ops/reference.py``.  All launches go to the
+(``ops/block.py``); blocks off the fused path (CPU, fp32) keep theirs as they are.  CPU tensors take the formulas of ``ops/reference.py``.  All launches go to the
 current stream of the tensors' device; workspaces belong to the call.  There is no counterpart in
 the reference, which recomputes blocks instead (reference ``models/imf_dit_video.py:909-972``).
 """
@@ -147,6 +147,20 @@ class Packed8:
 
     def __repr__(self) -> str:
         return f"Packed8({tuple(self.shape)}, {self.dtype}, {self.nbytes} bytes, {self.device})"
+
+
+def buffer(ps: Sequence[Packed8]) -> Tensor:
+    """The buffer that the tensors of one ``store8`` call share (what an autograd node saves)."""
+    return ps[0]._arena
+
+
+def layout(ps: Sequence[Packed8]) -> list:
+    """Where in it they are; with the buffer, ``in_buffer`` makes them again."""
+    return [(p._at, p.shape, p.dtype) for p in ps]
+
+
+def in_buffer(arena: Tensor, where: list) -> List[Packed8]:
+    return [Packed8._in(arena, at, shape, dtype) for at, shape, dtype in where]
 
 
 def _row_dims(t: Tensor) -> Optional[List[int]]:

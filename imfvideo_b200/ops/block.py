@@ -15,6 +15,11 @@ Block structure (reference ``models/imf_dit_video.py:909-972``, ``:422-467``):
     p2  = (fresh ? 0 : prefix) + a * attn_scale ; snaps2 = snaps (+ prefix if fresh)
     n2  = norm2(remix(p2, snaps2; w2))
     m   = situ(n2 [w1 | w3]^T) w2^T ;  out = p2 + m * mlp_scale
+
+With ``BlockGeom.act8`` the node keeps its activations in 8 bits (``ops/act8.py``): one launch at
+the end of the forward packs them, the backward reads n1, n2 and the latents in 8 bits as they
+are (weight gradients), [gate | up] as well (gated activation, which is recomputed there), q and k
+for the attention, and restores the rest in one launch.  The output gate's product is recomputed.
 """
 
 from __future__ import annotations
@@ -24,6 +29,7 @@ from typing import List, Optional, Sequence, Tuple
 
 import torch
 
+from . import act8 as A8
 from . import kernels as K
 from . import rowops as R
 
@@ -97,9 +103,13 @@ class GradSinks:
                     return False       # r0: the TMA view of dY[:, r0:] must start 16-byte aligned
         return True
 
-    def accumulate(self, name: str, dy: torch.Tensor, x: torch.Tensor) -> None:
-        """grad(piece) += dy[:, rows of the piece]^T x[:, :cols of the piece]"""
+    def accumulate(self, name: str, dy: torch.Tensor, x) -> None:
+        """grad(piece) += dy[:, rows of the piece]^T x[:, :cols of the piece]; ``x`` may be packed
+        in 8 bits (pieces of its whole width)"""
         for p, r0, n, c in self.pieces[name]:
+            if isinstance(x, A8.Packed8):
+                A8.gemm_wgrad8(dy[:, r0:r0 + n], x, out=p.grad.view(n, c), accumulate=True)
+                continue
             K.gemm_wgrad(dy[:, r0:r0 + n], x[:, :c] if c != x.shape[1] else x,
                          out=p.grad.view(n, c), accumulate=True)
 
@@ -107,8 +117,9 @@ class GradSinks:
 class BlockGeom:
     """Static geometry of a block (python ints only)."""
 
-    def __init__(self, attn, hidden: int, fpad: int):
+    def __init__(self, attn, hidden: int, fpad: int, act8: bool = False):
         self.d = hidden
+        self.act8 = act8              # activations are kept in 8 bits for the backward pass
         self.H = attn.num_heads
         self.dq, self.dc = attn.q_lora_rank, attn.kv_lora_rank
         self.dn, self.dr, self.dv = attn.qk_nope_head_dim, attn.qk_rope_head_dim, attn.v_head_dim
@@ -204,11 +215,21 @@ class _BlockFn(torch.autograd.Function):
                                      float(lbeta or 0.0), stream), "imf_block_post")
         K.LAUNCHES.count += 7 if g.gate else 6
         if need_bwd:
+            if g.act8:
+                # q, k and o go to the dense core's backward in 8 bits; another core has its own form
+                # of them, and they stay as they are
+                dense = isinstance(core, DenseCore)
+                packed = A8.store8([n1[0], a_[:rows], qlat[0], kvlat[0], qb[:rows], kvb[:rows],
+                                    a_out[:rows], n2[0], gu[:rows], m[:rows]] +
+                                   ([q[0], k[0], o] if dense else []))
+                ctx.packed = A8.layout(packed)
+                kept = (A8.buffer(packed),) + (() if dense else (q[0], k[0], o))
+            else:
+                kept = (n1[0], a_[:rows], qlat[0], kvlat[0], qb[:rows], kvb[:rows], q[0], k[0], o, og[0],
+                        a_out[:rows], n2[0], gu[:rows], act[:rows], m[:rows])
             ctx.save_for_backward(prefix, *snaps, w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn,
                                   a_scale, m_scale, W_a, W_qb, W_kvb, W_out, W13, W2, cos, sin,
-                                  n1[0], a_[:rows], qlat[0], kvlat[0], qb[:rows], kvb[:rows],
-                                  q[0], k[0], o, og[0], a_out[:rows], p2[0], n2[0], gu[:rows],
-                                  act[:rows], m[:rows], *core_saved)
+                                  *core_saved, *kept)
             ctx.meta = (g, core, fresh, use_res, eps, beta, lbeta, nsnap, B, L, len(core_saved))
             ctx.sinks = sinks
             ctx.mats_cached = bool(getattr(sinks, "mats_cached", False))
@@ -224,10 +245,17 @@ class _BlockFn(torch.autograd.Function):
         prefix = sv[0]
         snaps = list(sv[1:1 + nsnap])
         (w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn, a_scale, m_scale, W_a, W_qb, W_kvb, W_out,
-         W13, W2, cos, sin, n1, a_, qlat, kvlat, qb, kvb, q, k, o, og, a_out, p2, n2, gu, act,
-         m) = sv[1 + nsnap:1 + nsnap + 34]
-        core_saved = sv[1 + nsnap + 34:]
+         W13, W2, cos, sin) = sv[1 + nsnap:1 + nsnap + 18]
+        core_saved, kept = sv[1 + nsnap + 18:1 + nsnap + 18 + ncore], sv[1 + nsnap + 18 + ncore:]
         rows, d = B * L, g.d
+        if g.act8:
+            n1, a_, qlat, kvlat, qb, kvb, a_out, n2, gu, m, *qko = A8.in_buffer(kept[0], ctx.packed)
+            q, k, o = qko or kept[1:]
+            og = act = None                      # recomputed where they are needed
+            a_, qb, kvb, a_out, m, *restored = A8.restore8([a_, qb, kvb, a_out, m] + ([o] if qko else []))
+            o = restored[0] if qko else o
+        else:
+            n1, a_, qlat, kvlat, qb, kvb, q, k, o, og, a_out, n2, gu, act, m = kept
         dev = prefix.device
         hv, na = g.H * g.dv, g.na
         pfx = prefix.reshape(rows, d)
@@ -249,8 +277,9 @@ class _BlockFn(torch.autograd.Function):
             # gradient buffers existed then; returned gradients would reach no parameter
             raise RuntimeError("the parameters' fp32 gradient buffers were removed between the "
                                "forward and the backward pass of a fused block")
+        product = lambda dy, x: A8.gemm_wgrad8(dy, x) if isinstance(x, A8.Packed8) else K.gemm_wgrad(dy, x)
         wgrad = (lambda name, dy, x: sinks.accumulate(name, dy, x)) if direct else \
-            (lambda name, dy, x: K.gemm_wgrad(dy, x).to(BF16))
+            (lambda name, dy, x: product(dy, x).to(BF16))
         cs = R.ColSums()
         small = (lambda name, part, col, D: (cs.add(part, col, D, sinks.small_dst(name)), None)[1]) \
             if direct else (lambda name, part, col, D: cs.add(part, col, D, None))
@@ -260,9 +289,12 @@ class _BlockFn(torch.autograd.Function):
         g_mscale = small("m_scale", part_ms, 0, d)
         # 10'. MLP
         g_act = K.gemm(g_m, W2, b_mn=True)                          # [rows, fp]
+        if g.act8:
+            g_gu, act = A8.situ_bwd8(gu, g_act, beta, lbeta)
+        else:
+            g_gu = new(rows, 2 * g.fp)
+            R.situ_bwd(gu, g_act, g_gu, rows, g.fp, beta, lbeta)
         gW2 = wgrad("W2", g_m, act)
-        g_gu = new(rows, 2 * g.fp)
-        R.situ_bwd(gu, g_act, g_gu, rows, g.fp, beta, lbeta)
         g_n2v = K.gemm(g_gu, W13, b_mn=True)
         gW13 = wgrad("W13", g_gu, n2)
         # 9'. residual + remix + norm2
@@ -275,12 +307,17 @@ class _BlockFn(torch.autograd.Function):
         g_ascale = small("a_scale", part2, 2, d)
         # 8'. output projection
         g_og = K.gemm(g_aout, W_out, b_mn=True)                     # [rows, hv]
+        o2 = o.view(rows, hv)
+        gcol = g.dq + g.dc + g.dr
+        if og is None:
+            og = o2
+            if g.gate:
+                og = new(rows, hv)
+                R.outgate_fwd(o2, None, a_[:, gcol:], None, og, None, rows, hv, hv, na)
         gW_out = wgrad("W_out", g_aout, og)
         # 7'. output gate (gate gradient goes straight into its band of g_a_)
         g_a = new(rows, na)
-        o2 = o.view(rows, hv)
         if g.gate:
-            gcol = g.dq + g.dc + g.dr
             g_o = new(rows, hv)
             R.outgate_bwd(o2, a_[:, gcol:], g_og, g_o, g_a[:, gcol:], rows, hv, hv, na, hv, na)
         else:
@@ -289,8 +326,12 @@ class _BlockFn(torch.autograd.Function):
         g_kvb = new(rows, g.H * (g.dn + g.dv))
         kv4 = kvb.view(B, L, g.H, g.dn + g.dv)
         gkv4 = g_kvb.view(B, L, g.H, g.dn + g.dv)
-        gq, gk, _gv = core.bwd(q, k, kv4[..., g.dn:], o, core_saved, g_o.view(B, L, g.H, g.dv),
-                               gv_out=gkv4[..., g.dn:])
+        if isinstance(q, A8.Packed8):
+            gq, gk, _gv = A8.attn_bwd8(q, k, kv4[..., g.dn:], o, core_saved[0], g_o.view(B, L, g.H, g.dv),
+                                       gv_out=gkv4[..., g.dn:])
+        else:
+            gq, gk, _gv = core.bwd(q, k, kv4[..., g.dn:], o, core_saved, g_o.view(B, L, g.H, g.dv),
+                                   gv_out=gkv4[..., g.dn:])
         # 5'. q / k preparation
         g_qb = new(rows, g.H * g.hd)
         part_qk = R.qkprep_bwd(qb, kvb, cos, sin, g_qn, g_kn, gq.contiguous(),

@@ -90,7 +90,7 @@ def build_model(cfg: Optional[Config] = None) -> Tuple[M.IMFDiTVideo, int, str]:
         rope_theta=m.rope_theta, eval_mode=m.eval_mode, attn_impl=attn,
         attn_res_block_size=m.attn_res_block_size, situ_beta=m.situ_beta,
         situ_linear_beta=m.situ_linear_beta, mla_use_output_gate=m.mla_use_output_gate,
-        grad_checkpoint=m.grad_checkpoint)
+        grad_checkpoint=m.grad_checkpoint, act_store=m.act_store)
     n = sum(p.numel() for p in net.parameters())
     assert n <= m.max_params, f"model has {n / 1e6:.1f}M params, cap {m.max_params / 1e6:.0f}M"
     return net, n, getattr(attn, "__name__", str(attn))

@@ -199,3 +199,16 @@ def test_refusals():
     small = act8.store8(torch.randn(1, 4, 2, 32).bfloat16())
     with no():
         act8.attn_bwd8(small, small, small, go[..., :32], lse, go[..., :32])
+
+
+def test_option_of_the_model():
+    from imfvideo_b200.config import apply_overrides, preset
+    from imfvideo_b200.models import IMFDiTVideo
+    from imfvideo_b200.train import build_model
+
+    cfg = apply_overrides(preset("tiny"), {"model.act_store": "int8"})
+    net = build_model(cfg)[0]
+    assert all(b.act_store == "int8" for b in net.shared_blocks) and preset("tiny").model.act_store == "bf16"
+    with pytest.raises(ValueError):
+        IMFDiTVideo(input_size=8, num_frames=1, hidden_size=64, depth=2, num_heads=2, aux_head_depth=1,
+                    act_store="int4")
