@@ -35,7 +35,8 @@ Tensor = torch.Tensor
 BF16, F32 = torch.bfloat16, torch.float32
 GROUP = 32
 _MAX_RECS = 16                 # tensors a launch takes
-_REC = struct.Struct("<3Q8q")  # x, codes, steps, n0, n1, n2, s0, s1, s2, cols, fp32
+# n records x, codes, steps, n0, n1, n2, s0, s1, s2, cols, fp32
+_RECS = [struct.Struct("<" + 11 * n * "q") for n in range(_MAX_RECS + 1)]
 _KERNELS = None
 
 
@@ -63,7 +64,8 @@ def _kernels():
 
 
 def _pitches(cols: int) -> Tuple[int, int]:
-    groups = -(-cols // GROUP)
+    """Channels and groups that a row of codes and of steps is rounded up to."""
+    groups = (cols + GROUP - 1) // GROUP
     return groups * GROUP, (groups + 3) // 4 * 4
 
 
@@ -76,35 +78,33 @@ class Packed8:
     __slots__ = ("shape", "dtype", "rows", "cols", "device", "_codes", "_steps", "_arena", "_at")
 
     def __init__(self, codes: Tensor, steps: Tensor, shape: Sequence[int], dtype: torch.dtype = BF16):
-        self._geometry(shape, dtype, codes.device)
-        pitch, spitch = _pitches(self.cols)
-        if codes.dtype != torch.int8 or tuple(codes.shape) != (self.rows, pitch) or not codes.is_contiguous():
-            raise ValueError(f"codes of {tuple(shape)}: contiguous int8 ({self.rows}, {pitch}) expected, got "
+        self.shape = shape = torch.Size(shape)
+        if len(shape) < 1 or min(shape) < 0:
+            raise ValueError(f"not the shape of an activation: {tuple(shape)}")
+        if dtype is not BF16 and dtype is not F32:
+            raise ValueError(f"8-bit activations are bf16 or fp32, not {dtype}")
+        self.cols = cols = shape[-1]
+        self.rows = rows = math.prod(shape[:-1])
+        self.dtype, self.device = dtype, codes.device
+        pitch, spitch = _pitches(cols)
+        if codes.dtype is not torch.int8 or codes.shape != (rows, pitch) or not codes.is_contiguous():
+            raise ValueError(f"codes of {tuple(shape)}: contiguous int8 ({rows}, {pitch}) expected, got "
                              f"{codes.dtype} {tuple(codes.shape)}")
-        if steps.dtype != torch.uint8 or tuple(steps.shape) != (self.rows, spitch) or not steps.is_contiguous():
-            raise ValueError(f"steps of {tuple(shape)}: contiguous uint8 ({self.rows}, {spitch}) expected, got "
+        if steps.dtype is not torch.uint8 or steps.shape != (rows, spitch) or not steps.is_contiguous():
+            raise ValueError(f"steps of {tuple(shape)}: contiguous uint8 ({rows}, {spitch}) expected, got "
                              f"{steps.dtype} {tuple(steps.shape)}")
-        if codes.device != steps.device:
+        if steps.device != self.device:
             raise ValueError("codes and steps are on different devices")
         if codes.data_ptr() % 16 or steps.data_ptr() % 4:
             raise ValueError("codes need a 16-byte, steps a 4-byte aligned address")
         self._codes, self._steps, self._arena, self._at = codes, steps, None, None
 
-    def _geometry(self, shape, dtype, device) -> None:
-        if dtype not in (BF16, F32):
-            raise ValueError(f"8-bit activations are bf16 or fp32, not {dtype}")
-        self.shape = torch.Size(shape)
-        if len(self.shape) < 1 or min(self.shape, default=1) < 0:
-            raise ValueError(f"not the shape of an activation: {tuple(shape)}")
-        self.dtype, self.device = dtype, device
-        self.cols = self.shape[-1]
-        self.rows = math.prod(self.shape[:-1])
-
     @classmethod
-    def _in(cls, arena: Tensor, at: Tuple[int, int], shape, dtype) -> "Packed8":
+    def _in(cls, arena: Tensor, at: Tuple[int, int], shape, dtype, rows: int) -> "Packed8":
         """In the buffer ``arena`` at byte offsets ``at`` of codes and steps."""
         p = cls.__new__(cls)
-        p._geometry(shape, dtype, arena.device)
+        p.shape, p.dtype, p.device = shape, dtype, arena.device
+        p.rows, p.cols = rows, shape[-1]
         p._codes = p._steps = None
         p._arena, p._at = arena, at
         return p
@@ -138,7 +138,7 @@ class Packed8:
         if shape[-1] != self.cols or math.prod(shape[:-1]) != self.rows:
             raise ValueError(f"{tuple(self.shape)} cannot be seen as {tuple(shape)}")
         p = Packed8.__new__(Packed8)
-        p._geometry(shape, self.dtype, self.device)
+        p.shape, p.dtype, p.device, p.rows, p.cols = torch.Size(shape), self.dtype, self.device, self.rows, self.cols
         p._codes, p._steps, p._arena, p._at = self._codes, self._steps, self._arena, self._at
         return p
 
@@ -156,20 +156,23 @@ def buffer(ps: Sequence[Packed8]) -> Tensor:
 
 def layout(ps: Sequence[Packed8]) -> list:
     """Where in it they are; with the buffer, ``in_buffer`` makes them again."""
-    return [(p._at, p.shape, p.dtype) for p in ps]
+    return [(p._at, p.shape, p.dtype, p.rows) for p in ps]
 
 
 def in_buffer(arena: Tensor, where: list) -> List[Packed8]:
-    return [Packed8._in(arena, at, shape, dtype) for at, shape, dtype in where]
+    return [Packed8._in(arena, *w) for w in where]
 
 
-def _row_dims(t: Tensor) -> Optional[List[int]]:
-    """[n0, n1, n2, s0, s1, s2] of a tensor's rows (all dimensions but the last, merged where the
+def _row_dims(t: Tensor, rows: int) -> Optional[Tuple[int, ...]]:
+    """(n0, n1, n2, s0, s1, s2) of a tensor's rows (all dimensions but the last, merged where the
     strides allow it), or None where more than three remain or the channels are not adjacent."""
-    if t.dim() > 1 and t.shape[-1] > 1 and t.stride(-1) != 1 or t.dim() == 1 and t.stride(0) != 1 < t.shape[0]:
+    if t.is_contiguous():
+        return 1, 1, rows, 0, 0, t.shape[-1]
+    shape, strides = t.shape, t.stride()
+    if shape[-1] > 1 and strides[-1] != 1:
         return None
     dims: List[List[int]] = []
-    for n, s in zip(t.shape[:-1], t.stride()[:-1]):
+    for n, s in zip(shape[:-1], strides[:-1]):
         if n == 1:
             continue
         if dims and dims[-1][1] == n * s:
@@ -179,31 +182,30 @@ def _row_dims(t: Tensor) -> Optional[List[int]]:
     if len(dims) > 3:
         return None
     dims = [[1, 0]] * (3 - len(dims)) + dims
-    return [d[0] for d in dims] + [d[1] for d in dims]
+    return tuple(d[0] for d in dims) + tuple(d[1] for d in dims)
 
 
-def _on(device: torch.device):
-    """Makes the tensors' device the current one for the launches inside."""
-    return torch.cuda.device(device)
-
-
-def _launch(fn_name: str, recs: List[bytes]) -> None:
+def _launch(fn_name: str, recs: List[int]) -> None:
+    """``recs``: eleven numbers for each tensor."""
     K = _kernels()
     fn = getattr(K._lib, fn_name)
-    for i in range(0, len(recs), _MAX_RECS):
-        part = recs[i:i + _MAX_RECS]
-        K._check(fn(b"".join(part), len(part), K._stream()), fn_name)
+    for i in range(0, len(recs), 11 * _MAX_RECS):
+        part = recs[i:i + 11 * _MAX_RECS]
+        n = len(part) // 11
+        K._check(fn(_RECS[n].pack(*part), n, K._stream()), fn_name)
         K.LAUNCHES.count += 1
 
 
-def _current(device: torch.device) -> bool:
-    return device.index == torch._C._cuda_getDevice()
+def _elsewhere(device: torch.device) -> bool:
+    """Whether the launches need another current device."""
+    return device.index != torch._C._cuda_getDevice()
 
 
 def _same_device(what: str, *ts) -> torch.device:
     dev = ts[0].device
-    if any(t.device != dev for t in ts):
-        raise ValueError(f"{what}: tensors on different devices")
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{what}: tensors on different devices")
     return dev
 
 
@@ -212,42 +214,46 @@ def store8(xs: Union[Tensor, Sequence[Tensor]]) -> Union[Packed8, List[Packed8]]
     any number of leading ones, rows at any strides).  Several share one launch and one buffer."""
     if isinstance(xs, Tensor):
         return store8([xs])[0]
-    xs = [x.detach() for x in xs]
+    xs = list(xs)
     if not xs:
         return []
+    dev = xs[0].device
     for x in xs:
-        if x.dtype not in (BF16, F32) or x.dim() < 1:
+        if (x.dtype is not BF16 and x.dtype is not F32) or x.dim() < 1:
             raise ValueError(f"store8 takes bf16 or fp32 activations, not {x.dtype} of {x.dim()} dimensions")
-    dev = _same_device("store8", *xs)
-    if not xs[0].is_cuda:
+        if x.device != dev:
+            raise ValueError("store8: tensors on different devices")
+    if dev.type != "cuda":
         out = []
         for x in xs:
-            codes, steps = ref.store8(x.reshape(math.prod(x.shape[:-1]), x.shape[-1]))
+            codes, steps = ref.store8(x.detach().reshape(math.prod(x.shape[:-1]), x.shape[-1]))
             out.append(Packed8(codes, steps, x.shape, x.dtype))
         return out
-    if not _current(dev):
-        with _on(dev):
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return store8(xs)
-    at, total = [], 0
+    geo, total = [], 0
     for x in xs:
-        pitch, spitch = _pitches(x.shape[-1])
-        rows = math.prod(x.shape[:-1])
-        o1 = total + (rows * pitch + 127) // 128 * 128
-        at.append((total, o1))
-        total = o1 + (rows * spitch + 127) // 128 * 128
+        shape = x.shape
+        cols = shape[-1]
+        rows = x.numel() // cols if cols else math.prod(shape[:-1])
+        groups = (cols + GROUP - 1) // GROUP
+        steps = total + (rows * groups * GROUP + 127) // 128 * 128
+        geo.append((total, steps, shape, rows, cols))
+        total = steps + (rows * ((groups + 3) // 4 * 4) + 127) // 128 * 128
     arena = torch.empty(total, dtype=torch.uint8, device=dev)
     base = arena.data_ptr()
     out, recs, hold = [], [], []
-    for x, (oc, os_) in zip(xs, at):
-        out.append(Packed8._in(arena, (oc, os_), x.shape, x.dtype))
-        if x.numel() == 0:
+    for x, (codes, steps, shape, rows, cols) in zip(xs, geo):
+        out.append(Packed8._in(arena, (codes, steps), shape, x.dtype, rows))
+        if rows == 0 or cols == 0:
             continue
-        dims = _row_dims(x)
+        dims = _row_dims(x, rows)
         if dims is None:                       # channels apart, or rows that are no three strides
-            x = x.contiguous()
+            x = x.detach().contiguous()
             hold.append(x)
-            dims = _row_dims(x)
-        recs.append(_REC.pack(x.data_ptr(), base + oc, base + os_, *dims, x.shape[-1], int(x.dtype == F32)))
+            dims = _row_dims(x, rows)
+        recs += (x.data_ptr(), base + codes, base + steps, *dims, cols, x.dtype is F32)
     if recs:
         _launch("imf_store8", recs)
     return out
@@ -265,7 +271,7 @@ def restore8(ps: Union[Packed8, Sequence[Packed8]], outs=None) -> Union[Tensor, 
     outs = [None] * len(ps) if outs is None else list(outs)
     if len(outs) != len(ps):
         raise ValueError(f"{len(ps)} packed tensors and {len(outs)} outputs")
-    dev = _same_device("restore8", *ps, *[o for o in outs if o is not None])
+    dev = _same_device("restore8", *ps, *outs)
     for p, o in zip(ps, outs):
         if o is not None and (o.shape != p.shape or o.dtype != p.dtype):
             raise ValueError(f"output {o.dtype} {tuple(o.shape)} for packed {p.dtype} {tuple(p.shape)}")
@@ -274,20 +280,20 @@ def restore8(ps: Union[Packed8, Sequence[Packed8]], outs=None) -> Union[Tensor, 
             v = ref.values8(p.codes, p.steps, p.cols).to(p.dtype).view(p.shape)
             outs[i] = v if outs[i] is None else outs[i].copy_(v)
         return outs
-    if not _current(dev):
-        with _on(dev):
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return restore8(ps, outs)
     recs = []
     for i, p in enumerate(ps):
-        if outs[i] is None:
-            outs[i] = torch.empty(p.shape, dtype=p.dtype, device=dev)
         o = outs[i]
-        if o.numel() == 0:
+        if o is None:
+            o = outs[i] = torch.empty(p.shape, dtype=p.dtype, device=dev)
+        if p.rows == 0 or p.cols == 0:
             continue
-        dims = _row_dims(o)
+        dims = _row_dims(o, p.rows)
         if dims is None:
             raise ValueError("restore8 output: the channels have to be adjacent and the rows at three strides at most")
-        recs.append(_REC.pack(o.data_ptr(), *p._ptrs(), *dims, p.cols, int(p.dtype == F32)))
+        recs += (o.data_ptr(), *p._ptrs(), *dims, p.cols, p.dtype is F32)
     if recs:
         _launch("imf_restore8", recs)
     return outs
@@ -306,7 +312,7 @@ def gemm_wgrad8(dy: Tensor, x8: Packed8, out: Optional[Tensor] = None, accumulat
         accumulate = False
     elif out.dtype != F32 or tuple(out.shape) != (N, C) or (C > 1 and out.stride(1) != 1):
         raise ValueError(f"out has to be fp32 ({N}, {C}) with adjacent columns")
-    dev = _same_device("gemm_wgrad8", dy, x8, *([] if out is None else [out]))
+    dev = _same_device("gemm_wgrad8", dy, x8, out)
     if out is None:
         out = torch.empty(N, C, dtype=F32, device=dev)
     if dy.numel() == 0 or C == 0:
@@ -314,8 +320,8 @@ def gemm_wgrad8(dy: Tensor, x8: Packed8, out: Optional[Tensor] = None, accumulat
     if dev.type != "cuda":
         g = dy.float().t() @ ref.values8(x8.codes, x8.steps, C)
         return out.add_(g) if accumulate else out.copy_(g)
-    if not _current(dev):
-        with _on(dev):
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return gemm_wgrad8(dy, x8, out, accumulate)
     rows = x8.rows
     ld = dy.stride(0) if rows > 1 else (N + 7) // 8 * 8
@@ -353,8 +359,8 @@ def situ_bwd8(gu8: Packed8, gout: Tensor, beta: float, lbeta: Optional[float]) -
         gu = ref.values8(gu8.codes, gu8.steps, 2 * F)
         a, b, y = ref.situ_mul_grad(gu[:, :F], gu[:, F:], gout, beta, lbeta)
         return g_gu.copy_(torch.cat([a, b], 1)), act.copy_(y)
-    if not _current(dev):
-        with _on(dev):
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return situ_bwd8(gu8, gout, beta, lbeta)
     if F > 1 and gout.stride(1) != 1:
         raise ValueError("gout needs adjacent columns")
@@ -390,7 +396,7 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
             raise ValueError(f"attn_bwd8: {name} is {t.dtype} {tuple(t.shape)}, q is bf16 {tuple(shape)}")
     if lse.dtype != F32 or tuple(lse.shape) != (B, H, L) or not lse.is_contiguous():
         raise ValueError(f"attn_bwd8: lse has to be contiguous fp32 {(B, H, L)}")
-    dev = _same_device("attn_bwd8", q8, k8, v8, o8, lse, go, *([] if gv_out is None else [gv_out]))
+    dev = _same_device("attn_bwd8", q8, k8, v8, o8, lse, go, gv_out)
     if 0 in shape:
         new = lambda: torch.empty(shape, dtype=BF16, device=dev)
         return new(), new(), new() if gv_out is None else gv_out
@@ -399,8 +405,8 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
         dq, dk, dv = ref.attention_grad(*(plain(t) for t in (q8, k8, v8, o8)), lse, go, scale)
         dv = dv.to(BF16) if gv_out is None else gv_out.copy_(dv)
         return dq.to(BF16), dk.to(BF16), dv
-    if not _current(dev):
-        with _on(dev):
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
             return attn_bwd8(q8, k8, v8, o8, lse, go, scale, gv_out)
     K = _kernels()
     packed = [t for t in (q8, k8, v8, o8) if isinstance(t, Packed8)]

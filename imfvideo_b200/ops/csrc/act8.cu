@@ -24,8 +24,8 @@ struct A8Rec {
   int64_t s0, s1, s2;
   uint32_t cols, pitch, spitch;
   uint32_t units, chunk0;              // units of eight channels; first chunk of this tensor
-  FastDiv upr, n1, n2;                 // units per row; dims
-  uint32_t fp32, flat, vec;            // flat: one row stride (s2); vec: 16-byte accesses
+  FastDiv upr, gpr, n1, n2;            // units and groups per row; dims
+  uint32_t fp32, flat;                 // flat: one row stride (s2)
 };
 struct A8Args {
   A8Rec r[A8_MAX_RECS];
@@ -42,125 +42,227 @@ __device__ __forceinline__ int64_t a8_row_offset(const A8Rec& r, uint32_t row) {
   const uint32_t t = r.n2.div(row), i2 = row - t * r.n2.d, i0 = r.n1.div(t), i1 = t - i0 * r.n1.d;
   return (int64_t)i0 * r.s0 + (int64_t)i1 * r.s1 + (int64_t)i2 * r.s2;
 }
+__device__ __forceinline__ uint32_t abs2(uint32_t w) { return w & 0x7fff7fffu; }
+__device__ __forceinline__ void halves(uint32_t w, float* v) {
+  v[0] = __uint_as_float(w << 16);
+  v[1] = __uint_as_float(w & 0xffff0000u);
+}
 
-// UNITS steps per thread, loads first
-template <int UNITS>
-__global__ void __launch_bounds__(A8_THREADS) store8_kernel(const __grid_constant__ A8Args args) {
-  const A8Rec& r = a8_find(args);
-  const uint32_t u0 = (blockIdx.x - r.chunk0) * (UNITS * A8_THREADS) + threadIdx.x;
-  float v[UNITS][A8_VEC];
+// A chunk is UNITS * 256 units of eight channels.  A tensor whose rows are 16-byte aligned is read and
+// written by whole units (a thread owns one, loads first); any other one, in a launch of its own, by the channel:
+// a warp takes eight groups at a time, a lane a channel of each, so that its accesses are contiguous whatever the
+// alignment.
+template <int UNITS, bool FP32>
+__device__ __forceinline__ void store_units(const A8Rec& r, uint32_t u0) {
+  const char* const x = static_cast<const char*>(r.x);
+  int8_t* const codes = r.codes;
+  uint8_t* const steps = r.steps;
+  const int64_t ld = r.s2 * (FP32 ? 4 : 2);
+  const uint32_t pitch = r.pitch, spitch = r.spitch, units = r.units, cols = r.cols;
+  const FastDiv upr = r.upr;
+  uint4 w[UNITS][FP32 ? 2 : 1];
   uint32_t row[UNITS], c[UNITS];
 #pragma unroll
   for (int k = 0; k < UNITS; ++k) {
     const uint32_t u = u0 + k * A8_THREADS;
-    const bool in = u < r.units;
-    row[k] = in ? r.upr.div(u) : 0u;
-    c[k] = in ? (u - row[k] * r.upr.d) * A8_VEC : 0u;
+    row[k] = upr.div(u);
+    c[k] = (u - row[k] * upr.d) * A8_VEC;
+    const bool in = u < units && c[k] < cols;
 #pragma unroll
-    for (int i = 0; i < A8_VEC; ++i) v[k][i] = 0.f;
-    if (!in) continue;
-    const int64_t off = a8_row_offset(r, row[k]) + c[k];
-    if (r.vec && c[k] + A8_VEC <= r.cols) {
-      if (r.fp32) {
-        const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(r.x) + off);
-        const float4 a = __ldcs(p), b = __ldcs(p + 1);
-        v[k][0] = a.x; v[k][1] = a.y; v[k][2] = a.z; v[k][3] = a.w;
-        v[k][4] = b.x; v[k][5] = b.y; v[k][6] = b.z; v[k][7] = b.w;
-      } else {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(r.x) + off));
-        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[k][2 * i] = __uint_as_float(ww[i] << 16);
-          v[k][2 * i + 1] = __uint_as_float(ww[i] & 0xffff0000u);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int i = 0; i < A8_VEC; ++i)
-        if (c[k] + i < r.cols)
-          v[k][i] = r.fp32 ? static_cast<const float*>(r.x)[off + i]
-                           : __bfloat162float(static_cast<const __nv_bfloat16*>(r.x)[off + i]);
-    }
+    for (int h = 0; h < (FP32 ? 2 : 1); ++h)
+      w[k][h] = in ? __ldcs(reinterpret_cast<const uint4*>(x + row[k] * ld + c[k] * (FP32 ? 4 : 2) + 16 * h))
+                   : make_uint4(0u, 0u, 0u, 0u);
   }
 #pragma unroll
   for (int k = 0; k < UNITS; ++k) {
-    uint32_t m = 0u;
+    float v[A8_VEC];
+    uint32_t m;                        // bits of the largest magnitude, as fp32
+    if (FP32) {
+      const uint4 a = w[k][0], b = w[k][FP32 ? 1 : 0];
+      const uint32_t ww[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      m = 0u;
 #pragma unroll
-    for (int i = 0; i < A8_VEC; ++i) m = max(m, __float_as_uint(v[k][i]) & 0x7fffffffu);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    if (u0 + k * A8_THREADS >= r.units) continue;
+      for (int i = 0; i < 8; ++i) {
+        m = max(m, ww[i] & 0x7fffffffu);
+        v[i] = __uint_as_float(ww[i]);
+      }
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    } else {
+      const uint4 a = w[k][0];
+      uint32_t h = __vmaxu2(__vmaxu2(abs2(a.x), abs2(a.y)), __vmaxu2(abs2(a.z), abs2(a.w)));
+      h = __vmaxu2(h, __shfl_xor_sync(0xffffffffu, h, 1));
+      h = __vmaxu2(h, __shfl_xor_sync(0xffffffffu, h, 2));
+      m = max(h << 16, h & 0xffff0000u);
+      halves(a.x, v); halves(a.y, v + 2); halves(a.z, v + 4); halves(a.w, v + 6);
+    }
+    if (u0 + k * A8_THREADS >= units) break;
+    uint2 out;
     const uint32_t s = a8_step_of(m);
-    uint2 w = make_uint2(0u, 0u);
     if (s < A8_MAX_STEP) {
       const float inv = a8_inv_step(s);
-      w = make_uint2(a8_encode4(v[k], inv), a8_encode4(v[k] + 4, inv));
+      out = make_uint2(a8_encode4(v, inv), a8_encode4(v + 4, inv));
     } else if (s == A8_MAX_STEP) {
       const float inv = a8_inv_step(s);
-      w = make_uint2(a8_encode4_top(v[k], inv), a8_encode4_top(v[k] + 4, inv));
+      out = make_uint2(a8_encode4_top(v, inv), a8_encode4_top(v + 4, inv));
+    } else {
+      out = make_uint2(0u, 0u);
     }
-    *reinterpret_cast<uint2*>(r.codes + (int64_t)row[k] * r.pitch + c[k]) = w;
+    *reinterpret_cast<uint2*>(codes + (int64_t)row[k] * pitch + c[k]) = out;
     // one byte a group; the last group's thread also clears the bytes that pad the row
     if ((c[k] & (A8_GROUP - 1)) == 0) {
-      uint8_t* st = r.steps + (int64_t)row[k] * r.spitch + c[k] / A8_GROUP;
+      uint8_t* st = steps + (int64_t)row[k] * spitch + c[k] / A8_GROUP;
       *st = (uint8_t)s;
-      if (c[k] + A8_GROUP == r.pitch)
-        for (uint32_t g = r.pitch / A8_GROUP; g < r.spitch; ++g) *++st = 0;
+      if (c[k] + A8_GROUP == pitch)
+        for (uint32_t g = pitch / A8_GROUP; g < spitch; ++g) *++st = 0;
     }
   }
 }
 
-template <int UNITS>
-__global__ void __launch_bounds__(A8_THREADS) restore8_kernel(const __grid_constant__ A8Args args) {
+template <int UNITS, bool FP32>
+__device__ __forceinline__ void store_channels(const A8Rec& r, uint32_t chunk) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t groups = r.units / 4, gpr = r.gpr.d, cols = r.cols, pitch = r.pitch, spitch = r.spitch;
+  int8_t* const codes = r.codes;
+  uint8_t* const steps = r.steps;
+#pragma unroll 1
+  for (int k = 0; k < UNITS; ++k) {
+    const uint32_t g0 = (chunk * UNITS + k) * (A8_THREADS / 4) + warp * 8;
+    if (g0 >= groups) return;
+    const uint32_t row0 = r.gpr.div(g0), c0 = g0 - row0 * gpr;
+    uint32_t bits[8], row = row0, g = c0;
+    int64_t off = a8_row_offset(r, row) + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t c = g * A8_GROUP + lane;
+      bits[j] = 0u;
+      if (g0 + j < groups && c < cols)
+        bits[j] = FP32 ? __ldg(static_cast<const uint32_t*>(r.x) + off + g * A8_GROUP)
+                       : (uint32_t)__ldg(static_cast<const uint16_t*>(r.x) + off + g * A8_GROUP) << 16;
+      if (++g == gpr) {
+        g = 0;
+        off = a8_row_offset(r, ++row) + lane;
+      }
+    }
+    row = row0;
+    g = c0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t s = a8_step_of(__reduce_max_sync(0xffffffffu, bits[j] & 0x7fffffffu));
+      if (g0 + j >= groups) break;
+      int code = 0;
+      if (s < A8_MAX_STEP)
+        code = (int)__float_as_uint(fmaf(__uint_as_float(bits[j]), a8_inv_step(s), 12582912.f));     // its low byte
+      else if (s == A8_MAX_STEP)
+        code = __float2int_rn(fminf(fmaxf(__uint_as_float(bits[j]) * a8_inv_step(s), -127.f), 127.f));
+      codes[(int64_t)row * pitch + g * A8_GROUP + lane] = (int8_t)code;
+      uint8_t* st = steps + (int64_t)row * spitch + g;
+      if (lane == 0) *st = (uint8_t)s;
+      if (++g == gpr) {
+        if (lane > 0 && gpr - 1 + lane < spitch) st[lane] = 0;                                       // pads the row
+        g = 0;
+        ++row;
+      }
+    }
+  }
+}
+
+template <int UNITS, bool VEC>
+__global__ void __launch_bounds__(A8_THREADS) store8_kernel(const __grid_constant__ A8Args args) {
   const A8Rec& r = a8_find(args);
-  const uint32_t u0 = (blockIdx.x - r.chunk0) * (UNITS * A8_THREADS) + threadIdx.x;
+  const uint32_t chunk = blockIdx.x - r.chunk0, u0 = chunk * (UNITS * A8_THREADS) + threadIdx.x;
+  if (!VEC) {
+    if (r.fp32) store_channels<UNITS, true>(r, chunk);
+    else store_channels<UNITS, false>(r, chunk);
+  } else if (r.fp32) store_units<UNITS, true>(r, u0);
+  else store_units<UNITS, false>(r, u0);
+}
+
+template <int UNITS, bool FP32>
+__device__ __forceinline__ void restore_units(const A8Rec& r, uint32_t u0) {
+  char* const x = static_cast<char*>(r.x);
+  const int8_t* const src = r.codes;
+  const uint8_t* const sts = r.steps;
+  const int64_t ld = r.s2 * (FP32 ? 4 : 2);
+  const uint32_t pitch = r.pitch, spitch = r.spitch, units = r.units, cols = r.cols;
+  const FastDiv upr = r.upr;
   uint2 codes[UNITS];
   uint32_t step[UNITS], row[UNITS], c[UNITS];
 #pragma unroll
   for (int k = 0; k < UNITS; ++k) {
     const uint32_t u = u0 + k * A8_THREADS;
-    if (u >= r.units) break;
-    row[k] = r.upr.div(u);
-    c[k] = (u - row[k] * r.upr.d) * A8_VEC;
-    codes[k] = __ldg(reinterpret_cast<const uint2*>(r.codes + (int64_t)row[k] * r.pitch + c[k]));
-    step[k] = __ldg(r.steps + (int64_t)row[k] * r.spitch + c[k] / A8_GROUP);
+    row[k] = upr.div(u);
+    c[k] = (u - row[k] * upr.d) * A8_VEC;
+    if (u >= units) c[k] = cols;                       // nothing to do
+    if (c[k] < cols) {
+      codes[k] = __ldcs(reinterpret_cast<const uint2*>(src + (int64_t)row[k] * pitch + c[k]));
+      step[k] = __ldg(sts + (int64_t)row[k] * spitch + c[k] / A8_GROUP);
+    }
   }
 #pragma unroll
   for (int k = 0; k < UNITS; ++k) {
-    if (u0 + k * A8_THREADS >= r.units) break;
-    if (c[k] >= r.cols) continue;
+    if (c[k] >= cols) continue;
     const uint4 w = a8_decode8(codes[k], a8_step2(step[k]));
-    const int64_t off = a8_row_offset(r, row[k]) + c[k];
-    const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-    const bool whole = r.vec && c[k] + A8_VEC <= r.cols;
-    if (r.fp32) {
-      float* dst = static_cast<float*>(r.x) + off;
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        f[2 * i] = __uint_as_float(ww[i] << 16);
-        f[2 * i + 1] = __uint_as_float(ww[i] & 0xffff0000u);
-      }
-      if (whole) {
-        reinterpret_cast<float4*>(dst)[0] = make_float4(f[0], f[1], f[2], f[3]);
-        reinterpret_cast<float4*>(dst)[1] = make_float4(f[4], f[5], f[6], f[7]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < A8_VEC; ++i)
-          if (c[k] + i < r.cols) dst[i] = f[i];
-      }
+    char* dst = x + row[k] * ld + c[k] * (FP32 ? 4 : 2);
+    if (FP32) {
+      float v[8];
+      halves(w.x, v); halves(w.y, v + 2); halves(w.z, v + 4); halves(w.w, v + 6);
+      reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+      reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
     } else {
-      uint16_t* dst = static_cast<uint16_t*>(r.x) + off;
-      if (whole) {
-        *reinterpret_cast<uint4*>(dst) = w;
-      } else {
+      *reinterpret_cast<uint4*>(dst) = w;
+    }
+  }
+}
+
+template <int UNITS, bool FP32>
+__device__ __forceinline__ void restore_channels(const A8Rec& r, uint32_t chunk) {
+  const uint32_t lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const uint32_t groups = r.units / 4, gpr = r.gpr.d, cols = r.cols, pitch = r.pitch, spitch = r.spitch;
+#pragma unroll 1
+  for (int k = 0; k < UNITS; ++k) {
+    const uint32_t g0 = (chunk * UNITS + k) * (A8_THREADS / 4) + warp * 8;
+    if (g0 >= groups) return;
+    const uint32_t row0 = r.gpr.div(g0), c0 = g0 - row0 * gpr;
+    uint32_t code[8], step[8], row = row0, g = c0;
 #pragma unroll
-        for (int i = 0; i < A8_VEC; ++i)
-          if (c[k] + i < r.cols) dst[i] = (uint16_t)(ww[i / 2] >> (16 * (i & 1)));
+    for (int j = 0; j < 8; ++j) {
+      if (g0 + j < groups) {                           // codes are there up to the pitch
+        code[j] = (uint8_t)__ldg(r.codes + (int64_t)row * pitch + g * A8_GROUP + lane);
+        step[j] = __ldg(r.steps + (int64_t)row * spitch + g);
+      }
+      if (++g == gpr) {
+        g = 0;
+        ++row;
+      }
+    }
+    row = row0;
+    g = c0;
+    int64_t off = a8_row_offset(r, row) + lane;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (g0 + j < groups && g * A8_GROUP + lane < cols) {
+        const uint32_t w = a8_decode2(code[j], a8_step2(step[j]));
+        if (FP32) static_cast<float*>(r.x)[off + g * A8_GROUP] = __uint_as_float(w << 16);
+        else static_cast<uint16_t*>(r.x)[off + g * A8_GROUP] = (uint16_t)w;
+      }
+      if (++g == gpr) {
+        g = 0;
+        off = a8_row_offset(r, ++row) + lane;
       }
     }
   }
+}
+
+template <int UNITS, bool VEC>
+__global__ void __launch_bounds__(A8_THREADS) restore8_kernel(const __grid_constant__ A8Args args) {
+  const A8Rec& r = a8_find(args);
+  const uint32_t chunk = blockIdx.x - r.chunk0, u0 = chunk * (UNITS * A8_THREADS) + threadIdx.x;
+  if (!VEC) {
+    if (r.fp32) restore_channels<UNITS, true>(r, chunk);
+    else restore_channels<UNITS, false>(r, chunk);
+  } else if (r.fp32) restore_units<UNITS, true>(r, u0);
+  else restore_units<UNITS, false>(r, u0);
 }
 
 // Reverse mode of y = situ(gate) up' from the checkpoint of [gate | up] (width 2F), and y itself, which the
@@ -255,28 +357,31 @@ struct A8HostRec {
   int64_t n0, n1, n2, s0, s1, s2, cols, fp32;
 };
 
-// a thread takes four steps where that still gives every SM several blocks, else one
-static bool a8_wide(uint64_t units) { return units >= 4ull * A8_THREADS * 148 * 4; }
-
-static int a8_build(const void* recs, int n, A8Args& a, int& per_thread, uint32_t& chunks) {
+// Checks the records and sorts them into a[0] (rows of aligned units) and a[1] (the others).  A thread takes four
+// steps where that still gives every SM several blocks, else one.
+static int a8_build(const void* recs, int n, A8Args* a, int& per_thread, uint32_t* chunks) {
   if (n <= 0 || n > A8_MAX_RECS) return IMF_ERR_ARG;
   const A8HostRec* h = static_cast<const A8HostRec*>(recs);
-  a.n = 0;
+  a[0].n = a[1].n = 0;
   uint64_t all = 0;
   for (int i = 0; i < n; ++i) {
-    const int64_t rows = h[i].n0 * h[i].n1 * h[i].n2;
     if (h[i].n0 <= 0 || h[i].n1 <= 0 || h[i].n2 <= 0 || h[i].cols <= 0 || !h[i].x || !h[i].codes || !h[i].steps)
       return IMF_ERR_ARG;
     if (h[i].n0 > 0x7fffffff || h[i].n1 > 0x7fffffff || h[i].n2 > 0x7fffffff || h[i].cols > 0x7fffffc0 ||
-        rows > 0x7fffffff)
+        h[i].n0 * h[i].n1 > 0x7fffffff || h[i].n0 * h[i].n1 * h[i].n2 > 0x7fffffff)
       return IMF_ERR_TOO_LARGE;
+    const int64_t rows = h[i].n0 * h[i].n1 * h[i].n2;
     const uint64_t pitch = ((uint64_t)h[i].cols + A8_GROUP - 1) / A8_GROUP * A8_GROUP;
     const uint64_t units = (uint64_t)rows * (pitch / A8_VEC);
-    if (units > 0x7fffffffu) return IMF_ERR_TOO_LARGE;
+    if (units > 0x7ffffff0u) return IMF_ERR_TOO_LARGE;
     if ((reinterpret_cast<uintptr_t>(h[i].codes) & 15u) || (reinterpret_cast<uintptr_t>(h[i].steps) & 3u))
       return IMF_ERR_ARG;
-    A8Rec& r = a.r[a.n++];
     const int es = h[i].fp32 ? 4 : 2;
+    const bool flat = h[i].n0 == 1 && h[i].n1 == 1;
+    const bool vec = flat && (reinterpret_cast<uintptr_t>(h[i].x) & 15u) == 0 && (h[i].s2 * es & 15) == 0 &&
+                     h[i].cols % A8_VEC == 0;
+    A8Args& t = a[vec ? 0 : 1];
+    A8Rec& r = t.r[t.n++];
     r.x = h[i].x;
     r.codes = static_cast<int8_t*>(h[i].codes);
     r.steps = static_cast<uint8_t*>(h[i].steps);
@@ -286,23 +391,40 @@ static int a8_build(const void* recs, int n, A8Args& a, int& per_thread, uint32_
     r.spitch = (uint32_t)((pitch / A8_GROUP + 3) / 4 * 4);
     r.units = (uint32_t)units;
     r.upr = FastDiv((uint32_t)(pitch / A8_VEC));
+    r.gpr = FastDiv((uint32_t)(pitch / A8_GROUP));
     r.n1 = FastDiv((uint32_t)h[i].n1);
     r.n2 = FastDiv((uint32_t)h[i].n2);
     r.fp32 = h[i].fp32 != 0;
-    r.flat = h[i].n0 == 1 && h[i].n1 == 1;
-    const int64_t q = 16 / es - 1;
-    r.vec = (reinterpret_cast<uintptr_t>(h[i].x) & 15u) == 0 && (r.s2 & q) == 0 &&
-            (r.flat || ((r.s0 & q) == 0 && (r.s1 & q) == 0));
+    r.flat = flat;
     all += units;
   }
-  per_thread = a8_wide(all) ? 4 : 1;
-  uint64_t c = 0;
-  for (int i = 0; i < a.n; ++i) {
-    a.r[i].chunk0 = (uint32_t)c;
-    c += (a.r[i].units + (uint64_t)per_thread * A8_THREADS - 1) / ((uint64_t)per_thread * A8_THREADS);
+  per_thread = all >= 4ull * A8_THREADS * 148 * 4 ? 4 : 1;
+  for (int k = 0; k < 2; ++k) {
+    uint64_t c = 0;
+    for (int i = 0; i < a[k].n; ++i) {
+      a[k].r[i].chunk0 = (uint32_t)c;
+      c += (a[k].r[i].units + (uint64_t)per_thread * A8_THREADS - 1) / ((uint64_t)per_thread * A8_THREADS);
+    }
+    if (c > 0x7fffffffu) return IMF_ERR_TOO_LARGE;
+    chunks[k] = (uint32_t)c;
   }
-  if (c > 0x7fffffffu) return IMF_ERR_TOO_LARGE;
-  chunks = (uint32_t)c;
+  return IMF_OK;
+}
+
+typedef void (*A8Kernel)(const A8Args);
+static int a8_run(const void* recs, int n, void* stream, A8Kernel units4, A8Kernel units1, A8Kernel channels4,
+                  A8Kernel channels1) {
+  A8Args a[2];
+  int per = 1;
+  uint32_t chunks[2] = {0, 0};
+  const int rc = a8_build(recs, n, a, per, chunks);
+  if (rc) return rc;
+  for (int k = 0; k < 2; ++k) {
+    if (!chunks[k]) continue;
+    (k == 0 ? (per == 4 ? units4 : units1) : (per == 4 ? channels4 : channels1))<<<chunks[k], A8_THREADS, 0,
+                                                                                  static_cast<cudaStream_t>(stream)>>>(a[k]);
+    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
+  }
   return IMF_OK;
 }
 
@@ -312,28 +434,14 @@ static int a8_build(const void* recs, int n, A8Args& a, int& per_thread, uint32_
 // n0 x n1 x n2 of `cols` bf16 (fp32) channels at element strides s0, s1, s2 into codes and steps, or back.
 extern "C" int imf_store8(const void* recs, int n, void* stream) {
   using namespace imf;
-  A8Args a;
-  int per = 1;
-  uint32_t chunks = 0;
-  const int rc = a8_build(recs, n, a, per, chunks);
-  if (rc) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (per == 4) store8_kernel<4><<<chunks, A8_THREADS, 0, st>>>(a);
-  else store8_kernel<1><<<chunks, A8_THREADS, 0, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? IMF_OK : IMF_ERR_LAUNCH;
+  return a8_run(recs, n, stream, store8_kernel<4, true>, store8_kernel<1, true>, store8_kernel<4, false>,
+                store8_kernel<1, false>);
 }
 
 extern "C" int imf_restore8(const void* recs, int n, void* stream) {
   using namespace imf;
-  A8Args a;
-  int per = 1;
-  uint32_t chunks = 0;
-  const int rc = a8_build(recs, n, a, per, chunks);
-  if (rc) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (per == 4) restore8_kernel<4><<<chunks, A8_THREADS, 0, st>>>(a);
-  else restore8_kernel<1><<<chunks, A8_THREADS, 0, st>>>(a);
-  return cudaGetLastError() == cudaSuccess ? IMF_OK : IMF_ERR_LAUNCH;
+  return a8_run(recs, n, stream, restore8_kernel<4, true>, restore8_kernel<1, true>, restore8_kernel<4, false>,
+                restore8_kernel<1, false>);
 }
 
 // codes / steps: checkpoint of [gate | up], rows x 2F; gout rows x F, g_gu rows x 2F, act rows x F (bf16, row
