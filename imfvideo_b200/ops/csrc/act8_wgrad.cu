@@ -14,9 +14,12 @@
 // k-block each.  R is cut into slices (split-K) where that fills the SMs; a second kernel adds their planes up
 // in a fixed order, so results repeat bit for bit.
 //
-// The tensor core's fp32 accumulator drops bits with every k-step, 1.2e-5 of the result's norm after 32,780
-// rows; so a chain ends after CHUNK_KB k-blocks, and the TMA unit adds the next one's sum to the stored one
-// (one CTA owns the place, and waits for one addition before the next: the order is fixed).
+// The tensor core's fp32 accumulator drops bits with every k-step, more the longer the chain (of the result's norm,
+// 32,780 rows of activations with outliers: 1.2e-5 in one chain, 4.0e-6 in chains of 103 k-blocks, 1.9e-6 of
+// 52, 0.8e-6 of 35); so a slice is cut into equal chains of CHAIN k-blocks at most, and the TMA unit adds the
+// next one's sum to the stored one (one CTA owns the place, and waits for one addition before the next: the order is
+// fixed).  Storing a chain's sum runs under the next one's products where TMEM holds two accumulators; with BN 512
+// it holds one, whose halves are stored and begun again one after the other, at some 4 us a chain.
 //
 // What bounds it: the way into shared memory.  TMA takes about three clocks for a box row of 128 bytes, so a
 // k-block of 128 rows of dY^T and 128 columns of codes (BN 256) takes 600 clocks alone and 820 with all SMs reading,
@@ -30,39 +33,45 @@
 #include "act8.cuh"
 #include "common.cuh"
 #include "host_util.h"
+#include <stddef.h>
 
 namespace imf {
 namespace w8 {
 
 constexpr int BM = 128, BK = 64;           // rows of dY^T per CTA; rows of a k-block
-constexpr int CHUNK_KB = 128;              // k-blocks that one chain of accumulations runs over
 
 template <int BN>
 struct Smem {
   static constexpr int BNL = BN / 2;                 // columns of this CTA
   static constexpr int NH = BN == 512 ? 2 : 1;       // products of 256 columns
-  static constexpr int ACCS = NH == 2 ? 1 : 2;       // accumulators that TMEM holds
   static constexpr int STAGES = BN == 512 ? 4 : BN == 256 ? 6 : 8;
   static constexpr int CONV = BN == 512 ? 2 : 3;     // converted tiles in flight, one group of warps each
   static constexpr int GROUP_WARPS = BN == 512 ? 8 : 4;
   static constexpr int THREADS = (6 + CONV * GROUP_WARPS) * 32;
-  static constexpr int OUT = BN == 512 ? 1 : 2;      // staging buffers of an epilogue warp
+  static constexpr int CHAIN = BN == 512 ? 44 : 20;  // k-blocks that one chain of accumulations runs over at most
   static constexpr int WORDS = BNL > 128 ? 2 : 1;    // 4-byte words of steps per row
   alignas(1024) uint8_t a[STAGES][BM * BK * 2];      // dY: two panels [64 rows][128 bytes], swizzled
   alignas(1024) uint8_t b[CONV][BNL * BK * 2];       // X as bf16: BNL / 64 such panels
-  alignas(1024) uint8_t c[4][OUT][32 * 128];         // per epilogue warp: 32 rows x 32 fp32, swizzled
+  alignas(1024) uint8_t c[4][2][32 * 128];           // per epilogue warp: 32 rows x 32 fp32, swizzled, twice
   alignas(1024) uint8_t b8[STAGES][BK * BNL];        // codes [64 rows][BNL]
   alignas(16) uint8_t st[STAGES][BK * 4 * WORDS];    // step bytes [64 rows][4 WORDS]
   uint64_t full[STAGES], empty[STAGES], conv_full[CONV], conv_empty[CONV], acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
 };
+// what a launch asks for: the members, and room to align them as far as an SM has it (the window starts on a
+// multiple of 1,024 bytes in practice; the kernel checks)
+template <int BN>
+constexpr size_t smem_bytes() {
+  const size_t used = (offsetof(Smem<BN>, abort_flag) + sizeof(int) + 15) / 16 * 16;
+  return used + 1024 < 232448 ? used + 1024 : 232448;
+}
 
 struct Params {
   const uint8_t* steps;
   int64_t spitch;
   int R, N, C;
-  int n_c, tiles, num_kb, splits, kb_per;
+  int n_c, tiles, num_kb, splits, kb_per, chain;
   int accumulate;          // what is stored is added to what the result holds
   int* status;
 };
@@ -143,10 +152,15 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               const __grid_constant__ CUtensorMap tm_c, const __grid_constant__ Params p) {
   extern __shared__ uint8_t smem_raw[];
   using S = Smem<BN>;
-  constexpr int STAGES = S::STAGES, BNL = S::BNL, CONV = S::CONV, GROUP_WARPS = S::GROUP_WARPS, ACCS = S::ACCS,
+  constexpr int STAGES = S::STAGES, BNL = S::BNL, CONV = S::CONV, GROUP_WARPS = S::GROUP_WARPS,
                 NH = S::NH, WORDS = S::WORDS, PN = BN / NH;      // PN: columns of a product
   // the same offset in both CTAs, whose windows start alike: the products address them by one descriptor
-  auto& s = *reinterpret_cast<S*>(smem_raw + (1024 - (smem_u32(smem_raw) & 1023)) % 1024);
+  const uint32_t pad = (1024 - (smem_u32(smem_raw) & 1023)) % 1024;
+  if (pad + offsetof(S, abort_flag) + sizeof(int) > smem_bytes<BN>()) {
+    if (threadIdx.x == 0 && p.status) atomicCAS(p.status, 0, STATUS_BAD_ARG);
+    return;
+  }
+  auto& s = *reinterpret_cast<S*>(smem_raw + pad);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
@@ -230,31 +244,33 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       uint32_t it = 0, ch = 0;                       // k-blocks and chains so far
       bool ok = true;
       while (ok && walk.next(w)) {
-        for (int c0 = w.kb0; c0 < w.kb1 && ok; c0 += CHUNK_KB, ++ch) {
-          const int c1 = min(c0 + CHUNK_KB, w.kb1);
-          const uint32_t buf = ch % ACCS, acc = tmem + buf * BN;
-          if (ch >= ACCS)
-            ok = mbar_wait(&s.acc_empty[buf], (ch / ACCS - 1) & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
-          if (!ok) break;
-          tc_fence_after();
+        for (int c0 = w.kb0; c0 < w.kb1 && ok; c0 += p.chain, ++ch) {
+          const int c1 = min(c0 + p.chain, w.kb1);
           for (int kb = c0; kb < c1; ++kb, ++it) {
             // a group's arrival says that its CTA's dY is there too
             const int st = it % STAGES, cs = it % CONV;
             ok = mbar_wait(&s.conv_full[cs], (it / CONV) & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA);
             if (!ok) break;
-            tc_fence_after();
             const uint32_t a_base = smem_u32(s.a[st]), b_base = smem_u32(s.b[cs]);
 #pragma unroll
-            for (int ks = 0; ks < BK / 16; ++ks)
+            for (int h = 0; h < NH; ++h) {
+              // the accumulator: one of two that take turns, or the half of the only one
+              const uint32_t acc = NH == 2 ? h : ch & 1, turns = NH == 2 ? ch : ch >> 1;
+              if (kb == c0 && turns > 0)
+                ok = mbar_wait(&s.acc_empty[acc], (turns - 1) & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
+              if (!ok) break;
+              tc_fence_after();
 #pragma unroll
-              for (int h = 0; h < NH; ++h)
-                mma_pair(acc + h * PN, sdesc_mnmajor(a_base + ks * 2048, BK * 128),
+              for (int ks = 0; ks < BK / 16; ++ks)
+                mma_pair(tmem + acc * 256, sdesc_mnmajor(a_base + ks * 2048, BK * 128),
                          sdesc_mnmajor(b_base + h * (PN / 2 * BK * 2) + ks * 2048, BK * 128), idesc,
                          kb != c0 || ks != 0);
+              if (kb + 1 == c1) commit_both(&s.acc_full[acc]);
+            }
+            if (!ok) break;
             commit_both(&s.conv_empty[cs]);
             commit_both(&s.empty[st]);               // the codes were read before conv_full
           }
-          if (ok) commit_both(&s.acc_full[buf]);
         }
       }
     }
@@ -312,29 +328,26 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     bool ok = true;
     while (ok && walk.next(w)) {
       const int row0 = m_of(w.tile) + warp * 32, n0 = n_of(w.tile);
-      for (int c0 = w.kb0; c0 < w.kb1; c0 += CHUNK_KB, ++ch) {
-        const uint32_t buf = ch % ACCS;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_full[buf], (ch / ACCS) & 1, abort_flag, p.status,
-                                                  STATUS_TIMEOUT_MMA));
-        if (!ok) break;
-        tc_fence_after();
+      for (int c0 = w.kb0; c0 < w.kb1 && ok; c0 += p.chain, ++ch) {
         const bool add = p.accumulate || c0 != w.kb0;
         if (c0 != w.kb0 && lane == 0) tma_store_wait_all();          // the chain before is in memory
-        if (row0 < p.N) {
 #pragma unroll 1
-          for (int c = 0; c < BN; c += 32) {
-            // column of the accumulator -> of the tile: a product's first half is the first CTA's
-            const int n = NH == 1 ? n0 + c : n0 + (c & 128) * 2 + (c >> 8) * 128 + (c & 127);
+        for (int h = 0; h < NH; ++h) {
+          const uint32_t acc = NH == 2 ? h : ch & 1, turns = NH == 2 ? ch : ch >> 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.acc_full[acc], turns & 1, abort_flag, p.status, STATUS_TIMEOUT_MMA));
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < PN && row0 < p.N; c += 32) {
+            // column of the product -> of the tile: its first half is the first CTA's
+            const int n = n0 + (NH == 1 ? c : (c & 128) * 2 + h * 128 + (c & 127));
             if (n >= p.C) continue;
             uint32_t r[32];
-            tmem_ld32(tmem_addr(tmem + buf * BN, warp * 32, c), r);
-            if (lane == 0) {
-              if (S::OUT == 2) tma_store_wait_read1();
-              else tma_store_wait_read();
-            }
+            tmem_ld32(tmem_addr(tmem + acc * 256, warp * 32, c), r);
+            if (lane == 0) tma_store_wait_read1();
             __syncwarp();
             tc_wait_ld();
-            uint8_t *stage = s.c[warp][step++ % S::OUT], *line = stage + lane * 128;
+            uint8_t *stage = s.c[warp][step++ & 1], *line = stage + lane * 128;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
               *reinterpret_cast<uint4*>(line + ((i ^ (lane & 7)) << 4)) =
@@ -347,10 +360,10 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               tma_store_commit();
             }
           }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_first(&s.acc_empty[acc]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) arrive_first(&s.acc_empty[buf]);
       }
     }
     if (lane == 0) tma_store_wait_all();
@@ -443,9 +456,11 @@ static int launch(const void* dy, int64_t ld_dy, const void* codes, const void* 
   p.num_kb = (R + BK - 1) / BK;
   p.splits = pl.splits;
   p.kb_per = pl.kb_per;
+  const int chains = (pl.kb_per + Smem<BN>::CHAIN - 1) / Smem<BN>::CHAIN;
+  p.chain = (pl.kb_per + chains - 1) / chains;
   p.accumulate = accumulate;
   p.status = status;
-  const size_t smem = sizeof(Smem<BN>) + 1024;
+  const size_t smem = smem_bytes<BN>();
   static bool allowed[HOST_MAX_DEVICES] = {false};
   if (!allow_smem((const void*)wgrad8_kernel<BN>, smem, allowed)) return IMF_ERR_LAUNCH;
   wgrad8_kernel<BN><<<(unsigned)pl.pairs * 2, Smem<BN>::THREADS, smem, st>>>(ta, tb, tc, p);

@@ -49,6 +49,7 @@
 // and V as TMEM operands with P^T over S^T 2.21 ms (the next S^T waits for dV), the two
 // warp groups half a tile apart 3.24 ms.
 #include "attn_bwd128.h"
+#include "act8.cuh"
 #include "attn_bwd_split.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -93,6 +94,7 @@ struct BwParams {
   int B, H, L, Lp;
   int64_t dk_sb, dk_sl, dk_sh, dv_sb, dv_sl, dv_sh;
   float scale;
+  float exp_scale;        // RAW_Q: scale * log2(e)
   int* status;
   // block-sparse mode (null = dense): per K/V tile the list of steps (-1 terminated, at most qmax
   // entries) and, per entry, 4 flag bits (kv half * 2 + q half) saying which 64 x 64 quadrants
@@ -141,7 +143,12 @@ IMF_DEVICE void tma_reduce_add_4d(const CUtensorMap* m, const void* src, int c0,
       : "memory");
 }
 
-template <bool SPARSE>      // block-sparse lists given (keeps the dense instance free of their tests)
+// SPARSE: block-sparse lists given (keeps the dense instance free of their tests).  RAW_Q: the query tile is Q
+// itself and the band -lse / scale, and the math warps multiply the accumulator by scale*log2e.  For a Q that was
+// kept in 8 bits, whose values bf16 holds exactly while Q * scale*log2e is rounded (all gradients 2.4e-3
+// of their norm off the 64-bit ones instead of 3.5e-3, 1,025 to 29,140 tokens), at one packed multiplication
+// a pair of elements.
+template <bool SPARSE, bool RAW_Q = false>
 __global__ void __launch_bounds__(BW_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                 const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
@@ -468,7 +475,13 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         for (int c = 0; c < 32; c += 2) {
           const int cg = hh * 32 + c;
           if (live) {
-            const float p0 = ex2(__uint_as_float(sv[cg])), p1 = ex2(__uint_as_float(sv[cg + 1]));
+            float x0 = __uint_as_float(sv[cg]), x1 = __uint_as_float(sv[cg + 1]);
+            if (RAW_Q) {
+              const f32x2 x = mul2(pair2(sv[cg], sv[cg + 1]), dup2(p.exp_scale));
+              x0 = lo2(x);
+              x1 = hi2(x);
+            }
+            const float p0 = ex2(x0), p1 = ex2(x1);
             pk[c / 2] = pack_bf16(p0, p1);
             sv[cg] = __float_as_uint(p0);
             sv[cg + 1] = __float_as_uint(p1);
@@ -529,7 +542,7 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
       tc_fence_after();
       const int kv_row = kvb * BW_T + row;
       // Q in shared memory is Q * scale * log2(e): dK = scale dS^T Q = ln(2) dS^T Q_scaled
-      const float mul = n_q == 0 ? 0.f : (wg == 0 ? 0.6931471805599453f : 1.f);
+      const float mul = n_q == 0 ? 0.f : (wg == 0 ? (RAW_Q ? p.scale : 0.6931471805599453f) : 1.f);
       __nv_bfloat16* base =
           wg == 0 ? p.dk + (int64_t)b * p.dk_sb + (int64_t)kv_row * p.dk_sl + (int64_t)h * p.dk_sh
                   : p.dv + (int64_t)b * p.dv_sb + (int64_t)kv_row * p.dv_sl + (int64_t)h * p.dv_sh;
@@ -679,6 +692,57 @@ __global__ void attn_bwd_prep_kernel(const __nv_bfloat16* __restrict__ q,
   }
 }
 
+// The rows of constants alone, for RAW_Q: delta from dO and an O in bf16 or in 8 bits, and the bands
+// -lse / scale and -delta.  Eight lanes a row, 16-byte (8-byte) accesses.
+template <bool O8>
+__global__ void attn_bwd_prep_raw_kernel(const __nv_bfloat16* __restrict__ o, const int8_t* __restrict__ o_codes,
+                                         const uint8_t* __restrict__ o_steps, const __nv_bfloat16* __restrict__ d_o,
+                                         const float* __restrict__ lse, uint32_t* __restrict__ augq,
+                                         uint32_t* __restrict__ augd, int B, int L, int H, int Lp, int64_t o_sb,
+                                         int64_t o_sl, int64_t o_sh, int64_t g_sb, int64_t g_sl, int64_t g_sh,
+                                         float inv_exp_scale) {
+  const int lane = threadIdx.x & 31, part = lane & 7, c0 = part * 8;
+  const long u = (((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5) * 4 + (lane >> 3);
+  const bool in = u < (long)B * H * Lp;          // no early exit: the shuffles below need every lane
+  int h = 0, l = 0, b = 0;
+  if (in) {
+    h = (int)(u % H);
+    l = (int)((u / H) % Lp);
+    b = (int)(u / ((long)H * Lp));
+  }
+  const bool live = in && l < L;
+  float v = 0.f;
+  if (live) {
+    uint4 a;
+    if (O8) {
+      const int64_t r = ((int64_t)b * L + l) * H + h;
+      a = a8_decode8(*reinterpret_cast<const uint2*>(o_codes + r * 64 + c0), a8_step2(o_steps[r * 4 + part / 4]));
+    } else {
+      a = *reinterpret_cast<const uint4*>(o + b * o_sb + (int64_t)l * o_sl + h * o_sh + c0);
+    }
+    const uint4 g = *reinterpret_cast<const uint4*>(d_o + b * g_sb + (int64_t)l * g_sl + h * g_sh + c0);
+    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v += bf16_lo(aw[i]) * bf16_lo(gw[i]) + bf16_hi(aw[i]) * bf16_hi(gw[i]);
+  }
+#pragma unroll
+  for (int off = 4; off > 0; off >>= 1) v += __shfl_xor_sync(0xffffffffu, v, off);
+  if (!in) return;
+  float x = 30000.f;                             // padding rows: exp2(.. - 30000) = 0
+  if (live) x = fminf(fmaxf(lse[((long)b * H + h) * L + l] * 1.4426950408889634f, -30000.f), 30000.f);
+  const float dl = live ? v : 0.f;
+  x *= inv_exp_scale;
+  uint32_t wq = 0u, wd = 0u;                     // 16 bf16 = 8 words per row, one per lane of the row
+  if (part == 0) {
+    const float xh = bf16_lo(pack_bf16(-x, 0.f)), dh = bf16_lo(pack_bf16(-dl, 0.f));
+    wq = pack_bf16(xh, -x - xh);
+    wd = pack_bf16(dh, -dl - dh);
+  }
+  const long row = ((long)b * H + h) * Lp + l;
+  augq[row * 8 + part] = wq;
+  augd[row * 8 + part] = wd;
+}
+
 // dq = bf16(acc * scale (+ add)); `add`: an fp32 (B, L, H, 64) gradient from another branch
 __global__ void attn_bwd_post_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq,
                                      long n4, float scale, const float* __restrict__ add) {
@@ -758,6 +822,158 @@ extern "C" long imf_attn_bwd_scratch_bytes_hd(int B, int L, int H, int head_dim)
   return imf_attn_bwd_scratch_bytes(B, L, H);
 }
 
+namespace imf {
+struct Bwd64Args {
+  const void *q, *k, *v, *o;
+  const int8_t* o_codes;
+  const uint8_t* o_steps;
+  const void* d_o;
+  const float* lse;
+  void *dq, *dk, *dv;
+  int B, L, H;
+  const int64_t *strides, *o_strides, *dk_strides, *dv_strides;
+  float scale;
+  void* scratch;
+  long scratch_bytes;
+  const int* qlist;
+  const uint8_t* qflags;
+  const uint16_t* qrank;
+  int qmax, qpairs, fixed_order;
+  const float* dq_add;
+  int* status;
+  void* stream;
+};
+
+// raw: see RAW_Q (dense only)
+static int bwd64_launch(const Bwd64Args& a, bool raw) {
+  const int B = a.B, L = a.L, H = a.H;
+  const int64_t *strides = a.strides, *o_strides = a.o_strides, *dk_strides = a.dk_strides, *dv_strides = a.dv_strides;
+  const int* qlist = a.qlist;
+  void *scratch = a.scratch, *dq = a.dq, *dk = a.dk, *dv = a.dv;
+  const void *q = a.q, *k = a.k, *v = a.v, *o = a.o, *d_o = a.d_o;
+  const float *lse = a.lse, *dq_add = a.dq_add;
+  const float scale = a.scale;
+  int* status = a.status;
+  const uint16_t* qrank = a.qrank;
+  const int qpairs = a.qpairs;
+  // the fixed order of additions is kept per 128-row query tile
+  if (qpairs && (qlist == nullptr || qrank != nullptr)) return IMF_ERR_ARG;
+  if (scratch == nullptr || a.scratch_bytes < imf_attn_bwd_scratch_bytes(B, L, H)) return IMF_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(scratch) & 255) || (reinterpret_cast<uintptr_t>(dq) & 15) ||
+      (reinterpret_cast<uintptr_t>(dk) & 15) || (reinterpret_cast<uintptr_t>(dv) & 15) ||
+      (reinterpret_cast<uintptr_t>(dq_add) & 15))
+    return IMF_ERR_ARG;
+  for (int i = 0; i < 3; ++i)
+    if ((dk_strides[i] & 7) || (dv_strides[i] & 7) || (o_strides[i] & 1)) return IMF_ERR_ARG;
+  cudaStream_t st = static_cast<cudaStream_t>(a.stream);
+  const int Lp = ((L + 127) / 128) * 128;
+  float* dq_acc = static_cast<float*>(scratch);
+  const size_t acc_bytes = ((size_t)B * L * H * 64 * 4 + 255) & ~size_t(255);
+  // the turn counters follow the accumulator, so one memset clears both.  Fixed order needs a
+  // status word (how a CTA that gave up tells the others) and, block-sparse, the rank table
+  const bool ordered = a.fixed_order && status != nullptr && (qlist == nullptr || qrank != nullptr);
+  int* turn = reinterpret_cast<int*>(static_cast<uint8_t*>(scratch) + acc_bytes);
+  const size_t turn_bytes = ((size_t)B * H * (Lp / 128) * 4 + 255) & ~size_t(255);
+  uint8_t* cur = static_cast<uint8_t*>(scratch) + acc_bytes + turn_bytes;
+  uint32_t* augq = reinterpret_cast<uint32_t*>(cur);
+  cur += (size_t)B * H * Lp * 32;
+  uint32_t* augd = reinterpret_cast<uint32_t*>(cur);
+  cur += (size_t)B * H * Lp * 32;
+  __nv_bfloat16* qs = reinterpret_cast<__nv_bfloat16*>(cur);
+  cur += ((size_t)B * L * H * 64 * 2 + 255) & ~size_t(255);
+  const int n_t = (L + BW_T - 1) / BW_T;
+  const BwdSplit sp = qlist ? BwdSplit{n_t * B * H, 1, 0} : bwd64_split(B, L, H);
+  if (cudaMemsetAsync(dq_acc, 0, acc_bytes + turn_bytes, st) != cudaSuccess) return IMF_ERR_LAUNCH;
+  if (raw) {
+    const long rows = (long)B * H * Lp, blocks = ((rows + 3) / 4 * 32 + 255) / 256;
+    (o ? attn_bwd_prep_raw_kernel<false> : attn_bwd_prep_raw_kernel<true>)<<<(unsigned)blocks, 256, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(o), a.o_codes, a.o_steps, static_cast<const __nv_bfloat16*>(d_o), lse, augq,
+        augd, B, L, H, Lp, o ? o_strides[0] : 0, o ? o_strides[1] : 0, o ? o_strides[2] : 0, strides[9], strides[10],
+        strides[11], 1.f / (scale * 1.4426950408889634f));
+    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
+  } else {
+    const long rows = (long)B * H * Lp;
+    const int threads = 256;
+    auto ok16 = [](const void* p, int64_t s0, int64_t s1, int64_t s2) {
+      return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
+    };
+    const bool wide = ok16(q, strides[0], strides[1], strides[2]) &&
+                      ok16(o, o_strides[0], o_strides[1], o_strides[2]) &&
+                      ok16(d_o, strides[9], strides[10], strides[11]);
+    const long warps = wide ? (rows + 3) / 4 : rows;
+    const long blocks = (warps * 32 + threads - 1) / threads;
+    (wide ? attn_bwd_prep_wide_kernel : attn_bwd_prep_kernel)<<<(unsigned)blocks, threads, 0, st>>>(
+        static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(o),
+        static_cast<const __nv_bfloat16*>(d_o), lse, qs, augq, augd, B, L, H, Lp, strides[0],
+        strides[1], strides[2], o_strides[0], o_strides[1], o_strides[2], strides[9], strides[10],
+        strides[11], scale * 1.4426950408889634f);
+    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
+  }
+  CUtensorMap mq, mk, mv, mdo, mdq, maq, mad;
+  int rc;
+  // the query operand is the scaled copy (contiguous (B, L, H, 64)), or Q itself
+  const int q_rows = qlist ? 64 : BW_T;        // query-side boxes: a step is two 64-row blocks
+  if ((rc = raw ? make_map64(&mq, q, B, L, H, strides[0], strides[1], strides[2], q_rows)
+                : make_map64(&mq, qs, B, L, H, (int64_t)L * H * 64, (int64_t)H * 64, 64, q_rows)))
+    return rc;
+  for (int which = 0; which < 2; ++which) {      // (B*H, Lp, 16) bf16, 32-byte rows
+    uint64_t dims[3] = {16, (uint64_t)Lp, (uint64_t)B * H};
+    uint64_t str[3] = {2, 32, (uint64_t)Lp * 32};
+    uint32_t box[3] = {16, (uint32_t)q_rows, 1};
+    if ((rc = make_tmap(which ? &mad : &maq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                        which ? (void*)augd : (void*)augq, dims, str, box,
+                        CU_TENSOR_MAP_SWIZZLE_32B)))
+      return rc;
+  }
+  if ((rc = make_map64(&mk, k, B, L, H, strides[3], strides[4], strides[5], BW_T))) return rc;
+  if ((rc = make_map64(&mv, v, B, L, H, strides[6], strides[7], strides[8], BW_T))) return rc;
+  if ((rc = make_map64(&mdo, d_o, B, L, H, strides[9], strides[10], strides[11], q_rows))) return rc;
+  {
+    uint64_t dims[4] = {(uint64_t)BW_HD, (uint64_t)H, (uint64_t)L, (uint64_t)B};
+    uint64_t str[4] = {4, (uint64_t)BW_HD * 4, (uint64_t)H * BW_HD * 4, (uint64_t)L * H * BW_HD * 4};
+    uint32_t box[4] = {32, 1, (uint32_t)q_rows, 1};
+    if ((rc = make_tmap(&mdq, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, dq_acc, dims, str, box)))
+      return rc;
+  }
+  BwParams prm;
+  prm.dq_acc = dq_acc;
+  prm.dk = static_cast<__nv_bfloat16*>(dk);
+  prm.dv = static_cast<__nv_bfloat16*>(dv);
+  prm.B = B; prm.H = H; prm.L = L; prm.Lp = Lp;
+  prm.dk_sb = dk_strides[0]; prm.dk_sl = dk_strides[1]; prm.dk_sh = dk_strides[2];
+  prm.dv_sb = dv_strides[0]; prm.dv_sl = dv_strides[1]; prm.dv_sh = dv_strides[2];
+  prm.scale = scale;
+  prm.exp_scale = scale * 1.4426950408889634f;
+  prm.status = status;
+  prm.qlist = qlist;
+  prm.qflags = qlist ? a.qflags : nullptr;
+  prm.qmax = qlist ? a.qmax : 0;
+  prm.qpairs = qpairs;
+  prm.n_t = n_t;
+  prm.n_whole = sp.n_whole;
+  prm.parts = sp.parts;
+  prm.part = sp.n_split ? reinterpret_cast<float*>(cur) : nullptr;
+  prm.turn = ordered ? turn : nullptr;
+  prm.qrank = ordered ? qrank : nullptr;
+  const size_t smem = sizeof(BwSmem) + 1024;
+  auto kern = qlist != nullptr ? attn_bwd_kernel<true> : raw ? attn_bwd_kernel<false, true> : attn_bwd_kernel<false>;
+  static bool smem_set[3][HOST_MAX_DEVICES] = {{false}};
+  if (!allow_smem((const void*)kern, smem, smem_set[qlist != nullptr ? 1 : raw ? 2 : 0])) return IMF_ERR_LAUNCH;
+  kern<<<sp.ctas(), BW_THREADS, smem, st>>>(mq, mk, mv, mdo, mdq, maq, mad, prm);
+  if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
+  if (sp.n_split) {
+    const int n = sp.n_split * 2 * BW_T * (BW_HD / 4);
+    attn_bwd_combine_kernel<<<(n + 255) / 256, 256, 0, st>>>(
+        prm, sp.n_split, raw ? scale : 0.6931471805599453f);      // partial dK = dS^T (Q scale log2e)
+    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
+  }
+  const long n4 = (long)B * L * H * 64 / 4;
+  attn_bwd_post_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(
+      dq_acc, static_cast<__nv_bfloat16*>(dq), n4, scale, dq_add);
+  return cudaGetLastError() == cudaSuccess ? IMF_OK : IMF_ERR_LAUNCH;
+}
+}  // namespace imf
+
 // All tensors (B, L, H, head_dim) bf16, head_dim 64 or 128 (128: dense only); strides[0..11]: (batch,row,head) for q,k,v,do;
 // o contiguous-like with its own strides; dq contiguous (B, L, H, 64); dq_add: optional fp32
 // (B, L, H, 64) contiguous, added to dq before the rounding to bf16 (another branch's gradient);
@@ -786,109 +1002,28 @@ extern "C" int imf_attn_bwd(const void* q, const void* k, const void* v, const v
                  fixed_order && status != nullptr};
     return attn_bwd128_launch(a);
   }
-  // the fixed order of additions is kept per 128-row query tile
-  if (qpairs && (qlist == nullptr || qrank != nullptr)) return IMF_ERR_ARG;
-  if (scratch == nullptr || scratch_bytes < imf_attn_bwd_scratch_bytes(B, L, H)) return IMF_ERR_ARG;
-  if ((reinterpret_cast<uintptr_t>(scratch) & 255) || (reinterpret_cast<uintptr_t>(dq) & 15) ||
-      (reinterpret_cast<uintptr_t>(dk) & 15) || (reinterpret_cast<uintptr_t>(dv) & 15) ||
-      (reinterpret_cast<uintptr_t>(dq_add) & 15))
+  Bwd64Args a{q, k, v, o, nullptr, nullptr, d_o, lse, dq, dk, dv, B, L, H, strides, o_strides, dk_strides, dv_strides,
+              scale, scratch, scratch_bytes, qlist, qflags, qrank, qmax, qpairs, fixed_order, dq_add, status, stream};
+  return bwd64_launch(a, false);
+}
+
+// head_dim 64 from restored checkpoints: the values of q, k, v in bf16 (exact), o in bf16 or, where that is null, in 8
+// bits ((B L H, 64) codes, (B L H, 4) step bytes).  As above otherwise; q, o and d_o have 16-byte aligned rows,
+// and |scale| is at least 1e-30 (the constants carry lse / scale).
+extern "C" int imf_attn_bwd8(const void* q, const void* k, const void* v, const void* o, const void* o_codes,
+                             const void* o_steps, const void* d_o, const float* lse, void* dq, void* dk, void* dv,
+                             int B, int L, int H, const int64_t* strides, const int64_t* o_strides,
+                             const int64_t* dk_strides, const int64_t* dv_strides, float scale, void* scratch,
+                             long scratch_bytes, int fixed_order, int* status, void* stream) {
+  using namespace imf;
+  if (B <= 0 || L <= 0 || H <= 0 || !(fabsf(scale) >= 1e-30f) || (!o && (!o_codes || !o_steps))) return IMF_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(o) & 15) || (reinterpret_cast<uintptr_t>(d_o) & 15) ||
+      (reinterpret_cast<uintptr_t>(o_codes) & 15))
     return IMF_ERR_ARG;
   for (int i = 0; i < 3; ++i)
-    if ((dk_strides[i] & 7) || (dv_strides[i] & 7) || (o_strides[i] & 1)) return IMF_ERR_ARG;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int Lp = ((L + 127) / 128) * 128;
-  float* dq_acc = static_cast<float*>(scratch);
-  const size_t acc_bytes = ((size_t)B * L * H * 64 * 4 + 255) & ~size_t(255);
-  // the turn counters follow the accumulator, so one memset clears both.  Fixed order needs a
-  // status word (how a CTA that gave up tells the others) and, block-sparse, the rank table
-  const bool ordered = fixed_order && status != nullptr && (qlist == nullptr || qrank != nullptr);
-  int* turn = reinterpret_cast<int*>(static_cast<uint8_t*>(scratch) + acc_bytes);
-  const size_t turn_bytes = ((size_t)B * H * (Lp / 128) * 4 + 255) & ~size_t(255);
-  uint8_t* cur = static_cast<uint8_t*>(scratch) + acc_bytes + turn_bytes;
-  uint32_t* augq = reinterpret_cast<uint32_t*>(cur);
-  cur += (size_t)B * H * Lp * 32;
-  uint32_t* augd = reinterpret_cast<uint32_t*>(cur);
-  cur += (size_t)B * H * Lp * 32;
-  __nv_bfloat16* qs = reinterpret_cast<__nv_bfloat16*>(cur);
-  cur += ((size_t)B * L * H * 64 * 2 + 255) & ~size_t(255);
-  const int n_t = (L + BW_T - 1) / BW_T;
-  const BwdSplit sp = qlist ? BwdSplit{n_t * B * H, 1, 0} : bwd64_split(B, L, H);
-  if (cudaMemsetAsync(dq_acc, 0, acc_bytes + turn_bytes, st) != cudaSuccess) return IMF_ERR_LAUNCH;
-  {
-    const long rows = (long)B * H * Lp;
-    const int threads = 256;
-    auto ok16 = [](const void* p, int64_t s0, int64_t s1, int64_t s2) {
-      return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && s0 % 8 == 0 && s1 % 8 == 0 && s2 % 8 == 0;
-    };
-    const bool wide = ok16(q, strides[0], strides[1], strides[2]) &&
-                      ok16(o, o_strides[0], o_strides[1], o_strides[2]) &&
-                      ok16(d_o, strides[9], strides[10], strides[11]);
-    const long warps = wide ? (rows + 3) / 4 : rows;
-    const long blocks = (warps * 32 + threads - 1) / threads;
-    (wide ? attn_bwd_prep_wide_kernel : attn_bwd_prep_kernel)<<<(unsigned)blocks, threads, 0, st>>>(
-        static_cast<const __nv_bfloat16*>(q), static_cast<const __nv_bfloat16*>(o),
-        static_cast<const __nv_bfloat16*>(d_o), lse, qs, augq, augd, B, L, H, Lp, strides[0],
-        strides[1], strides[2], o_strides[0], o_strides[1], o_strides[2], strides[9], strides[10],
-        strides[11], scale * 1.4426950408889634f);
-    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
-  }
-  CUtensorMap mq, mk, mv, mdo, mdq, maq, mad;
-  int rc;
-  // the query operand is the scaled copy (contiguous (B, L, H, 64))
-  const int q_rows = qlist ? 64 : BW_T;        // query-side boxes: a step is two 64-row blocks
-  if ((rc = make_map64(&mq, qs, B, L, H, (int64_t)L * H * 64, (int64_t)H * 64, 64, q_rows))) return rc;
-  for (int which = 0; which < 2; ++which) {      // (B*H, Lp, 16) bf16, 32-byte rows
-    uint64_t dims[3] = {16, (uint64_t)Lp, (uint64_t)B * H};
-    uint64_t str[3] = {2, 32, (uint64_t)Lp * 32};
-    uint32_t box[3] = {16, (uint32_t)q_rows, 1};
-    if ((rc = make_tmap(which ? &mad : &maq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                        which ? (void*)augd : (void*)augq, dims, str, box,
-                        CU_TENSOR_MAP_SWIZZLE_32B)))
-      return rc;
-  }
-  if ((rc = make_map64(&mk, k, B, L, H, strides[3], strides[4], strides[5], BW_T))) return rc;
-  if ((rc = make_map64(&mv, v, B, L, H, strides[6], strides[7], strides[8], BW_T))) return rc;
-  if ((rc = make_map64(&mdo, d_o, B, L, H, strides[9], strides[10], strides[11], q_rows))) return rc;
-  {
-    uint64_t dims[4] = {(uint64_t)BW_HD, (uint64_t)H, (uint64_t)L, (uint64_t)B};
-    uint64_t str[4] = {4, (uint64_t)BW_HD * 4, (uint64_t)H * BW_HD * 4, (uint64_t)L * H * BW_HD * 4};
-    uint32_t box[4] = {32, 1, (uint32_t)q_rows, 1};
-    if ((rc = make_tmap(&mdq, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, dq_acc, dims, str, box)))
-      return rc;
-  }
-  BwParams prm;
-  prm.dq_acc = dq_acc;
-  prm.dk = static_cast<__nv_bfloat16*>(dk);
-  prm.dv = static_cast<__nv_bfloat16*>(dv);
-  prm.B = B; prm.H = H; prm.L = L; prm.Lp = Lp;
-  prm.dk_sb = dk_strides[0]; prm.dk_sl = dk_strides[1]; prm.dk_sh = dk_strides[2];
-  prm.dv_sb = dv_strides[0]; prm.dv_sl = dv_strides[1]; prm.dv_sh = dv_strides[2];
-  prm.scale = scale;
-  prm.status = status;
-  prm.qlist = qlist;
-  prm.qflags = qlist ? qflags : nullptr;
-  prm.qmax = qlist ? qmax : 0;
-  prm.qpairs = qpairs;
-  prm.n_t = n_t;
-  prm.n_whole = sp.n_whole;
-  prm.parts = sp.parts;
-  prm.part = sp.n_split ? reinterpret_cast<float*>(cur) : nullptr;
-  prm.turn = ordered ? turn : nullptr;
-  prm.qrank = ordered ? qrank : nullptr;
-  const size_t smem = sizeof(BwSmem) + 1024;
-  auto kern = qlist != nullptr ? attn_bwd_kernel<true> : attn_bwd_kernel<false>;
-  static bool smem_set[2][HOST_MAX_DEVICES] = {{false}};
-  if (!allow_smem((const void*)kern, smem, smem_set[qlist != nullptr])) return IMF_ERR_LAUNCH;
-  kern<<<sp.ctas(), BW_THREADS, smem, st>>>(mq, mk, mv, mdo, mdq, maq, mad, prm);
-  if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
-  if (sp.n_split) {
-    const int n = sp.n_split * 2 * BW_T * (BW_HD / 4);
-    attn_bwd_combine_kernel<<<(n + 255) / 256, 256, 0, st>>>(
-        prm, sp.n_split, 0.6931471805599453f);      // partial dK = dS^T (Q scale log2e)
-    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
-  }
-  const long n4 = (long)B * L * H * 64 / 4;
-  attn_bwd_post_kernel<<<(unsigned)((n4 + 255) / 256), 256, 0, st>>>(
-      dq_acc, static_cast<__nv_bfloat16*>(dq), n4, scale, dq_add);
-  return cudaGetLastError() == cudaSuccess ? IMF_OK : IMF_ERR_LAUNCH;
+    if ((o && (o_strides[i] & 7)) || (strides[9 + i] & 7)) return IMF_ERR_ARG;
+  Bwd64Args a{q, k, v, o, static_cast<const int8_t*>(o_codes), static_cast<const uint8_t*>(o_steps), d_o, lse, dq, dk,
+              dv, B, L, H, strides, o_strides, dk_strides, dv_strides, scale, scratch, scratch_bytes, nullptr, nullptr,
+              nullptr, 0, 0, fixed_order, nullptr, status, stream};
+  return bwd64_launch(a, true);
 }

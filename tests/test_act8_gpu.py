@@ -310,6 +310,12 @@ def test_attention_fixed_order_and_views(A, K):
     got = A.attn_bwd8(*ps, lse, go.transpose(1, 2).contiguous().transpose(1, 2))
     _near(got, [t.double() for t in a], "order of go")
     _near(A.attn_bwd8(*ps, lse, go, scale=0.05), _oracle(ps, lse, go, 0.05), "scale")
+    low = torch.logsumexp(-0.1 * torch.einsum("blhd,bmhd->bhlm", *(p.restore().float() for p in ps[:2])), -1)
+    _near(A.attn_bwd8(*ps, low, go, scale=-0.1), _oracle(ps, low, go, -0.1), "a scale below zero")
+    flat = torch.full_like(lse, math.log(1500))                          # scale 0: P = 1 / L, dQ = dK = 0
+    dq, dk, dv = A.attn_bwd8(*ps, flat, go, scale=0.0)
+    assert (dq == 0).all() and (dk == 0).all()
+    _near((dv,), _oracle(ps, flat, go, 0.0)[2:], "a scale of zero")
     none = torch.empty(0, 5, 2, 64, dtype=BF16, device="cuda")
     assert A.attn_bwd8(*A.store8([none] * 4), torch.empty(0, 2, 5, device="cuda"), none)[0].shape == none.shape
     with pytest.raises(ValueError):
