@@ -316,7 +316,7 @@ class TransformerBlock(nn.Module):
 
             f = self.mlp.w1.out_features
             g = self._geom = BlockGeom(self.attn, self.norm1.weight.shape[0], f + (-f) % 8,
-                                       act8=self.act_store == "int8")
+                                       act8=getattr(self, "act_store", "bf16") == "int8")
         return g
 
     def fused_ok(self, x: Tensor, compute_dtype) -> bool:

@@ -146,7 +146,7 @@ class _BlockFn(torch.autograd.Function):
     def forward(ctx, geom, core, fresh, use_res, eps, beta, lbeta, cos, sin, nsnap, prefix,
                 dprefix, *rest):
         g: BlockGeom = geom
-        core, sinks = core if isinstance(core, tuple) else (core, None)
+        core, sinks, grad_on = core
         snaps = list(rest[:nsnap])
         dsnaps = list(rest[nsnap:2 * nsnap])
         (w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn, a_scale, m_scale,
@@ -215,7 +215,9 @@ class _BlockFn(torch.autograd.Function):
                                      float(lbeta or 0.0), stream), "imf_block_post")
         K.LAUNCHES.count += 7 if g.gate else 6
         if need_bwd:
-            if g.act8:
+            if g.act8 and not grad_on:        # under no_grad: nothing to keep (parameters still ask for gradients)
+                kept = ()
+            elif g.act8:
                 # q, k and o go to the dense core's backward in 8 bits; another core has its own form
                 # of them, and they stay as they are
                 dense = isinstance(core, DenseCore)
@@ -383,8 +385,7 @@ def run_block(geom: BlockGeom, core, fresh: bool, use_res: bool, eps: float, bet
     W_a, W_qb, W_kvb, W_out, W13, W2) with bf16 weight matrices; ``sinks`` says which
     parameters those matrices were built from (see ``GradSinks``)."""
     nsnap = len(snaps)
-    if sinks is not None:
-        core = (core, sinks)
+    core = (core, sinks, torch.is_grad_enabled())
     args = list(snaps) + ([s for s in dsnaps] if dprefix is not None else [None] * nsnap)
     p, t = _BlockFn.apply(geom, core, fresh, use_res, eps, beta, lbeta, cos, sin, nsnap, prefix,
                           dprefix, *args, *params)

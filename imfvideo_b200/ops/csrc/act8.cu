@@ -60,6 +60,8 @@ __device__ __forceinline__ void store_units(const A8Rec& r, uint32_t u0) {
   const int64_t ld = r.s2 * (FP32 ? 4 : 2);
   const uint32_t pitch = r.pitch, spitch = r.spitch, units = r.units, cols = r.cols;
   const FastDiv upr = r.upr;
+  const uint32_t gpr = r.gpr.d;
+  const bool words = gpr % 4 == 0 || gpr <= 2;
   uint4 w[UNITS][FP32 ? 2 : 1];
   uint32_t row[UNITS], c[UNITS];
 #pragma unroll
@@ -96,25 +98,37 @@ __device__ __forceinline__ void store_units(const A8Rec& r, uint32_t u0) {
       m = max(h << 16, h & 0xffff0000u);
       halves(a.x, v); halves(a.y, v + 2); halves(a.z, v + 4); halves(a.w, v + 6);
     }
-    if (u0 + k * A8_THREADS >= units) break;
-    uint2 out;
     const uint32_t s = a8_step_of(m);
-    if (s < A8_MAX_STEP) {
-      const float inv = a8_inv_step(s);
-      out = make_uint2(a8_encode4(v, inv), a8_encode4(v + 4, inv));
-    } else if (s == A8_MAX_STEP) {
-      const float inv = a8_inv_step(s);
-      out = make_uint2(a8_encode4_top(v, inv), a8_encode4_top(v + 4, inv));
-    } else {
-      out = make_uint2(0u, 0u);
+    // the steps of four groups are one word, which the first of them writes, where a warp holds whole words (a byte
+    // a group cost rows of two groups, q and k by the head, twice the time of wide ones)
+    uint32_t word = s;
+    if (words) {                       // the same for the whole launch's tensor: every lane shuffles
+      const uint32_t s1 = __shfl_down_sync(0xffffffffu, s, 4), s2 = __shfl_down_sync(0xffffffffu, s, 8),
+                     s3 = __shfl_down_sync(0xffffffffu, s, 12);
+      if (gpr > 1) word |= s1 << 8;
+      if (gpr > 2) word |= s2 << 16 | s3 << 24;
     }
-    *reinterpret_cast<uint2*>(codes + (int64_t)row[k] * pitch + c[k]) = out;
-    // one byte a group; the last group's thread also clears the bytes that pad the row
-    if ((c[k] & (A8_GROUP - 1)) == 0) {
-      uint8_t* st = steps + (int64_t)row[k] * spitch + c[k] / A8_GROUP;
-      *st = (uint8_t)s;
-      if (c[k] + A8_GROUP == pitch)
-        for (uint32_t g = pitch / A8_GROUP; g < spitch; ++g) *++st = 0;
+    if (u0 + k * A8_THREADS < units) {
+      uint2 out;
+      if (s < A8_MAX_STEP) {
+        const float inv = a8_inv_step(s);
+        out = make_uint2(a8_encode4(v, inv), a8_encode4(v + 4, inv));
+      } else if (s == A8_MAX_STEP) {
+        const float inv = a8_inv_step(s);
+        out = make_uint2(a8_encode4_top(v, inv), a8_encode4_top(v + 4, inv));
+      } else {
+        out = make_uint2(0u, 0u);
+      }
+      *reinterpret_cast<uint2*>(codes + (int64_t)row[k] * pitch + c[k]) = out;
+      const uint32_t g = c[k] / A8_GROUP;
+      uint8_t* st = steps + (int64_t)row[k] * spitch + g;
+      if (words) {
+        if (c[k] % (4 * A8_GROUP) == 0) *reinterpret_cast<uint32_t*>(st) = word;
+      } else if (c[k] % A8_GROUP == 0) {
+        *st = (uint8_t)s;
+        if (g + 1 == gpr)              // the last group's thread also clears the bytes that pad the row
+          for (uint32_t j = gpr; j < spitch; ++j) *++st = 0;
+      }
     }
   }
 }

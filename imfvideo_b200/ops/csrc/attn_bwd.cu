@@ -107,6 +107,7 @@ struct BwParams {
   const uint8_t* qflags;
   int qmax, qpairs;
   int n_t;                // K/V tiles per (batch, head)
+  int group;              // chains that are worked on at a time (bwd_item)
   // dense mode: the query tiles of each K/V tile from n_whole on are split over `parts` CTAs to
   // even out the last wave (attn_bwd_split.h); each writes unscaled fp32 partial dK / dV to
   // part[(tile - n_whole) * parts + r] = [dK | dV][128][64] and a second kernel adds them up
@@ -146,8 +147,8 @@ IMF_DEVICE void tma_reduce_add_4d(const CUtensorMap* m, const void* src, int c0,
 // SPARSE: block-sparse lists given (keeps the dense instance free of their tests).  RAW_Q: the query tile is Q
 // itself and the band -lse / scale, and the math warps multiply the accumulator by scale*log2e.  For a Q that was
 // kept in 8 bits, whose values bf16 holds exactly while Q * scale*log2e is rounded (all gradients 2.4e-3
-// of their norm off the 64-bit ones instead of 3.5e-3, 1,025 to 29,140 tokens), at one packed multiplication
-// a pair of elements.
+// of their norm off the 64-bit ones instead of 3.5e-3, 1,025 to 29,140 tokens), at one multiplication an element
+// (4 heads of 29,140 tokens 2.21 ms either way).
 template <bool SPARSE, bool RAW_Q = false>
 __global__ void __launch_bounds__(BW_THREADS, 1)
 attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
@@ -160,13 +161,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   // block-sparse lists can be very uneven (the always-attended tail tiles are attended by every
   // query tile and sit at the end): walk the K/V tiles from the back so the long ones start first
-  // item = chain (batch, head) + chains * K/V tile: the resident CTAs are a few K/V tiles of
-  // EVERY chain rather than many of one
   const int idx = (int)blockIdx.x;
   const bool split = idx >= p.n_whole;
   const int item = split ? p.n_whole + (idx - p.n_whole) / p.parts : idx;
   const int qpart = split ? (idx - p.n_whole) % p.parts : 0;
-  const int chains = p.B * p.H, kv_ord = item / chains, chain = item % chains;
+  int chain, kv_ord;
+  bwd_item(item, p.B * p.H, p.n_t, p.group, chain, kv_ord);
   const int kvb = SPARSE ? p.n_t - 1 - kv_ord : kv_ord;
   const int h = chain % p.H, b = chain / p.H;
   const size_t lrow = ((size_t)chain * p.n_t + kvb) * (size_t)p.qmax;
@@ -477,9 +477,8 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
           if (live) {
             float x0 = __uint_as_float(sv[cg]), x1 = __uint_as_float(sv[cg + 1]);
             if (RAW_Q) {
-              const f32x2 x = mul2(pair2(sv[cg], sv[cg + 1]), dup2(p.exp_scale));
-              x0 = lo2(x);
-              x1 = hi2(x);
+              x0 *= p.exp_scale;
+              x1 *= p.exp_scale;
             }
             const float p0 = ex2(x0), p1 = ex2(x1);
             pk[c / 2] = pack_bf16(p0, p1);
@@ -767,9 +766,10 @@ __global__ void attn_bwd_combine_kernel(const BwParams p, int n_split, float sca
   const int i = (int)(blockIdx.x * blockDim.x + threadIdx.x);
   if (i >= n_split * 2 * TILE4) return;
   const int c = (i % ROW4) * 4, row = (i / ROW4) % BW_T, which = (i / TILE4) & 1, t = i / (2 * TILE4);
-  const int item = p.n_whole + t, chains = p.B * p.H, chain = item % chains;
+  int chain, kv_ord;
+  bwd_item(p.n_whole + t, p.B * p.H, p.n_t, p.group, chain, kv_ord);
   const int h = chain % p.H, b = chain / p.H;
-  const int kv_row = (item / chains) * BW_T + row;
+  const int kv_row = kv_ord * BW_T + row;
   if (kv_row >= p.L) return;
   const float* src = p.part + (((size_t)t * p.parts * 2 + which) * BW_T + row) * BW_HD + c;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -950,6 +950,7 @@ static int bwd64_launch(const Bwd64Args& a, bool raw) {
   prm.qmax = qlist ? a.qmax : 0;
   prm.qpairs = qpairs;
   prm.n_t = n_t;
+  prm.group = bwd_group(B * H, L, BW_HD, qlist || ordered);
   prm.n_whole = sp.n_whole;
   prm.parts = sp.parts;
   prm.part = sp.n_split ? reinterpret_cast<float*>(cur) : nullptr;

@@ -79,6 +79,7 @@ struct Params {
   // the query tiles of each K/V tile from n_whole on are split over `parts` CTAs to even out the
   // last wave (attn_bwd_split.h); each writes unscaled fp32 partial dK / dV to
   // part[(tile - n_whole) * parts + r] = [dK | dV][128][128] and a second kernel adds them up
+  int n_t, group;         // K/V tiles of a chain; chains that are worked on at a time (bwd_item)
   int n_whole, parts;
   float* part;
   // fixed-order dQ (null = arrival order): one counter per (batch, head, 64-row query step),
@@ -101,14 +102,14 @@ attn_bwd128_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
   auto& s = *reinterpret_cast<Smem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                      ~uintptr_t(1023));
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // item = chain (batch, head) + chains * K/V tile: a CTA waits (fixed-order dQ) only for the K/V
-  // tile before it in its chain, whose block index is smaller, and the resident CTAs are a few
-  // tiles of every chain
+  // (bwd_item) a CTA waits (fixed-order dQ) only for the K/V tile before it in its chain, whose
+  // block index is smaller
   const int idx = (int)blockIdx.x;
   const bool split = idx >= p.n_whole;
   const int item = split ? p.n_whole + (idx - p.n_whole) / p.parts : idx;
   const int qpart = split ? (idx - p.n_whole) % p.parts : 0, parts = split ? p.parts : 1;
-  const int chains = p.B * p.H, kvb = item / chains, chain = item % chains;
+  int chain, kvb;
+  bwd_item(item, p.B * p.H, p.n_t, p.group, chain, kvb);
   const int h = chain % p.H, b = chain / p.H;
   int n_q = (p.L + QT - 1) / QT;
   int* turn = p.turn ? p.turn + ((size_t)b * p.H + h) * n_q : nullptr;
@@ -476,9 +477,10 @@ __global__ void attn_bwd128_combine_kernel(const Params p, int n_split, float sc
   const int i = (int)(blockIdx.x * blockDim.x + threadIdx.x);
   if (i >= n_split * 2 * TILE4) return;
   const int c = (i % ROW4) * 4, row = (i / ROW4) % KT, which = (i / TILE4) & 1, t = i / (2 * TILE4);
-  const int item = p.n_whole + t, chains = p.B * p.H, chain = item % chains;
+  int chain, kv_ord;
+  bwd_item(p.n_whole + t, p.B * p.H, p.n_t, p.group, chain, kv_ord);
   const int h = chain % p.H, b = chain / p.H;
-  const int kv_row = (item / chains) * KT + row;
+  const int kv_row = kv_ord * KT + row;
   if (kv_row >= p.L) return;
   const float* src = p.part + (((size_t)t * p.parts * 2 + which) * KT + row) * HD + c;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -571,6 +573,8 @@ int attn_bwd128_launch(const Bwd128Args& a) {
   prm.dv_sb = a.dv_strides[0]; prm.dv_sl = a.dv_strides[1]; prm.dv_sh = a.dv_strides[2];
   prm.scale = a.scale;
   prm.status = a.status;
+  prm.n_t = (L + KT - 1) / KT;
+  prm.group = bwd_group(B * H, L, HD, a.fixed_order && a.status != nullptr);
   prm.n_whole = sp.n_whole;
   prm.parts = sp.parts;
   prm.part = sp.n_split ? reinterpret_cast<float*>(end) : nullptr;

@@ -68,4 +68,24 @@ inline BwdSplit bwd_split(long items, int n_steps, int sms, float cta_steps) {
   return r;
 }
 
+// How many chains (batch, head) are worked on at a time.  Every K/V tile of a chain reads all of its Q and dO and
+// adds to all of its dQ, 8 bytes a channel; the resident CTAs drift apart along them, and what of the chains at work
+// does not fit in L2 comes from DRAM again and again (16 chains of 32,780 rows, head_dim 64: 26 GB read for the
+// 7.5 that one pass per wave takes).  34 MB of them leave the L2 room for what drifts.  All chains at once / in
+// groups, ms: 16 chains of 32,780 rows, head_dim 64 12.3 / 10.8; 8 chains 5.63 / 5.46; 16 of 16,384 2.92 / 2.81;
+// 12 of 32,780, head_dim 128 18.3 / 16.5; 4 of 29,140, head_dim 64 2.20 / 2.21 (two at a time).  In the fixed order of dQ
+// additions all chains stay in one group: a CTA waits for the one before it in its chain, and more
+// of a chain's CTAs at once wait longer.
+inline int bwd_group(int chains, int L, int head_dim, bool ordered) {
+  const long n = 34000000L / ((long)L * head_dim * 8);
+  return ordered || n >= chains ? chains : n < 1 ? 1 : (int)n;
+}
+// Item -> chain and K/V tile: within a group, consecutive items are one K/V tile of each chain, so the resident CTAs
+// are a few K/V tiles of every chain of the group.
+__device__ __forceinline__ void bwd_item(int item, int chains, int n_t, int group, int& chain, int& kv_tile) {
+  const int g = item / (group * n_t), first = g * group, n = min(group, chains - first), r = item - first * n_t;
+  kv_tile = r / n;
+  chain = first + r % n;
+}
+
 }  // namespace imf

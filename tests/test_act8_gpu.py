@@ -115,6 +115,10 @@ def test_restore_into_views_leaves_the_rest(A):
         A.restore8(q, torch.empty(77, 66, device="cuda").t())
     with pytest.raises(ValueError):
         A.restore8([p], [torch.empty(2, 33, 3, 45, dtype=BF16)])         # on the CPU
+    with pytest.raises(ValueError):
+        A.restore8(p, torch.empty(2, 1, 3, 45, dtype=BF16, device="cuda").expand(2, 33, 3, 45))
+    with pytest.raises(ValueError):
+        A.restore8(q, torch.empty(1, 77, device="cuda").expand(66, 77))
 
 
 def test_offsets_beyond_32_bits(A):
@@ -186,6 +190,8 @@ def test_weight_gradient_views(A, K):
         A.gemm_wgrad8(_randn(g, 777, 208)[:, 1:], p)
     with pytest.raises(ValueError):
         A.gemm_wgrad8(_randn(g, 208, 777).t(), p)
+    with pytest.raises(ValueError):
+        A.gemm_wgrad8(dy, p, out=torch.empty(1, 100, device="cuda").expand(203, 100))
     K.check_status()
 
 
@@ -381,6 +387,37 @@ def test_another_stream_and_two_graphs(A, K):
     torch.cuda.synchronize()
     for got, w in zip(outs, want):
         assert all(torch.equal(x, y) for x, y in zip(got, w))
+    K.check_status()
+
+
+def test_threads_at_once(A, K):
+    """Two host threads, a stream each: every call has its own workspace."""
+    import threading
+
+    g = _gen(42)
+    mk = lambda: (_randn(g, 3000, 256), _randn(g, 3000, 2 * 344), _randn(g, 3000, 528), _randn(g, 3000, 344))
+    data = [mk(), mk()]
+    want = [_linear_step(A, *t) for t in data]
+    torch.cuda.synchronize()
+    got, errors = [None, None], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(20):
+                    got[i] = _linear_step(A, *data[i])
+                torch.cuda.current_stream().synchronize()
+        except Exception as exc:      # noqa: BLE001
+            errors.append(exc)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for i in range(2):
+        assert all(torch.equal(x, y) for x, y in zip(got[i], want[i]))
     K.check_status()
 
 
