@@ -63,7 +63,7 @@ def _check_store(A, x, p=None):
 # ------------------------------------------------------------- store, restore ---
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("rows,C", [(1, 1), (1, 32), (3, 7), (5, 33), (2, 64), (77, 48), (130, 528), (31, 1021),
-                                    (2068, 682), (4099, 1376), (9000, 2064)])
+                                    (2068, 682), (4099, 1376), (9000, 2064), (9000, 2048), (6000, 1021), (90000, 64)])
 def test_store_and_restore(A, dtype, rows, C):
     _check_store(A, _activations(_gen(rows + C), rows, C, dtype))
 
