@@ -58,7 +58,7 @@ def _kernels():
         K._lib.imf_wgrad8.restype = ci
         K._lib.imf_wgrad8.argtypes = [vp, i64, vp, vp, ci, ci, ci, vp, i64, ci, vp, i64, vp, vp]
         K._lib.imf_attn_bwd8.restype = ci
-        K._lib.imf_attn_bwd8.argtypes = [vp] * 11 + [ci] * 3 + [vp] * 4 + [cf, vp, cl, ci, vp, vp]
+        K._lib.imf_attn_bwd8.argtypes = [vp] * 10 + [ci] * 3 + [vp] * 4 + [cf, vp, cl, ci, vp, vp]
         K._lib.imf_situ_bwd8.restype = ci
         K._lib.imf_situ_bwd8.argtypes = [vp] * 5 + [cl, ci] + [i64] * 3 + [cf, cf, ci, vp]
         _KERNELS = K
@@ -429,45 +429,45 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
     dv = _new(shape, BF16, dev) if gv_out is None else gv_out
     if dv.stride(3) != 1 or dv.data_ptr() % 16 or any(s % 8 for s in dv.stride()[:3]):
         raise ValueError("attn_bwd8: the dv output needs 16-byte aligned rows")
-    # head_dim 64: the kernel's form for an exact Q, which reads o in 8 bits (its constants are lse / scale)
+    # what is packed gets its values in bf16 in front of the kernel's own scratch.  head_dim 64: the kernel's form for
+    # an exact Q, whose first launch does that too and reads o in 8 bits (its constants are lse / scale)
     raw = hd == 64 and abs(scale) >= 1e-30
-    keep8 = o8 if raw and isinstance(o8, Packed8) else None
-    # the values of what else is packed, in bf16, in front of the kernel's own scratch
-    n, rows = 2 * B * L * H * hd, B * L * H
+    n, rows, row = 2 * B * L * H * hd, B * L * H, (L * H * hd, H * hd, hd)
     size = (n + 255) // 256 * 256
     nscr = lib.imf_attn_bwd_scratch_bytes_hd(B, L, H, hd)
-    count = sum(isinstance(t, Packed8) for t in (q8, k8, v8, o8)) - (keep8 is not None)
-    work = _new(count * size + nscr, torch.uint8, dev)
-    at = work.data_ptr()
-    recs, ptrs, strides, hold = [], [], [], []
-    for i, t in enumerate((q8, k8, v8, o8, go)):
-        if i == 3 and keep8 is not None:
-            ptrs.append(None)
-            strides.append((0, 0, 0))
-        elif isinstance(t, Packed8):
-            recs += (at, *t._ptrs(), 1, 1, rows, 0, 0, hd, hd, 0)
-            ptrs.append(at)
-            strides.append((L * H * hd, H * hd, hd))
-            at += size
-        else:
+    space = sum(isinstance(t, Packed8) for t in ((q8, k8, v8) if raw else (q8, k8, v8, o8))) * size
+    work = _new(space + nscr, torch.uint8, dev)
+    at = base = work.data_ptr()
+    codes, recs, ptrs, strides, hold = [], [], [], [], []
+    for t in (q8, k8, v8, o8, go):
+        if not isinstance(t, Packed8):
             t = K._tma_ok(t)
             strides.append(t.stride()[:3])
             ptrs.append(t.data_ptr())
             hold.append(t)                     # a copy lives until the launch
-    _launch("imf_restore8", recs)
-    scr = work.data_ptr() + count * size
+            codes += (None, None)
+            continue
+        pair = t._ptrs()
+        codes += pair
+        strides.append(row)
+        if raw and len(ptrs) == 3:             # o stays as it is
+            ptrs.append(None)
+            continue
+        recs += (at, *pair, 1, 1, rows, 0, 0, hd, hd, 0)
+        ptrs.append(at)
+        at += size
     i64 = ctypes.c_int64
     q_, k_, v_, o_, g_ = strides
-    q, k, v, o, g = ptrs
-    outs = (lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, L, H)
-    geo = ((i64 * 12)(*q_, *k_, *v_, *g_), (i64 * 3)(*o_), (i64 * 3)(L * H * hd, H * hd, hd),
-           (i64 * 3)(*dv.stride()[:3]), scale, scr, nscr)
+    common = (*ptrs, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, L, H)
+    geo = ((i64 * 12)(*q_, *k_, *v_, *g_), (i64 * 3)(*o_), (i64 * 3)(*row), (i64 * 3)(*dv.stride()[:3]), scale,
+           base + space, nscr)
     fixed, status = int(K.DETERMINISTIC), K.status_word(dev).data_ptr()
     if raw:
-        codes, steps = (None, None) if keep8 is None else keep8._ptrs()
-        K._check(lib.imf_attn_bwd8(q, k, v, o, codes, steps, g, *outs, *geo, fixed, status, stream), "imf_attn_bwd8")
+        K._check(lib.imf_attn_bwd8((ctypes.c_void_p * 8)(*codes[:8]), *common, *geo, fixed, status, stream),
+                 "imf_attn_bwd8")
     else:
-        K._check(lib.imf_attn_bwd(q, k, v, o, g, *outs, hd, *geo, None, None, None, 0, 0, fixed, None, status,
-                                  stream), "imf_attn_bwd")
+        _launch("imf_restore8", recs)
+        K._check(lib.imf_attn_bwd(*common, hd, *geo, None, None, None, 0, 0, fixed, None, status, stream),
+                 "imf_attn_bwd")
     K.LAUNCHES.count += 3
     return dq, dk, dv
