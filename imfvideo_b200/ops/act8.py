@@ -14,9 +14,11 @@ stored.  A group that holds a NaN or an infinity reads as NaN throughout.
     attn_bwd8(q8, k8, v8, o8, lse, go)        # dense attention, probabilities recomputed
 
 ``model.act_store = "int8"`` keeps the activations of the fused blocks this way
-(``ops/block.py``); blocks off the fused path (CPU, fp32) keep theirs as they are.  CPU tensors take the formulas of ``ops/reference.py``.  All launches go to the
-current stream of the tensors' device; workspaces belong to the call.  There is no counterpart in
-the reference, which recomputes blocks instead (reference ``models/imf_dit_video.py:909-972``).
+(``ops/block.py``); blocks off the fused path (CPU, fp32) keep theirs as they are.  These are
+operators of a backward pass: none of them is differentiable.  CPU tensors take the formulas of
+``ops/reference.py``.  All launches go to the current stream of the tensors' device; workspaces
+belong to the call.  There is no counterpart in the reference, which recomputes blocks instead
+(reference ``models/imf_dit_video.py:909-972``).
 """
 
 from __future__ import annotations
@@ -342,6 +344,8 @@ def gemm_wgrad8(dy: Tensor, x8: Packed8, out: Optional[Tensor] = None, accumulat
     ld = dy.stride(0) if rows > 1 else (N + 7) // 8 * 8
     if dy.stride(1) != 1 and N > 1 or ld % 8 or dy.data_ptr() % 16:
         raise ValueError("dy needs adjacent columns and 16-byte aligned rows")
+    if max(rows, N, C) >= 2 ** 31 - 512:
+        raise ValueError(f"gemm_wgrad8: sizes of 2^31 and more ({rows}, {N}, {C})")
     K = _kernels()
     ldo = out.stride(0) if N > 1 else (C + 3) // 4 * 4
     floats = K._lib.imf_wgrad8_work(rows, N, C, int(ldo % 4 == 0 and out.data_ptr() % 16 == 0))
@@ -414,7 +418,7 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
     if 0 in shape:
         new = lambda: _new(shape, BF16, dev)
         return new(), new(), new() if gv_out is None else gv_out
-    scale = hd ** -0.5 if scale is None else scale
+    scale = hd ** -0.5 if scale is None else float(scale)
     if dev.type != "cuda":
         plain = lambda t: t.restore() if isinstance(t, Packed8) else t
         dq, dk, dv = ref.attention_grad(*(plain(t) for t in (q8, k8, v8, o8)), lse, go, scale)

@@ -318,6 +318,18 @@ def test_attention_fixed_order_and_views(A, K):
     _near(A.attn_bwd8(*ps, lse, go, scale=0.05), _oracle(ps, lse, go, 0.05), "scale")
     low = torch.logsumexp(-0.1 * torch.einsum("blhd,bmhd->bhlm", *(p.restore().float() for p in ps[:2])), -1)
     _near(A.attn_bwd8(*ps, low, go, scale=-0.1), _oracle(ps, low, go, -0.1), "a scale below zero")
+    # bf16 v and o that are not laid out for TMA: copied first
+    v, o_ = ps[2].restore(), ps[3].restore()
+    odd = torch.empty(1, 1500, 3, 68, dtype=BF16, device="cuda")[..., 4:]
+    odd.copy_(v)
+    K.set_deterministic(True)
+    try:
+        a = A.attn_bwd8(ps[0], ps[1], v, o_, lse, go)
+        b = A.attn_bwd8(ps[0], ps[1], odd, o_.transpose(1, 3).contiguous().transpose(1, 3), lse, go)
+        c = A.attn_bwd8(*ps, lse, go)
+    finally:
+        K.set_deterministic(was)
+    assert all(torch.equal(x, y) and torch.equal(x, z) for x, y, z in zip(a, b, c))
     flat = torch.full_like(lse, math.log(1500))                          # scale 0: P = 1 / L, dQ = dK = 0
     dq, dk, dv = A.attn_bwd8(*ps, flat, go, scale=0.0)
     assert (dq == 0).all() and (dk == 0).all()
