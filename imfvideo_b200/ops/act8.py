@@ -60,7 +60,7 @@ def _kernels():
         K._lib.imf_wgrad8.restype = ci
         K._lib.imf_wgrad8.argtypes = [vp, i64, vp, vp, ci, ci, ci, vp, i64, ci, vp, i64, vp, vp]
         K._lib.imf_attn_bwd8.restype = ci
-        K._lib.imf_attn_bwd8.argtypes = [vp] * 10 + [ci] * 3 + [vp] * 4 + [cf, vp, cl, ci, vp, vp]
+        K._lib.imf_attn_bwd8.argtypes = [vp] * 10 + [ci] * 4 + [vp] * 4 + [cf, vp, cl, ci, vp, vp]
         K._lib.imf_situ_bwd8.restype = ci
         K._lib.imf_situ_bwd8.argtypes = [vp] * 5 + [cl, ci] + [i64] * 3 + [cf, cf, ci, vp]
         _KERNELS = K
@@ -433,13 +433,13 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
     dv = _new(shape, BF16, dev) if gv_out is None else gv_out
     if dv.stride(3) != 1 or dv.data_ptr() % 16 or any(s % 8 for s in dv.stride()[:3]):
         raise ValueError("attn_bwd8: the dv output needs 16-byte aligned rows")
-    # what is packed gets its values in bf16 in front of the kernel's own scratch.  head_dim 64: the kernel's form for
-    # an exact Q, whose first launch does that too and reads o in 8 bits (its constants are lse / scale)
-    raw = hd == 64 and abs(scale) >= 1e-30
+    # what is packed but o gets its values in bf16 in front of the kernel's own scratch, in the call's first launch.
+    # (head_dim 64 at a scale of zero: the kernel's form for an exact Q divides by it, so the other one runs)
+    first = hd == 128 or abs(scale) >= 1e-30
     n, rows, row = 2 * B * L * H * hd, B * L * H, (L * H * hd, H * hd, hd)
     size = (n + 255) // 256 * 256
     nscr = lib.imf_attn_bwd_scratch_bytes_hd(B, L, H, hd)
-    space = sum(isinstance(t, Packed8) for t in ((q8, k8, v8) if raw else (q8, k8, v8, o8))) * size
+    space = sum(isinstance(t, Packed8) for t in ((q8, k8, v8) if first else (q8, k8, v8, o8))) * size
     work = _new(space + nscr, torch.uint8, dev)
     at = base = work.data_ptr()
     codes, recs, ptrs, strides, hold = [], [], [], [], []
@@ -454,7 +454,7 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
         pair = t._ptrs()
         codes += pair
         strides.append(row)
-        if raw and len(ptrs) == 3:             # o stays as it is
+        if first and len(ptrs) == 3:           # o stays as it is
             ptrs.append(None)
             continue
         recs += (at, *pair, 1, 1, rows, 0, 0, hd, hd, 0)
@@ -462,16 +462,14 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
         at += size
     i64 = ctypes.c_int64
     q_, k_, v_, o_, g_ = strides
-    common = (*ptrs, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, L, H)
-    geo = ((i64 * 12)(*q_, *k_, *v_, *g_), (i64 * 3)(*o_), (i64 * 3)(*row), (i64 * 3)(*dv.stride()[:3]), scale,
-           base + space, nscr)
+    common = (*ptrs, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, L, H, hd,
+              (i64 * 12)(*q_, *k_, *v_, *g_), (i64 * 3)(*o_), (i64 * 3)(*row), (i64 * 3)(*dv.stride()[:3]), scale,
+              base + space, nscr)
     fixed, status = int(K.DETERMINISTIC), K.status_word(dev).data_ptr()
-    if raw:
-        K._check(lib.imf_attn_bwd8((ctypes.c_void_p * 8)(*codes[:8]), *common, *geo, fixed, status, stream),
-                 "imf_attn_bwd8")
+    if first:
+        K._check(lib.imf_attn_bwd8((ctypes.c_void_p * 8)(*codes[:8]), *common, fixed, status, stream), "imf_attn_bwd8")
     else:
         _launch("imf_restore8", recs)
-        K._check(lib.imf_attn_bwd(*common, hd, *geo, None, None, None, 0, 0, fixed, None, status, stream),
-                 "imf_attn_bwd")
+        K._check(lib.imf_attn_bwd(*common, None, None, None, 0, 0, fixed, None, status, stream), "imf_attn_bwd")
     K.LAUNCHES.count += 3
     return dq, dk, dv

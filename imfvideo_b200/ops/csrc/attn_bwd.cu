@@ -49,10 +49,11 @@
 // and V as TMEM operands with P^T over S^T 2.21 ms (the next S^T waits for dV), the two
 // warp groups half a tile apart 3.24 ms.
 #include "attn_bwd128.h"
-#include "act8.cuh"
+#include "attn_bwd8.cuh"
 #include "attn_bwd_split.h"
 #include "common.cuh"
 #include "host_util.h"
+#include <initializer_list>
 
 namespace imf {
 
@@ -691,68 +692,6 @@ __global__ void attn_bwd_prep_kernel(const __nv_bfloat16* __restrict__ q,
   }
 }
 
-// A checkpoint of a (B, L, H, 64) tensor, contiguous rows of 64 codes and 4 step bytes
-struct Bwd8Tensor {
-  const int8_t* codes;
-  const uint8_t* steps;
-  IMF_DEVICE uint4 at(int64_t row, int part) const {
-    return a8_decode8(*reinterpret_cast<const uint2*>(codes + row * 64 + part * 8), a8_step2(steps[row * 4 + part / 4]));
-  }
-};
-// Everything that the kernel of RAW_Q wants from checkpoints, in one launch (short sequences are all launches): the
-// values of q, k and (V8) v in bf16, exact; delta from dO and an O in 8 bits (O8) or bf16; the bands -lse / scale and
-// -delta; and zeros for the dQ additions.  Eight lanes a row, 8-byte accesses to codes and 16-byte ones besides.
-template <bool V8, bool O8>
-__global__ void attn_bwd_prep8_kernel(Bwd8Tensor q8, Bwd8Tensor k8, Bwd8Tensor v8, Bwd8Tensor o8,
-                                      __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ k,
-                                      __nv_bfloat16* __restrict__ v, const __nv_bfloat16* __restrict__ o,
-                                      const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse,
-                                      uint32_t* __restrict__ augq, uint32_t* __restrict__ augd, float* __restrict__ dq_acc,
-                                      int B, int L, int H, int Lp, int64_t o_sb, int64_t o_sl, int64_t o_sh, int64_t g_sb,
-                                      int64_t g_sl, int64_t g_sh, float inv_exp_scale) {
-  const int lane = threadIdx.x & 31, part = lane & 7, c0 = part * 8;
-  const long u = (((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5) * 4 + (lane >> 3);
-  const bool in = u < (long)B * H * Lp;          // no early exit: the shuffles below need every lane
-  int h = 0, l = 0, b = 0;
-  if (in) {
-    h = (int)(u % H);
-    l = (int)((u / H) % Lp);
-    b = (int)(u / ((long)H * Lp));
-  }
-  const bool live = in && l < L;
-  float d = 0.f;
-  if (live) {
-    const int64_t r = ((int64_t)b * L + l) * H + h, at = r * 64 + c0;
-    const uint4 a = O8 ? o8.at(r, part)
-                       : *reinterpret_cast<const uint4*>(o + b * o_sb + (int64_t)l * o_sl + h * o_sh + c0);
-    const uint4 g = *reinterpret_cast<const uint4*>(d_o + b * g_sb + (int64_t)l * g_sl + h * g_sh + c0);
-    *reinterpret_cast<uint4*>(q + at) = q8.at(r, part);
-    *reinterpret_cast<uint4*>(k + at) = k8.at(r, part);
-    if (V8) *reinterpret_cast<uint4*>(v + at) = v8.at(r, part);
-    const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-    reinterpret_cast<float4*>(dq_acc + at)[0] = zero;
-    reinterpret_cast<float4*>(dq_acc + at)[1] = zero;
-    const uint32_t aw[4] = {a.x, a.y, a.z, a.w}, gw[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) d += bf16_lo(aw[i]) * bf16_lo(gw[i]) + bf16_hi(aw[i]) * bf16_hi(gw[i]);
-  }
-#pragma unroll
-  for (int off = 4; off > 0; off >>= 1) d += __shfl_xor_sync(0xffffffffu, d, off);
-  if (!in) return;
-  float x = 30000.f;                             // padding rows: exp2(.. - 30000) = 0
-  if (live) x = fminf(fmaxf(lse[((long)b * H + h) * L + l] * 1.4426950408889634f, -30000.f), 30000.f);
-  x *= inv_exp_scale;
-  uint32_t wq = 0u, wd = 0u;                     // 16 bf16 = 8 words per row, one per lane of the row
-  if (part == 0) {
-    const float xh = bf16_lo(pack_bf16(-x, 0.f)), dh = bf16_lo(pack_bf16(-d, 0.f));
-    wq = pack_bf16(xh, -x - xh);
-    wd = pack_bf16(dh, -d - dh);
-  }
-  const long row = ((long)b * H + h) * Lp + l;
-  augq[row * 8 + part] = wq;
-  augd[row * 8 + part] = wd;
-}
-
 // dq = bf16(acc * scale (+ add)); `add`: an fp32 (B, L, H, 64) gradient from another branch
 __global__ void attn_bwd_post_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq,
                                      long n4, float scale, const float* __restrict__ add) {
@@ -852,13 +791,9 @@ struct Bwd64Args {
   int* status;
   void* stream;
 };
-// checkpoints of q, k and, where given, v and o; q, k (and v) of the call are where their values go
-struct Bwd64Packed {
-  Bwd8Tensor q, k, v, o;
-};
 
 // packed: see RAW_Q (dense only)
-static int bwd64_launch(const Bwd64Args& a, const Bwd64Packed* packed) {
+static int bwd64_launch(const Bwd64Args& a, const Bwd8Packed* packed) {
   const bool raw = packed != nullptr;
   const int B = a.B, L = a.L, H = a.H;
   const int64_t *strides = a.strides, *o_strides = a.o_strides, *dk_strides = a.dk_strides, *dv_strides = a.dv_strides;
@@ -903,17 +838,8 @@ static int bwd64_launch(const Bwd64Args& a, const Bwd64Packed* packed) {
     return IMF_ERR_LAUNCH;
   }
   if (raw) {
-    const long rows = (long)B * H * Lp, blocks = ((rows + 3) / 4 * 32 + 255) / 256;
-    const bool v8 = packed->v.codes != nullptr, o8 = packed->o.codes != nullptr;
-    auto prep = v8 ? (o8 ? attn_bwd_prep8_kernel<true, true> : attn_bwd_prep8_kernel<true, false>)
-                   : (o8 ? attn_bwd_prep8_kernel<false, true> : attn_bwd_prep8_kernel<false, false>);
-    typedef __nv_bfloat16 bf;
-    prep<<<(unsigned)blocks, 256, 0, st>>>(
-        packed->q, packed->k, packed->v, packed->o, static_cast<bf*>(const_cast<void*>(q)),
-        static_cast<bf*>(const_cast<void*>(k)), static_cast<bf*>(const_cast<void*>(v)), static_cast<const bf*>(o),
-        static_cast<const bf*>(d_o), lse, augq, augd, dq_acc, B, L, H, Lp, o_strides[0], o_strides[1], o_strides[2],
-        strides[9], strides[10], strides[11], 1.f / (scale * 1.4426950408889634f));
-    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
+    const Bwd8Rows r{q, k, v, o, d_o, lse, dq_acc, B, L, H, Lp, o_strides, strides + 9};
+    if (attn_bwd_prep8<64>(*packed, r, augq, augd, 1.f / (scale * 1.4426950408889634f), st) != IMF_OK) return IMF_ERR_LAUNCH;
   } else {
     const long rows = (long)B * H * Lp;
     const int threads = 256;
@@ -1024,24 +950,27 @@ extern "C" int imf_attn_bwd(const void* q, const void* k, const void* v, const v
     Bwd128Args a{q, k, v, o, d_o, lse, dq, dk, dv, B, L, H, strides, o_strides, dk_strides,
                  dv_strides, scale, scratch, scratch_bytes, status, stream,
                  fixed_order && status != nullptr};
-    return attn_bwd128_launch(a);
+    return attn_bwd128_launch(a, nullptr);
   }
   Bwd64Args a{q, k, v, o, d_o, lse, dq, dk, dv, B, L, H, strides, o_strides, dk_strides, dv_strides,
               scale, scratch, scratch_bytes, qlist, qflags, qrank, qmax, qpairs, fixed_order, dq_add, status, stream};
   return bwd64_launch(a, nullptr);
 }
 
-// head_dim 64 from checkpoints: packed[0..7] = codes and steps of q, k, v, o ((B L H, 64) bytes, (B L H, 4) bytes; v and
-// o may be null: then they come in bf16, with strides[6..8] and o_strides).  q, k and a packed v get their values here,
-// contiguous bf16 (strides[0..8] say so).  As above otherwise; o and d_o have 16-byte aligned rows, and |scale| is at
-// least 1e-30 (the constants carry lse / scale).
+// From checkpoints: packed[0..7] = codes and steps of q, k, v, o ((B L H, head_dim) bytes, (B L H, 4) bytes; v and o may
+// be null: then they come in bf16, with strides[6..8] and o_strides).  q, k and a packed v get their values here,
+// contiguous bf16 (strides[0..8] say so).  As above otherwise; o and d_o have 16-byte aligned rows; head_dim 64:
+// |scale| is at least 1e-30 (the constants carry lse / scale).
 extern "C" int imf_attn_bwd8(const void* const* packed, void* q, void* k, const void* v, const void* o, const void* d_o,
-                             const float* lse, void* dq, void* dk, void* dv, int B, int L, int H, const int64_t* strides,
-                             const int64_t* o_strides, const int64_t* dk_strides, const int64_t* dv_strides, float scale,
-                             void* scratch, long scratch_bytes, int fixed_order, int* status, void* stream) {
+                             const float* lse, void* dq, void* dk, void* dv, int B, int L, int H, int head_dim,
+                             const int64_t* strides, const int64_t* o_strides, const int64_t* dk_strides,
+                             const int64_t* dv_strides, float scale, void* scratch, long scratch_bytes, int fixed_order,
+                             int* status, void* stream) {
   using namespace imf;
-  if (B <= 0 || L <= 0 || H <= 0 || !(fabsf(scale) >= 1e-30f) || !q || !k || !v || (!o && !packed[6])) return IMF_ERR_ARG;
-  Bwd64Packed pk;
+  if ((head_dim != BW_HD && head_dim != 128) || B <= 0 || L <= 0 || H <= 0 || !q || !k || !v || (!o && !packed[6]))
+    return IMF_ERR_ARG;
+  if (head_dim == BW_HD && !(fabsf(scale) >= 1e-30f)) return IMF_ERR_ARG;
+  Bwd8Packed pk;
   Bwd8Tensor* const t[4] = {&pk.q, &pk.k, &pk.v, &pk.o};
   for (int i = 0; i < 4; ++i) {
     t[i]->codes = static_cast<const int8_t*>(packed[2 * i]);
@@ -1049,15 +978,19 @@ extern "C" int imf_attn_bwd8(const void* const* packed, void* q, void* k, const 
     if ((i < 2 && !t[i]->codes) || (t[i]->codes && !t[i]->steps) || (reinterpret_cast<uintptr_t>(t[i]->codes) & 15))
       return IMF_ERR_ARG;
   }
-  if ((reinterpret_cast<uintptr_t>(q) & 15) || (reinterpret_cast<uintptr_t>(k) & 15) ||
-      (reinterpret_cast<uintptr_t>(v) & 15) || (reinterpret_cast<uintptr_t>(o) & 15) ||
-      (reinterpret_cast<uintptr_t>(d_o) & 15))
-    return IMF_ERR_ARG;
-  const int64_t row[3] = {(int64_t)L * H * 64, (int64_t)H * 64, 64};
+  for (const void* p : {(const void*)q, (const void*)k, v, o, d_o, (const void*)dq, (const void*)dk, (const void*)dv})
+    if (reinterpret_cast<uintptr_t>(p) & 15) return IMF_ERR_ARG;
+  if (reinterpret_cast<uintptr_t>(scratch) & 255) return IMF_ERR_ARG;
+  const int64_t row[3] = {(int64_t)L * H * head_dim, (int64_t)H * head_dim, head_dim};
   for (int i = 0; i < 3; ++i)
     if ((!packed[6] && (o_strides[i] & 7)) || (strides[9 + i] & 7) || strides[i] != row[i] || strides[3 + i] != row[i] ||
-        (packed[4] && strides[6 + i] != row[i]))
+        (packed[4] && strides[6 + i] != row[i]) || (dk_strides[i] & 7) || (dv_strides[i] & 7))
       return IMF_ERR_ARG;
+  if (head_dim == 128) {
+    Bwd128Args a{q, k, v, o, d_o, lse, dq, dk, dv, B, L, H, strides, o_strides, dk_strides, dv_strides, scale, scratch,
+                 scratch_bytes, status, stream, fixed_order && status != nullptr};
+    return attn_bwd128_launch(a, &pk);
+  }
   Bwd64Args a{q, k, v, o, d_o, lse, dq, dk, dv, B, L, H, strides, o_strides, dk_strides, dv_strides, scale, scratch,
               scratch_bytes, nullptr, nullptr, nullptr, 0, 0, fixed_order, nullptr, status, stream};
   return bwd64_launch(a, &pk);

@@ -23,6 +23,7 @@
 // issuer; warp 13: TMA producer.  S^T / dP^T of tile i+1 are issued as soon as
 // tile i has been pulled into registers.
 #include "attn_bwd128.h"
+#include "attn_bwd8.cuh"
 #include "attn_bwd_split.h"
 #include "common.cuh"
 #include "host_util.h"
@@ -523,7 +524,7 @@ long attn_bwd128_scratch_bytes(int B, int L, int H) {
   return (long)B * L * H * b128::HD * 4 + turns + 2 * (long)B * H * Lp * 4 + 512 + part;
 }
 
-int attn_bwd128_launch(const Bwd128Args& a) {
+int attn_bwd128_launch(const Bwd128Args& a, const Bwd8Packed* packed) {
   using namespace b128;
   const int B = a.B, L = a.L, H = a.H;
   if (a.scratch == nullptr || a.scratch_bytes < attn_bwd128_scratch_bytes(B, L, H)) return IMF_ERR_ARG;
@@ -538,8 +539,12 @@ int attn_bwd128_launch(const Bwd128Args& a) {
   float* delta = lse2 + (size_t)B * H * Lp;
   const BwdSplit sp = split_for(B, L, H);
   const uintptr_t end = (reinterpret_cast<uintptr_t>(delta + (size_t)B * H * Lp) + 255) & ~uintptr_t(255);
-  if (cudaMemsetAsync(dq_acc, 0, acc_bytes + turn_bytes, st) != cudaSuccess) return IMF_ERR_LAUNCH;
-  {
+  if (packed) {
+    if (a.fixed_order && cudaMemsetAsync(turn, 0, turn_bytes, st) != cudaSuccess) return IMF_ERR_LAUNCH;
+    const Bwd8Rows r{a.q, a.k, a.v, a.o, a.d_o, a.lse, dq_acc, B, L, H, Lp, a.o_strides, a.strides + 9};
+    if (attn_bwd_prep8<128>(*packed, r, lse2, delta, 0.f, st) != IMF_OK) return IMF_ERR_LAUNCH;
+  } else {
+    if (cudaMemsetAsync(dq_acc, 0, acc_bytes + turn_bytes, st) != cudaSuccess) return IMF_ERR_LAUNCH;
     const long warps = (long)B * H * Lp;
     const int threads = 256;
     const long blocks = (warps * 32 + threads - 1) / threads;

@@ -23,6 +23,8 @@ struct Bwd128Args {
 };
 
 long attn_bwd128_scratch_bytes(int B, int L, int H);
-int attn_bwd128_launch(const Bwd128Args& a);
+struct Bwd8Packed;
+// packed: checkpoints that q, k (and v) get their values from, or null
+int attn_bwd128_launch(const Bwd128Args& a, const Bwd8Packed* packed);
 
 }  // namespace imf

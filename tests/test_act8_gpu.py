@@ -301,9 +301,10 @@ def test_attention_of_one_token(A, K, hd):
     assert (dk.double().abs() <= size * q.abs() * 1.2 + 1e-12).all()
 
 
-def test_attention_fixed_order_and_views(A, K):
-    ps, lse, go, o = _attention(A, K, 1, 1500, 3, 64, 21)
-    wide = torch.empty(1, 1500, 3, 96, dtype=BF16, device="cuda")
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_fixed_order_and_views(A, K, hd):
+    ps, lse, go, o = _attention(A, K, 1, 1500, 3, hd, 21)
+    wide = torch.empty(1, 1500, 3, hd + 32, dtype=BF16, device="cuda")
     wide[..., 32:] = go
     was = K.DETERMINISTIC
     try:
@@ -320,7 +321,7 @@ def test_attention_fixed_order_and_views(A, K):
     _near(A.attn_bwd8(*ps, low, go, scale=-0.1), _oracle(ps, low, go, -0.1), "a scale below zero")
     # bf16 v and o that are not laid out for TMA: copied first
     v, o_ = ps[2].restore(), ps[3].restore()
-    odd = torch.empty(1, 1500, 3, 68, dtype=BF16, device="cuda")[..., 4:]
+    odd = torch.empty(1, 1500, 3, hd + 4, dtype=BF16, device="cuda")[..., 4:]
     odd.copy_(v)
     K.set_deterministic(True)
     try:
@@ -334,7 +335,7 @@ def test_attention_fixed_order_and_views(A, K):
     dq, dk, dv = A.attn_bwd8(*ps, flat, go, scale=0.0)
     assert (dq == 0).all() and (dk == 0).all()
     _near((dv,), _oracle(ps, flat, go, 0.0)[2:], "a scale of zero")
-    none = torch.empty(0, 5, 2, 64, dtype=BF16, device="cuda")
+    none = torch.empty(0, 5, 2, hd, dtype=BF16, device="cuda")
     assert A.attn_bwd8(*A.store8([none] * 4), torch.empty(0, 2, 5, device="cuda"), none)[0].shape == none.shape
     with pytest.raises(ValueError):
         A.attn_bwd8(*ps, lse.transpose(1, 2).contiguous().transpose(1, 2), go)
