@@ -56,7 +56,7 @@ def _kernels():
             getattr(K._lib, name).restype = ci
             getattr(K._lib, name).argtypes = [vp, ci, vp]
         K._lib.imf_wgrad8_work.restype = i64
-        K._lib.imf_wgrad8_work.argtypes = [ci] * 4
+        K._lib.imf_wgrad8_work.argtypes = [ci] * 3 + [vp, i64]
         K._lib.imf_wgrad8.restype = ci
         K._lib.imf_wgrad8.argtypes = [vp, i64, vp, vp, ci, ci, ci, vp, i64, ci, vp, i64, vp, vp]
         K._lib.imf_attn_bwd8.restype = ci
@@ -348,7 +348,7 @@ def gemm_wgrad8(dy: Tensor, x8: Packed8, out: Optional[Tensor] = None, accumulat
         raise ValueError(f"gemm_wgrad8: sizes of 2^31 and more ({rows}, {N}, {C})")
     K = _kernels()
     ldo = out.stride(0) if N > 1 else (C + 3) // 4 * 4
-    floats = K._lib.imf_wgrad8_work(rows, N, C, int(ldo % 4 == 0 and out.data_ptr() % 16 == 0))
+    floats = K._lib.imf_wgrad8_work(rows, N, C, out.data_ptr(), ldo)
     work = _new(floats, F32, dev) if floats else None
     codes, steps = x8._ptrs()
     K._check(K._lib.imf_wgrad8(dy.data_ptr(), ld, codes, steps, rows, N, C, out.data_ptr(), ldo, int(accumulate),

@@ -472,12 +472,18 @@ static int64_t plane_floats(int N, int C) { return (int64_t)N * (((int64_t)C + 3
 }  // namespace w8
 }  // namespace imf
 
-// Floats of workspace that imf_wgrad8 wants.  `direct`: the result's address and row pitch are 16-byte multiples.
-extern "C" int64_t imf_wgrad8_work(int R, int N, int C, int direct) {
+// Whether TMA may write a result in place: 16-byte rows, and a width of whole 16 bytes, for it writes those of the last
+// columns whole (what lies behind a band's 738 columns was overwritten up to 740).
+static bool in_place(const float* out, int64_t ldo, int C) {
+  return (ldo & 3) == 0 && (C & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+}
+
+// Floats of workspace that imf_wgrad8 wants for these sizes and this result.
+extern "C" int64_t imf_wgrad8_work(int R, int N, int C, const float* out, int64_t ldo) {
   using namespace imf;
   if (R <= 0 || N <= 0 || C <= 0) return 0;
   const w8::Plan pl = w8::plan(R, N, C, w8::sm_count());
-  return pl.splits > 1 || !direct ? pl.splits * w8::plane_floats(N, C) : 0;
+  return pl.splits > 1 || !in_place(out, ldo, C) ? pl.splits * w8::plane_floats(N, C) : 0;
 }
 
 extern "C" int imf_splitk_reduce_ld(const float* partial, int splits, int M, int N, int64_t ldp, int64_t plane, float* out,
@@ -493,7 +499,7 @@ extern "C" int imf_wgrad8(const void* dy, int64_t ld_dy, const void* codes, cons
   if ((reinterpret_cast<uintptr_t>(codes) & 15u) || (reinterpret_cast<uintptr_t>(steps) & 3u)) return IMF_ERR_ARG;
   const w8::Plan pl = w8::plan(R, N, C, w8::sm_count());
   if ((int64_t)((N + 255) / 256) * ((C + pl.bn - 1) / pl.bn) * pl.splits > 0x7fffffff) return IMF_ERR_TOO_LARGE;
-  const bool direct = pl.splits == 1 && (ldo & 3) == 0 && (reinterpret_cast<uintptr_t>(out) & 15u) == 0;
+  const bool direct = pl.splits == 1 && in_place(out, ldo, C);
   const int64_t plane = w8::plane_floats(N, C), cp = plane / N;
   if (!direct && (!work || work_floats < pl.splits * plane || (reinterpret_cast<uintptr_t>(work) & 15u)))
     return IMF_ERR_ARG;

@@ -195,6 +195,21 @@ def test_weight_gradient_views(A, K):
     K.check_status()
 
 
+@pytest.mark.parametrize("rows,N,C", [(1, 406, 78), (63, 607, 738), (129, 82, 625), (127, 338, 486), (700, 40, 99)])
+@pytest.mark.parametrize("accumulate", [False, True])
+def test_weight_gradient_leaves_what_is_beside_it(A, K, rows, N, C, accumulate):
+    """Widths that are no whole 16 bytes, in front of a wider buffer's other columns and rows."""
+    g = _gen(13)
+    dy, p = _randn(g, rows, (N + 7) // 8 * 8)[:, :N], A.store8(_randn(g, rows, C))
+    for pitch in (C + 1, (C + 3) // 4 * 4, (C + 7) // 4 * 4):
+        buf = torch.randn(N + 2, pitch, device="cuda", generator=g)
+        was = buf.clone()
+        A.gemm_wgrad8(dy, p, out=buf[:N, :C], accumulate=accumulate)
+        _wgrad_check(buf[:N, :C], dy, p, was[:N, :C] if accumulate else None)
+        assert torch.equal(buf[:N, C:], was[:N, C:]) and torch.equal(buf[N:], was[N:])
+    K.check_status()
+
+
 def test_weight_gradient_bad_values(A, K):
     """A group with an infinity makes NaN of its own 32 columns, an infinity of dY of its own row."""
     g = _gen(12)
