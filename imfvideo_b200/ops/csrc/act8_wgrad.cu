@@ -24,12 +24,15 @@
 // What bounds it: the way into shared memory.  TMA takes about three clocks for a box row of 128 bytes, so a
 // k-block of 128 rows of dY^T and 128 columns of codes (BN 256) takes 600 clocks alone and 820 with all SMs reading,
 // against 512 of tcgen05.mma; with BN 512 (two accumulators share the rows of dY^T) 1,570 against 1,024.
-// 32,780 rows x 5,472 x 1,024: 315 us (1,166 TFLOP/s) with BN 512, 381 with 256; one CTA per tile 372 (256 x
-// 256) to 620 us (128 x 256), conversion included; restoring X to bf16 first and the bf16 kernel of gemm.cu 428.
-// 29,140 x 1,376 x 256: 39 us, the bf16 kernel alone 45.  Tried and slower: codes loaded into registers by the
-// converting warps (594 us at 5,472 x 1,024: the proxy fence waits for the loads), remote arrivals and
-// waits with cluster scope (627 us: the release waits for everything the thread has in flight), the k-blocks of
-// all tiles dealt to the pairs in equal runs (356 us: pairs at different rows share nothing in L2).
+// 32,780 rows x 5,472 x 1,024: 334 us (1,100 TFLOP/s) with BN 512, 381 with 256; without chains 315, and then one CTA
+// per tile 372 (256 x 256) to 620 us (128 x 256); restoring X to bf16 first and the bf16 kernel of gemm.cu 428.
+// 29,140 x 1,376 x 256: 37 us, the bf16 kernel alone 45.  Tried and slower: codes loaded into registers by the
+// converting warps (594 us at 5,472 x 1,024: the proxy fence waits for the loads) or by cp.async of the loading
+// warp (463; no difference at 1,376 x 256); remote arrivals and
+// waits with cluster scope (627 us: the release waits for everything the thread has in flight); the k-blocks of
+// all tiles dealt to the pairs in equal runs (356 us: pairs at different rows share nothing in L2); sums added from
+// registers, eight lanes a line (362 instead of 338 by TMA).  Chains that end at other times in other
+// pairs gain 0.6 %.
 #include "act8.cuh"
 #include "common.cuh"
 #include "host_util.h"
