@@ -342,8 +342,8 @@ def gemm_wgrad8(dy: Tensor, x8: Packed8, out: Optional[Tensor] = None, accumulat
             return gemm_wgrad8(dy, x8, out, accumulate)
     rows = x8.rows
     ld = dy.stride(0) if rows > 1 else (N + 7) // 8 * 8
-    if dy.stride(1) != 1 and N > 1 or ld % 8 or dy.data_ptr() % 16:
-        raise ValueError("dy needs adjacent columns and 16-byte aligned rows")
+    if dy.stride(1) != 1 and N > 1 or ld % 8 or ld < N or dy.data_ptr() % 16:
+        raise ValueError("dy needs adjacent columns and 16-byte aligned rows that do not overlap")
     if max(rows, N, C) >= 2 ** 31 - 512:
         raise ValueError(f"gemm_wgrad8: sizes of 2^31 and more ({rows}, {N}, {C})")
     K = _kernels()
@@ -431,8 +431,8 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
     lib, stream = K._lib, K._stream()
     dq, dk = _new(shape, BF16, dev), _new(shape, BF16, dev)
     dv = _new(shape, BF16, dev) if gv_out is None else gv_out
-    if dv.stride(3) != 1 or dv.data_ptr() % 16 or any(s % 8 for s in dv.stride()[:3]):
-        raise ValueError("attn_bwd8: the dv output needs 16-byte aligned rows")
+    if dv.stride(3) != 1 or dv.data_ptr() % 16 or any(s % 8 or s == 0 and n > 1 for n, s in zip(shape[:3], dv.stride())):
+        raise ValueError("attn_bwd8: the dv output needs 16-byte aligned rows, no two of them in one place")
     # what is packed but o gets its values in bf16 in front of the kernel's own scratch, in the call's first launch.
     # (head_dim 64 at a scale of zero: the kernel's form for an exact Q divides by it, so the other one runs)
     first = hd == 128 or abs(scale) >= 1e-30
@@ -446,7 +446,9 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
     for t in (q8, k8, v8, o8, go):
         if not isinstance(t, Packed8):
             t = K._tma_ok(t)
-            strides.append(t.stride()[:3])
+            if 0 in t.stride():                # a broadcast gradient, shared heads
+                t = t.contiguous()
+            strides.append(row if t.is_contiguous() else t.stride()[:3])
             ptrs.append(t.data_ptr())
             hold.append(t)                     # a copy lives until the launch
             codes += (None, None)

@@ -357,6 +357,31 @@ def test_attention_fixed_order_and_views(A, K, hd):
     K.check_status()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("B", [1, 2])
+def test_attention_of_broadcast_tensors(A, K, hd, B):
+    """Output gradients that are one row for all (of a mean), V and O shared by the heads: as their copies."""
+    g, (L, H) = _gen(31), (150, 3)
+    q8, k8 = A.store8([_randn(g, B, L, H, hd), _randn(g, B, L, H, hd)])
+    lse = torch.full((B, H, L), math.log(L) + 1.0, device="cuda")
+    v, o = (_randn(g, B, L, 1, hd).expand(B, L, H, hd) for _ in range(2))
+    was = K.DETERMINISTIC
+    K.set_deterministic(True)
+    try:
+        for go in (_randn(g, B, 1, H, hd), _randn(g, 1, 1, 1, hd), _randn(g, 1, L, H, hd)):
+            go = go.expand(B, L, H, hd)
+            a = A.attn_bwd8(q8, k8, v, o, lse, go)
+            b = A.attn_bwd8(q8, k8, v.contiguous(), o.contiguous(), lse, go.contiguous())
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+        with pytest.raises(ValueError):
+            A.attn_bwd8(q8, k8, v, o, lse, go, gv_out=torch.empty(B, 1, H, hd, dtype=BF16, device="cuda").expand(B, L, H, hd))
+    finally:
+        K.set_deterministic(was)
+    with pytest.raises(ValueError):
+        A.gemm_wgrad8(_randn(g, 1, 64).expand(96, 64), A.store8(_randn(g, 96, 40)))
+    K.check_status()
+
+
 def test_attention_gradient_is_a_difference_quotient(A, K):
     """Along a random direction of q, k and v the loss changes as the gradients say (64-bit differences)."""
     B, L, H, hd = 1, 40, 2, 64
