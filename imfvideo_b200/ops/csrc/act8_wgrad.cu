@@ -9,9 +9,11 @@
 //
 // Two CTAs (a cluster) share a 256 (N) x BN (C) tile and its products (cta_group::2): each holds 128 of the
 // rows of dY^T and half of X's columns, so each converts half a tile for 256 rows of products.  k-blocks are
-// 64 rows of R.  Warps 0-3: epilogue; warp 4: loads (dY and codes by TMA, the steps by cp.async: their rows
-// are no 16-byte multiples); warp 5 of the first CTA: tcgen05.mma; then CONV groups of warps that convert a
-// k-block each.  R is cut into slices (split-K) where that fills the SMs; a second kernel adds their planes up
+// 64 rows of R.  Warps 0-3: epilogue; warp 4: loads of dY; warp 5: tcgen05.mma in the first CTA, word of the
+// other's dY in the second; warp 6: loads of the codes (TMA) and steps (cp.async: their rows
+// are no 16-byte multiples); then CONV groups of warps that convert a k-block each.  dY and the codes have rings
+// of their own: dY's stages wait for products alone, those of the codes for the conversion.
+// R is cut into slices (split-K) where that fills the SMs; a second kernel adds their planes up
 // in a fixed order, so results repeat bit for bit.
 //
 // The tensor core's fp32 accumulator drops bits with every k-step, more the longer the chain (of the result's norm,
@@ -21,15 +23,18 @@
 // fixed).  Storing a chain's sum runs under the next one's products where TMEM holds two accumulators; with BN 512
 // it holds one, whose halves are stored and begun again one after the other, at some 4 us a chain.
 //
-// What bounds it: the way into shared memory.  TMA takes about three clocks for a box row of 128 bytes, so a
-// k-block of 128 rows of dY^T and 128 columns of codes (BN 256) takes 600 clocks alone and 820 with all SMs reading,
-// against 512 of tcgen05.mma; with BN 512 (two accumulators share the rows of dY^T) 1,570 against 1,024.
-// 32,780 rows x 5,472 x 1,024: 334 us (1,100 TFLOP/s) with BN 512, 381 with 256; without chains 315, and then one CTA
+// What bounds it: shared memory.  For a k-block of BN 256 a CTA moves 24 KB in by TMA, 24 KB through the conversion and
+// 32 KB into the tensor core, 640 clocks at 128 bytes against 512 of tcgen05.mma (BN 512, whose two accumulators
+// share the rows of dY^T: 1,152 against 1,024); 900 and 1,230 are measured.  Without the converted tile's stores it
+// would take 12 % less, without three of four products 6 %; rings of five or seven stages make no difference.
+// 32,780 rows x 5,472 x 1,024: 328 us (1,120 TFLOP/s) with BN 512, 381 with 256; without chains 310, and then one CTA
 // per tile 372 (256 x 256) to 620 us (128 x 256); restoring X to bf16 first and the bf16 kernel of gemm.cu 428.
-// 29,140 x 1,376 x 256: 37 us, the bf16 kernel alone 45.  Tried and slower: codes loaded into registers by the
-// converting warps (594 us at 5,472 x 1,024: the proxy fence waits for the loads) or by cp.async of the loading
-// warp (463; no difference at 1,376 x 256); remote arrivals and
-// waits with cluster scope (627 us: the release waits for everything the thread has in flight); the k-blocks of
+// 29,140 x 1,376 x 256: 36 us, the bf16 kernel alone 45.  One ring and one loading warp for dY, codes and steps took 2 to 6
+// % longer (its instructions, 730 clocks a k-block, were the pace).  Tried and slower: codes loaded into registers
+// by the converting warps (594 us at 5,472 x 1,024: the proxy fence waits for the loads) or by cp.async
+// (463; no difference at 1,376 x 256); remote arrivals and
+// waits with cluster scope (627 us: the release waits for everything the thread has in flight); one barrier for dY
+// and the converted tile (2 to 4 %); more polls before the clock is read (2 %), or fewer; the k-blocks of
 // all tiles dealt to the pairs in equal runs (356 us: pairs at different rows share nothing in L2); sums added from
 // registers, eight lanes a line (362 instead of 338 by TMA).  Chains that end at other times in other
 // pairs gain 0.6 %.
@@ -50,7 +55,7 @@ struct Smem {
   static constexpr int STAGES = BN == 512 ? 4 : BN == 256 ? 6 : 8;
   static constexpr int CONV = BN == 512 ? 2 : 3;     // converted tiles in flight, one group of warps each
   static constexpr int GROUP_WARPS = BN == 512 ? 8 : 4;
-  static constexpr int THREADS = (6 + CONV * GROUP_WARPS) * 32;
+  static constexpr int THREADS = (7 + CONV * GROUP_WARPS) * 32;
   static constexpr int CHAIN = BN == 512 ? 44 : 20;  // k-blocks that one chain of accumulations runs over at most
   static constexpr int WORDS = BNL > 128 ? 2 : 1;    // 4-byte words of steps per row
   alignas(1024) uint8_t a[STAGES][BM * BK * 2];      // dY: two panels [64 rows][128 bytes], swizzled
@@ -58,7 +63,8 @@ struct Smem {
   alignas(1024) uint8_t c[4][2][32 * 128];           // per epilogue warp: 32 rows x 32 fp32, swizzled, twice
   alignas(1024) uint8_t b8[STAGES][BK * BNL];        // codes [64 rows][BNL]
   alignas(16) uint8_t st[STAGES][BK * 4 * WORDS];    // step bytes [64 rows][4 WORDS]
-  uint64_t full[STAGES], empty[STAGES], conv_full[CONV], conv_empty[CONV], acc_full[2], acc_empty[2];
+  uint64_t full_a[STAGES], empty_a[STAGES], full_8[STAGES], empty_8[STAGES];
+  uint64_t conv_full[CONV], conv_empty[CONV], acc_full[2], acc_empty[2];
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -115,6 +121,13 @@ IMF_DEVICE void tma_reduce_add_3d(const CUtensorMap* m, const void* src, int c0,
 // all but the newest bulk store have read their source
 IMF_DEVICE void tma_store_wait_read1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 
+// given up after `it` k-blocks: see the copies in flight land (bounded)
+IMF_DEVICE void see_landed(uint64_t* full, uint32_t stages, uint32_t it) {
+  for (uint32_t j = it < stages ? 0 : it - stages; j < it; ++j)
+    for (int spin = 0; spin < 100000 && !mbar_test(&full[j % stages], (j / stages) & 1); ++spin) {
+    }
+}
+
 // ---- the pair of CTAs
 IMF_DEVICE uint32_t cluster_rank() {
   uint32_t r;
@@ -168,8 +181,10 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(&s.full[i], 1 + 32);                 // the bytes' announcement, and each lane's step bytes
-      mbar_init(&s.empty[i], 1);
+      mbar_init(&s.full_8[i], 1 + 32);               // the bytes' announcement, and each lane's step bytes
+      mbar_init(&s.empty_8[i], GROUP_WARPS);
+      mbar_init(&s.full_a[i], rank == 0 ? 2 : 1);    // the bytes' announcement; in the first CTA: the other has its own
+      mbar_init(&s.empty_a[i], 1);
     }
     for (int i = 0; i < CONV; ++i) {
       mbar_init(&s.conv_full[i], 2 * GROUP_WARPS);   // one arrival per warp of the group, from both CTAs
@@ -200,30 +215,43 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   const auto n_of = [&](int tile) { return tile % p.n_c * BN; };
 
   if (warp == 4) {
-    // ------------------------------------------------------------- loads --
-    if (lane == 0) {
+    // ---------------------------------------------------------------- dY --
+    if (elect_one()) {
       prefetch_tmap(&tm_a);
-      prefetch_tmap(&tm_b);
       prefetch_tmap(&tm_c);
+      uint32_t it = 0;
+      bool ok = true;
+      while (ok && walk.next(w)) {
+        const int m0 = m_of(w.tile);
+        for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
+          const int st = it % STAGES, k0 = kb * BK;
+          if (it >= STAGES)
+            ok = mbar_wait(&s.empty_a[st], ((it / STAGES) & 1) ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&s.full_a[st], BM * BK * 2);
+          tma_load_2d(s.a[st], &tm_a, &s.full_a[st], m0, k0);
+          tma_load_2d(s.a[st] + BK * 128, &tm_a, &s.full_a[st], m0 + 64, k0);
+        }
+      }
+      if (!ok) see_landed(s.full_a, STAGES, it);
     }
-    constexpr uint32_t bytes = BM * BK * 2 + BK * BNL;
+  } else if (warp == 6) {
+    // --------------------------------------------------- codes and steps --
+    if (lane == 0) prefetch_tmap(&tm_b);
     uint32_t it = 0;
     bool ok = true;
     while (ok && walk.next(w)) {
-      const int m0 = m_of(w.tile), n0 = n_of(w.tile) + rank * BNL;
+      const int n0 = n_of(w.tile) + rank * BNL;
       const int64_t g = n0 / 128 * 4;                // the word with the steps of these columns
       for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
-        const int st = it % STAGES;
+        const int st = it % STAGES, k0 = kb * BK;
         if (it >= STAGES)
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.empty[st], ((it / STAGES) & 1) ^ 1, abort_flag, p.status,
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.empty_8[st], ((it / STAGES) & 1) ^ 1, abort_flag, p.status,
                                                     STATUS_TIMEOUT_EMPTY));
         if (!ok) break;
-        const int k0 = kb * BK;
         if (lane == 0) {
-          mbar_arrive_expect_tx(&s.full[st], bytes);
-          tma_load_2d(s.b8[st], &tm_b, &s.full[st], n0, k0);
-          tma_load_2d(s.a[st], &tm_a, &s.full[st], m0, k0);
-          tma_load_2d(s.a[st] + BK * 128, &tm_a, &s.full[st], m0 + 64, k0);
+          mbar_arrive_expect_tx(&s.full_8[st], BK * BNL);
+          tma_load_2d(s.b8[st], &tm_b, &s.full_8[st], n0, k0);
         }
 #pragma unroll
         for (int i = 0; i < 2 * WORDS; ++i) {        // rows and words past the end: zeros, nothing is read
@@ -232,17 +260,25 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           cp_async4(s.st[st] + (r * WORDS + w4) * 4, in ? p.steps + (int64_t)(k0 + r) * p.spitch + g + 4 * w4 : p.steps,
                     in);
         }
-        cp_async_arrive(&s.full[st]);
+        cp_async_arrive(&s.full_8[st]);
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-    if (!ok)                                         // given up: see the copies in flight land (bounded)
-      for (uint32_t j = it < STAGES ? 0 : it - STAGES; j < it; ++j)
-        for (int spin = 0; spin < 100000 && !mbar_test(&s.full[j % STAGES], (j / STAGES) & 1); ++spin) {
+    if (!ok) see_landed(s.full_8, STAGES, it);
+  } else if (warp == 5 && rank == 1) {
+    // ------------------------------------ tells the first CTA of its dY --
+    if (elect_one()) {
+      uint32_t it = 0;
+      bool ok = true;
+      while (ok && walk.next(w))
+        for (int kb = w.kb0; kb < w.kb1 && ok; ++kb, ++it) {
+          ok = mbar_wait(&s.full_a[it % STAGES], (it / STAGES) & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA);
+          if (ok) arrive_first(&s.full_a[it % STAGES]);
         }
+    }
   } else if (warp == 5) {
     // --------------------------------------------------------------- MMA --
-    if (rank == 0 && elect_one()) {
+    if (elect_one()) {
       constexpr uint32_t idesc = idesc_bf16(2 * BM, PN, 1, 1);
       uint32_t it = 0, ch = 0;                       // k-blocks and chains so far
       bool ok = true;
@@ -250,9 +286,9 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
         for (int c0 = w.kb0; c0 < w.kb1 && ok; c0 += p.chain, ++ch) {
           const int c1 = min(c0 + p.chain, w.kb1);
           for (int kb = c0; kb < c1; ++kb, ++it) {
-            // a group's arrival says that its CTA's dY is there too
             const int st = it % STAGES, cs = it % CONV;
-            ok = mbar_wait(&s.conv_full[cs], (it / CONV) & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA);
+            ok = mbar_wait(&s.full_a[st], (it / STAGES) & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA) &&
+                 mbar_wait(&s.conv_full[cs], (it / CONV) & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA);
             if (!ok) break;
             const uint32_t a_base = smem_u32(s.a[st]), b_base = smem_u32(s.b[cs]);
 #pragma unroll
@@ -272,12 +308,12 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
             }
             if (!ok) break;
             commit_both(&s.conv_empty[cs]);
-            commit_both(&s.empty[st]);               // the codes were read before conv_full
+            commit_both(&s.empty_a[st]);
           }
         }
       }
     }
-  } else if (warp >= 6) {
+  } else if (warp >= 7) {
     // -------------------------------------------------------- conversion --
     // a lane owns eight codes of a row: a warp reads whole rows, and eight lanes write the eight 16-byte
     // chunks of a panel's line, no bank twice.  Its rows are a multiple of eight apart, so its place in a
@@ -285,8 +321,8 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     constexpr int LANES = BNL / 8, ROWS = 32 / LANES;    // lanes of a row, rows a warp takes at a time
     constexpr int STEP = GROUP_WARPS * ROWS, UNITS = BK / STEP;
     static_assert(STEP % 8 == 0, "rows of a lane keep their place in the swizzle");
-    const int grp = (warp - 6) / GROUP_WARPS, col = lane % LANES;
-    const int r0 = ((warp - 6) % GROUP_WARPS) * ROWS + lane / LANES;
+    const int grp = (warp - 7) / GROUP_WARPS, col = lane % LANES;
+    const int r0 = ((warp - 7) % GROUP_WARPS) * ROWS + lane / LANES;
     uint8_t* const dst = s.b[grp] + (col / 8) * (BK * 128) + r0 * 128 + (((col & 7) ^ (r0 & 7)) << 4);
     uint32_t it = 0;
     bool ok = true;
@@ -295,7 +331,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
       for (int kb = w.kb0; kb < w.kb1; ++kb, ++it) {
         if ((int)(it % CONV) != grp) continue;
         const int st = it % STAGES;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s.full[st], (it / STAGES) & 1, abort_flag, p.status,
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.full_8[st], (it / STAGES) & 1, abort_flag, p.status,
                                                STATUS_TIMEOUT_TMA));
         if (!ok) break;
         // converted into registers while products still read the tile; what is left between their end
@@ -314,9 +350,11 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           v[j] = a8_decode8(codes[j], a8_step2(step[j]));
           asm volatile("" : "+r"(v[j].x), "+r"(v[j].y), "+r"(v[j].z), "+r"(v[j].w));   // here, not behind the wait
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.empty_8[st]);
         if (it >= CONV)
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.conv_empty[grp], ((it / CONV) & 1) ^ 1, abort_flag, p.status,
-                                                    STATUS_TIMEOUT_MMA));
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.conv_empty[grp], ((it / CONV) & 1) ^ 1, abort_flag,
+                                                    p.status, STATUS_TIMEOUT_MMA));
         if (!ok) break;
 #pragma unroll
         for (int j = 0; j < UNITS; ++j) *reinterpret_cast<uint4*>(dst + j * STEP * 128) = v[j];
