@@ -27,7 +27,7 @@
 // 32 KB into the tensor core, 640 clocks at 128 bytes against 512 of tcgen05.mma (BN 512, whose two accumulators
 // share the rows of dY^T: 1,152 against 1,024); 900 and 1,230 are measured.  Without the converted tile's stores it
 // would take 12 % less, without three of four products 6 %; rings of five or seven stages make no difference.
-// 32,780 rows x 5,472 x 1,024: 328 us (1,120 TFLOP/s) with BN 512, 381 with 256; without chains 310, and then one CTA
+// 32,780 rows x 5,472 x 1,024: 322 us (1,140 TFLOP/s) with BN 512, 381 with 256; without chains 305, and then one CTA
 // per tile 372 (256 x 256) to 620 us (128 x 256); restoring X to bf16 first and the bf16 kernel of gemm.cu 428.
 // 29,140 x 1,376 x 256: 36 us, the bf16 kernel alone 45.  One ring and one loading warp for dY, codes and steps took 2 to 6
 // % longer (its instructions, 730 clocks a k-block, were the pace).  Tried and slower: codes loaded into registers
@@ -80,7 +80,8 @@ struct Params {
   const uint8_t* steps;
   int64_t spitch;
   int R, N, C;
-  int n_c, tiles, num_kb, splits, kb_per, chain;
+  int n_c, tiles, num_kb, kb_per, chain;
+  int run, runs, rest;     // slices of an owner's piece, such pieces and single slices of a tile
   int accumulate;          // what is stored is added to what the result holds
   int* status;
 };
@@ -89,19 +90,26 @@ struct Params {
 struct Piece {
   int tile, plane, kb0, kb1;
 };
-// the pieces of a pair of CTAs: all tiles of a slice before the next one's, so that pairs read the same rows
+// The pieces of a pair of CTAs.  Where the slices of all tiles take `run` rounds of the pairs, a pair of the first
+// runs * tiles ones takes that many slices of one tile, one after the other, into one plane; what slices are left the
+// others take, all tiles of a slice before the next one's, a plane a slice.  So at any time the pairs read few
+// different rows, and planes are few (32,780 x 5,472 x 1,024: three for five slices, 356 us against 361 in a row).
 struct Walk {
   const Params& p;
   int64_t pos;
   int pairs;
   IMF_DEVICE Walk(const Params& prm, int pair, int n) : p(prm), pos(pair), pairs(n) {}
   IMF_DEVICE bool next(Piece& w) {
-    if (pos >= (int64_t)p.tiles * p.splits) return false;
-    w.plane = (int)(pos / p.tiles);
-    w.tile = (int)(pos - (int64_t)w.plane * p.tiles);
-    w.kb0 = w.plane * p.kb_per;
-    w.kb1 = min(w.kb0 + p.kb_per, p.num_kb);
-    pos += pairs;
+    const int64_t owners = (int64_t)p.runs * p.tiles;
+    if (pos >= owners + (int64_t)p.tiles * p.rest) return false;
+    const int64_t row = pos / p.tiles;
+    w.tile = (int)(pos - row * p.tiles);
+    w.plane = (int)row;
+    const bool owner = pos < owners;
+    const int first = owner ? (int)row * p.run : p.runs * p.run + (int)(row - p.runs);
+    w.kb0 = first * p.kb_per;
+    w.kb1 = min(w.kb0 + (owner ? p.run * p.kb_per : p.kb_per), p.num_kb);
+    pos += owner ? owners + (int64_t)p.tiles * p.rest : pairs - owners;
     return true;
   }
 };
@@ -432,7 +440,9 @@ static int sm_count() {
 }
 
 struct Plan {
-  int bn, splits, kb_per, pairs;
+  int bn, kb_per, pairs;
+  int run, runs, rest;     // see Walk
+  int planes() const { return runs + rest; }
 };
 
 // Tile width and slices: the least time among the counts that fill one, two or three rounds of pairs (and one
@@ -442,7 +452,7 @@ struct Plan {
 // x 256 20.5 (256) and 18.4 (128).
 static Plan plan(int R, int N, int C, int sms) {
   const int num_kb = (R + BK - 1) / BK, most = sms > 1 ? sms / 2 : 1;
-  Plan best{128, 1, num_kb, 1};
+  Plan best{128, num_kb, 1, 1, 1, 0};
   double least = 1e30;
   for (int bn = 128; bn <= 512; bn *= 2) {
     const double kb_us = bn == 512 ? 0.82 : bn == 256 ? 0.50 : 0.45, tile_us = bn == 512 ? 6 : bn == 256 ? 3.5 : 2.5;
@@ -452,12 +462,14 @@ static Plan plan(int R, int N, int C, int sms) {
       if (want > num_kb / 2) want = num_kb / 2;        // two k-blocks a slice at least
       if (want < 1) want = 1;
       const int per = (int)((num_kb + want - 1) / want), sp = (num_kb + per - 1) / per;
-      const double lines = (double)((tiles * sp + most - 1) / most);
-      double cost = lines * (per * kb_us + tile_us);
-      if (sp > 1) cost += 5.0 + 0.22 * (sp * (4e-6 * N * C));
+      const int64_t pieces = tiles * sp, lines = (pieces + most - 1) / most;
+      const int run = (int)(lines < sp ? lines : sp), runs = tiles <= most ? sp / run : 0, rest = sp - runs * run;
+      double cost = (double)lines * (per * kb_us + tile_us);
+      if (runs + rest > 1) cost += 5.0 + 0.22 * ((runs + rest) * (4e-6 * N * C));
       if (cost < least) {
         least = cost;
-        best = Plan{bn, sp, per, (int)(tiles * sp < most ? tiles * sp : most)};
+        const int64_t walks = tiles * (runs + rest);
+        best = Plan{bn, per, (int)(walks < most ? walks : most), run, runs, rest};
       }
     }
   }
@@ -483,7 +495,7 @@ static int launch(const void* dy, int64_t ld_dy, const void* codes, const void* 
       return rc;
   }
   {
-    uint64_t dims[3] = {(uint64_t)C, (uint64_t)N, (uint64_t)pl.splits};
+    uint64_t dims[3] = {(uint64_t)C, (uint64_t)N, (uint64_t)pl.planes()};
     uint64_t str[3] = {4, (uint64_t)ld_dst * 4, (uint64_t)plane * 4};
     uint32_t box[3] = {32, 32, 1};
     if ((rc = make_tmap(&tc, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, dst, dims, str, box))) return rc;
@@ -495,7 +507,9 @@ static int launch(const void* dy, int64_t ld_dy, const void* codes, const void* 
   p.n_c = (C + BN - 1) / BN;
   p.tiles = (N + 2 * BM - 1) / (2 * BM) * p.n_c;
   p.num_kb = (R + BK - 1) / BK;
-  p.splits = pl.splits;
+  p.run = pl.run;
+  p.runs = pl.runs;
+  p.rest = pl.rest;
   p.kb_per = pl.kb_per;
   const int chains = (pl.kb_per + Smem<BN>::CHAIN - 1) / Smem<BN>::CHAIN;
   p.chain = (pl.kb_per + chains - 1) / chains;
@@ -524,7 +538,7 @@ extern "C" int64_t imf_wgrad8_work(int R, int N, int C, const float* out, int64_
   using namespace imf;
   if (R <= 0 || N <= 0 || C <= 0) return 0;
   const w8::Plan pl = w8::plan(R, N, C, w8::sm_count());
-  return pl.splits > 1 || !in_place(out, ldo, C) ? pl.splits * w8::plane_floats(N, C) : 0;
+  return pl.planes() > 1 || !in_place(out, ldo, C) ? pl.planes() * w8::plane_floats(N, C) : 0;
 }
 
 extern "C" int imf_splitk_reduce_ld(const float* partial, int splits, int M, int N, int64_t ldp, int64_t plane, float* out,
@@ -539,15 +553,15 @@ extern "C" int imf_wgrad8(const void* dy, int64_t ld_dy, const void* codes, cons
   if (R > 0x7fffff00 || N > 0x7fffff00 || C > 0x7ffffe00) return IMF_ERR_TOO_LARGE;
   if ((reinterpret_cast<uintptr_t>(codes) & 15u) || (reinterpret_cast<uintptr_t>(steps) & 3u)) return IMF_ERR_ARG;
   const w8::Plan pl = w8::plan(R, N, C, w8::sm_count());
-  if ((int64_t)((N + 255) / 256) * ((C + pl.bn - 1) / pl.bn) * pl.splits > 0x7fffffff) return IMF_ERR_TOO_LARGE;
-  const bool direct = pl.splits == 1 && in_place(out, ldo, C);
+  if ((int64_t)((N + 255) / 256) * ((C + pl.bn - 1) / pl.bn) * pl.planes() > 0x7fffffff) return IMF_ERR_TOO_LARGE;
+  const bool direct = pl.planes() == 1 && in_place(out, ldo, C);
   const int64_t plane = w8::plane_floats(N, C), cp = plane / N;
-  if (!direct && (!work || work_floats < pl.splits * plane || (reinterpret_cast<uintptr_t>(work) & 15u)))
+  if (!direct && (!work || work_floats < pl.planes() * plane || (reinterpret_cast<uintptr_t>(work) & 15u)))
     return IMF_ERR_ARG;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto go = pl.bn == 512 ? w8::launch<512> : pl.bn == 256 ? w8::launch<256> : w8::launch<128>;
   const int rc = direct ? go(dy, ld_dy, codes, steps, R, N, C, out, ldo, (int64_t)N * ldo, accumulate, pl, status, st)
                         : go(dy, ld_dy, codes, steps, R, N, C, work, cp, plane, 0, pl, status, st);
   if (rc || direct) return rc;
-  return imf_splitk_reduce_ld(work, pl.splits, N, C, cp, plane, out, ldo, 1.f, accumulate, stream);
+  return imf_splitk_reduce_ld(work, pl.planes(), N, C, cp, plane, out, ldo, 1.f, accumulate, stream);
 }
