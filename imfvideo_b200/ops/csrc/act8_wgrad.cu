@@ -29,7 +29,7 @@
 // would take 12 % less, without three of four products 6 %; rings of five or seven stages make no difference.
 // 32,780 rows x 5,472 x 1,024: 322 us (1,140 TFLOP/s) with BN 512, 381 with 256; without chains 305, and then one CTA
 // per tile 372 (256 x 256) to 620 us (128 x 256); restoring X to bf16 first and the bf16 kernel of gemm.cu 428.
-// 29,140 x 1,376 x 256: 36 us, the bf16 kernel alone 45.  One ring and one loading warp for dY, codes and steps took 2 to 6
+// 29,140 x 1,376 x 256: 35 us, the bf16 kernel alone 45.  One ring and one loading warp for dY, codes and steps took 2 to 6
 // % longer (its instructions, 730 clocks a k-block, were the pace).  Tried and slower: codes loaded into registers
 // by the converting warps (594 us at 5,472 x 1,024: the proxy fence waits for the loads) or by cp.async
 // (463; no difference at 1,376 x 256); remote arrivals and
@@ -142,9 +142,8 @@ IMF_DEVICE uint32_t cluster_rank() {
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
   return r;
 }
-IMF_DEVICE void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
-}
+IMF_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+IMF_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // arrive on the first CTA's barrier
 IMF_DEVICE void arrive_first(uint64_t* bar) {
   asm volatile(
@@ -188,6 +187,9 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_rank(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   if (threadIdx.x == 0) {
+    prefetch_tmap(&tm_a);
+    prefetch_tmap(&tm_b);
+    prefetch_tmap(&tm_c);
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&s.full_8[i], 1 + 32);               // the bytes' announcement, and each lane's step bytes
       mbar_init(&s.empty_8[i], GROUP_WARPS);
@@ -205,6 +207,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     s.abort_flag = 0;
     fence_barrier_init();
   }
+  __syncthreads();
   if (warp == 5) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s.tmem_base)),
                  "r"(512u)
@@ -212,10 +215,12 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
-  cluster_sync();
+  cluster_arrive();
+  // the loading warps touch nothing of the other CTA, nor TMEM: they begin, and wait for it at their end
+  const bool loads = warp == 4 || warp == 6;
+  if (!loads) cluster_wait();
   tc_fence_after();
-  const uint32_t tmem = s.tmem_base;
+  const uint32_t tmem = loads ? 0u : s.tmem_base;
   volatile int* abort_flag = &s.abort_flag;
   Walk walk(p, pair, pairs);
   Piece w;
@@ -225,8 +230,6 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
   if (warp == 4) {
     // ---------------------------------------------------------------- dY --
     if (elect_one()) {
-      prefetch_tmap(&tm_a);
-      prefetch_tmap(&tm_c);
       uint32_t it = 0;
       bool ok = true;
       while (ok && walk.next(w)) {
@@ -245,7 +248,6 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
   } else if (warp == 6) {
     // --------------------------------------------------- codes and steps --
-    if (lane == 0) prefetch_tmap(&tm_b);
     uint32_t it = 0;
     bool ok = true;
     while (ok && walk.next(w)) {
@@ -418,8 +420,10 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     if (lane == 0) tma_store_wait_all();
     tc_fence_before();
   }
+  if (loads) cluster_wait();
   __syncthreads();
-  cluster_sync();            // the other CTA's products have read this one's tiles
+  cluster_arrive();
+  cluster_wait();            // the other CTA's products have read this one's tiles
   if (warp == 5) {
     __syncwarp();
     tc_fence_after();
