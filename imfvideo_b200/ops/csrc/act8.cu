@@ -60,8 +60,8 @@ __device__ __forceinline__ void halves(uint32_t w, float* v) {
 //
 // PLAIN: the tensor has no gaps and whole words of steps (a multiple of 128 channels), so unit u is 16 (32) bytes at
 // 16 u, its codes are at 8 u and its step at u / 4: no division, one address computation each.  Storing is bound by the
-// instructions: 574 M channels in 13 tensors 324 us with two units a thread, 338 with four, 356 with divisions
-// throughout (130 instructions a unit); a copy's rate would be 282.  Restoring is at it: 277 us with four, 305 with two.
+// instructions: 574 M channels in 13 tensors 313 us with two units a thread, 330 with four, 318 with codes rounded in fp32,
+// 356 with divisions besides; a copy's rate would be 282.  Restoring is at it: 270 us with four, 305 with two.
 template <int UNITS, bool FP32, bool PLAIN>
 __device__ __forceinline__ void store_units(const A8Rec& r, uint32_t u0) {
   constexpr int ES = FP32 ? 4 : 2;
@@ -95,7 +95,7 @@ __device__ __forceinline__ void store_units(const A8Rec& r, uint32_t u0) {
 #pragma unroll
   for (int k = 0; k < UNITS; ++k) {
     float v[A8_VEC];
-    uint32_t m;                        // bits of the largest magnitude, as fp32
+    uint32_t m, mag[4];                // bits of the largest magnitude, as fp32; bf16: the pairs' magnitudes
     if (FP32) {
       const uint4 a = w[k][0], b = w[k][FP32 ? 1 : 0];
       const uint32_t ww[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -109,11 +109,11 @@ __device__ __forceinline__ void store_units(const A8Rec& r, uint32_t u0) {
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
     } else {
       const uint4 a = w[k][0];
-      uint32_t h = max2(max2(abs2(a.x), abs2(a.y)), max2(abs2(a.z), abs2(a.w)));
+      mag[0] = abs2(a.x); mag[1] = abs2(a.y); mag[2] = abs2(a.z); mag[3] = abs2(a.w);
+      uint32_t h = max2(max2(mag[0], mag[1]), max2(mag[2], mag[3]));
       h = max2(h, __shfl_xor_sync(0xffffffffu, h, 1));
       h = max2(h, __shfl_xor_sync(0xffffffffu, h, 2));
       m = max(h << 16, h & 0xffff0000u);
-      halves(a.x, v); halves(a.y, v + 2); halves(a.z, v + 4); halves(a.w, v + 6);
     }
     const uint32_t s = a8_step_of(m);
     // the steps of four groups are one word, which the first of them writes, where a warp holds whole words (by
@@ -129,10 +129,20 @@ __device__ __forceinline__ void store_units(const A8Rec& r, uint32_t u0) {
     if (u < units) {
       uint2 out;
       if (s < A8_MAX_STEP) {
-        const float inv = a8_inv_step(s);
-        out = make_uint2(a8_encode4(v, inv), a8_encode4(v + 4, inv));
+        if (FP32) {
+          const float inv = a8_inv_step(s);
+          out = make_uint2(a8_encode4(v, inv), a8_encode4(v + 4, inv));
+        } else {
+          const uint4 a = w[k][0];
+          const __nv_bfloat162 inv = a8_inv_step2(s);
+          out = make_uint2(a8_encode4(a.x, a.y, mag[0], mag[1], inv), a8_encode4(a.z, a.w, mag[2], mag[3], inv));
+        }
       } else if (s == A8_MAX_STEP) {
         const float inv = a8_inv_step(s);
+        if (!FP32) {
+          const uint4 a = w[k][0];
+          halves(a.x, v); halves(a.y, v + 2); halves(a.z, v + 4); halves(a.w, v + 6);
+        }
         out = make_uint2(a8_encode4_top(v, inv), a8_encode4_top(v + 4, inv));
       } else {
         out = make_uint2(0u, 0u);

@@ -25,8 +25,12 @@ __device__ __forceinline__ uint32_t a8_step_of(uint32_t amax_bits) {
   const int s = (int)((amax_bits + 0x10000u) >> 23) - 6;
   return s < 0 ? 0u : s > (int)A8_MAX_STEP ? A8_MAX_STEP : (uint32_t)s;
 }
-// 2^(127 - s), s <= 248
+// 2^(127 - s), s <= 248 (as a pair of bf16: s <= 247)
 __device__ __forceinline__ float a8_inv_step(uint32_t s) { return __uint_as_float((254u - s) << 23); }
+__device__ __forceinline__ __nv_bfloat162 a8_inv_step2(uint32_t s) {
+  const uint32_t w = (254u - s) * 0x00800080u;
+  return *reinterpret_cast<const __nv_bfloat162*>(&w);
+}
 
 // four codes of v[0..3] as one word.  Adding 1.5 * 2^23 leaves the nearest whole number (ties to even)
 // in the low bits; the product with a power of two is exact (or below half a step), so the one rounding
@@ -43,6 +47,22 @@ __device__ __forceinline__ uint32_t a8_encode4_top(const float* v, float inv) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) c[i] = fminf(fmaxf(v[i] * inv, -127.f), 127.f);
   return a8_encode4(c, 1.f);
+}
+
+// four codes of the bf16 pairs a and b, whose magnitudes are ma and mb, times 2^(127 - s) (in both halves of inv), below
+// the largest step.  128 + |x| has a spacing of one in bf16, so the one rounding of the fma is that of the code, whose
+// magnitude is the result's low byte; negative codes are then ~m + 1, a byte at a time.
+__device__ __forceinline__ uint32_t a8_encode4(uint32_t a, uint32_t b, uint32_t ma, uint32_t mb, __nv_bfloat162 inv) {
+  const uint32_t one28 = 0x43004300u;
+  const auto mag = [&](uint32_t m) {
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&m), inv,
+                                     *reinterpret_cast<const __nv_bfloat162*>(&one28));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  };
+  uint32_t neg;                        // 0xff where the sign is set: prmt repeats the top bit of bytes 1, 3 of both
+  asm("prmt.b32 %0, %1, %2, 0xfdb9;" : "=r"(neg) : "r"(a), "r"(b));
+  const uint32_t c = __byte_perm(mag(ma), mag(mb), 0x6420) ^ neg;
+  return ((c & 0x7f7f7f7fu) + (neg & 0x01010101u)) ^ (c & 0x80808080u);
 }
 
 // the step in both halves, as bf16: the byte is the exponent.  2^-127 is half the smallest normal number
