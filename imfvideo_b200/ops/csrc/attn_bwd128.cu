@@ -319,6 +319,11 @@ attn_bwd128_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int row = wl * 32 + lane;     // kv row of this thread (TMEM lane)
     const uint32_t tb = tmem_addr(tmem, wl * 32, 0);
     const float scale_log2 = p.scale * 1.4426950408889634f;
+    // a row behind the last key has the score zero, and P = exp(-lse) is infinite from lse = -89 on: then dQ would be
+    // infinity times a key of zeros.  Its scores become such that the exponent is -infinity (NaN at a scale of zero,
+    // where P = exp(-lse) is what every key has)
+    const bool no_key = kvb * KT + row >= p.L && scale_log2 != 0.f;
+    const uint32_t no_score = scale_log2 < 0.f ? 0x7f800000u : 0xff800000u;
     bool ok = true;
     for (int i = 0; i < n_q && ok; ++i) {
       const int st = i % QSTAGES;
@@ -332,6 +337,10 @@ attn_bwd128_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       tmem_ld32(tb + BC_DP + wg * 32, dp);
       tc_wait_ld();
       tc_fence_before();
+      if (no_key) {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) sv[c] = no_score;
+      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.s_taken);
       const float4* lse4 = reinterpret_cast<const float4*>(s.lse2[st] + wg * 32);

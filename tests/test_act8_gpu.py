@@ -382,6 +382,36 @@ def test_attention_of_broadcast_tensors(A, K, hd, B):
     K.check_status()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("L", [1, 65, 128, 200, 333])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_scores_far_below_zero(A, K, hd, L, sign):
+    """All scores near -100: exp(-lse) of the rows behind the last key is no number of 32 bits."""
+    g, H = _gen(50 + L), 2
+    q, k, v, go = (_randn(g, 1, L, H, hd) for _ in range(4))
+    q[..., 0], k[..., 0] = 16.0, -100.0 * sign * hd ** 0.5 / 16      # the scores; the other channels tell them apart
+    k[..., 0] = k[..., 0].float().round().to(BF16)
+    scale = sign * hd ** -0.5
+    q8, k8, v8 = A.store8([q, k, v])
+    z = [p.restore().double() for p in (q8, k8, v8)]
+    s = torch.einsum("blhd,bmhd->bhlm", z[0], z[1]) * scale
+    lse = torch.logsumexp(s, -1).float()
+    assert (lse < -89).all()
+    o8 = A.store8(torch.einsum("bhlm,bmhd->blhd", torch.softmax(s, -1), z[2]).to(BF16))
+    got = A.attn_bwd8(q8, k8, v8, o8, lse, go, scale=scale)
+    want = _oracle((q8, k8, v8, o8), lse, go, scale)
+    assert all(torch.isfinite(t).all() for t in got)
+    # P, dS and the results are rounded to bf16 (1.6e-3 of the norm each); the exponent is off by the (hi, lo) pair of
+    # lse / scale, 2^-16 of 110 at most, and 32-bit sums of scores, 2^-23 of a few 110: 2e-3
+    if L > 1:             # (one token: dQ and dK are nothing but roundings; channel 0 of k is one value, its dQ too)
+        _near((got[0][..., 1:], got[1], got[2]), [want[0][..., 1:], want[1], want[2]], (hd, L, sign))
+    else:
+        _near((got[2],) * 3, [want[2]] * 3, (hd, L, sign))
+    gq, gk, gv = K.attn_bwd(q, k, v, o8.restore(), lse, go, scale=scale)
+    assert torch.isfinite(gq).all() and torch.isfinite(gk).all() and torch.isfinite(gv).all()
+    K.check_status()
+
+
 def test_attention_gradient_is_a_difference_quotient(A, K):
     """Along a random direction of q, k and v the loss changes as the gradients say (64-bit differences)."""
     B, L, H, hd = 1, 40, 2, 64
