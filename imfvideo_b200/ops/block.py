@@ -218,9 +218,9 @@ class _BlockFn(torch.autograd.Function):
             if g.act8 and not grad_on:        # under no_grad: nothing to keep (parameters still ask for gradients)
                 kept = ()
             elif g.act8:
-                # q, k and o go to the dense core's backward in 8 bits; another core has its own form
-                # of them, and they stay as they are
-                dense = isinstance(core, DenseCore)
+                # q, k and o go to the dense core's backward in 8 bits; another core, one derived from it
+                # too, has its own form of them or its own backward, and they stay as they are
+                dense = type(core) is DenseCore
                 packed = A8.store8([n1[0], a_[:rows], qlat[0], kvlat[0], qb[:rows], kvb[:rows],
                                     a_out[:rows], n2[0], gu[:rows], m[:rows]] +
                                    ([q[0], k[0], o] if dense else []))

@@ -153,6 +153,42 @@ def test_block_from_8_bit_activations(kernels, monkeypatch, gate, wide, fresh, t
         assert (a - c).norm() <= 0.1 * c.norm(), n
 
 
+@pytest.mark.parametrize("own", ["bwd", "both"])
+def test_cores_derived_from_the_dense_one(kernels, monkeypatch, own):
+    """A core that overrides the dense one's methods runs its own backward pass, from q, k and o as they are."""
+    from imfvideo_b200.ops.block import DenseCore
+
+    calls = []
+
+    class Core(DenseCore):
+        scale = 0.2 if own == "both" else None
+
+        def fwd(self, q, k, v, dq, dk, dv, need_bwd):
+            o, do, lse = kernels.attn_fwd(q, k, v, dq, dk, dv, scale=self.scale, need_lse=need_bwd)
+            return o, do, (lse,)
+
+        def bwd(self, q, k, v, o, saved, go, gv_out=None):
+            calls.append((q, k, o))
+            dq, dk, dv = kernels.attn_bwd(q, k, v, o, saved[0], go, scale=self.scale, gv_out=gv_out)
+            return dq * 0.5, dk, dv
+
+    kernels.set_deterministic(True)
+    monkeypatch.setattr("imfvideo_b200.ops.block.DENSE_CORE", Core())
+    try:
+        grads = []
+        for store in ("int8", "bf16"):
+            blk = _block(store)
+            xs, cos, sin, go = _inputs(blk)
+            grads.append(_run(blk, xs, cos, sin, go, False)[1])
+    finally:
+        kernels.set_deterministic(False)
+    kernels.check_status()
+    assert len(calls) == 2 and all(torch.equal(a, b) for a, b in zip(*calls))
+    for a, b in zip(*grads):
+        # (see test_block_from_8_bit_activations)
+        assert (a is None) == (b is None) and (a is None or (a - b).norm() <= 0.1 * b.norm())
+
+
 def test_straight_into_gradient_buffers(kernels):
     """Weight gradients accumulated into existing fp32 buffers equal those returned to autograd."""
     kernels.set_deterministic(True)
