@@ -290,7 +290,8 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     // --------------------------------------------------------------- MMA --
     if (elect_one()) {
       constexpr uint32_t idesc = idesc_bf16(2 * BM, PN, 1, 1);
-      uint32_t it = 0, ch = 0;                       // k-blocks and chains so far
+      uint32_t it = 0, ch = 0, total = 0;            // k-blocks and chains so far, k-blocks in all
+      for (Walk all = walk; all.next(w);) total += w.kb1 - w.kb0;
       bool ok = true;
       while (ok && walk.next(w)) {
         for (int c0 = w.kb0; c0 < w.kb1 && ok; c0 += p.chain, ++ch) {
@@ -317,8 +318,10 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
               if (kb + 1 == c1) commit_both(&s.acc_full[acc]);
             }
             if (!ok) break;
-            commit_both(&s.conv_empty[cs]);
-            commit_both(&s.empty_a[st]);
+            // slots that are used again; nobody would wait for the other arrivals, which might then find the other
+            // CTA gone
+            if (it + CONV < total) commit_both(&s.conv_empty[cs]);
+            if (it + STAGES < total) commit_both(&s.empty_a[st]);
           }
         }
       }

@@ -210,6 +210,24 @@ def test_weight_gradient_leaves_what_is_beside_it(A, K, rows, N, C, accumulate):
     K.check_status()
 
 
+@pytest.mark.parametrize("N,C", [(9216, 1024), (18800, 256), (18800, 128)])
+@pytest.mark.parametrize("blocks", [1, 2, 3, 4, 5, 6, 7, 8, 9, 17])
+def test_weight_gradient_of_walks_about_the_rings(A, K, N, C, blocks):
+    """One tile a pair of CTAs (of 512, 256 and 128 columns), of fewer k-blocks than a ring has stages, as many
+    and more, launch after launch: an arrival left over from one would disturb the next.  Whole numbers, so
+    that every sum is exact."""
+    g, rows = _gen(blocks), 64 * blocks - 5
+    dy = torch.randint(-2, 3, (rows, N), device="cuda", generator=g).to(BF16)
+    x = torch.randint(-60, 61, (rows, C), device="cuda", generator=g).to(BF16)
+    x[:, ::32] = 100.0                                                   # so that the step is one
+    p = A.store8(x)
+    assert torch.equal(p.restore(), x)
+    want = (dy.double().t() @ x.double()).float()
+    outs = [A.gemm_wgrad8(dy, p) for _ in range(12)]
+    assert want.abs().max() < 2 ** 24 and all(torch.equal(o, want) for o in outs)
+    K.check_status()
+
+
 def test_weight_gradient_bad_values(A, K):
     """A group with an infinity makes NaN of its own 32 columns, an infinity of dY of its own row."""
     g = _gen(12)
