@@ -228,6 +228,23 @@ def test_weight_gradient_of_walks_about_the_rings(A, K, N, C, blocks):
     K.check_status()
 
 
+@pytest.mark.parametrize("rows,N,C", [(16384, 2048, 1024), (29140, 1376, 256), (9000, 1000, 100)])
+def test_weight_gradient_repeats(A, K, rows, N, C):
+    """Two hundred launches, several chains of products each, give the same bits, which are the exact sums."""
+    g = _gen(rows)
+    dy = torch.randint(-2, 3, (rows, N), device="cuda", generator=g).to(BF16)
+    x = torch.randint(-60, 61, (rows, C), device="cuda", generator=g).to(BF16)
+    x[:, ::32] = 100.0                                                   # so that the step is one
+    p = A.store8(x)
+    want = dy.double().t() @ x.double()
+    assert want.abs().max() < 2 ** 24 and (dy.double().abs().t() @ x.double().abs()).max() < 2 ** 24
+    want, same = want.float(), torch.ones((), dtype=torch.bool, device="cuda")
+    for _ in range(200):
+        same &= (A.gemm_wgrad8(dy, p) == want).all()
+    assert bool(same)
+    K.check_status()
+
+
 def test_weight_gradient_bad_values(A, K):
     """A group with an infinity makes NaN of its own 32 columns, an infinity of dY of its own row."""
     g = _gen(12)
