@@ -200,6 +200,47 @@ def _row_dims(t: Tensor, rows: int) -> Optional[Tuple[int, ...]]:
     return tuple(d[0] for d in dims) + tuple(d[1] for d in dims)
 
 
+def _places(t: Tensor) -> Tuple[List[Tuple[int, int]], int]:
+    """((stride, n) of the dimensions that count but adjacent channels, smallest first; how many those are)."""
+    dims = sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1)
+    return (dims[1:], dims[0][1]) if dims and dims[0][0] == 1 else (dims, 1)
+
+
+def _starts(dims: List[Tuple[int, int]]) -> Tensor:
+    at = torch.zeros(1, dtype=torch.int64)
+    for s, n in dims:
+        at = (at[:, None] + torch.arange(n) * s).flatten()
+    return at
+
+
+def _apart(dims: List[Tuple[int, int]], run: int) -> bool:
+    """Whether runs of ``run`` elements at these strides lie in different places."""
+    reach = run
+    for s, n in dims:
+        if s < reach:
+            break
+        reach += s * (n - 1)
+    else:
+        return True
+    return dims[0][0] > 0 and bool((_starts(dims).sort().values.diff() >= run).all())      # strides that interleave
+
+
+def _in_one_place(a: Tensor, b: Tensor) -> bool:
+    """Whether two tensors, each of elements apart, share memory."""
+    if a.data_ptr() > b.data_ptr():
+        a, b = b, a
+    (da, ra), (db, rb), es, d = _places(a), _places(b), a.element_size(), b.data_ptr() - a.data_ptr()
+    if a.numel() == 0 or b.numel() == 0 or d >= (sum(s * (n - 1) for s, n in da) + ra) * es:
+        return False
+    if da == db and b.element_size() == es and d % es == 0 and d >= ra * es and _apart(da, d // es + rb):
+        return False                           # two bands of one buffer
+    at = torch.cat([_starts(da) * es, _starts(db) * b.element_size() + d])
+    end = at + torch.tensor([ra * es, rb * b.element_size()]).repeat_interleave(
+        torch.tensor([a.numel() // ra, b.numel() // rb]))
+    at, order = at.sort()
+    return bool((at[1:] < end[order][:-1]).any())
+
+
 def _launch(fn_name: str, recs: List[int]) -> None:
     """``recs``: eleven numbers for each tensor."""
     K = _kernels()
@@ -277,7 +318,7 @@ def store8(xs: Union[Tensor, Sequence[Tensor]]) -> Union[Packed8, List[Packed8]]
 def restore8(ps: Union[Packed8, Sequence[Packed8]], outs=None) -> Union[Tensor, List[Tensor]]:
     """The values of one packed tensor or of several, in one launch; ``outs``: where they go (one
     tensor, or a list with None for a new one), of the packed shape and type, rows at any three
-    strides, channels adjacent."""
+    strides, channels adjacent, no two elements in one place."""
     if isinstance(ps, Packed8):
         return restore8([ps], None if outs is None else [outs])[0]
     ps = list(ps)
@@ -290,6 +331,10 @@ def restore8(ps: Union[Packed8, Sequence[Packed8]], outs=None) -> Union[Tensor, 
     for p, o in zip(ps, outs):
         if o is not None and (o.shape != p.shape or o.dtype != p.dtype):
             raise ValueError(f"output {o.dtype} {tuple(o.shape)} for packed {p.dtype} {tuple(p.shape)}")
+    given = [o for o in outs if o is not None]
+    if not all(o.is_contiguous() or _apart(*_places(o)) for o in given) or \
+            any(_in_one_place(a, b) for i, a in enumerate(given) for b in given[:i]):
+        raise ValueError("restore8 output: no two elements in one place, of one output or of two")
     if dev.type != "cuda":
         for i, p in enumerate(ps):
             v = ref.values8(p.codes, p.steps, p.cols).to(p.dtype).view(p.shape)
@@ -306,9 +351,8 @@ def restore8(ps: Union[Packed8, Sequence[Packed8]], outs=None) -> Union[Tensor, 
         if p.rows == 0 or p.cols == 0:
             continue
         dims = _row_dims(o, p.rows)
-        if dims is None or not o.is_contiguous() and 0 in [s for n, s in zip(o.shape, o.stride()) if n > 1]:
-            raise ValueError("restore8 output: the channels have to be adjacent, the rows at three strides at most "
-                             "and no two of them in one place")
+        if dims is None:
+            raise ValueError("restore8 output: the channels have to be adjacent, the rows at three strides at most")
         recs += (o.data_ptr(), *p._ptrs(), *dims, p.cols, p.dtype is F32)
     if recs:
         _launch("imf_restore8", recs)

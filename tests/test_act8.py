@@ -201,6 +201,34 @@ def test_refusals():
         act8.attn_bwd8(small, small, small, go[..., :32], lse, go[..., :32])
 
 
+def test_outputs_that_share_memory():
+    """Elements of one output, or of two, in one place are refused; bands and rows that interleave are not."""
+    a, b = act8.store8([torch.randn(6, 40).bfloat16(), torch.randn(6, 24).bfloat16()])
+    f = act8.store8(torch.randn(6, 20))
+    c = act8.store8(torch.randn(3, 2, 8).bfloat16())
+    flat = lambda n=2000, dt=BF16: torch.full((n,), 7.0, dtype=dt)
+    buf = flat()
+    row = lambda p, o, s: buf.as_strided(p.shape, (s, 1), o)
+    for ps, outs in (([a], [row(a, 0, 39)]), ([a], [row(a, 0, 1)]), ([a], [row(a, 0, 0)]),
+                     ([a], [buf[:40].expand(6, 40)]), ([c], [buf.as_strided((3, 2, 8), (16, 12, 1))]),
+                     ([c], [buf.as_strided((3, 2, 8), (8, 16, 1))]),
+                     ([a, a], [row(a, 0, 40), row(a, 0, 40)]), ([a, b], [row(a, 0, 64), row(b, 39, 64)]),
+                     ([a, b], [row(a, 24, 63), row(b, 0, 63)]), ([b, a], [row(b, 0, 24), row(a, 143, 40)]),
+                     ([a, b], [row(a, 0, 80), row(b, 60, 81)])):
+        with pytest.raises(ValueError):
+            act8.restore8(ps, outs)
+    assert (buf == 7).all()
+    for ps, outs in (([a, b], [row(a, 0, 64), row(b, 40, 64)]), ([a, b], [row(a, 24, 64), row(b, 0, 64)]),
+                     ([a, b], [row(a, 0, 40), row(b, 240, 24)]), ([c], [buf.as_strided((3, 2, 8), (16, 24, 1))]),
+                     ([c], [buf.as_strided((3, 2, 8), (8, 24, 1))]), ([a, b], [row(a, 0, 80), row(b, 40, 160)][:2]),
+                     ([a], [row(a, 5, 40)]), ([b, a, b], [None, row(a, 0, 64), row(b, 40, 64)])):
+        buf.fill_(7.0)
+        for p, o in zip(ps, act8.restore8(ps, outs)):
+            assert torch.equal(o, p.restore())
+    out = flat(6 * 20, F32).view(6, 20)
+    assert torch.equal(act8.restore8([f, a], [out, None])[0], f.restore())
+
+
 def test_option_of_the_model():
     from imfvideo_b200.config import apply_overrides, preset
     from imfvideo_b200.models import IMFDiTVideo
