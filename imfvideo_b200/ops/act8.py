@@ -463,6 +463,8 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
         new = lambda: _new(shape, BF16, dev)
         return new(), new(), new() if gv_out is None else gv_out
     scale = hd ** -0.5 if scale is None else float(scale)
+    if gv_out is not None and not _apart(*_places(gv_out)):
+        raise ValueError("attn_bwd8: no two elements of the dv output in one place")
     if dev.type != "cuda":
         plain = lambda t: t.restore() if isinstance(t, Packed8) else t
         dq, dk, dv = ref.attention_grad(*(plain(t) for t in (q8, k8, v8, o8)), lse, go, scale)
@@ -475,12 +477,14 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
     lib, stream = K._lib, K._stream()
     dq, dk = _new(shape, BF16, dev), _new(shape, BF16, dev)
     dv = _new(shape, BF16, dev) if gv_out is None else gv_out
-    if dv.stride(3) != 1 or dv.data_ptr() % 16 or any(s % 8 or s == 0 and n > 1 for n, s in zip(shape[:3], dv.stride())):
-        raise ValueError("attn_bwd8: the dv output needs 16-byte aligned rows, no two of them in one place")
+    row = (L * H * hd, H * hd, hd)
+    dv_strides = [s if m > 1 else r for m, s, r in zip(shape, dv.stride(), row)]      # no address depends on the others
+    if dv.stride(3) != 1 or dv.data_ptr() % 16 or any(s % 8 for s in dv_strides):
+        raise ValueError("attn_bwd8: the dv output needs 16-byte aligned rows")
     # what is packed but o gets its values in bf16 in front of the kernel's own scratch, in the call's first launch.
     # (head_dim 64 at a scale of zero: the kernel's form for an exact Q divides by it, so the other one runs)
     first = hd == 128 or abs(scale) >= 1e-30
-    n, rows, row = 2 * B * L * H * hd, B * L * H, (L * H * hd, H * hd, hd)
+    n, rows = 2 * B * L * H * hd, B * L * H
     size = (n + 255) // 256 * 256
     nscr = lib.imf_attn_bwd_scratch_bytes_hd(B, L, H, hd)
     space = sum(isinstance(t, Packed8) for t in ((q8, k8, v8) if first else (q8, k8, v8, o8))) * size
@@ -509,7 +513,7 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
     i64 = ctypes.c_int64
     q_, k_, v_, o_, g_ = strides
     common = (*ptrs, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), B, L, H, hd,
-              (i64 * 12)(*q_, *k_, *v_, *g_), (i64 * 3)(*o_), (i64 * 3)(*row), (i64 * 3)(*dv.stride()[:3]), scale,
+              (i64 * 12)(*q_, *k_, *v_, *g_), (i64 * 3)(*o_), (i64 * 3)(*row), (i64 * 3)(*dv_strides), scale,
               base + space, nscr)
     fixed, status = int(K.DETERMINISTIC), K.status_word(dev).data_ptr()
     if first:

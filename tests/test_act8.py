@@ -229,6 +229,19 @@ def test_outputs_that_share_memory():
     assert torch.equal(act8.restore8([f, a], [out, None])[0], f.restore())
 
 
+def test_attention_outputs_that_share_memory():
+    q = act8.store8(torch.randn(2, 4, 2, 64).bfloat16())
+    go, lse = torch.randn(2, 4, 2, 64).bfloat16(), torch.zeros(2, 2, 4)
+    buf = torch.zeros(4096, dtype=BF16)
+    for strides in ((512, 128, 32, 1), (512, 128, 0, 1), (0, 128, 64, 1), (512, 64, 64, 1), (448, 128, 64, 1)):
+        with pytest.raises(ValueError):
+            act8.attn_bwd8(q, q, q, go, lse, go, gv_out=buf.as_strided((2, 4, 2, 64), strides))
+    want = act8.attn_bwd8(q, q, q, go, lse, go)[2]
+    for strides in ((512, 128, 64, 1), (128, 256, 64, 1), (64, 128, 512, 1)):
+        got = act8.attn_bwd8(q, q, q, go, lse, go, gv_out=buf.as_strided((2, 4, 2, 64), strides))[2]
+        assert torch.equal(got, want)
+
+
 def test_option_of_the_model():
     from imfvideo_b200.config import apply_overrides, preset
     from imfvideo_b200.models import IMFDiTVideo

@@ -447,6 +447,24 @@ def test_attention_of_scores_far_below_zero(A, K, hd, L, sign):
     K.check_status()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_strides_of_single_dimensions(A, K, hd):
+    """The stride of a dimension of one element is anything: no address depends on it."""
+    for shape, strides in (((1, 65, 2, hd), (1, 2 * hd, hd, 1)), ((1, 65, 1, hd), (3, hd, 5, 1)),
+                           ((2, 1, 3, hd), (3 * hd, 7, hd, 1)), ((1, 1, 1, hd), (1, 1, 1, 1))):
+        B, L, H, _ = shape
+        ps, lse, go, _ = _attention(A, K, B, L, H, hd, 60)
+        buf = torch.full((B * L * H * hd + 64,), 3.0, dtype=BF16, device="cuda")
+        got = A.attn_bwd8(*ps, lse, go, gv_out=buf.as_strided(shape, strides))[2]
+        assert torch.equal(got, A.attn_bwd8(*ps, lse, go)[2])
+        assert torch.equal(buf[:-64].view(shape), got) and (buf[-64:] == 3).all()
+        with pytest.raises(ValueError):
+            A.attn_bwd8(*ps, lse, go, gv_out=buf[1:].as_strided(shape, strides, 1))
+    with pytest.raises(ValueError):
+        A.attn_bwd8(*ps, lse, go, gv_out=buf.new_empty(2 * hd)[::2].view(shape))
+    K.check_status()
+
+
 def test_attention_gradient_is_a_difference_quotient(A, K):
     """Along a random direction of q, k and v the loss changes as the gradients say (64-bit differences)."""
     B, L, H, hd = 1, 40, 2, 64
