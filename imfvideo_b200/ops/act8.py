@@ -150,7 +150,7 @@ class Packed8:
 
     def view(self, *shape: int) -> "Packed8":
         """The same rows under other leading dimensions."""
-        if shape[-1] != self.cols or math.prod(shape[:-1]) != self.rows:
+        if not shape or shape[-1] != self.cols or math.prod(shape[:-1]) != self.rows or min(shape) < 0:
             raise ValueError(f"{tuple(self.shape)} cannot be seen as {tuple(shape)}")
         p = Packed8.__new__(Packed8)
         p.shape, p.dtype, p.device, p.rows, p.cols = torch.Size(shape), self.dtype, self.device, self.rows, self.cols

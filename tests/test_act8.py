@@ -242,6 +242,15 @@ def test_attention_outputs_that_share_memory():
         assert torch.equal(got, want)
 
 
+def test_views_of_packed_tensors():
+    p = act8.store8(torch.randn(4, 64).bfloat16())
+    for shape in ((-2, -2, 64), (-1, 64), (64,), (), (4, -64)):
+        with pytest.raises(ValueError):
+            p.view(*shape)
+    v = p.view(2, 1, 2, 64)
+    assert v.shape == (2, 1, 2, 64) and torch.equal(v.restore().view(4, 64), p.restore())
+
+
 def test_option_of_the_model():
     from imfvideo_b200.config import apply_overrides, preset
     from imfvideo_b200.models import IMFDiTVideo
