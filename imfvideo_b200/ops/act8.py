@@ -36,6 +36,7 @@ from . import reference as ref
 Tensor = torch.Tensor
 BF16, F32 = torch.bfloat16, torch.float32
 GROUP = 32
+_F32_MIN, _F32_MAX = torch.finfo(F32).tiny, torch.finfo(F32).max
 _MAX_RECS = 16                 # tensors a launch takes
 # n records x, codes, steps, n0, n1, n2, s0, s1, s2, cols, fp32
 _RECS = [struct.Struct("<" + 11 * n * "q") for n in range(_MAX_RECS + 1)]
@@ -463,6 +464,8 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
         new = lambda: _new(shape, BF16, dev)
         return new(), new(), new() if gv_out is None else gv_out
     scale = hd ** -0.5 if scale is None else float(scale)
+    if not abs(scale) <= _F32_MAX:
+        raise ValueError(f"attn_bwd8: scale {scale}")
     if gv_out is not None and not _apart(*_places(gv_out)):
         raise ValueError("attn_bwd8: no two elements of the dv output in one place")
     if dev.type != "cuda":

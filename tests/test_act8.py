@@ -251,6 +251,14 @@ def test_views_of_packed_tensors():
     assert v.shape == (2, 1, 2, 64) and torch.equal(v.restore().view(4, 64), p.restore())
 
 
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e39])
+def test_scales_that_are_no_number_of_32_bits(scale):
+    q = act8.store8(torch.randn(1, 4, 2, 64).bfloat16())
+    go, lse = torch.randn(1, 4, 2, 64).bfloat16(), torch.zeros(1, 2, 4)
+    with pytest.raises(ValueError):
+        act8.attn_bwd8(q, q, q, go, lse, go, scale)
+
+
 def test_option_of_the_model():
     from imfvideo_b200.config import apply_overrides, preset
     from imfvideo_b200.models import IMFDiTVideo
