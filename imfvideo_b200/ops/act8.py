@@ -412,8 +412,8 @@ def situ_bwd8(gu8: Packed8, gout: Tensor, beta: float, lbeta: Optional[float]) -
     rows, F = gu8.rows, gu8.cols // 2
     if gout.dtype != BF16 or gout.dim() != 2 or tuple(gout.shape) != (rows, F):
         raise ValueError(f"gout {gout.dtype} {tuple(gout.shape)}: bf16 ({rows}, {F}) expected")
-    if not beta > 0 or (lbeta is not None and not lbeta > 0):
-        raise ValueError(f"beta {beta} and linear beta {lbeta} have to be positive")
+    if not _F32_MIN <= beta <= _F32_MAX or (lbeta is not None and not _F32_MIN <= lbeta <= _F32_MAX):
+        raise ValueError(f"beta {beta} and linear beta {lbeta} have to be positive normal numbers of 32 bits")
     dev = _same_device("situ_bwd8", gu8, gout)
     g_gu, act = _new((rows, 2 * F), BF16, dev), _new((rows, F), BF16, dev)
     if rows == 0 or F == 0:

@@ -259,6 +259,17 @@ def test_scales_that_are_no_number_of_32_bits(scale):
         act8.attn_bwd8(q, q, q, go, lse, go, scale)
 
 
+@pytest.mark.parametrize("bad", [math.inf, math.nan, 1e39, 1e-39, 1e-60, 0.0, -4.0])
+def test_betas_that_are_no_positive_number_of_32_bits(bad):
+    """(their reciprocals, or products with a tanh of zero, would be NaN where the formula has a value)"""
+    gu, gout = act8.store8(torch.zeros(2, 16).bfloat16()), torch.ones(2, 8).bfloat16()
+    for beta, lbeta in ((bad, 25.0), (4.0, bad), (bad, None)):
+        with pytest.raises(ValueError):
+            act8.situ_bwd8(gu, gout, beta, lbeta)
+    for t in act8.situ_bwd8(gu, gout, 2.0 ** -126, 3.4e38):
+        assert torch.isfinite(t).all()
+
+
 def test_option_of_the_model():
     from imfvideo_b200.config import apply_overrides, preset
     from imfvideo_b200.models import IMFDiTVideo
