@@ -15,6 +15,7 @@ Numerics policy on CUDA: fp32 master parameters, fp32 residual stream,
 from __future__ import annotations
 
 import math
+import warnings
 from functools import partial
 from typing import Callable, List, Optional, Sequence, Tuple
 
@@ -554,6 +555,10 @@ class IMFDiTVideo(nn.Module):
         self.head_dim = hidden_size // num_heads
         self.attn_res_block_size = attn_res_block_size
         self.grad_checkpoint = grad_checkpoint
+        if grad_checkpoint and act_store != "bf16":
+            warnings.warn(f"act_store={act_store!r} together with grad_checkpoint saves no memory: each block is packed "
+                          "when it is recomputed and unpacked at once, at the price in accuracy and time of both",
+                          stacklevel=2)
         self.compute_dtype = compute_dtype
         self.rmsnorm_eps = rmsnorm_eps
         hd = self.head_dim

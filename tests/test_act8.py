@@ -281,3 +281,20 @@ def test_option_of_the_model():
     with pytest.raises(ValueError):
         IMFDiTVideo(input_size=8, num_frames=1, hidden_size=64, depth=2, num_heads=2, aux_head_depth=1,
                     act_store="int4")
+
+
+def test_option_with_block_recomputation_warns():
+    import warnings
+
+    from imfvideo_b200.config import apply_overrides, preset
+    from imfvideo_b200.train import build_model
+
+    def build(**model):
+        return build_model(apply_overrides(preset("tiny"), {"model." + k: v for k, v in model.items()}))
+
+    with pytest.warns(UserWarning, match="saves no memory"):
+        build(act_store="int8", grad_checkpoint=True)
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        build(act_store="int8", grad_checkpoint=False)
+        build(act_store="bf16", grad_checkpoint=True)
