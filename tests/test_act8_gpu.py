@@ -447,6 +447,34 @@ def test_attention_of_scores_far_below_zero(A, K, hd, L, sign):
     K.check_status()
 
 
+def test_attention_of_more_heads_than_are_worked_on_at_once(A, K, hd, L, B, H):
+    """Heads go in groups (34 MB of what they read and add to), the last of them smaller, whose tiles are split;
+    every head against the formula, from 8 bits and in bf16, and against the fixed order, which has one group."""
+    group = 34000000 // (L * hd * 8)
+    assert 1 <= group < B * H and B * H % group
+    ps, lse, go, o = _attention(A, K, B, L, H, hd, L + H)
+    q, k, v, o8 = (p.restore() for p in ps)
+    got, got16 = A.attn_bwd8(*ps, lse, go), K.attn_bwd(q, k, v, o8, lse, go)
+    was = K.DETERMINISTIC
+    K.set_deterministic(True)
+    try:
+        fixed, fixed16 = A.attn_bwd8(*ps, lse, go), K.attn_bwd(q, k, v, o8, lse, go)
+    finally:
+        K.set_deterministic(was)
+    K.check_status()
+    cut = lambda t, b, h: t[b:b + 1, :, h:h + 1]
+    for b in range(B):
+        for h in range(H):
+            one = [cut(t, b, h).double().transpose(1, 2) for t in (q, k, v, o8, go)]
+            s = one[0] @ one[1].transpose(-1, -2) * hd ** -0.5
+            P = torch.exp(s - lse[b:b + 1, h:h + 1, :, None].double())
+            dS = P * (one[4] @ one[2].transpose(-1, -2) - (one[4] * one[3]).sum(-1, keepdim=True))
+            want = [(dS @ one[1] * hd ** -0.5), (dS.transpose(-1, -2) @ one[0] * hd ** -0.5), P.transpose(-1, -2) @ one[4]]
+            want = [t.transpose(1, 2) for t in want]
+            for res in (got, got16, fixed, fixed16):
+                _near([cut(t, b, h) for t in res], want, (b, h))
+
+
 @pytest.mark.parametrize("hd", [64, 128])
 def test_attention_strides_of_single_dimensions(A, K, hd):
     """The stride of a dimension of one element is anything: no address depends on it."""
