@@ -228,6 +228,24 @@ def test_weight_gradient_of_walks_about_the_rings(A, K, N, C, blocks):
     K.check_status()
 
 
+@pytest.mark.parametrize("rows,N,C,bound", [(32780, 5472, 1024, 2e-6), (29140, 1376, 256, 5.5e-7)])
+def test_weight_gradient_sums_in_chains(A, K, rows, N, C, bound):
+    """The tensor core drops what is below 2^-25 of a running sum, half of that on average and always towards zero.  The
+    sums of a random walk of n steps add up to n / sqrt(3) times its end, so a chain of n products of 16 rows
+    loses 0.5 x 0.72 (the mean of a number's unit over it) x 2^-25 n / sqrt(3) = 6.2e-9 n of the result: 0.87e-6 for
+    the 35 x 4 products of a chain at 1,024 columns (2.6e-6 for a slice of 103 x 4 in one chain), 4.7e-7 for the 19 x 4 at
+    256 (9.4e-7 for a slice of 38 x 4).  Sums of chains and slices in 32 bits add 2^-24 each."""
+    g = _gen(rows)
+    dy, p = _randn(g, rows, N, s=0.02), A.store8(_activations(g, rows, C))
+    want = dy.double().t() @ p.restore().double()
+    base = torch.randn(N, C, device="cuda", generator=g) * want.std().float()
+    out = base.clone()
+    A.gemm_wgrad8(dy, p, out=out, accumulate=True)
+    assert (A.gemm_wgrad8(dy, p).double() - want).norm() <= bound * want.norm()
+    assert (out.double() - want - base.double()).norm() <= bound * (want + base.double()).norm()
+    K.check_status()
+
+
 @pytest.mark.parametrize("rows,N,C", [(16384, 2048, 1024), (29140, 1376, 256), (9000, 1000, 100)])
 def test_weight_gradient_repeats(A, K, rows, N, C):
     """Two hundred launches, several chains of products each, give the same bits, which are the exact sums."""
