@@ -465,6 +465,8 @@ def test_attention_of_scores_far_below_zero(A, K, hd, L, sign):
     K.check_status()
 
 
+@pytest.mark.parametrize("hd,L,B,H", [(64, 2100, 1, 40), (64, 2100, 3, 25), (64, 9000, 1, 9), (128, 2100, 1, 20),
+                                      (128, 2100, 2, 19), (128, 5000, 1, 7)])
 def test_attention_of_more_heads_than_are_worked_on_at_once(A, K, hd, L, B, H):
     """Heads go in groups (34 MB of what they read and add to), the last of them smaller, whose tiles are split;
     every head against the formula, from 8 bits and in bf16, and against the fixed order, which has one group."""
