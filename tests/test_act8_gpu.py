@@ -465,6 +465,34 @@ def test_attention_of_scores_far_below_zero(A, K, hd, L, sign):
     K.check_status()
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("L", [333, 1025, 2049])
+def test_attention_rounds_twice_on_the_way(A, K, hd, L):
+    """What is rounded to bf16 is P or dS and then the result, 1.66e-3 of the norm each (half a unit, evenly spread,
+    over normally distributed values), together 2.35e-3.  A q multiplied by a constant and rounded too would
+    make it 3.0e-3 to 3.6e-3."""
+    ps, lse, go, o = _attention(A, K, 1, L, 3, hd, L)
+    for a, b, name in zip(A.attn_bwd8(*ps, lse, go), _oracle(ps, lse, go), ("dq", "dk", "dv")):
+        rel = ((a.double() - b).norm() / b.norm()).item()
+        assert rel < 2.7e-3, (name, rel)
+    K.check_status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_attention_of_one_token_exponent(A, K, hd):
+    """dV = P go of a single token, where P is the exponential of a difference: off by the (hi, lo) pair of bf16 that
+    holds lse, 2^-16 of it, and by 32-bit sums; then P and dV are rounded to bf16, 2^-8 each."""
+    ps, lse, go, o = _attention(A, K, 3, 1, 5, hd, 4, s=2.0)
+    _, _, want = _oracle(ps, lse, go)
+    q, k = (p.restore().double() for p in ps[:2])
+    size = lse.double().abs().transpose(1, 2)[..., None]
+    exponent = 2.0 ** -16 * size + 8 * 2.0 ** -23 * (size + hd ** -0.5 * (q * k).abs().sum(-1, keepdim=True))
+    rel = (1 + torch.expm1(exponent)) * (1 + 2.0 ** -22) * (1 + 2.0 ** -8) ** 2 - 1
+    dv = A.attn_bwd8(*ps, lse, go)[2]
+    assert ((dv.double() - want).abs() <= rel * want.abs() + 1e-30).all()
+    K.check_status()
+
+
 @pytest.mark.parametrize("hd,L,B,H", [(64, 2100, 1, 40), (64, 2100, 3, 25), (64, 9000, 1, 9), (128, 2100, 1, 20),
                                       (128, 2100, 2, 19), (128, 5000, 1, 7)])
 def test_attention_of_more_heads_than_are_worked_on_at_once(A, K, hd, L, B, H):
