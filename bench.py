@@ -236,6 +236,7 @@ def run_ours(args):
                        "global_batch": B * world, "seq_len": TOKENS[args.config],
                        "parallelism": f"dp{world}", "grad_sync": cfg.parallel.grad_sync
                        if world > 1 else "none", "optimizer": cfg.optim.optimizer,
+                       "activations": cfg.model.act_store + (", blocks recomputed" if cfg.model.grad_checkpoint else ""),
                        "l2": "256 MiB buffer written between timed steps (inside the timed "
                              "region); per-step working set is several GB"},
             "clocks": clocks,
@@ -243,6 +244,7 @@ def run_ours(args):
                     "h2d_bytes_per_step": h2d, "d2h_bytes_per_step": 3 * 8 + 8,
                     "loss": last.get("loss")},
             "gpu_launches": n_launch,
+            "peak_memory_bytes": torch.cuda.max_memory_allocated(device) if device.type == "cuda" else None,
         }
         if phases is not None:
             out["phases_ms_max_over_ranks"] = phases
