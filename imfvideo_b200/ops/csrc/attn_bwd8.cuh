@@ -25,8 +25,8 @@ struct Bwd8Rows {
   const int64_t *o_strides, *g_strides;
 };
 
-// head_dim 64: c1, c2 = bands of 16 bf16 a row, -lse / scale and -delta as (hi, lo) pairs and zeros (padding rows: the
-// exponent -30000); inv_exp_scale = 1 / (scale * log2 e).  head_dim 128: c1, c2 = lse * log2 e (padding: infinity) and
+// head_dim 64: c1, c2 = bands of 16 bf16 a row that the tensor core adds up, -lse / scale and -delta in three parts and
+// zeros (padding rows: the exponent -30000); inv_exp_scale = 1 / (scale * log2 e).  head_dim 128: c1, c2 = lse * log2 e (padding: infinity) and
 // delta, one fp32 a row.  head_dim / 8 lanes a row, 8-byte accesses to codes and 16-byte ones besides.
 template <int HD, bool V8, bool O8>
 __global__ void attn_bwd_prep8_kernel(Bwd8Packed p, __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ k,
@@ -78,10 +78,13 @@ __global__ void attn_bwd_prep8_kernel(Bwd8Packed p, __nv_bfloat16* __restrict__ 
   }
   x = (live ? fminf(fmaxf(x, -30000.f), 30000.f) : 30000.f) * inv_exp_scale;
   uint32_t wq = 0u, wd = 0u;                     // 16 bf16 = 8 words per row, one per lane of the row
-  if (part == 0) {
-    const float xh = bf16_lo(pack_bf16(-x, 0.f)), dh = bf16_lo(pack_bf16(-d, 0.f));
-    wq = pack_bf16(xh, -x - xh);
-    wd = pack_bf16(dh, -d - dh);
+  if (part < 2) {                                // three parts of 8 bits each hold all 24 of a 32-bit number
+    const auto word = [part](float v) {
+      const float hi = bf16_lo(pack_bf16(v, 0.f)), mid = bf16_lo(pack_bf16(v - hi, 0.f));
+      return part == 0 ? pack_bf16(hi, mid) : pack_bf16(v - hi - mid, 0.f);
+    };
+    wq = word(-x);
+    wd = word(-d);
   }
   c1[row * 8 + part] = wq;
   c2[row * 8 + part] = wd;

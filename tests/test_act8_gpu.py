@@ -524,6 +524,34 @@ def test_attention_of_more_heads_than_are_worked_on_at_once(A, K, hd, L, B, H):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [500, 2000])
+def test_attention_of_large_scores(A, K, hd, size):
+    """Scores near 500 and 2,000, and delta of that size: P and dS are exponentials and products of differences of numbers
+    that large, which 16 bits (a pair of bf16) would get wrong by 2^-17 of them: 0.8 and 3 % of P."""
+    B, L, H = 1, 300, 2
+    g = _gen(70)
+    q, k, v, go = (_randn(g, B, L, H, hd) for _ in range(4))
+    q[..., 0], k[..., 0] = 16.0, round(size * hd ** 0.5 / 16 / 4) * 4.0
+    v[..., 0], go[..., 0] = 64.0, size / 64
+    q8, k8, v8 = A.store8([q, k, v])
+    z = [p.restore().double() for p in (q8, k8, v8)]
+    s = torch.einsum("blhd,bmhd->bhlm", z[0], z[1]) * hd ** -0.5
+    lse = torch.logsumexp(s, -1).float()
+    o8 = A.store8(torch.einsum("bhlm,bmhd->blhd", torch.softmax(s, -1), z[2]).to(BF16))
+    assert lse.min() > 0.9 * size and (o8.restore()[..., 0] == 64).all()
+    got = A.attn_bwd8(q8, k8, v8, o8, lse, go)
+    want = _oracle((q8, k8, v8, o8), lse, go)
+    # two roundings to bf16 (2.35e-3, see test_attention_rounds_twice_on_the_way); lse in 32 bits, 2^-25 of it on the
+    # average, is the oracle's too; what the tensor core drops of sums of `size`, 2^-25 of the sum in each of 5 (9)
+    # steps and its conversion by scale, less than 2^-21 size = 1e-3 at 2,000.  (Channel 0 of k is one value: its
+    # dQ is a sum that cancels.)
+    for a, b, name in zip((got[0][..., 1:], got[1], got[2]), (want[0][..., 1:], want[1], want[2]), ("dq", "dk", "dv")):
+        rel = ((a.double() - b).norm() / b.norm()).item()
+        assert rel < 4e-3, (name, rel)
+    K.check_status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 def test_attention_strides_of_single_dimensions(A, K, hd):
     """The stride of a dimension of one element is anything: no address depends on it."""
     for shape, strides in (((1, 65, 2, hd), (1, 2 * hd, hd, 1)), ((1, 65, 1, hd), (3, hd, 5, 1)),
