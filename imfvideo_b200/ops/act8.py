@@ -3,9 +3,10 @@
 
 What a training step keeps of every transformer block is most of its memory.  ``store8`` writes
 activations as one signed byte a channel and one step byte for each 32 channels of a row; the value
-is code * 2^(step - 127), at most half a step (1/127.5 of the group's largest magnitude) off.  The
-step is a power of two, so the values are exact in bf16 and the tensor cores multiply what was
-stored.  A group that holds a NaN or an infinity reads as NaN throughout.
+is code * 2^(step - 127), at most half a step off: 1/127.5 of the group's largest magnitude, or 2^-128
+in groups below 2^-121 or so, and up to a step for fp32 above the largest bf16.  The step is a
+power of two, so the values are exact in bf16 and the tensor cores multiply what was stored.  A
+group that holds a NaN or an infinity reads as NaN throughout.
 
     packed = store8([x, y, z])                # one launch, one allocation
     x, y, z = restore8(packed)                # back to their types

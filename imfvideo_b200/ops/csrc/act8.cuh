@@ -3,8 +3,9 @@
 // A row is cut into groups of 32 channels.  A group has one step byte s and a signed code for every
 // channel; the value is code * 2^(s - 127).  With amax the group's largest magnitude,
 //     s = clamp(floor(log2 amax) + 127 - 6 (+ 1 where amax would round to 128 steps), 0, 248)
-// so the largest code is 64 .. 127 and a value is off by half a step at most, amax / 127.5.  (Above
-// 127.5 * 2^121, the last 1/256 below the largest bf16, codes stop at 127.)  The step is a power of two
+// so the largest code of a step above the smallest is 64 .. 127 and a value is off by half a step at most, amax / 127.5.
+// Groups below 64 steps of 2^-127 have that smallest step, half of which is 2^-128 whatever amax is; above the
+// largest bf16, 127.5 * 2^121, which only fp32 has, codes stop at 127, up to a step off.  The step is a power of two
 // because the value is then exact in bf16 -- 7 bits of significand -- and a tensor core that is fed the
 // codes converted to bf16 multiplies what was stored, with no second rounding.
 // s = 255: the group held a NaN or an infinity; all of it reads as NaN.

@@ -23,21 +23,17 @@
 // fixed).  Storing a chain's sum runs under the next one's products where TMEM holds two accumulators; with BN 512
 // it holds one, whose halves are stored and begun again one after the other, at some 4 us a chain.
 //
-// What bounds it: shared memory.  For a k-block of BN 256 a CTA moves 24 KB in by TMA, 24 KB through the conversion and
-// 32 KB into the tensor core, 640 clocks at 128 bytes against 512 of tcgen05.mma (BN 512, whose two accumulators
-// share the rows of dY^T: 1,152 against 1,024); 900 and 1,230 are measured.  Without the converted tile's stores it
-// would take 12 % less, without three of four products 6 %; rings of five or seven stages make no difference.
-// 32,780 rows x 5,472 x 1,024: 322 us (1,140 TFLOP/s) with BN 512, 381 with 256; without chains 305, and then one CTA
-// per tile 372 (256 x 256) to 620 us (128 x 256); restoring X to bf16 first and the bf16 kernel of gemm.cu 428.
-// 29,140 x 1,376 x 256: 35 us, the bf16 kernel alone 45.  One ring and one loading warp for dY, codes and steps took 2 to 6
-// % longer (its instructions, 730 clocks a k-block, were the pace).  Tried and slower: codes loaded into registers
-// by the converting warps (594 us at 5,472 x 1,024: the proxy fence waits for the loads) or by cp.async
-// (463; no difference at 1,376 x 256); remote arrivals and
-// waits with cluster scope (627 us: the release waits for everything the thread has in flight); one barrier for dY
-// and the converted tile (2 to 4 %); more polls before the clock is read (2 %), or fewer; the k-blocks of
-// all tiles dealt to the pairs in equal runs (356 us: pairs at different rows share nothing in L2); sums added from
-// registers, eight lanes a line (362 instead of 338 by TMA).  Chains that end at other times in other
-// pairs gain 0.6 %.
+// What bounds it.  For a k-block of BN 256 a CTA moves 24 KB in by TMA, 24 KB through the conversion and 32 KB into the
+// tensor core, 640 clocks of shared memory at 128 bytes, against 512 of tcgen05.mma (BN 512, whose two accumulators share
+// the rows of dY^T: 1,152 against 1,024); 900 and 1,230 are measured.  Neither sets the pace alone: without the
+// converted tile's stores it takes 12 % less, without three of four products 6 %.  What makes up the rest is not known;
+// rings of five or seven stages and fewer or more polls of the barriers do not change it.
+// 32,780 rows x 5,472 x 1,024: 334 us alone (1,100 TFLOP/s; among other passes, at the power cap, some 400), of which
+// the ends of the chains are 20 and the kernel that adds the planes up 20 to 27; restoring X to bf16 first and the bf16
+// kernel of gemm.cu 428.  29,140 x 1,376 x 256: 37 us, the bf16 kernel alone 45.  Into a gradient buffer 4 and 2 us more.
+// Tried and slower: one ring and one loading warp for dY, codes and steps (2 to 6 %); codes loaded into registers by
+// the converting warps (594 us: the proxy fence waits for the loads) or by cp.async (463); the k-blocks of all tiles
+// dealt to the pairs in equal runs (9 %: pairs at different rows share nothing in L2); sums added from registers (10 %).
 #include "act8.cuh"
 #include "common.cuh"
 #include "host_util.h"
