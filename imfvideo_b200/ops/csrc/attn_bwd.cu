@@ -207,8 +207,12 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     fence_barrier_init();
   }
   {
-    uint32_t* o32 = reinterpret_cast<uint32_t*>(s.ones);       // every element 1.0: the swizzle
-    for (int i = threadIdx.x; i < BW_T * 32 / 4; i += BW_THREADS) o32[i] = 0x3f803f80u;   // is moot
+    // every element 1.0 (the swizzle is moot, it stays within a row), but zero in rows behind the last key.  Those have
+    // the score zero, and P = exp(-lse) would be infinite from lse = -89 on, dQ infinity times a key of zeros;
+    // this way P is 1 there and dS zero
+    uint32_t* o32 = reinterpret_cast<uint32_t*>(s.ones);
+    for (int i = threadIdx.x; i < BW_T * 32 / 4; i += BW_THREADS)
+      o32[i] = kvb * BW_T + i / 8 < p.L ? 0x3f803f80u : 0u;
     fence_proxy_async_smem();
   }
   if (warp == 12) {
@@ -445,10 +449,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
     const int wl = warp & 3;
     const int row = wl * 32 + lane;     // kv row of this thread (TMEM lane)
     const uint32_t tb = tmem_addr(tmem, wl * 32, 0);
-    // a row behind the last key has the score zero, and P = exp(-lse) is infinite from lse = -89 on: then dQ would be
-    // infinity times a key of zeros.  Its exponents are set to -infinity (before RAW_Q's factor, whose sign counts)
-    const bool no_key = kvb * BW_T + row >= p.L;
-    const uint32_t no_exponent = RAW_Q && p.exp_scale < 0.f ? 0x7f800000u : 0xff800000u;
     bool ok = true;
     for (int i = 0; i < n_q && ok; ++i) {
       const uint32_t par = (uint32_t)(i & 1);
@@ -470,10 +470,6 @@ attn_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant_
         tmem_ld32(tb + BC_S + wg * 64 + 32, sv + 32);
         tc_wait_ld();
         tc_fence_before();
-        if (no_key) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c) sv[c] = no_exponent;
-        }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.s_taken);

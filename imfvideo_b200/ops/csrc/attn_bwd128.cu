@@ -54,7 +54,9 @@ struct Smem {
   alignas(1024) uint8_t d_o[QSTAGES][2 * QPANEL];
   alignas(1024) uint8_t ds[2][KT * 128];              // dS^T: [kv 128][q 64] bf16, one panel
   alignas(1024) uint8_t dq_stage[4 * DQPANEL];        // dQ tile [q 64][hd 128] fp32, 4 panels
-  alignas(16) float lse2[QSTAGES][QT];
+  // the last row is infinity, for the rows behind the last key: their score is zero, and P = exp(-lse) would be infinite
+  // from lse = -89 on, dQ infinity times a key of zeros
+  alignas(16) float lse2[QSTAGES + 1][QT];
   alignas(16) float delta[QSTAGES][QT];
   uint64_t kv_full;
   uint64_t q_full[QSTAGES], q_empty[QSTAGES];
@@ -136,6 +138,7 @@ attn_bwd128_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     s.abort_flag = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x < QT) s.lse2[QSTAGES][threadIdx.x] = INFINITY;
   if (warp == 12) {
     tmem_alloc(&s.tmem_base, 512);
     tmem_relinquish();
@@ -319,11 +322,7 @@ attn_bwd128_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
     const int row = wl * 32 + lane;     // kv row of this thread (TMEM lane)
     const uint32_t tb = tmem_addr(tmem, wl * 32, 0);
     const float scale_log2 = p.scale * 1.4426950408889634f;
-    // a row behind the last key has the score zero, and P = exp(-lse) is infinite from lse = -89 on: then dQ would be
-    // infinity times a key of zeros.  Its scores become such that the exponent is -infinity (NaN at a scale of zero,
-    // where P = exp(-lse) is what every key has)
-    const bool no_key = kvb * KT + row >= p.L && scale_log2 != 0.f;
-    const uint32_t no_score = scale_log2 < 0.f ? 0x7f800000u : 0xff800000u;
+    const bool no_key = kvb * KT + row >= p.L;
     bool ok = true;
     for (int i = 0; i < n_q && ok; ++i) {
       const int st = i % QSTAGES;
@@ -337,13 +336,9 @@ attn_bwd128_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_consta
       tmem_ld32(tb + BC_DP + wg * 32, dp);
       tc_wait_ld();
       tc_fence_before();
-      if (no_key) {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) sv[c] = no_score;
-      }
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.s_taken);
-      const float4* lse4 = reinterpret_cast<const float4*>(s.lse2[st] + wg * 32);
+      const float4* lse4 = reinterpret_cast<const float4*>(s.lse2[no_key ? QSTAGES : st] + wg * 32);
       const float4* dl4 = reinterpret_cast<const float4*>(s.delta[st] + wg * 32);
       // all of the tile's math first, from registers only: it overlaps the dV / dK / dQ MMAs
       // of the previous tile, which still read P^T (TMEM) and dS^T (shared memory)
