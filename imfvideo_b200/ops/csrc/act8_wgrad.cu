@@ -399,7 +399,8 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
     }
   } else {
     // ---------------------------------------------------------- epilogue --
-    uint32_t ch = 0, step = 0;
+    uint32_t ch = 0, step = 0, chains = 0;           // chains so far, in all
+    for (Walk all = walk; all.next(w);) chains += (w.kb1 - w.kb0 + p.chain - 1) / p.chain;
     bool ok = true;
     while (ok && walk.next(w)) {
       const int row0 = m_of(w.tile) + warp * 32, n0 = n_of(w.tile);
@@ -416,7 +417,7 @@ wgrad8_kernel(const __grid_constant__ CUtensorMap tm_a, const __grid_constant__ 
           const auto done = [&] {
             tc_fence_before();
             __syncwarp();
-            if (lane == 1) arrive_first_cluster(&s.acc_empty[acc]);
+            if (lane == 1 && ch + (NH == 2 ? 1 : 2) < chains) arrive_first_cluster(&s.acc_empty[acc]);   // used again
             read = true;
           };
 #pragma unroll 1
