@@ -28,7 +28,7 @@
 // the rows of dY^T: 1,152 against 1,024); 900 and 1,230 are measured.  Neither sets the pace alone: without the
 // converted tile's stores it takes 12 % less, without three of four products 6 %.  What makes up the rest is not known;
 // rings of five or seven stages and fewer or more polls of the barriers do not change it.
-// 32,780 rows x 5,472 x 1,024: 334 us alone (1,100 TFLOP/s; among other passes, at the power cap, some 400), of which
+// 32,780 rows x 5,472 x 1,024: 334 us alone (1,100 TFLOP/s; among other passes, at the power cap, 380 to 410), of which
 // the ends of the chains are 20 and the kernel that adds the planes up 20 to 27; restoring X to bf16 first and the bf16
 // kernel of gemm.cu 428.  29,140 x 1,376 x 256: 37 us, the bf16 kernel alone 45.  Into a gradient buffer 4 and 2 us more.
 // Tried and slower: one ring and one loading warp for dY, codes and steps (2 to 6 %); codes loaded into registers by

@@ -77,8 +77,8 @@ struct BwSmem {
   alignas(1024) uint8_t ds[2 * BW_T * 128];          // dS^T: [kv 128][q 128] as two 64-col panels
   alignas(1024) float dq_stage[BW_T * BW_HD];        // dQ tile staged for the TMA reduce-add
   alignas(1024) uint8_t ones[BW_T * 32];             // [128][16] bf16 1.0, 32-byte rows (SWIZZLE_32B)
-  alignas(1024) uint8_t augq[BW_QSTAGES][BW_T * 32]; // [q 128][16]: -lse2 as (hi, lo), zeros
-  alignas(1024) uint8_t augd[BW_QSTAGES][BW_T * 32]; // [q 128][16]: -delta as (hi, lo), zeros
+  alignas(1024) uint8_t augq[BW_QSTAGES][BW_T * 32]; // [q 128][16]: -lse2 as (hi, lo) (RAW_Q: in three parts), zeros
+  alignas(1024) uint8_t augd[BW_QSTAGES][BW_T * 32]; // [q 128][16]: -delta likewise
   uint64_t kv_full;
   uint64_t q_full[BW_QSTAGES], q_empty[BW_QSTAGES];
   uint64_t s_full, s_taken, dp_full, p_ready, p_free, ds_ready;
