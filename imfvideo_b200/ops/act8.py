@@ -227,13 +227,22 @@ def _apart(dims: List[Tuple[int, int]], run: int) -> bool:
     return dims[0][0] > 0 and bool((_starts(dims).sort().values.diff() >= run).all())      # strides that interleave
 
 
+def _span(t: Tensor) -> Tuple[int, int]:
+    """First and last byte + 1 of a tensor."""
+    at, n = t.data_ptr(), t.numel()
+    if n and not t.is_contiguous():
+        n = 1 + sum(s * (m - 1) for m, s in zip(t.shape, t.stride()))
+    return at, at + n * t.element_size()
+
+
 def _in_one_place(a: Tensor, b: Tensor) -> bool:
     """Whether two tensors, each of elements apart, share memory."""
-    if a.data_ptr() > b.data_ptr():
-        a, b = b, a
-    (da, ra), (db, rb), es, d = _places(a), _places(b), a.element_size(), b.data_ptr() - a.data_ptr()
-    if a.numel() == 0 or b.numel() == 0 or d >= (sum(s * (n - 1) for s, n in da) + ra) * es:
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    if a1 <= b0 or b1 <= a0 or a0 == a1 or b0 == b1:
         return False
+    if a0 > b0:
+        a, b, a0, b0 = b, a, b0, a0
+    (da, ra), (db, rb), es, d = _places(a), _places(b), a.element_size(), b0 - a0
     if da == db and b.element_size() == es and d % es == 0 and d >= ra * es and _apart(da, d // es + rb):
         return False                           # two bands of one buffer
     at = torch.cat([_starts(da) * es, _starts(db) * b.element_size() + d])
@@ -241,6 +250,16 @@ def _in_one_place(a: Tensor, b: Tensor) -> bool:
         torch.tensor([a.numel() // ra, b.numel() // rb]))
     at, order = at.sort()
     return bool((at[1:] < end[order][:-1]).any())
+
+
+def _share(ts: Sequence[Tensor]) -> bool:
+    """Whether any two of several tensors share memory."""
+    if len(ts) < 2:
+        return False
+    spans = sorted((*_span(t), i) for i, t in enumerate(ts))
+    if all(a[1] <= b[0] for a, b in zip(spans, spans[1:])):
+        return False
+    return any(_in_one_place(a, b) for i, a in enumerate(ts) for b in ts[:i])
 
 
 def _launch(fn_name: str, recs: List[int]) -> None:
@@ -334,8 +353,7 @@ def restore8(ps: Union[Packed8, Sequence[Packed8]], outs=None) -> Union[Tensor, 
         if o is not None and (o.shape != p.shape or o.dtype != p.dtype):
             raise ValueError(f"output {o.dtype} {tuple(o.shape)} for packed {p.dtype} {tuple(p.shape)}")
     given = [o for o in outs if o is not None]
-    if not all(o.is_contiguous() or _apart(*_places(o)) for o in given) or \
-            any(_in_one_place(a, b) for i, a in enumerate(given) for b in given[:i]):
+    if not all(o.is_contiguous() or _apart(*_places(o)) for o in given) or _share(given):
         raise ValueError("restore8 output: no two elements in one place, of one output or of two")
     if dev.type != "cuda":
         for i, p in enumerate(ps):

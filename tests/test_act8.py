@@ -229,6 +229,33 @@ def test_outputs_that_share_memory():
     assert torch.equal(act8.restore8([f, a], [out, None])[0], f.restore())
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_sharing_of_memory_is_found(seed):
+    """Two or three random outputs of a small buffer: refused exactly where two of their elements have one place."""
+    import random
+
+    rng = random.Random(seed)
+    refused = taken = 0
+    for _ in range(30):
+        buf, ps, outs, places = torch.zeros(400, dtype=BF16), [], [], []
+        for _ in range(rng.choice([1, 2, 3])):
+            shape = [rng.choice([1, 1, 2, 3]) for _ in range(rng.choice([1, 2]))] + [rng.choice([1, 2, 5, 8])]
+            strides = [rng.choice([0, 1, 3, 8, 8, 16, 16, 24, 40]) for _ in shape[:-1]] + [1]
+            out = buf.as_strided(shape, strides, rng.choice([0, 5, 8, 16, 100, 200, 200 + rng.randrange(60)]))
+            ps.append(act8.store8(torch.randn(shape).bfloat16()))
+            outs.append(out)
+            places += torch.arange(400).as_strided(shape, strides, out.storage_offset()).flatten().tolist()
+        if len(set(places)) == len(places):
+            for p, o in zip(ps, act8.restore8(ps, outs)):
+                assert torch.equal(o, p.restore())
+            taken += 1
+        else:
+            with pytest.raises(ValueError):
+                act8.restore8(ps, outs)
+            refused += 1
+    assert refused and taken
+
+
 def test_attention_outputs_that_share_memory():
     q = act8.store8(torch.randn(2, 4, 2, 64).bfloat16())
     go, lse = torch.randn(2, 4, 2, 64).bfloat16(), torch.zeros(2, 2, 4)
