@@ -569,6 +569,37 @@ def test_attention_strides_of_single_dimensions(A, K, hd):
     K.check_status()
 
 
+@pytest.mark.parametrize("hd,L", [(64, 67001), (128, 34001)])
+def test_attention_of_one_head_at_a_time(A, K, hd, L):
+    """Sequences so long that a single head is more than a group: as in the fixed order, which has one group.  The two
+    differ in the order of 32-bit sums, which moves a result across a rounding to bf16 (2^-8) now and then."""
+    assert 34000000 // (L * hd * 8) == 0
+    ps, lse, go, o = _attention(A, K, 1, L, 2, hd, 8)
+    got = A.attn_bwd8(*ps, lse, go)
+    was = K.DETERMINISTIC
+    K.set_deterministic(True)
+    try:
+        fixed = A.attn_bwd8(*ps, lse, go)
+    finally:
+        K.set_deterministic(was)
+    K.check_status()
+    for h in range(2):
+        for a, b in zip(got, fixed):
+            a, b = a[:, :, h].double(), b[:, :, h].double()
+            assert (a - b).norm() <= 1e-3 * b.norm() and (a - b).abs().max() <= 2.0 ** -7 * b.abs().max()
+    # rows of dQ in the first, a middle and the last tile, and the same of dK and dV, against the formula
+    q, k, v, o8 = (p.restore() for p in ps)
+    rows = torch.tensor([0, 1, 127, L // 2, L - 2, L - 1], device="cuda")
+    for h in range(2):
+        Q, Kk, V, O, G = (t[0, :, h].double() for t in (q, k, v, o8, go))
+        stat, delta = lse[0, h].double(), (G * O).sum(1)
+        P = torch.exp(Q[rows] @ Kk.t() * hd ** -0.5 - stat[rows, None])
+        dq = (P * (G[rows] @ V.t() - delta[rows, None])) @ Kk * hd ** -0.5
+        P = torch.exp(Kk[rows] @ Q.t() * hd ** -0.5 - stat)
+        want = (dq, (P * (V[rows] @ G.t() - delta)) @ Q * hd ** -0.5, P @ G)
+        _near([t[0, rows, h] for t in got], want, h)
+
+
 def test_attention_gradient_is_a_difference_quotient(A, K):
     """Along a random direction of q, k and v the loss changes as the gradients say (64-bit differences)."""
     B, L, H, hd = 1, 40, 2, 64
