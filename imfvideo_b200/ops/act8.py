@@ -425,7 +425,8 @@ def gemm_wgrad8(dy: Tensor, x8: Packed8, out: Optional[Tensor] = None, accumulat
 def situ_bwd8(gu8: Packed8, gout: Tensor, beta: float, lbeta: Optional[float]) -> Tuple[Tensor, Tensor]:
     """Reverse mode of y = situ(gate) up' from the packed [gate | up] (rows, 2F): returns (its
     gradient (rows, 2F), y (rows, F)), bf16 -- y is what the next layer's weight gradient multiplies, so
-    it need not be kept.  ``gout`` (rows, F) bf16, adjacent columns."""
+    it need not be kept.  ``gout`` (rows, F) bf16, adjacent columns; the betas are positive normal numbers of
+    32 bits."""
     if not isinstance(gu8, Packed8) or gu8.dtype != BF16 or gu8.cols % 2:
         raise ValueError("situ_bwd8 takes a bf16 [gate | up] packed by store8")
     rows, F = gu8.rows, gu8.cols // 2
@@ -465,7 +466,8 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
         dQ = scale dS k,  dK = scale dS^T q
 
     v and o may also be bf16 tensors (a band of a wider buffer that is restored anyway).  ``gv_out``
-    takes dv, as in ``kernels.attn_bwd``, whose fixed-order mode holds here too."""
+    takes dv (16-byte aligned rows, no two elements in one place), as in ``kernels.attn_bwd``, whose
+    fixed-order mode holds here too.  ``scale`` is finite, of either sign."""
     for name, t in (("q", q8), ("k", k8)):
         if not isinstance(t, Packed8):
             raise ValueError(f"attn_bwd8: {name} has to be packed by store8")
@@ -483,7 +485,7 @@ def attn_bwd8(q8: Packed8, k8: Packed8, v8: Union[Packed8, Tensor], o8: Union[Pa
         new = lambda: _new(shape, BF16, dev)
         return new(), new(), new() if gv_out is None else gv_out
     scale = hd ** -0.5 if scale is None else float(scale)
-    if not abs(scale) <= _F32_MAX:
+    if not abs(scale) <= _F32_MAX / 2:         # the kernels multiply it by log2 e
         raise ValueError(f"attn_bwd8: scale {scale}")
     if gv_out is not None and not _apart(*_places(gv_out)):
         raise ValueError("attn_bwd8: no two elements of the dv output in one place")
