@@ -76,7 +76,8 @@ __global__ void attn_bwd_prep8_kernel(Bwd8Packed p, __nv_bfloat16* __restrict__ 
     }
     return;
   }
-  x = (live ? fminf(fmaxf(x, -30000.f), 30000.f) : 30000.f) * inv_exp_scale;
+  // (infinities become what is still finite over the smallest scale, 1e-30)
+  x = (live ? fminf(fmaxf(x, -1e8f), 1e8f) : 30000.f) * inv_exp_scale;
   uint32_t wq = 0u, wd = 0u;                     // 16 bf16 = 8 words per row, one per lane of the row
   if (part < 2) {                                // three parts of 8 bits each hold all 24 of a 32-bit number
     const auto word = [part](float v) {

@@ -552,6 +552,31 @@ def test_attention_of_large_scores(A, K, hd, size):
 
 
 @pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_attention_of_scores_beyond_the_exponents_of_32_bits(A, K, hd, sign):
+    """Scores near +-25,000, where lse is beyond 2^15 in powers of two."""
+    B, L, H = 1, 200, 2
+    g = _gen(71)
+    q, k, v, go = (_randn(g, B, L, H, hd) for _ in range(4))
+    q[..., 0], k[..., 0] = 512.0, sign * round(25000 * hd ** 0.5 / 512 / 4) * 4.0
+    q8, k8, v8 = A.store8([q, k, v])
+    z = [p.restore().double() for p in (q8, k8, v8)]
+    s = torch.einsum("blhd,bmhd->bhlm", z[0], z[1]) * hd ** -0.5
+    lse = torch.logsumexp(s, -1).float()
+    assert (lse.abs() > 22000).all()
+    o8 = A.store8(torch.einsum("bhlm,bmhd->blhd", torch.softmax(s, -1), z[2]).to(BF16))
+    got = A.attn_bwd8(q8, k8, v8, o8, lse, go)
+    want = _oracle((q8, k8, v8, o8), lse, go)
+    # two roundings to bf16, 2.4e-3; lse log2 e and the scale are each rounded, 2^-24 of 36,000 = 2.2e-3; sums of 2^18 in the
+    # tensor core drop up to 2^-7 a step (with a bit or two below 32 bits' last), 5 or 9 steps over a scale of 1 / 8 or
+    # 1 / 11: 6e-3; all together 1.3e-2, mostly of one sign
+    for a, b, name in zip((got[0][..., 1:], got[1], got[2]), (want[0][..., 1:], want[1], want[2]), ("dq", "dk", "dv")):
+        rel = ((a.double() - b).norm() / b.norm()).item()
+        assert rel < 1.3e-2, (name, rel)
+    K.check_status()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
 def test_attention_strides_of_single_dimensions(A, K, hd):
     """The stride of a dimension of one element is anything: no address depends on it."""
     for shape, strides in (((1, 65, 2, hd), (1, 2 * hd, hd, 1)), ((1, 65, 1, hd), (3, hd, 5, 1)),
