@@ -1,0 +1,58 @@
+// Host-side interface of differential attention (attn_diff_fwd.cu, attn_diff_bwd.cu).
+//
+// Heads 2j and 2j + 1 of q, k, v (B, L, 2H, 64) form pair j.  Both maps of a pair multiply the pair's
+// values side by side, V = [v_2j | v_2j+1] (128 channels):
+//   A_m = softmax(scale q_m k_m^T),  O_m = A_m V,  o = O_1 - lam O_2
+//
+// The backward pass needs delta_m = rowsum(dO .* O_m), and an error of delta moves every dS of its row the same
+// way: from o and O_2 in bf16, dQ was 1.1 % of its norm off at 29,140 tokens whose values have an offset (what
+// the keys of a row have in common adds up, what tells them apart averages out).  So the forward pass also
+// keeps a signed byte for each value, what bf16 dropped in 1/256 of its last place: 16 bits in all.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace imf {
+
+// The pairs' weights: bf16 or fp32, `stride` elements apart (0: one weight for all pairs).
+struct DiffWeights {
+  const void* p;
+  int64_t stride;
+  int is_bf16;
+  __device__ __forceinline__ float at(int pair) const {
+    return is_bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p)[pair * stride])
+                   : static_cast<const float*>(p)[pair * stride];
+  }
+};
+
+// Eight values as bf16 and what that dropped, and back.
+__device__ __forceinline__ void diff_split8(const float* x, uint4& hi, uint2& low) {
+  uint32_t w[4], c[2] = {0u, 0u};
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i / 2]) : "f"(x[i + 1]), "f"(x[i]));
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const uint32_t bits = u ? w[i / 2] & 0xffff0000u : w[i / 2] << 16;
+      // last place 2^(e - 134), e the exponent's field; below 2^-112 the codes are zero
+      const int e = max((int)((bits >> 23) & 255u), 15);
+      const int code = __float2int_rn((x[i + u] - __uint_as_float(bits)) * __uint_as_float((uint32_t)(269 - e) << 23));
+      c[(i + u) / 4] |= (uint32_t)(max(-127, min(127, code)) & 255) << (8 * ((i + u) & 3));
+    }
+  }
+  hi = make_uint4(w[0], w[1], w[2], w[3]);
+  low = make_uint2(c[0], c[1]);
+}
+__device__ __forceinline__ void diff_join8(const uint4& hi, const uint2& low, float* x) {
+  const uint32_t w[4] = {hi.x, hi.y, hi.z, hi.w}, c[2] = {low.x, low.y};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t bits = (i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16;
+    const int e = (int)((bits >> 23) & 255u), code = (int)(c[i / 4] << (24 - 8 * (i & 3))) >> 24;
+    const float step = e > 15 ? __uint_as_float((uint32_t)(e - 15) << 23) : 0.f;
+    x[i] = fmaf((float)code, step, __uint_as_float(bits));
+  }
+}
+
+}  // namespace imf

@@ -1,0 +1,982 @@
+// Differential attention forward on tcgen05 / TMEM, primal and fused forward-mode tangent
+// (see attn_diff.h for the pairing of heads):
+//
+//   S_m = Q_m K_m^T * scale,  A_m = softmax(S_m),  O_m = A_m V,  o = O_1 - lam O_2
+//   dS_m = (dQ_m K_m^T + Q_m dK_m^T) * scale,  T_m = A_m .* (dS_m - rowsum(A_m dS_m)),
+//   do = (T_1 V + A_1 dV) - lam (T_2 V + A_2 dV)
+//
+// Each map is a flash attention of its own, q and k 64 wide and V 128, with its own running maximum
+// and sum; what they share is V.  O_1 and O_2 are divided and subtracted in 32 bits and rounded once.
+//
+// TMEM (512 columns of fp32 per SM) decides the shapes:
+//   primal  : an item is 128 query rows of a pair.  Each map has a slot of its own: S (64), O (128),
+//             P (bf16, 32) and four softmax warps, so K_1, K_2 and V are read once for both maps, and
+//             the epilogue reads both O (the warps of a lane quadrant see its lanes in every column).
+//   tangent : O | dO of one map (256) and two S | dS buffers leave no room for the other map.  A segment
+//             runs map 1, then map 2, over the same K/V tiles; map 1's finished rows wait in global
+//             memory (128 KB a CTA, in L2) and come back to the thread that wrote them.
+// Q K^T and P V of the primal are issued by two warps, so that neither waits for the other's barriers.
+// Scheduling, shares and records of split items are those of attn_fwd_split.h, with a record for each
+// map; the kernel that merges the parts also subtracts.
+#include "attn_diff.h"
+#include "attn_fwd_split.h"
+#include "common.cuh"
+#include "host_util.h"
+
+namespace imf {
+namespace diff {
+
+constexpr int HD = 64;               // channels of a query or key
+constexpr int VD = 128;              // channels of a pair's values
+constexpr int TM = 128;              // query rows per item
+constexpr int BN = 64;               // K/V rows per tile
+constexpr int QPANEL = TM * 128;     // bytes of a query tile (64 columns)
+constexpr int KPANEL = BN * 128;     // bytes of 64 columns of a K/V tile
+constexpr int SOFT_WARPS = 8;
+constexpr int WARP_MMA = 8, WARP_TMA = 9, WARP_PV = 10;   // primal: WARP_MMA issues Q K^T only
+constexpr int THREADS = 12 * 32;
+constexpr int REG_SOFT = 216, REG_OTHER = 72, REG_LAUNCH = 168;
+static_assert(SOFT_WARPS * 32 * REG_SOFT + (THREADS - SOFT_WARPS * 32) * REG_OTHER <= THREADS * REG_LAUNCH,
+              "register pool exceeded");
+constexpr float LOG2E = 1.4426950408889634f;
+
+// A record of a partial segment, for each map: accumulators [column][row] (o, then do), m, l, mu.
+template <bool TANGENT>
+struct Rec {
+  static constexpr int ACC = TANGENT ? 2 * VD : VD;
+  static constexpr int STATS = ACC * TM;
+  static constexpr size_t MAP = (size_t)TM * (ACC + 3), ALL = 2 * MAP;
+  static constexpr float PART_COST = TANGENT ? 0.9f : 0.6f;  // see fwd_share_cost
+};
+constexpr size_t HOLD = (size_t)TM * 2 * VD;      // floats a CTA holds of map 1 (tangent)
+
+struct Params {
+  __nv_bfloat16 *o, *dout, *o2;      // o2: O_2 for the backward pass, or null
+  int8_t* low;                       // what bf16 dropped of o, then (plane elements on) of o2; null with o2
+  int64_t plane;
+  float* lse;                        // (B, 2H, L) or null
+  float* scratch;                    // records of split items
+  float* hold;                       // tangent: the held rows of map 1, HOLD a CTA
+  DiffWeights lam;
+  int B, H, L;                       // H pairs
+  int n_qblk;
+  FwdShares sh;
+  int64_t o_sb, o_sl, o_sh;          // o, dout and o2
+  float scale;
+  int* status;
+};
+
+IMF_DEVICE void item_coords(const Params& p, int item, int& q0, int& h, int& b) {
+  q0 = (item % p.n_qblk) * TM;
+  h = (item / p.n_qblk) % p.H;
+  b = item / (p.n_qblk * p.H);
+}
+
+// Eight channels of o or (which = 1) O_2 at element `at`.
+IMF_DEVICE void store_out8(const Params& p, int which, int64_t at, const float* x) {
+  uint4 hi;
+  uint2 low;
+  diff_split8(x, hi, low);
+  *reinterpret_cast<uint4*>((which ? p.o2 : p.o) + at) = hi;
+  if (p.low) *reinterpret_cast<uint2*>(p.low + which * p.plane + at) = low;
+}
+
+// ------------------------------------------------------------------ primal ---
+constexpr int P_STAGES = 4;
+constexpr int P_SLOT = 256, P_COL_S = 0, P_COL_O = BN, P_COL_P = BN + VD;    // TMEM columns of a map
+static_assert(P_COL_P + BN / 2 <= P_SLOT, "TMEM budget");
+
+struct PSmem {
+  alignas(1024) uint8_t q[2][QPANEL];
+  alignas(1024) uint8_t k[P_STAGES][2][KPANEL];      // K_1, K_2
+  alignas(1024) uint8_t v[P_STAGES][2][KPANEL];      // the two halves of V
+  float inv_l[2][TM];                                // 1 / l of either map
+  uint64_t q_full, q_empty;
+  uint64_t k_full[P_STAGES], k_empty[P_STAGES];
+  uint64_t v_full[P_STAGES], v_empty[P_STAGES];
+  uint64_t s_full[2], s_taken[2], p_full[2];
+  uint64_t o_done[2];      // every P V
+  uint64_t o_final[2];     // last P V of a segment (one phase per segment, never skipped)
+  uint64_t o_free;
+  uint64_t xbar;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__global__ void __launch_bounds__(THREADS, 1)
+attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  auto& s = *reinterpret_cast<PSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x, G = gridDim.x;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&s.q_full, 1);
+    mbar_init(&s.q_empty, 1);
+    for (int i = 0; i < P_STAGES; ++i) {
+      mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.v_full[i], 1);
+      mbar_init(&s.v_empty[i], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&s.s_full[t], 1);
+      mbar_init(&s.s_taken[t], 4);
+      mbar_init(&s.p_full[t], 4);
+      mbar_init(&s.o_done[t], 1);
+      mbar_init(&s.o_final[t], 1);
+    }
+    mbar_init(&s.o_free, SOFT_WARPS);
+    mbar_init(&s.xbar, SOFT_WARPS);
+    s.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == WARP_MMA) {
+    tmem_alloc(&s.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* abort_flag = &s.abort_flag;
+
+  if (warp >= SOFT_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_OTHER));
+    if (warp == WARP_TMA) {
+      // ------------------------------------------------------ TMA producer --
+      if (elect_one()) {
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+        unsigned kv_it = 0;
+        Segment sg;
+        bool ok = true;
+        for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
+          int q0, h, b;
+          item_coords(p, sg.item, q0, h, b);
+          if (si > 0) ok = mbar_wait(&s.q_empty, (si - 1) & 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&s.q_full, 2 * QPANEL);
+          for (int m = 0; m < 2; ++m) tma_load_4d(s.q[m], &tm_q, &s.q_full, 0, 2 * h + m, q0, b);
+          for (int j = sg.j0; j < sg.j1; ++j, ++kv_it) {
+            const int st = (int)(kv_it % P_STAGES);
+            const uint32_t par = (uint32_t)((kv_it / P_STAGES) & 1) ^ 1;
+            if (kv_it >= P_STAGES) {
+              ok = mbar_wait(&s.k_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+              if (!ok) break;
+            }
+            mbar_arrive_expect_tx(&s.k_full[st], 2 * KPANEL);
+            for (int m = 0; m < 2; ++m) tma_load_4d(s.k[st][m], &tm_k, &s.k_full[st], 0, 2 * h + m, j * BN, b);
+            if (kv_it >= P_STAGES) {
+              ok = mbar_wait(&s.v_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+              if (!ok) break;
+            }
+            mbar_arrive_expect_tx(&s.v_full[st], 2 * KPANEL);
+            for (int m = 0; m < 2; ++m) tma_load_4d(s.v[st][m], &tm_v, &s.v_full[st], 0, 2 * h + m, j * BN, b);
+          }
+        }
+      }
+    } else if (warp == WARP_MMA) {
+      // ---------------------------------------------------- Q K^T issuer --
+      if (elect_one()) {
+        constexpr uint32_t idesc_qk = idesc_bf16(TM, BN, 0, 0);
+        const uint64_t q_desc = sdesc_kmajor(smem_u32(s.q[0])), k_desc = sdesc_kmajor(smem_u32(s.k[0][0]));
+        unsigned kv_it = 0;
+        Segment sg;
+        bool ok = true;
+        for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
+          ok = mbar_wait(&s.q_full, si & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA);
+          for (int j = sg.j0; j < sg.j1 && ok; ++j, ++kv_it) {
+            const int st = (int)(kv_it % P_STAGES);
+            ok = mbar_wait(&s.k_full[st], (uint32_t)((kv_it / P_STAGES) & 1), abort_flag, p.status,
+                           STATUS_TIMEOUT_TMA);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              ok = ok && mbar_wait(&s.s_taken[t], (uint32_t)(kv_it & 1) ^ 1, abort_flag, p.status,
+                                   STATUS_TIMEOUT_SOFTMAX);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t qd = q_desc + (uint32_t)(t * (QPANEL >> 4));
+              const uint64_t kd = k_desc + (uint32_t)((2 * st + t) * (KPANEL >> 4));
+#pragma unroll
+              for (int ks = 0; ks < HD / 16; ++ks)
+                mma_ss(tmem + t * P_SLOT + P_COL_S, qd + ks * 2, kd + ks * 2, idesc_qk, ks != 0);
+              tc_commit(&s.s_full[t]);
+            }
+            if (!ok) break;
+            tc_commit(&s.k_empty[st]);
+            if (j + 1 == sg.j1) tc_commit(&s.q_empty);
+          }
+        }
+      }
+    } else if (warp == WARP_PV) {
+      // ------------------------------------------------------ P V issuer --
+      if (elect_one()) {
+        constexpr uint32_t idesc_pv = idesc_bf16(TM, VD, 0, 1);
+        const uint64_t v_desc = sdesc_mnmajor(smem_u32(s.v[0][0]), KPANEL);
+        unsigned kv_it = 0;
+        Segment sg;
+        bool ok = true;
+        for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
+          for (int j = sg.j0; j < sg.j1 && ok; ++j, ++kv_it) {
+            const int st = (int)(kv_it % P_STAGES);
+            ok = mbar_wait(&s.v_full[st], (uint32_t)((kv_it / P_STAGES) & 1), abort_flag, p.status,
+                           STATUS_TIMEOUT_TMA);
+            const uint64_t vd = v_desc + (uint32_t)(st * (2 * KPANEL >> 4));
+            if (j == sg.j0 && si > 0)        // epilogue of the previous segment has drained both O
+              ok = ok && mbar_wait(&s.o_free, (uint32_t)((si - 1) & 1), abort_flag, p.status,
+                                   STATUS_TIMEOUT_SOFTMAX);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              ok = ok && mbar_wait(&s.p_full[t], (uint32_t)(kv_it & 1), abort_flag, p.status,
+                                   STATUS_TIMEOUT_SOFTMAX);
+              if (!ok) break;
+              tc_fence_after();
+              const uint32_t tb = tmem + t * P_SLOT;
+#pragma unroll
+              for (int ks = 0; ks < BN / 16; ++ks)
+                mma_ts(tb + P_COL_O, tb + P_COL_P + ks * 8, vd + 128 * ks, idesc_pv, !(j == sg.j0 && ks == 0));
+              tc_commit(&s.o_done[t]);
+              if (j + 1 == sg.j1) tc_commit(&s.o_final[t]);
+            }
+            if (ok) tc_commit(&s.v_empty[st]);
+          }
+        }
+      }
+    }
+  } else {
+    // --------------------------------------- softmax / correction / epilogue --
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFT));
+    const int t = warp >> 2, wl = warp & 3;         // map; lane quadrant
+    const int row = wl * 32 + lane;
+    const uint32_t tq = tmem_addr(tmem, wl * 32, 0), tb = tq + t * P_SLOT;
+    const float scale_log2 = p.scale * LOG2E;
+    unsigned it = 0;
+    uint32_t xn = 0;                                // exchanges done so far (phase of xbar)
+    Segment sg;
+    bool ok = true;
+    for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
+      int q0, h, b;
+      item_coords(p, sg.item, q0, h, b);
+      const int q_row = q0 + row;
+      float m_used = -INFINITY, l_sum = 0.f, l_sum2 = 0.f;
+      for (int j = sg.j0; j < sg.j1 && ok; ++j, ++it) {
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[t], (uint32_t)(it & 1), abort_flag, p.status,
+                                               STATUS_TIMEOUT_MMA));
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t sv[BN];
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) tmem_ld32(tb + P_COL_S + c, sv + c);
+        // P of the step before has been read, probed here
+        const bool p_ok = it == 0 || mbar_test(&s.o_done[t], (uint32_t)((it - 1) & 1));
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.s_taken[t]);
+        const int kv_rem = p.L - j * BN;
+        if (kv_rem < BN) {
+#pragma unroll
+          for (int i = 0; i < BN; ++i)
+            if (i >= kv_rem) sv[i] = 0xff800000u;  // -inf
+        }
+        const bool first = j == sg.j0;
+        float alpha = 1.f;
+        // Maximum first, so that P can be stored as it is made.  The reference moves only when a row
+        // has outgrown it by more than 2^8.
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < BN; i += 2)
+          asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[(i / 2) & 3]) : "f"(__uint_as_float(sv[i])), "f"(__uint_as_float(sv[i + 1])));
+        mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        const bool need = first || (mx[0] - m_used) * scale_log2 > 8.0f;
+        if (__any_sync(0xffffffffu, need)) {
+          if (need) {
+            if (!first) alpha = ex2((m_used - mx[0]) * scale_log2);
+            m_used = mx[0];
+          }
+          if (!first) {
+            // O, once P V of the step before has run, to the reference that the rows have now
+            ok = __all_sync(0xffffffffu, mbar_wait(&s.o_done[t], (uint32_t)((it - 1) & 1), abort_flag,
+                                                   p.status, STATUS_TIMEOUT_MMA));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c = 0; c < VD; c += 32) {
+              uint32_t ov[32];
+              tmem_ld32(tb + P_COL_O + c, ov);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+              tmem_st32(tb + P_COL_O + c, ov);
+            }
+            tc_wait_st();
+          }
+        }
+        if (!__all_sync(0xffffffffu, p_ok)) {      // P of the step before is still being read
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.o_done[t], (uint32_t)((it - 1) & 1), abort_flag,
+                                                 p.status, STATUS_TIMEOUT_MMA));
+          if (!ok) break;
+        }
+        tc_fence_after();
+        const f32x2 neg_m2 = dup2(-m_used * scale_log2);
+        f32x2 l_new = dup2(0.f);
+#pragma unroll
+        for (int c = 0; c < BN; c += 32) {
+          uint32_t pk[32 / 2];
+#pragma unroll
+          for (int i = 0; i < 32; i += 2) {
+            const f32x2 e = fma2(pair2(sv[c + i], sv[c + i + 1]), dup2(scale_log2), neg_m2);
+            const float p0 = ex2(lo2(e)), p1 = ex2(hi2(e));
+            pk[i / 2] = pack_bf16(p0, p1);
+            l_new = add2(l_new, pair2(__float_as_uint(p0), __float_as_uint(p1)));
+          }
+          tmem_st16(tb + P_COL_P + c / 2, pk);
+        }
+        l_sum = fmaf(l_sum, alpha, lo2(l_new));
+        l_sum2 = fmaf(l_sum2, alpha, hi2(l_new));
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.p_full[t]);
+      }
+      // ---- epilogue of this segment ----
+      const float l_tot = l_sum + l_sum2;
+      const bool live = q_row < p.L;
+      if (sg.rec < 0) {
+        // Both maps have finished; this warp takes the rows of its quadrant and the channels of head
+        // 2h + t, from both O.
+        const float lam = p.lam.at(h);
+        s.inv_l[t][row] = 1.f / l_tot;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.xbar);
+        if (ok)
+          ok = mbar_wait(&s.o_final[0], (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA) &&
+               mbar_wait(&s.o_final[1], (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA) &&
+               mbar_wait(&s.xbar, xn & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
+        ++xn;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const float w1 = s.inv_l[0][row], inv_l2 = s.inv_l[1][row], w2 = lam * inv_l2;
+        const int64_t off = (int64_t)b * p.o_sb + (int64_t)q_row * p.o_sl + (int64_t)(2 * h + t) * p.o_sh;
+#pragma unroll 1
+        for (int c = 0; c < VD / 2; c += 32) {
+          uint32_t a[32], e[32];
+          tmem_ld32(tq + P_COL_O + t * (VD / 2) + c, a);
+          tmem_ld32(tq + P_SLOT + P_COL_O + t * (VD / 2) + c, e);
+          tc_wait_ld();
+          if (live) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              float r[8];
+#pragma unroll
+              for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(a[i + u]) * w1 - __uint_as_float(e[i + u]) * w2;
+              store_out8(p, 0, off + c + i, r);
+              if (!p.o2) continue;
+#pragma unroll
+              for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(e[i + u]) * inv_l2;
+              store_out8(p, 1, off + c + i, r);
+            }
+          }
+        }
+        if (live && p.lse)
+          p.lse[((int64_t)b * 2 * p.H + 2 * h + t) * p.L + q_row] = m_used * p.scale + __logf(l_tot);
+      } else {
+        if (ok) ok = mbar_wait(&s.o_final[t], (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        // partial result of a split item: raw accumulators, [column][row] so that a warp stores 128
+        // consecutive bytes, + (m, l, mu)
+        float* part = p.scratch + (size_t)sg.rec * Rec<false>::ALL + t * Rec<false>::MAP;
+        for (int c = 0; c < VD; c += 32) {
+          uint32_t ov[32];
+          tmem_ld32(tb + P_COL_O + c, ov);
+          tc_wait_ld();
+          float* acc = part + (size_t)c * TM + row;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) acc[i * TM] = __uint_as_float(ov[i]);
+        }
+        float* stats = part + Rec<false>::STATS;
+        stats[row] = m_used;
+        stats[TM + row] = l_tot;
+        stats[2 * TM + row] = 0.f;
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.o_free);
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == WARP_MMA) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ----------------------------------------------------------------- tangent ---
+constexpr int T_STAGES = 3;
+constexpr int T_COL_O = 128, T_COL_DO = 256;
+__host__ __device__ constexpr int t_col_s(int buf) { return buf ? 384 : 0; }
+__host__ __device__ constexpr int t_col_ds(int buf) { return t_col_s(buf) + BN; }
+constexpr int NC = BN / 2;             // score columns of a thread: two threads per query row
+
+struct TSmem {
+  alignas(1024) uint8_t q[2][QPANEL];                // q, dq of the map at work
+  alignas(1024) uint8_t k[T_STAGES][2][KPANEL];      // k, dk
+  alignas(1024) uint8_t v[T_STAGES][4][KPANEL];      // V, dV
+  float xmx[2][2][TM];      // row-maximum exchange [parity][half][row]
+  float xlm[2][2][TM];      // (l, mu) exchange [half][which][row]
+  uint64_t q_full, q_empty;
+  uint64_t k_full[T_STAGES], k_empty[T_STAGES];
+  uint64_t v_full[T_STAGES], v_empty[T_STAGES];
+  uint64_t s_full[2], p_full[2];
+  uint64_t o_done;      // every P V
+  uint64_t o_final;     // last P V of a map's walk (one phase per walk, never skipped)
+  uint64_t o_free;
+  uint64_t xbar;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+__global__ void __launch_bounds__(THREADS, 1)
+attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
+                     const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_dq,
+                     const __grid_constant__ CUtensorMap tm_dk, const __grid_constant__ CUtensorMap tm_dv,
+                     const Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  auto& s = *reinterpret_cast<TSmem*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x, G = gridDim.x;
+
+  if (threadIdx.x == 0) {
+    mbar_init(&s.q_full, 1);
+    mbar_init(&s.q_empty, 1);
+    for (int i = 0; i < T_STAGES; ++i) {
+      mbar_init(&s.k_full[i], 1);
+      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.v_full[i], 1);
+      mbar_init(&s.v_empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.s_full[i], 1);
+      mbar_init(&s.p_full[i], SOFT_WARPS);
+    }
+    mbar_init(&s.o_done, 1);
+    mbar_init(&s.o_final, 1);
+    mbar_init(&s.o_free, SOFT_WARPS);
+    mbar_init(&s.xbar, SOFT_WARPS);
+    s.abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == WARP_MMA) {
+    tmem_alloc(&s.tmem_base, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s.tmem_base;
+  volatile int* abort_flag = &s.abort_flag;
+
+  // A walk is one map over the K/V tiles of a segment: walk 2 si + m of the CTA.
+  if (warp >= SOFT_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_OTHER));
+    if (warp == WARP_TMA) {
+      // ------------------------------------------------------ TMA producer --
+      if (elect_one()) {
+        prefetch_tmap(&tm_q);
+        prefetch_tmap(&tm_k);
+        prefetch_tmap(&tm_v);
+        unsigned kv_it = 0;
+        int walk = 0;
+        Segment sg;
+        bool ok = true;
+        for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
+          int q0, h, b;
+          item_coords(p, sg.item, q0, h, b);
+          for (int m = 0; m < 2 && ok; ++m, ++walk) {
+            if (walk > 0) ok = mbar_wait(&s.q_empty, (walk - 1) & 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+            if (!ok) break;
+            mbar_arrive_expect_tx(&s.q_full, 2 * QPANEL);
+            tma_load_4d(s.q[0], &tm_q, &s.q_full, 0, 2 * h + m, q0, b);
+            tma_load_4d(s.q[1], &tm_dq, &s.q_full, 0, 2 * h + m, q0, b);
+            for (int j = sg.j0; j < sg.j1; ++j, ++kv_it) {
+              const int st = (int)(kv_it % T_STAGES);
+              const uint32_t par = (uint32_t)((kv_it / T_STAGES) & 1) ^ 1;
+              if (kv_it >= T_STAGES) {
+                ok = mbar_wait(&s.k_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+                if (!ok) break;
+              }
+              mbar_arrive_expect_tx(&s.k_full[st], 2 * KPANEL);
+              tma_load_4d(s.k[st][0], &tm_k, &s.k_full[st], 0, 2 * h + m, j * BN, b);
+              tma_load_4d(s.k[st][1], &tm_dk, &s.k_full[st], 0, 2 * h + m, j * BN, b);
+              if (kv_it >= T_STAGES) {
+                ok = mbar_wait(&s.v_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+                if (!ok) break;
+              }
+              mbar_arrive_expect_tx(&s.v_full[st], 4 * KPANEL);
+              for (int i = 0; i < 2; ++i) {
+                tma_load_4d(s.v[st][i], &tm_v, &s.v_full[st], 0, 2 * h + i, j * BN, b);
+                tma_load_4d(s.v[st][2 + i], &tm_dv, &s.v_full[st], 0, 2 * h + i, j * BN, b);
+              }
+            }
+          }
+        }
+      }
+    } else if (warp == WARP_MMA) {
+      // -------------------------------------------------------- MMA issuer --
+      if (elect_one()) {
+        // Q [K | dK]^T -> S | dS and P [V | dV] -> O | dO are one product each (operands adjacent in
+        // shared memory, accumulators adjacent in TMEM); then dS += dQ K^T, dO += T V.
+        constexpr uint32_t idesc_qk = idesc_bf16(TM, 2 * BN, 0, 0);
+        constexpr uint32_t idesc_dqk = idesc_bf16(TM, BN, 0, 0);
+        constexpr uint32_t idesc_pv = idesc_bf16(TM, 2 * VD, 0, 1);
+        constexpr uint32_t idesc_tv = idesc_bf16(TM, VD, 0, 1);
+        const uint64_t q_desc = sdesc_kmajor(smem_u32(s.q[0])), dq_desc = sdesc_kmajor(smem_u32(s.q[1]));
+        const uint64_t k_desc = sdesc_kmajor(smem_u32(s.k[0][0]));
+        const uint64_t v_desc = sdesc_mnmajor(smem_u32(s.v[0][0]), KPANEL);
+        auto issue_qk = [&](int buf, int st) {
+          const uint64_t kd = k_desc + (uint32_t)(st * (2 * KPANEL >> 4));
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks)
+            mma_ss(tmem + t_col_s(buf), q_desc + ks * 2, kd + ks * 2, idesc_qk, ks != 0);
+#pragma unroll
+          for (int ks = 0; ks < HD / 16; ++ks)
+            mma_ss(tmem + t_col_ds(buf), dq_desc + ks * 2, kd + ks * 2, idesc_dqk, 1);
+          tc_commit(&s.s_full[buf]);
+          tc_commit(&s.k_empty[st]);
+        };
+        auto issue_pv = [&](int buf, int st, bool first, bool last) {
+          const uint64_t vd = v_desc + (uint32_t)(st * (4 * KPANEL >> 4));
+#pragma unroll
+          for (int ks = 0; ks < BN / 16; ++ks)
+            mma_ts(tmem + T_COL_O, tmem + t_col_s(buf) + ks * 8, vd + 128 * ks, idesc_pv, !(first && ks == 0));
+#pragma unroll
+          for (int ks = 0; ks < BN / 16; ++ks)
+            mma_ts(tmem + T_COL_DO, tmem + t_col_ds(buf) + ks * 8, vd + 128 * ks, idesc_tv, 1);
+          tc_commit(&s.o_done);
+          if (last) tc_commit(&s.o_final);
+        };
+        unsigned it = 0;          // K/V tiles so far: stage it % T_STAGES, buffer it & 1
+        int walk = 0;
+        Segment sg;
+        bool ok = true;
+        for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
+          const int n_j = sg.j1 - sg.j0;
+          for (int m = 0; m < 2 && ok; ++m, ++walk) {
+            ok = mbar_wait(&s.q_full, walk & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA) &&
+                 mbar_wait(&s.k_full[it % T_STAGES], (uint32_t)((it / T_STAGES) & 1), abort_flag, p.status,
+                           STATUS_TIMEOUT_TMA);
+            if (!ok) break;
+            tc_fence_after();
+            // Q K^T of the next tile is issued before waiting for the softmax of this one
+            issue_qk((int)(it & 1), (int)(it % T_STAGES));
+            if (n_j == 1) tc_commit(&s.q_empty);
+            for (int jj = 0; jj < n_j && ok; ++jj, ++it) {
+              const int st = (int)(it % T_STAGES);
+              if (jj + 1 < n_j) {
+                const int st1 = (int)((it + 1) % T_STAGES);
+                ok = mbar_wait(&s.k_full[st1], (uint32_t)(((it + 1) / T_STAGES) & 1), abort_flag, p.status,
+                               STATUS_TIMEOUT_TMA);
+                if (!ok) break;
+                tc_fence_after();
+                issue_qk((int)((it + 1) & 1), st1);
+                if (jj + 2 == n_j) tc_commit(&s.q_empty);
+              }
+              ok = mbar_wait(&s.p_full[it & 1], (uint32_t)((it >> 1) & 1), abort_flag, p.status,
+                             STATUS_TIMEOUT_SOFTMAX) &&
+                   mbar_wait(&s.v_full[st], (uint32_t)((it / T_STAGES) & 1), abort_flag, p.status,
+                             STATUS_TIMEOUT_TMA);
+              if (ok && jj == 0 && walk > 0)
+                ok = mbar_wait(&s.o_free, (uint32_t)((walk - 1) & 1), abort_flag, p.status,
+                               STATUS_TIMEOUT_SOFTMAX);
+              if (!ok) break;
+              tc_fence_after();
+              issue_pv((int)(it & 1), st, jj == 0, jj + 1 == n_j);
+              tc_commit(&s.v_empty[st]);
+            }
+          }
+        }
+      }
+    }
+  } else {
+    // --------------------------------------- softmax / correction / epilogue --
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFT));
+    const int half = warp >> 2, wl = warp & 3;      // column half; lane quadrant
+    const int c0 = half * NC;                       // first score column of this thread
+    const int row = wl * 32 + lane;
+    const uint32_t tb = tmem_addr(tmem, wl * 32, 0);
+    const float scale_log2 = p.scale * LOG2E;
+    // 64 columns of o, then of do, of this thread's half: [column][row]
+    float* const hold = p.hold + (size_t)cta * HOLD + (size_t)half * VD * TM + row;
+    unsigned it = 0;
+    uint32_t xn = 0;                                // exchanges done so far (phase of xbar)
+    int walk = 0;
+    Segment sg;
+    bool ok = true;
+    for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
+      int q0, h, b;
+      item_coords(p, sg.item, q0, h, b);
+      const int q_row = q0 + row;
+      const bool live = q_row < p.L;
+#pragma unroll 1
+      for (int m = 0; m < 2 && ok; ++m, ++walk) {
+        float m_used = -INFINITY, l_sum = 0.f, l_sum2 = 0.f, mu_sum = 0.f, mu_sum2 = 0.f;
+        for (int j = sg.j0; j < sg.j1 && ok; ++j, ++it) {
+          const int buf = (int)(it & 1);
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[buf], (uint32_t)((it >> 1) & 1), abort_flag, p.status,
+                                                 STATUS_TIMEOUT_MMA));
+          if (!ok) break;
+          tc_fence_after();
+          uint32_t sv[NC], dsv[NC];
+          tmem_ld32(tb + t_col_s(buf) + c0, sv);
+          tmem_ld32(tb + t_col_ds(buf) + c0, dsv);
+          tc_wait_ld();
+          const int kv_rem = p.L - j * BN - c0;
+          if (kv_rem < NC) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+              if (i >= kv_rem) sv[i] = 0xff800000u;  // -inf
+          }
+          const bool first = j == sg.j0;
+          float alpha = 1.f;
+          // The exponentials are taken against the reference maximum that the rows already have
+          // while the new maximum is formed alongside; only when a row has outgrown its reference
+          // by more than 2^8 (or has none yet) is the reference moved, O and dO rescaled and the tile
+          // done again from the scores, which are still in registers.
+          uint32_t pk[NC / 2];
+          uint32_t tk[NC / 2];
+          f32x2 l_new, mu_new;
+          for (bool redo = false;; redo = true) {
+            const f32x2 neg_m2 = dup2(-m_used * scale_log2);
+            l_new = mu_new = dup2(0.f);
+            float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < NC; i += 2) {
+              float& mxi = (i & 2) ? mx1 : mx0;
+              asm("max.f32 %0, %0, %1, %2;" : "+f"(mxi) : "f"(__uint_as_float(sv[i])), "f"(__uint_as_float(sv[i + 1])));
+              const f32x2 e = fma2(pair2(sv[i], sv[i + 1]), dup2(scale_log2), neg_m2);
+              const float p0 = ex2(lo2(e)), p1 = ex2(hi2(e));
+              const f32x2 pp = pair2(__float_as_uint(p0), __float_as_uint(p1));
+              pk[i / 2] = pack_bf16(p0, p1);
+              l_new = add2(l_new, pp);
+              const f32x2 tt = mul2(mul2(pp, pair2(dsv[i], dsv[i + 1])), dup2(p.scale));
+              mu_new = add2(mu_new, tt);
+              tk[i / 2] = pack_bf16(lo2(tt), hi2(tt));
+            }
+            if (redo) break;
+            float mx = fmaxf(mx0, mx1);
+            // both column halves of a row must use the same maximum.  The exchange is also the
+            // point after which every S / dS column of this buffer has been read, so the bf16
+            // P / T written below may overlap the partner's score columns.
+            s.xmx[it & 1][half][row] = mx;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.xbar);
+            ok = __all_sync(0xffffffffu, mbar_wait(&s.xbar, xn & 1, abort_flag, p.status,
+                                                   STATUS_TIMEOUT_SOFTMAX));
+            ++xn;
+            if (!ok) break;
+            mx = fmaxf(mx, s.xmx[it & 1][half ^ 1][row]);
+            const bool need = first || (mx - m_used) * scale_log2 > 8.0f;
+            if (!__any_sync(0xffffffffu, need)) break;
+            if (need) {
+              if (!first) alpha = ex2((m_used - mx) * scale_log2);
+              m_used = mx;
+            }
+            if (first) continue;               // nothing in O yet
+            // half 0 rescales O, half 1 dO, once P V of the step before has run
+            ok = __all_sync(0xffffffffu, mbar_wait(&s.o_done, (uint32_t)((it - 1) & 1), abort_flag, p.status,
+                                                   STATUS_TIMEOUT_MMA));
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t rb = tb + (half ? T_COL_DO : T_COL_O);
+#pragma unroll 1
+            for (int c = 0; c < VD; c += 32) {
+              uint32_t ov[32];
+              tmem_ld32(rb + c, ov);
+              tc_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+              tmem_st32(rb + c, ov);
+            }
+            tc_wait_st();
+          }
+          if (!ok) break;
+          l_sum = fmaf(l_sum, alpha, lo2(l_new));
+          l_sum2 = fmaf(l_sum2, alpha, hi2(l_new));
+          mu_sum = fmaf(mu_sum, alpha, lo2(mu_new));
+          mu_sum2 = fmaf(mu_sum2, alpha, hi2(mu_new));
+          tmem_st16(tb + t_col_s(buf) + c0 / 2, pk);
+          tmem_st16(tb + t_col_ds(buf) + c0 / 2, tk);
+          tc_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.p_full[buf]);
+        }
+        // ---- epilogue of this walk ----
+        float l_tot = l_sum + l_sum2, mu_tot = mu_sum + mu_sum2;
+        s.xlm[half][0][row] = l_tot;
+        s.xlm[half][1][row] = mu_tot;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.xbar);
+        if (ok)
+          ok = mbar_wait(&s.xbar, xn & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX) &&
+               mbar_wait(&s.o_final, (uint32_t)(walk & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA);
+        ++xn;
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        l_tot += s.xlm[half ^ 1][0][row];
+        mu_tot += s.xlm[half ^ 1][1][row];
+        if (sg.rec < 0) {
+          // this thread takes the 64 channels of head 2h + half, of o and of do
+          const float inv_l = 1.f / l_tot, mul = mu_tot * inv_l, lam = p.lam.at(h);
+          const int64_t off = (int64_t)b * p.o_sb + (int64_t)q_row * p.o_sl + (int64_t)(2 * h + half) * p.o_sh;
+#pragma unroll 1
+          for (int c = 0; c < VD / 2; c += 32) {
+            uint32_t ov[32], dv_[32];
+            tmem_ld32(tb + T_COL_O + half * (VD / 2) + c, ov);
+            tmem_ld32(tb + T_COL_DO + half * (VD / 2) + c, dv_);
+            tc_wait_ld();
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+              const float o = __uint_as_float(ov[i]) * inv_l;
+              ov[i] = __float_as_uint(o);
+              dv_[i] = __float_as_uint(__uint_as_float(dv_[i]) * inv_l - mul * o);
+            }
+            float* ho = hold + (size_t)c * TM;
+            float* hd = ho + (size_t)(VD / 2) * TM;
+            if (m == 0) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) {
+                ho[i * TM] = __uint_as_float(ov[i]);
+                hd[i * TM] = __uint_as_float(dv_[i]);
+              }
+            } else if (live) {
+#pragma unroll
+              for (int i = 0; i < 32; i += 8) {
+                float r[8];
+                if (p.o2) {
+#pragma unroll
+                  for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(ov[i + u]);
+                  store_out8(p, 1, off + c + i, r);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) r[u] = ho[(i + u) * TM] - lam * __uint_as_float(ov[i + u]);
+                store_out8(p, 0, off + c + i, r);
+#pragma unroll
+                for (int u = 0; u < 8; ++u) r[u] = hd[(i + u) * TM] - lam * __uint_as_float(dv_[i + u]);
+                *reinterpret_cast<uint4*>(p.dout + off + c + i) =
+                    make_uint4(pack_bf16(r[0], r[1]), pack_bf16(r[2], r[3]), pack_bf16(r[4], r[5]), pack_bf16(r[6], r[7]));
+              }
+            }
+          }
+          if (live && p.lse && half == 0)
+            p.lse[((int64_t)b * 2 * p.H + 2 * h + m) * p.L + q_row] = m_used * p.scale + __logf(l_tot);
+        } else {
+          // half 0 stores the O accumulators (columns 0-127), half 1 those of dO (128-255)
+          float* part = p.scratch + (size_t)sg.rec * Rec<true>::ALL + m * Rec<true>::MAP;
+          const uint32_t rb = tb + (half ? T_COL_DO : T_COL_O);
+          for (int c = 0; c < VD; c += 32) {
+            uint32_t ov[32];
+            tmem_ld32(rb + c, ov);
+            tc_wait_ld();
+            float* acc = part + (size_t)(c + half * VD) * TM + row;
+#pragma unroll
+            for (int i = 0; i < 32; ++i) acc[i * TM] = __uint_as_float(ov[i]);
+          }
+          if (half == 0) {
+            float* stats = part + Rec<true>::STATS;
+            stats[row] = m_used;
+            stats[TM + row] = l_tot;
+            stats[2 * TM + row] = mu_tot;
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.o_free);
+      }
+    }
+    tc_fence_before();
+  }
+  __syncthreads();
+  if (warp == WARP_MMA) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// ------------------------------------------------------------------- merge ---
+// Merge the parts of every split item and subtract map 2 (as combine_split_items, a record for each
+// map).  A CTA takes 32 query rows (a lane each), a warp 8 of the 128 columns.
+template <bool TANGENT>
+__global__ void __launch_bounds__(32 * VD / COMBINE_COLS) attn_diff_combine_kernel(const Params p, int G) {
+  using R = Rec<TANGENT>;
+  const int c = blockIdx.x;
+  int item, parts;
+  if (!split_item(p.sh, c, G, item, parts)) return;
+  int q0, h, b;
+  item_coords(p, item, q0, h, b);
+  const float scale_log2 = p.scale * LOG2E, lam = p.lam.at(h);
+  const int r = blockIdx.y * COMBINE_ROWS + (threadIdx.x & 31);
+  const int col = (threadIdx.x >> 5) * COMBINE_COLS;
+  const int q_row = q0 + r;
+  if (q_row >= p.L) return;
+  const int64_t off = (int64_t)b * p.o_sb + (int64_t)q_row * p.o_sl + (int64_t)(2 * h + col / HD) * p.o_sh + col % HD;
+  float y[COMBINE_COLS], dy[COMBINE_COLS];
+#pragma unroll
+  for (int map = 0; map < 2; ++map) {
+    const float* x = p.scratch + (size_t)(2 * c + 1) * R::ALL + map * R::MAP + r;   // then records 2c + 2, 2c + 4, ...
+    float m = x[R::STATS], l = 0.f, mu = 0.f;
+    float o[COMBINE_COLS], d[COMBINE_COLS];
+#pragma unroll
+    for (int i = 0; i < COMBINE_COLS; ++i) o[i] = d[i] = 0.f;
+#pragma unroll 2
+    for (int k = 0; k < parts; ++k, x += k == 1 ? R::ALL : 2 * R::ALL) {
+      const float mk = x[R::STATS], mn = fmaxf(m, mk);
+      const float w0 = ex2((m - mn) * scale_log2), w1 = ex2((mk - mn) * scale_log2);
+      m = mn;
+      l = l * w0 + x[R::STATS + TM] * w1;
+      mu = mu * w0 + x[R::STATS + 2 * TM] * w1;
+#pragma unroll
+      for (int i = 0; i < COMBINE_COLS; ++i) {
+        o[i] = o[i] * w0 + x[(col + i) * TM] * w1;
+        if (TANGENT) d[i] = d[i] * w0 + x[(VD + col + i) * TM] * w1;
+      }
+    }
+    const float inv_l = 1.f / l, mul = mu * inv_l;
+#pragma unroll
+    for (int i = 0; i < COMBINE_COLS; ++i) {
+      o[i] *= inv_l;
+      d[i] = d[i] * inv_l - mul * o[i];
+      y[i] = map == 0 ? o[i] : y[i] - lam * o[i];
+      dy[i] = map == 0 ? d[i] : dy[i] - lam * d[i];
+    }
+    if (map == 1 && p.o2) store_out8(p, 1, off, o);
+    if (p.lse && col == 0)
+      p.lse[((int64_t)b * 2 * p.H + 2 * h + map) * p.L + q_row] = m * p.scale + __logf(l);
+  }
+  store_out8(p, 0, off, y);
+  if (TANGENT)
+    *reinterpret_cast<uint4*>(p.dout + off) =
+        make_uint4(pack_bf16(dy[0], dy[1]), pack_bf16(dy[2], dy[3]), pack_bf16(dy[4], dy[5]), pack_bf16(dy[6], dy[7]));
+}
+
+// 4-D map over a (B, L, 2H, 64) bf16 tensor whose box is `rows` rows of one head
+static int make_map(CUtensorMap* m, const void* ptr, int B, int L, int heads, const int64_t* st, int rows) {
+  uint64_t dims[4] = {(uint64_t)HD, (uint64_t)heads, (uint64_t)L, (uint64_t)B};
+  uint64_t str[4] = {2, (uint64_t)st[2] * 2, (uint64_t)st[1] * 2, (uint64_t)st[0] * 2};
+  uint32_t box[4] = {(uint32_t)HD, 1, (uint32_t)rows, 1};
+  return make_tmap(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(ptr), dims, str, box);
+}
+
+static FwdShares shares(int B, int L, int H) {
+  FwdShares sh;
+  sh.n_items = (L + TM - 1) / TM * H * B;
+  sh.n_kv = (L + BN - 1) / BN;
+  sh.total = (long)sh.n_items * sh.n_kv;
+  return sh;
+}
+
+// Floats of scratch of a grid of G CTAs: with a tangent the held rows, then the records if items are split.
+template <bool TANGENT>
+static size_t scratch_floats(int G, bool split) {
+  return (TANGENT ? (size_t)G * HOLD : 0) + (split ? (size_t)G * 2 * Rec<TANGENT>::ALL : 0);
+}
+
+template <bool TANGENT>
+static int grid(const FwdShares& sh) {
+  return fwd_grid(sh.n_items, sh.n_kv, Rec<TANGENT>::PART_COST);
+}
+
+}  // namespace diff
+}  // namespace imf
+
+// Bytes of scratch that imf_attn_diff_fwd needs (0: none).
+extern "C" long imf_attn_diff_fwd_scratch_bytes(int B, int L, int H, int tangent) {
+  using namespace imf;
+  using namespace imf::diff;
+  if (B <= 0 || L <= 0 || H <= 0 || (long)B * H * ((L + TM - 1) / TM) > 0x3fffffffL) return 0;
+  const FwdShares sh = shares(B, L, H);
+  const int G = tangent ? grid<true>(sh) : grid<false>(sh);
+  return 4L * (long)(tangent ? scratch_floats<true>(G, G != sh.n_items) : scratch_floats<false>(G, G != sh.n_items));
+}
+
+// q, k, v (, dq, dk, dv): (B, L, 2H, 64) bf16 with (batch, row, head) element strides in strides[0..17]; o, dout, o2
+// share (batch, row, head) strides o_strides; dout null without a tangent.  Where a backward pass follows: o2, lse
+// (B, 2H, L) and low, the bytes of o at o's strides and `plane` bytes on those of o2 (see attn_diff.h).  lam: H weights, lam_stride elements apart.
+extern "C" int imf_attn_diff_fwd(const void* q, const void* k, const void* v, const void* dq, const void* dk,
+                                 const void* dv, const void* lam, int64_t lam_stride, int lam_bf16, void* o, void* dout,
+                                 void* o2, void* low, int64_t plane, float* lse, int B, int L, int H, const int64_t* strides,
+                                 const int64_t* o_strides, float scale, void* scratch, long scratch_bytes, int* status,
+                                 void* stream) {
+  using namespace imf;
+  using namespace imf::diff;
+  const bool tangent = dq != nullptr;
+  if (!q || !k || !v || !lam || !o || B <= 0 || L <= 0 || H <= 0) return IMF_ERR_ARG;
+  if (tangent != (dk != nullptr) || tangent != (dv != nullptr) || tangent != (dout != nullptr)) return IMF_ERR_ARG;
+  if ((o2 != nullptr) != (low != nullptr) || (reinterpret_cast<uintptr_t>(low) & 7) || (plane & 7)) return IMF_ERR_ARG;
+  if (!(scale > 0.f) || scale > 1e30f) return IMF_ERR_ARG;
+  if ((long)B * H * ((L + TM - 1) / TM) > 0x3fffffffL) return IMF_ERR_TOO_LARGE;
+  for (const void* x : {(const void*)o, (const void*)dout, (const void*)o2})
+    if (reinterpret_cast<uintptr_t>(x) & 15) return IMF_ERR_ARG;
+  for (int i = 0; i < 3; ++i)
+    if (o_strides[i] & 7) return IMF_ERR_ARG;
+  Params prm;
+  prm.o = static_cast<__nv_bfloat16*>(o);
+  prm.dout = static_cast<__nv_bfloat16*>(dout);
+  prm.o2 = static_cast<__nv_bfloat16*>(o2);
+  prm.low = static_cast<int8_t*>(low);
+  prm.plane = plane;
+  prm.lse = lse;
+  prm.lam = {lam, lam_stride, lam_bf16};
+  prm.B = B; prm.H = H; prm.L = L;
+  prm.n_qblk = (L + TM - 1) / TM;
+  prm.sh = shares(B, L, H);
+  prm.o_sb = o_strides[0]; prm.o_sl = o_strides[1]; prm.o_sh = o_strides[2];
+  prm.scale = scale;
+  prm.status = status;
+  const int G = tangent ? grid<true>(prm.sh) : grid<false>(prm.sh);
+  const bool split = G != prm.sh.n_items;
+  const size_t need = 4 * (tangent ? scratch_floats<true>(G, split) : scratch_floats<false>(G, split));
+  if (need && (scratch == nullptr || (size_t)scratch_bytes < need || (reinterpret_cast<uintptr_t>(scratch) & 15)))
+    return IMF_ERR_ARG;
+  prm.hold = static_cast<float*>(scratch);
+  prm.scratch = prm.hold + (tangent ? (size_t)G * HOLD : 0);
+  CUtensorMap mq, mk, mv, mdq, mdk, mdv;
+  int rc;
+  if ((rc = make_map(&mq, q, B, L, 2 * H, strides, TM))) return rc;
+  if ((rc = make_map(&mk, k, B, L, 2 * H, strides + 3, BN))) return rc;
+  if ((rc = make_map(&mv, v, B, L, 2 * H, strides + 6, BN))) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  static bool smem_set[2][HOST_MAX_DEVICES] = {{false}};
+  if (tangent) {
+    if ((rc = make_map(&mdq, dq, B, L, 2 * H, strides + 9, TM))) return rc;
+    if ((rc = make_map(&mdk, dk, B, L, 2 * H, strides + 12, BN))) return rc;
+    if ((rc = make_map(&mdv, dv, B, L, 2 * H, strides + 15, BN))) return rc;
+    const size_t smem = sizeof(TSmem) + 1024;
+    if (!allow_smem((const void*)attn_diff_jvp_kernel, smem, smem_set[1])) return IMF_ERR_LAUNCH;
+    attn_diff_jvp_kernel<<<G, THREADS, smem, st>>>(mq, mk, mv, mdq, mdk, mdv, prm);
+  } else {
+    const size_t smem = sizeof(PSmem) + 1024;
+    if (!allow_smem((const void*)attn_diff_fwd_kernel, smem, smem_set[0])) return IMF_ERR_LAUNCH;
+    attn_diff_fwd_kernel<<<G, THREADS, smem, st>>>(mq, mk, mv, prm);
+  }
+  if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
+  if (split) {
+    const dim3 g(G - 1, TM / COMBINE_ROWS);
+    if (tangent)
+      attn_diff_combine_kernel<true><<<g, 32 * VD / COMBINE_COLS, 0, st>>>(prm, G);
+    else
+      attn_diff_combine_kernel<false><<<g, 32 * VD / COMBINE_COLS, 0, st>>>(prm, G);
+    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
+  }
+  return IMF_OK;
+}

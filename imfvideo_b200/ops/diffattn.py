@@ -1,0 +1,199 @@
+"""Differential attention on the sm_100a kernels (``csrc/attn_diff_fwd.cu``, ``csrc/attn_diff_bwd.cu``).
+
+Heads 2j and 2j + 1 of q, k, v (B, L, 2H, 64) are a pair.  Both heads' values lie side by side, and the
+second softmax map is subtracted with the pair's learned weight:
+
+    A_m = softmax(scale q_m k_m^T),  V = [v_2j | v_2j+1],  o = (A_1 - lam_j A_2) V
+
+so the tensors are those of ordinary attention with 2H heads and nothing is copied to form pairs.
+``ops.dual.diff_attention`` is the entry point for models (dual numbers, any device);
+``diff_attn_fwd`` / ``diff_attn_bwd`` are the launches.  bf16, head_dim 64, any length from one token on,
+any number of pairs; lam is fp32 or bf16 and its gradient has its type.  Launches go to the current
+stream of the tensors' device; workspaces belong to the call.  The reference has no such attention.
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import cuda as _cuda
+from .act8 import _apart, _elsewhere, _in_one_place, _new, _places, _same_device
+from .dual import Dual
+
+Tensor = torch.Tensor
+BF16, F32 = torch.bfloat16, torch.float32
+HEAD_DIM = 64
+_KERNELS = None
+
+
+def _kernels():
+    """``ops.kernels`` with the argument types of this module's launchers set (loads the library)."""
+    global _KERNELS
+    if _KERNELS is None:
+        if not _cuda.available():
+            raise RuntimeError("differential attention on a GPU needs the kernel library")
+        from . import kernels as K
+
+        vp, ci, cl, i64, cf = (ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_int64,
+                               ctypes.c_float)
+        lib = K._lib
+        for name, n in (("imf_attn_diff_fwd_scratch_bytes", 4), ("imf_attn_diff_bwd_scratch_bytes", 3)):
+            getattr(lib, name).restype = cl
+            getattr(lib, name).argtypes = [ci] * n
+        lib.imf_attn_diff_fwd.restype = ci
+        lib.imf_attn_diff_fwd.argtypes = [vp] * 7 + [i64, ci] + [vp] * 4 + [i64, vp] + [ci] * 3 + [vp, vp, cf, vp, cl, vp, vp]
+        lib.imf_attn_diff_bwd.restype = ci
+        lib.imf_attn_diff_bwd.argtypes = [vp] * 6 + [i64] + [vp] * 3 + [i64, ci] + [vp] * 4 + [ci] * 3 + [vp] * 4 + [cf, vp, cl, ci, vp, vp]
+        _KERNELS = K
+    return _KERNELS
+
+
+def _check(what: str, shape, lam: Tensor, scale: Optional[float], **tensors) -> Tuple[torch.device, float]:
+    if len(shape) != 4 or shape[3] != HEAD_DIM or shape[2] % 2:
+        raise ValueError(f"{what} takes (B, L, an even number of heads, {HEAD_DIM}), not {tuple(shape)}")
+    for name, t in tensors.items():
+        if t is not None and (t.shape != shape or t.dtype != BF16):
+            raise ValueError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, bf16 {tuple(shape)} expected")
+    if lam.dtype not in (BF16, F32) or tuple(lam.shape) != (shape[2] // 2,):
+        raise ValueError(f"{what}: lam is {lam.dtype} {tuple(lam.shape)}, fp32 or bf16 ({shape[2] // 2},) expected")
+    scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+    if not 1e-30 <= scale <= 1e30:
+        raise ValueError(f"{what}: scale {scale} is not a positive number between 1e-30 and 1e30")
+    return _same_device(what, *tensors.values(), lam), scale
+
+
+def _operand(t: Tensor):
+    """(the tensor or a copy with 16-byte aligned rows, its (batch, row, head) strides); strides of
+    single dimensions are replaced, no address depends on them."""
+    B, L, H, D = t.shape
+    row = (L * H * D, H * D, D)
+    if not t.is_contiguous():
+        s = [s_ if n > 1 else r for n, s_, r in zip(t.shape, t.stride(), row)]
+        if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(x % 8 or x == 0 for x in s):
+            return t, tuple(s)
+        t = t.contiguous()                 # a broadcast, transposed or unaligned tensor
+    return (t, row) if t.data_ptr() % 16 == 0 else (t.clone(), row)
+
+
+def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Tensor] = None,
+                  dk: Optional[Tensor] = None, dv: Optional[Tensor] = None, scale: Optional[float] = None,
+                  need_bwd: bool = True) -> Tuple[Tensor, Optional[Tensor], tuple]:
+    """(o, do | None, saved) of (B, L, 2H, 64) bf16 CUDA tensors at any strides; lam (H,).  With tangents
+    dq, dk, dv (all or none) also do.  ``need_bwd``: saved is what ``diff_attn_bwd`` takes, O_2 in bf16, the
+    bytes that o and O_2 lost when they were rounded (int8, two planes of o's shape) and the log-sum-exp
+    (B, 2H, L) of both maps; otherwise it is empty."""
+    shape, tang = q.shape, dq is not None
+    if (dk is None) == tang or (dv is None) == tang:
+        raise ValueError("diff_attn_fwd: tangents of q, k and v come together")
+    dev, scale = _check("diff_attn_fwd", shape, lam, scale, q=q, k=k, v=v, dq=dq, dk=dk, dv=dv)
+    if dev.type != "cuda":
+        raise ValueError("diff_attn_fwd launches on a GPU; dual.diff_attention also takes CPU tensors")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return diff_attn_fwd(q, k, v, lam, dq, dk, dv, scale, need_bwd)
+    B, L, H2, D = shape
+    o = _new(shape, BF16, dev)
+    do = _new(shape, BF16, dev) if tang else None
+    o2, low, lse = saved = (_new(shape, BF16, dev), _new((2, *shape), torch.int8, dev),
+                            _new((B, H2, L), F32, dev)) if need_bwd else (None,) * 3
+    saved = saved if need_bwd else ()
+    if 0 in shape:
+        return o, do, saved
+    K = _kernels()
+    ops = [_operand(t) for t in ((q, k, v, dq, dk, dv) if tang else (q, k, v))]
+    ptrs = [t.data_ptr() for t, _ in ops] + ([] if tang else [None] * 3)
+    strides = [s for _, st in ops for s in st]
+    nscr = K._lib.imf_attn_diff_fwd_scratch_bytes(B, L, H2 // 2, int(tang))
+    scr = _new(nscr, torch.uint8, dev) if nscr else None
+    K._check(K._lib.imf_attn_diff_fwd(
+        *ptrs, lam.data_ptr(), lam.stride(0), int(lam.dtype == BF16), o.data_ptr(), K._ptr(do), K._ptr(o2),
+        K._ptr(low), o.numel(), K._ptr(lse), B, L, H2 // 2, (ctypes.c_int64 * 18)(*strides), (ctypes.c_int64 * 3)(L * H2 * D, H2 * D, D),
+        scale, K._ptr(scr), nscr, K.status_word(dev).data_ptr(), K._stream()), "imf_attn_diff_fwd")
+    K.LAUNCHES.count += 1
+    return o, do, saved
+
+
+def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved: tuple, go: Tensor,
+                  scale: Optional[float] = None, gv_out: Optional[Tensor] = None
+                  ) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
+    """(dq, dk, dv, dlam) from what ``diff_attn_fwd`` returned and the output gradient ``go``.  ``gv_out``
+    takes dv (16-byte aligned rows, no two elements in one place, apart from the inputs), as in
+    ``kernels.attn_bwd``, whose fixed-order mode holds here too."""
+    shape = q.shape
+    o2, low, lse = saved
+    dev, scale = _check("diff_attn_bwd", shape, lam, scale, q=q, k=k, v=v, o=o, o2=o2, go=go, gv_out=gv_out)
+    _same_device("diff_attn_bwd", q, low, lse)
+    if dev.type != "cuda":
+        raise ValueError("diff_attn_bwd launches on a GPU; dual.diff_attention also takes CPU tensors")
+    B, L, H2, D = shape
+    if lse.dtype != F32 or tuple(lse.shape) != (B, H2, L) or not lse.is_contiguous():
+        raise ValueError(f"diff_attn_bwd: lse has to be contiguous fp32 {(B, H2, L)}")
+    if low.dtype != torch.int8 or low.shape != (2, *shape) or not (low.is_contiguous() and o2.is_contiguous()):
+        raise ValueError("diff_attn_bwd: saved has to be what diff_attn_fwd returned")
+    row = (L * H2 * D, H2 * D, D)
+    dv_strides = row
+    if gv_out is not None and 0 not in shape:
+        dv_strides = [s if n > 1 else r for n, s, r in zip(shape, gv_out.stride(), row)]
+        if gv_out.stride(3) != 1 or gv_out.data_ptr() % 16 or any(s % 8 for s in dv_strides):
+            raise ValueError("diff_attn_bwd: the dv output needs 16-byte aligned rows")
+        if not _apart(*_places(gv_out)):
+            raise ValueError("diff_attn_bwd: no two elements of the dv output in one place")
+        if any(_apart(*_places(t)) and _in_one_place(gv_out, t) for t in (q, k, v, go)):
+            raise ValueError("diff_attn_bwd: the dv output lies over an input")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return diff_attn_bwd(q, k, v, lam, o, saved, go, scale, gv_out)
+    dq, dk = _new(shape, BF16, dev), _new(shape, BF16, dev)
+    dv = _new(shape, BF16, dev) if gv_out is None else gv_out
+    dlam = _new((H2 // 2,), lam.dtype, dev)
+    if 0 in shape:
+        return dq, dk, dv, dlam.zero_()
+    K = _kernels()
+    (q_, sq), (k_, sk), (v_, sv), (g_, sg) = (_operand(t) for t in (q, k, v, go))
+    o_ = o.contiguous()
+    nscr = K._lib.imf_attn_diff_bwd_scratch_bytes(B, L, H2 // 2)
+    scr = _new(nscr, torch.uint8, dev)
+    i64 = ctypes.c_int64
+    K._check(K._lib.imf_attn_diff_bwd(
+        q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), o_.data_ptr(), o2.data_ptr(), low.data_ptr(), o.numel(),
+        g_.data_ptr(), lse.data_ptr(), lam.data_ptr(), lam.stride(0), int(lam.dtype == BF16), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        dlam.data_ptr(), B, L, H2 // 2, (i64 * 12)(*sq, *sk, *sv, *sg), (i64 * 3)(*row), (i64 * 3)(*row),
+        (i64 * 3)(*dv_strides), scale, scr.data_ptr(), nscr, int(K.DETERMINISTIC), K.status_word(dev).data_ptr(),
+        K._stream()), "imf_attn_diff_bwd")
+    K.LAUNCHES.count += 3
+    return dq, dk, dv, dlam
+
+
+class _DiffAttnFn(torch.autograd.Function):
+    """o and the detached tangent do; reverse mode through the primal only."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, lam, dq, dk, dv, scale):
+        need_bwd = any(ctx.needs_input_grad[:4])
+        o, do, saved = diff_attn_fwd(q, k, v, lam, dq, dk, dv, scale, need_bwd)
+        if need_bwd:
+            ctx.save_for_backward(q, k, v, lam, o, *saved)
+            ctx.scale = scale
+        if do is None:
+            do = o.new_empty(0)
+        ctx.mark_non_differentiable(do)
+        return o, do
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, go, _gdo):
+        q, k, v, lam, o, *saved = ctx.saved_tensors
+        return (*diff_attn_bwd(q, k, v, lam, o, saved, go, ctx.scale), None, None, None, None)
+
+
+def diff_attention_dual(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[float] = None) -> Dual:
+    """``ops.dual.diff_attention`` on CUDA tensors; lam (H,)."""
+    t = (q.t, k.t, v.t)
+    if any(x is not None for x in t):
+        t = tuple(torch.zeros_like(p.p) if x is None else x.detach() for p, x in zip((q, k, v), t))
+        return Dual(*_DiffAttnFn.apply(q.p, k.p, v.p, lam, *t, scale))
+    return Dual(_DiffAttnFn.apply(q.p, k.p, v.p, lam, None, None, None, scale)[0], None)

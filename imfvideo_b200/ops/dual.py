@@ -187,6 +187,78 @@ def dense_attention(q: Dual, k: Dual, v: Dual, impl: str = "auto") -> Dual:
     return Dual(p, t)
 
 
+def diff_attention(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[float] = None,
+                   impl: str = "auto") -> Dual:
+    """Differential attention on (b, l, 2H, d) tensors: heads 2j and 2j + 1 are a pair,
+
+        o = (softmax(scale q_2j k_2j^T) - lam_j softmax(scale q_2j+1 k_2j+1^T)) [v_2j | v_2j+1]
+
+    with learned weights ``lam`` (H,), or one (a number's tensor) for all pairs; scale 1/sqrt(d) unless
+    given.  The output's heads 2j and 2j + 1 are the two halves of pair j's channels.  lam carries no
+    tangent.  impl: "auto" (kernels for CUDA tensors: bf16, d = 64; formulas on CPU) or "math"."""
+    if impl not in ("auto", "math"):
+        raise ValueError(f"diff_attention: impl is 'auto' or 'math', not {impl!r}")
+    if q.p.dim() != 4 or q.p.shape[2] % 2 or k.p.shape != q.p.shape or v.p.shape != q.p.shape:
+        raise ValueError("diff_attention takes q, k, v of one shape (b, l, an even number of heads, d), not "
+                         f"{tuple(q.p.shape)}, {tuple(k.p.shape)}, {tuple(v.p.shape)}")
+    H = q.p.shape[2] // 2
+    if lam.numel() != 1 and tuple(lam.shape) != (H,):
+        raise ValueError(f"diff_attention: lam is {tuple(lam.shape)}, one weight or ({H},) expected")
+    lam = lam.reshape(-1).expand(H)
+    cu = _cuda_ops(q.p)
+    if impl == "auto" and cu is not None:
+        from . import diffattn
+
+        return diffattn.diff_attention_dual(q, k, v, lam, scale)
+    p = ref.diff_attention(q.p, k.p, v.p, lam, scale)
+    t = None
+    if any(x.t is not None for x in (q, k, v)):
+        dq, dk, dv = (torch.zeros_like(x.p) if x.t is None else x.t for x in (q, k, v))
+        _, t = ref.diff_attention_jvp(q.p.detach(), k.p.detach(), v.p.detach(), lam.detach(), dq, dk, dv, scale)
+    return Dual(p, t)
+
+
+# ------------------------------------------- norms around a branch --------
+def norm_add_norm(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor, eps: float,
+                  res_scale: Optional[Tensor] = None, pre: Optional[Tensor] = None,
+                  out_dtype: Optional[torch.dtype] = None):
+    """The update of a residual stream whose branch is normed before it is added, with the norm that the
+    next branch begins with:
+
+        x = res_scale * res + gate * post * y / rms(y),    n = pre * x / rms(x)
+
+    (rms(z) = sqrt(mean z^2 + eps); post, gate, res_scale and pre are learned, per channel, and carry no
+    tangent).  Returns (x, n) as duals; n is None without ``pre``.  ``res`` None: the stream begins with
+    this branch; ``res_scale`` None: 1.  x has the type of ``res`` (without one, 32 bits or y's), n
+    ``out_dtype`` or y's.  CUDA: y bf16 or fp32 and res fp32 take one kernel a direction
+    (``ops/postnorm.py``)."""
+    if res_scale is not None and res is None:
+        raise ValueError("norm_add_norm: res_scale without res")
+    D = y.p.shape[-1]
+    for name, w in (("post", post), ("gate", gate), ("res_scale", res_scale), ("pre", pre)):
+        if w is not None and tuple(w.shape) != (D,):
+            raise ValueError(f"norm_add_norm: {name} is {tuple(w.shape)}, ({D},) expected")
+    if res is not None and res.p.shape != y.p.shape:
+        raise ValueError(f"norm_add_norm: res is {tuple(res.p.shape)}, y {tuple(y.p.shape)}")
+    xd = res.p.dtype if res is not None else torch.promote_types(y.p.dtype, torch.float32)
+    nd = out_dtype or y.p.dtype
+    cu = _cuda_ops(y.p)
+    if cu is not None:
+        from . import postnorm
+
+        if postnorm.supported(y.p, xd, nd, post, gate, res_scale, pre):
+            return postnorm.norm_add_norm_dual(res, y, post, gate, eps, res_scale, pre)
+    rp, rt = (None, None) if res is None else res
+    x, n = ref.norm_add_norm(rp, y.p, post, gate, eps, res_scale, pre)
+    dx = dn = None
+    if y.t is not None or rt is not None:
+        det = lambda t: None if t is None else t.detach()
+        dy = torch.zeros_like(y.p) if y.t is None else y.t
+        dx, dn = ref.norm_add_norm_jvp(det(rp), rt, det(y.p), dy, det(post), det(gate), eps, det(res_scale), det(pre))
+    to = lambda t, d: None if t is None else t.to(d)
+    return Dual(x.to(xd), to(dx, xd)), None if n is None else Dual(n.to(nd), to(dn, nd))
+
+
 def cat(parts: List[Dual], dim: int) -> Dual:
     p = torch.cat([x.p for x in parts], dim=dim)
     if all(x.t is None for x in parts):

@@ -1,0 +1,191 @@
+"""Norms around a block's branch on the sm_100a kernels (``csrc/rowops_postnorm.cu``):
+
+    x = res_scale * res + gate * post * y / rms(y),    n = pre * x / rms(x)
+
+``ops.dual.norm_add_norm`` is the entry point for models (dual numbers, any device);
+``norm_add_norm_fwd`` / ``norm_add_norm_bwd`` are the launches.  Rows are all leading dimensions; D a
+multiple of 8 up to 8,192; y and n bf16 or fp32 (one type), the residual stream and the learned vectors
+fp32.  Launches go to the current stream of the tensors' device; workspaces belong to the call.  The
+reference norms a branch's input only (reference ``models/imf_dit_video.py:909-972``).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from typing import Optional, Tuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import cuda as _cuda
+from .act8 import _elsewhere, _new, _same_device
+from .dual import Dual
+
+Tensor = torch.Tensor
+BF16, F32 = torch.bfloat16, torch.float32
+MAX_WIDTH = 8192
+_PTRS = ctypes.c_void_p * 17
+_KERNELS = None
+
+
+def _kernels():
+    """``ops.kernels`` with the argument types of this module's launchers set (loads the library)."""
+    global _KERNELS
+    if _KERNELS is None:
+        if not _cuda.available():
+            raise RuntimeError("norm_add_norm on a GPU needs the kernel library")
+        from . import kernels as K
+
+        vp, ci = ctypes.c_void_p, ctypes.c_int
+        K._lib.imf_norm_add_norm_grid.restype = ci
+        K._lib.imf_norm_add_norm_grid.argtypes = [ci, ci]
+        K._lib.imf_norm_add_norm.restype = ci
+        K._lib.imf_norm_add_norm.argtypes = [vp, ci, ci, ctypes.c_float, ci, ci, vp]
+        _KERNELS = K
+    return _KERNELS
+
+
+def supported(y: Tensor, x_dtype: torch.dtype, n_dtype: torch.dtype, *vectors: Optional[Tensor]) -> bool:
+    """Whether the kernels take these types and this width."""
+    D = y.shape[-1]
+    return (y.dtype in (BF16, F32) and n_dtype == y.dtype and x_dtype == F32 and D % 8 == 0 and 0 < D <= MAX_WIDTH
+            and y.numel() // D < 1 << 31 and all(w is None or w.dtype == F32 for w in vectors))
+
+
+def _rows(what: str, shape, dtype: torch.dtype, t: Optional[Tensor]) -> Optional[Tensor]:
+    """Contiguous, 16-byte aligned rows of a tensor (the tensor itself where it has them)."""
+    if t is None:
+        return None
+    if t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} where {dtype} {tuple(shape)} is expected")
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _prepare(what: str, res, y, post, gate, res_scale, pre):
+    D = y.shape[-1] if y.dim() else 0
+    if not supported(y, F32, y.dtype, post, gate, res_scale, pre):
+        raise ValueError(f"{what}: y bf16 or fp32 with a multiple of 8 up to {MAX_WIDTH} channels and fp32 vectors, "
+                         f"not {y.dtype} {tuple(y.shape)}")
+    if res_scale is not None and res is None:
+        raise ValueError(f"{what}: res_scale without res")
+    vec = [_rows(f"{what}: a vector", (D,), F32, w) for w in (post, gate, res_scale, pre)]
+    return _rows(f"{what}: res", y.shape, F32, res), _rows(f"{what}: y", y.shape, y.dtype, y), vec
+
+
+def norm_add_norm_fwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tensor, eps: float,
+                      res_scale: Optional[Tensor] = None, pre: Optional[Tensor] = None,
+                      dres: Optional[Tensor] = None, dy: Optional[Tensor] = None
+                      ) -> Tuple[Tensor, Optional[Tensor], Optional[Tensor], Optional[Tensor]]:
+    """(x, n | None, dx | None, dn | None) of CUDA tensors; with ``dy`` the tangents too (``dres`` None: the
+    residual stands still)."""
+    what = "norm_add_norm_fwd"
+    dev = _same_device(what, y, res, post, gate, res_scale, pre, dres, dy)
+    if dres is not None and (dy is None or res is None):
+        raise ValueError(f"{what}: dres without dy or res")
+    res, y, (post, gate, res_scale, pre) = _prepare(what, res, y, post, gate, res_scale, pre)
+    dres, dy = _rows(f"{what}: dres", y.shape, F32, dres), _rows(f"{what}: dy", y.shape, y.dtype, dy)
+    if dev.type != "cuda":
+        raise ValueError(f"{what} launches on a GPU; dual.norm_add_norm also takes CPU tensors")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return norm_add_norm_fwd(res, y, post, gate, eps, res_scale, pre, dres, dy)
+    shape, D = y.shape, y.shape[-1]
+    x = _new(shape, F32, dev)
+    n = None if pre is None else _new(shape, y.dtype, dev)
+    dx = None if dy is None else _new(shape, F32, dev)
+    dn = None if dy is None or pre is None else _new(shape, y.dtype, dev)
+    rows = y.numel() // D
+    if rows:
+        K = _kernels()
+        p = K._ptr
+        ptrs = _PTRS(p(res), p(dres), p(y), p(dy), p(post), p(gate), p(res_scale), p(pre), p(x), p(dx), p(n), p(dn))
+        K._check(K._lib.imf_norm_add_norm(ptrs, rows, D, float(eps), int(y.dtype == F32), int(dy is not None),
+                                          K._stream()), "imf_norm_add_norm")
+        K.LAUNCHES.count += 1
+    return x, n, dx, dn
+
+
+def norm_add_norm_bwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tensor, eps: float,
+                      res_scale: Optional[Tensor], pre: Optional[Tensor], gx: Optional[Tensor], gn: Optional[Tensor],
+                      want_g_res: bool = True, raw: bool = False):
+    """(g_res | None, g_y, g_pre | None, g_r | None, g_gate, g_post) from the gradients of x and n (None: zero;
+    ``gn`` together with ``pre``).  With ``raw`` the last four are replaced by the [g, 4, D] buffer of their
+    partial sums (columns pre, r, gate, post) for a later ``rowops.ColSums`` reduction; columns of vectors that
+    are not there are not written."""
+    what = "norm_add_norm_bwd"
+    dev = _same_device(what, y, res, post, gate, res_scale, pre, gx, gn)
+    if (gn is None) != (pre is None):
+        raise ValueError(f"{what}: gn and pre come together")
+    res, y, (post, gate, res_scale, pre) = _prepare(what, res, y, post, gate, res_scale, pre)
+    gx, gn = _rows(f"{what}: gx", y.shape, F32, gx), _rows(f"{what}: gn", y.shape, y.dtype, gn)
+    if dev.type != "cuda":
+        raise ValueError(f"{what} launches on a GPU; dual.norm_add_norm also takes CPU tensors")
+    if _elsewhere(dev):
+        with torch.cuda.device(dev):
+            return norm_add_norm_bwd(res, y, post, gate, eps, res_scale, pre, gx, gn, want_g_res, raw)
+    shape, D = y.shape, y.shape[-1]
+    rows = y.numel() // D
+    want_g_res = want_g_res and res is not None
+    # without a second norm and a scale the residual's gradient is x's
+    passed = want_g_res and pre is None and res_scale is None and gx is not None
+    g_res = gx if passed else _new(shape, F32, dev) if want_g_res else None
+    g_y = _new(shape, y.dtype, dev)
+    if rows == 0:
+        zero = lambda w: None if w is None else torch.zeros_like(w)
+        part = torch.zeros(1, 4, D, dtype=F32, device=dev)
+        return (g_res, g_y, part) if raw else (g_res, g_y, zero(pre), zero(res_scale), zero(gate), zero(post))
+    K = _kernels()
+    part = _new((K._lib.imf_norm_add_norm_grid(rows, D), 4, D), F32, dev)
+    p = K._ptr
+    ptrs = _PTRS(p(res), None, p(y), None, p(post), p(gate), p(res_scale), p(pre), None, None, None, None, p(gx), p(gn),
+                 None if passed else p(g_res), p(g_y), p(part))
+    K._check(K._lib.imf_norm_add_norm(ptrs, rows, D, float(eps), int(y.dtype == F32), 2, K._stream()),
+             "imf_norm_add_norm")
+    K.LAUNCHES.count += 1
+    if raw:
+        return g_res, g_y, part
+    from .rowops import ColSums
+
+    cs = ColSums()
+    sums = [None if w is None else cs.add(part, i, D, None) for i, w in enumerate((pre, res_scale, gate, post))]
+    cs.flush()
+    return (g_res, g_y, *sums)
+
+
+class _NormAddNormFn(torch.autograd.Function):
+    """x, n and their detached tangents; reverse mode through the primal only."""
+
+    @staticmethod
+    def forward(ctx, res, y, post, gate, res_scale, pre, dres, dy, eps):
+        x, n, dx, dn = norm_add_norm_fwd(res, y, post, gate, eps, res_scale, pre, dres, dy)
+        ctx.set_materialize_grads(False)
+        if any(ctx.needs_input_grad[:6]):
+            ctx.save_for_backward(res, y, post, gate, res_scale, pre)
+            ctx.eps = eps
+        ctx.mark_non_differentiable(*[t for t in (dx, dn) if t is not None])
+        return x, n, dx, dn
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gx, gn, _gdx, _gdn):
+        res, y, post, gate, res_scale, pre = ctx.saved_tensors
+        if gx is None and gn is None:
+            return (None,) * 9
+        if pre is not None and gn is None:
+            gn = torch.zeros_like(y)
+        g_res, g_y, g_pre, g_r, g_gate, g_post = norm_add_norm_bwd(
+            res, y, post, gate, ctx.eps, res_scale, pre, gx, gn, want_g_res=ctx.needs_input_grad[0])
+        return g_res, g_y, g_post, g_gate, g_r, g_pre, None, None, None
+
+
+def norm_add_norm_dual(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor, eps: float,
+                       res_scale: Optional[Tensor], pre: Optional[Tensor]):
+    """``ops.dual.norm_add_norm`` on CUDA tensors of the kernels' types."""
+    rp, rt = (None, None) if res is None else res
+    dy = y.t
+    if dy is None and rt is not None:
+        dy = torch.zeros_like(y.p)
+    x, n, dx, dn = _NormAddNormFn.apply(rp, y.p, post, gate, res_scale, pre, None if rt is None else rt.detach(),
+                                        None if dy is None else dy.detach(), eps)
+    return Dual(x, dx), None if n is None else Dual(n, dn)

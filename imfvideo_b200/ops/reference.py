@@ -141,6 +141,83 @@ def attention_jvp(q: Tensor, k: Tensor, v: Tensor, dq: Tensor, dk: Tensor,
 
 
 # --------------------------------------------------------------------------
+# Differential attention: heads 2j and 2j + 1 are a pair whose values lie side by side,
+# o = (softmax(q_2j k_2j^T) - lam_j softmax(q_2j+1 k_2j+1^T)) [v_2j | v_2j+1]
+# --------------------------------------------------------------------------
+def _pair_maps(t: Tensor) -> Tensor:
+    """(b, l, 2H, d) -> (b, l, H, 2, d): the two heads of a pair"""
+    return t.reshape(*t.shape[:2], t.shape[2] // 2, 2, t.shape[3])
+
+
+def diff_attention(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, scale: Optional[float] = None) -> Tensor:
+    """(b, l, 2H, d) tensors, lam (H,) or one weight for all; einsum form, so that forward- and
+    reverse-mode AD both work."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    up = lambda t: t if t.dtype == torch.float64 else t.float()
+    qp, kp = _pair_maps(up(q)), _pair_maps(up(k))
+    vp = up(v).reshape(*v.shape[:2], v.shape[2] // 2, 2 * v.shape[3])
+    p = torch.softmax(torch.einsum("blhmd,bshmd->bhmls", qp, kp) * scale, dim=-1)
+    w = up(lam).expand(v.shape[2] // 2)[None, :, None, None]
+    # each map times V first: flat maps are nearly equal, and their difference would be rounded
+    o = torch.einsum("bhmls,bshd->bhmld", p, vp)
+    o = o[:, :, 0] - w * o[:, :, 1]
+    return o.transpose(1, 2).reshape(v.shape).to(v.dtype)
+
+
+@torch.no_grad()
+def diff_attention_jvp(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Tensor, dk: Tensor, dv: Tensor,
+                       scale: Optional[float] = None) -> Tuple[Tensor, Tensor]:
+    """(o, do); the weights carry no tangent."""
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    up = lambda t: t if t.dtype == torch.float64 else t.float()
+    qp, kp, dqp, dkp = (_pair_maps(up(t)) for t in (q, k, dq, dk))
+    wide = lambda t: up(t).reshape(*t.shape[:2], t.shape[2] // 2, 2 * t.shape[3])
+    vp, dvp = wide(v), wide(dv)
+    score = lambda a, b: torch.einsum("blhmd,bshmd->bhmls", a, b) * scale
+    p = torch.softmax(score(qp, kp), dim=-1)
+    ds = score(dqp, kp) + score(qp, dkp)
+    t = p * (ds - (p * ds).sum(-1, keepdim=True))
+    w = up(lam).expand(v.shape[2] // 2)[None, :, None, None]
+    prod = lambda a, b: torch.einsum("bhmls,bshd->bhmld", a, b)
+    back = lambda z: (z[:, :, 0] - w * z[:, :, 1]).transpose(1, 2).reshape(v.shape).to(v.dtype)
+    return back(prod(p, vp)), back(prod(t, vp) + prod(p, dvp))
+
+
+# --------------------------------------------------------------------------
+# Norms around a branch: x = r res + gate post y / rms(y),  n = pre x / rms(x)
+# --------------------------------------------------------------------------
+def norm_add_norm(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tensor, eps: float,
+                  res_scale: Optional[Tensor] = None, pre: Optional[Tensor] = None
+                  ) -> Tuple[Tensor, Optional[Tensor]]:
+    """(x, n or None) in 32 bits or more, unrounded."""
+    up = lambda t: t if t is None or t.dtype == torch.float64 else t.float()
+    unit = lambda t: t * torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + eps)
+    x = unit(up(y)) * (up(gate) * up(post))
+    if res is not None:
+        x = x + (up(res) if res_scale is None else up(res) * up(res_scale))
+    return x, None if pre is None else unit(x) * up(pre)
+
+
+@torch.no_grad()
+def norm_add_norm_jvp(res: Optional[Tensor], dres: Optional[Tensor], y: Tensor, dy: Tensor, post: Tensor,
+                      gate: Tensor, eps: float, res_scale: Optional[Tensor] = None, pre: Optional[Tensor] = None
+                      ) -> Tuple[Tensor, Optional[Tensor]]:
+    """(dx, dn or None): parameters carry no tangent; without ``dres`` the residual stands still."""
+    up = lambda t: t if t is None or t.dtype == torch.float64 else t.float()
+
+    def unit_jvp(t, dt):
+        r = torch.rsqrt(t.pow(2).mean(-1, keepdim=True) + eps)
+        return r * (dt - t * r * r * (t * dt).mean(-1, keepdim=True))
+    dx = unit_jvp(up(y), up(dy)) * (up(gate) * up(post))
+    if dres is not None:
+        dx = dx + (up(dres) if res_scale is None else up(dres) * up(res_scale))
+    if pre is None:
+        return dx, None
+    x, _ = norm_add_norm(res, y, post, gate, eps, res_scale)
+    return dx, unit_jvp(x, dx) * up(pre)
+
+
+# --------------------------------------------------------------------------
 # Attention residual (Kimi-style per-token softmax over residual history)
 # --------------------------------------------------------------------------
 def attn_res(cands: Sequence[Tensor], w: Tensor, eps: float) -> Tensor:
