@@ -23,6 +23,8 @@
 #include "common.cuh"
 #include "host_util.h"
 
+#include <math.h>
+
 namespace imf {
 namespace diff {
 
@@ -40,7 +42,8 @@ static_assert(SOFT_WARPS * 32 * REG_SOFT + (THREADS - SOFT_WARPS * 32) * REG_OTH
               "register pool exceeded");
 constexpr float LOG2E = 1.4426950408889634f;
 
-// A record of a partial segment, for each map: accumulators [column][row] (o, then do), m, l, mu.
+// A record of a partial segment, for each map: accumulators [column][row] (o, then do), m of the scaled
+// scores, l, mu.
 template <bool TANGENT>
 struct Rec {
   static constexpr int ACC = TANGENT ? 2 * VD : VD;
@@ -81,6 +84,34 @@ IMF_DEVICE void store_out8(const Params& p, int which, int64_t at, const float* 
   if (p.low) *reinterpret_cast<uint2*>(p.low + which * p.plane + at) = low;
 }
 
+// The row's reference maximum as step `n` of its map left it goes to the warp of the other group in one
+// 64-bit word, the step's number in its upper half.  One scalar access each way: a vector of two words is
+// two accesses in no order, and the number could be seen before the maximum that it stands for.
+IMF_DEVICE uint64_t ref_word(float m, int n) { return (uint64_t)(uint32_t)n << 32 | __float_as_uint(m); }
+IMF_DEVICE void publish_ref(uint64_t* addr, float m, int n) {
+  asm volatile("st.volatile.shared.b64 [%0], %1;" ::"r"(smem_u32(addr)), "l"(ref_word(m, n)) : "memory");
+}
+// From the other group's warp, which decided long before as a rule.  Bounded; false: gave up.
+IMF_DEVICE bool ref_of_step(const uint64_t* addr, int n, float& m, volatile int* abort_flag, int* status) {
+  uint64_t t0 = 0;
+  for (uint32_t spins = 1;; ++spins) {
+    uint64_t word;
+    asm volatile("ld.volatile.shared.b64 %0, [%1];" : "=l"(word) : "r"(smem_u32(addr)) : "memory");
+    m = __uint_as_float((uint32_t)word);
+    if (__all_sync(0xffffffffu, (int)(word >> 32) >= n)) return true;
+    if ((spins & 63u) == 0) {
+      if (__any_sync(0xffffffffu, *abort_flag)) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (__any_sync(0xffffffffu, now - t0 > IMF_WAIT_LIMIT_NS)) {
+        *abort_flag = 1;
+        if (status) atomicCAS(status, 0, STATUS_TIMEOUT_SOFTMAX);
+        return false;
+      }
+    }
+  }
+}
+
 // ------------------------------------------------------------------ primal ---
 constexpr int P_STAGES = 4;
 constexpr int P_SLOT = 256, P_COL_S = 0, P_COL_O = BN, P_COL_P = BN + VD;    // TMEM columns of a map
@@ -99,6 +130,7 @@ struct PSmem {
   uint64_t o_final[2];     // last P V of a segment (one phase per segment, never skipped)
   uint64_t o_free;
   uint64_t xbar;
+  uint64_t turn[2][4];     // whose exponentials are next, for each pair of warps of a scheduler
   uint32_t tmem_base;
   int abort_flag;
 };
@@ -126,6 +158,7 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       mbar_init(&s.p_full[t], 4);
       mbar_init(&s.o_done[t], 1);
       mbar_init(&s.o_final[t], 1);
+      for (int w = 0; w < 4; ++w) mbar_init(&s.turn[t][w], 1);
     }
     mbar_init(&s.o_free, SOFT_WARPS);
     mbar_init(&s.xbar, SOFT_WARPS);
@@ -321,6 +354,11 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           if (!ok) break;
         }
         tc_fence_after();
+        if (t == 1 || it > 0) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.turn[t][wl], (uint32_t)((it - (t ^ 1)) & 1), abort_flag,
+                                                 p.status, STATUS_TIMEOUT_SOFTMAX));
+          if (!ok) break;
+        }
         const f32x2 neg_m2 = dup2(-m_used * scale_log2);
         f32x2 l_new = dup2(0.f);
 #pragma unroll
@@ -332,6 +370,10 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             const float p0 = ex2(lo2(e)), p1 = ex2(hi2(e));
             pk[i / 2] = pack_bf16(p0, p1);
             l_new = add2(l_new, pair2(__float_as_uint(p0), __float_as_uint(p1)));
+          }
+          if (c + 32 == BN) {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s.turn[t ^ 1][wl]);
           }
           tmem_st16(tb + P_COL_P + c / 2, pk);
         }
@@ -401,7 +443,7 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           for (int i = 0; i < 32; ++i) acc[i * TM] = __uint_as_float(ov[i]);
         }
         float* stats = part + Rec<false>::STATS;
-        stats[row] = m_used;
+        stats[row] = m_used * p.scale;
         stats[TM + row] = l_tot;
         stats[2 * TM + row] = 0.f;
       }
@@ -420,30 +462,46 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 }
 
 // ----------------------------------------------------------------- tangent ---
-constexpr int T_STAGES = 3;
-constexpr int T_COL_O = 128, T_COL_DO = 256;
-__host__ __device__ constexpr int t_col_s(int buf) { return buf ? 384 : 0; }
-__host__ __device__ constexpr int t_col_ds(int buf) { return t_col_s(buf) + BN; }
-constexpr int NC = BN / 2;             // score columns of a thread: two threads per query row
+constexpr int T_KSTAGES = 3, T_VSTAGES = 3;
+constexpr int T_COL_O = 0, T_COL_DO = VD;
+__host__ __device__ constexpr int t_col_s(int buf) { return 2 * VD + buf * 2 * BN; }      // S, dS; then P and T over them
 
 struct TSmem {
-  alignas(1024) uint8_t q[2][QPANEL];                // q, dq of the map at work
-  alignas(1024) uint8_t k[T_STAGES][2][KPANEL];      // k, dk
-  alignas(1024) uint8_t v[T_STAGES][4][KPANEL];      // V, dV
-  float xmx[2][2][TM];      // row-maximum exchange [parity][half][row]
-  float xlm[2][2][TM];      // (l, mu) exchange [half][which][row]
-  uint64_t q_full, q_empty;
-  uint64_t k_full[T_STAGES], k_empty[T_STAGES];
-  uint64_t v_full[T_STAGES], v_empty[T_STAGES];
+  alignas(1024) uint8_t q[2][2][QPANEL];             // of two walks: q, dq
+  alignas(1024) uint8_t k[T_KSTAGES][2][KPANEL];     // k, dk
+  alignas(1024) uint8_t v[T_VSTAGES][4][KPANEL];     // V, dV
+  uint64_t m_ref[TM];       // reference maximum of the row as of the last step decided | that step's number
+  float xst[2][3][TM];      // l, mu and reference maximum of either group, at a walk's end
+  uint64_t q_full[2], q_empty[2], q_ready;
+  uint64_t k_full[T_KSTAGES], k_empty[T_KSTAGES];
+  uint64_t v_full[T_VSTAGES], v_empty[T_VSTAGES];
   uint64_t s_full[2], p_full[2];
-  uint64_t o_done;      // every P V
-  uint64_t o_final;     // last P V of a map's walk (one phase per walk, never skipped)
-  uint64_t o_free;
-  uint64_t xbar;
+  uint64_t o_done[2];       // every O product
+  uint64_t o_final;         // the last one of a walk (one phase per walk, never skipped)
+  uint64_t o_free, sums;
   uint32_t tmem_base;
   int abort_flag;
 };
 
+// q and dq times a power of two, in place, by the softmax warps
+IMF_DEVICE void scale_queries(uint8_t (&q)[2][QPANEL], float f) {
+  uint4* qs = reinterpret_cast<uint4*>(q);
+#pragma unroll 4
+  for (int i = threadIdx.x; i < (int)(sizeof(q) / 16); i += SOFT_WARPS * 32) {
+    uint4 x = qs[i];
+    x.x = pack_bf16(bf16_lo(x.x) * f, bf16_hi(x.x) * f);
+    x.y = pack_bf16(bf16_lo(x.y) * f, bf16_hi(x.y) * f);
+    x.z = pack_bf16(bf16_lo(x.z) * f, bf16_hi(x.z) * f);
+    x.w = pack_bf16(bf16_lo(x.w) * f, bf16_hi(x.w) * f);
+    qs[i] = x;
+  }
+  fence_proxy_async_smem();
+  __syncwarp();
+}
+
+// UNIT: the scale is a power of two, which is multiplied into q and dq in shared memory, exactly, instead
+// of into every T.
+template <bool UNIT>
 __global__ void __launch_bounds__(THREADS, 1)
 attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_dq,
@@ -455,25 +513,29 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const int cta = blockIdx.x, G = gridDim.x;
 
   if (threadIdx.x == 0) {
-    mbar_init(&s.q_full, 1);
-    mbar_init(&s.q_empty, 1);
-    for (int i = 0; i < T_STAGES; ++i) {
+    for (int i = 0; i < T_KSTAGES; ++i) {
       mbar_init(&s.k_full[i], 1);
       mbar_init(&s.k_empty[i], 1);
+    }
+    for (int i = 0; i < T_VSTAGES; ++i) {
       mbar_init(&s.v_full[i], 1);
       mbar_init(&s.v_empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
+      mbar_init(&s.q_full[i], 1);
+      mbar_init(&s.q_empty[i], 1);
       mbar_init(&s.s_full[i], 1);
-      mbar_init(&s.p_full[i], SOFT_WARPS);
+      mbar_init(&s.p_full[i], SOFT_WARPS / 2);
+      mbar_init(&s.o_done[i], 1);
     }
-    mbar_init(&s.o_done, 1);
+    mbar_init(&s.q_ready, SOFT_WARPS);
     mbar_init(&s.o_final, 1);
     mbar_init(&s.o_free, SOFT_WARPS);
-    mbar_init(&s.xbar, SOFT_WARPS);
+    mbar_init(&s.sums, SOFT_WARPS);
     s.abort_flag = 0;
     fence_barrier_init();
   }
+  if (threadIdx.x < TM) s.m_ref[threadIdx.x] = ref_word(0.f, -1);
   if (warp == WARP_MMA) {
     tmem_alloc(&s.tmem_base, 512);
     tmem_relinquish();
@@ -493,37 +555,43 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
-        unsigned kv_it = 0;
-        int walk = 0;
+        prefetch_tmap(&tm_dq);
+        prefetch_tmap(&tm_dk);
+        prefetch_tmap(&tm_dv);
+        int kst = 0, vst = 0, walk = 0;
+        uint32_t kpar = 1, vpar = 1;         // an "empty" wait passes in the first round of a ring
         Segment sg;
         bool ok = true;
         for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
           int q0, h, b;
           item_coords(p, sg.item, q0, h, b);
           for (int m = 0; m < 2 && ok; ++m, ++walk) {
-            if (walk > 0) ok = mbar_wait(&s.q_empty, (walk - 1) & 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+            const int qs = walk & 1;
+            ok = mbar_wait(&s.q_empty[qs], (uint32_t)((walk >> 1) & 1) ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
             if (!ok) break;
-            mbar_arrive_expect_tx(&s.q_full, 2 * QPANEL);
-            tma_load_4d(s.q[0], &tm_q, &s.q_full, 0, 2 * h + m, q0, b);
-            tma_load_4d(s.q[1], &tm_dq, &s.q_full, 0, 2 * h + m, q0, b);
-            for (int j = sg.j0; j < sg.j1; ++j, ++kv_it) {
-              const int st = (int)(kv_it % T_STAGES);
-              const uint32_t par = (uint32_t)((kv_it / T_STAGES) & 1) ^ 1;
-              if (kv_it >= T_STAGES) {
-                ok = mbar_wait(&s.k_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
-                if (!ok) break;
+            mbar_arrive_expect_tx(&s.q_full[qs], 2 * QPANEL);
+            tma_load_4d(s.q[qs][0], &tm_q, &s.q_full[qs], 0, 2 * h + m, q0, b);
+            tma_load_4d(s.q[qs][1], &tm_dq, &s.q_full[qs], 0, 2 * h + m, q0, b);
+            for (int j = sg.j0; j < sg.j1; ++j) {
+              ok = mbar_wait(&s.k_empty[kst], kpar, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&s.k_full[kst], 2 * KPANEL);
+              tma_load_4d(s.k[kst][0], &tm_k, &s.k_full[kst], 0, 2 * h + m, j * BN, b);
+              tma_load_4d(s.k[kst][1], &tm_dk, &s.k_full[kst], 0, 2 * h + m, j * BN, b);
+              if (++kst == T_KSTAGES) {
+                kst = 0;
+                kpar ^= 1;
               }
-              mbar_arrive_expect_tx(&s.k_full[st], 2 * KPANEL);
-              tma_load_4d(s.k[st][0], &tm_k, &s.k_full[st], 0, 2 * h + m, j * BN, b);
-              tma_load_4d(s.k[st][1], &tm_dk, &s.k_full[st], 0, 2 * h + m, j * BN, b);
-              if (kv_it >= T_STAGES) {
-                ok = mbar_wait(&s.v_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
-                if (!ok) break;
-              }
-              mbar_arrive_expect_tx(&s.v_full[st], 4 * KPANEL);
+              ok = mbar_wait(&s.v_empty[vst], vpar, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&s.v_full[vst], 4 * KPANEL);
               for (int i = 0; i < 2; ++i) {
-                tma_load_4d(s.v[st][i], &tm_v, &s.v_full[st], 0, 2 * h + i, j * BN, b);
-                tma_load_4d(s.v[st][2 + i], &tm_dv, &s.v_full[st], 0, 2 * h + i, j * BN, b);
+                tma_load_4d(s.v[vst][i], &tm_v, &s.v_full[vst], 0, 2 * h + i, j * BN, b);
+                tma_load_4d(s.v[vst][2 + i], &tm_dv, &s.v_full[vst], 0, 2 * h + i, j * BN, b);
+              }
+              if (++vst == T_VSTAGES) {
+                vst = 0;
+                vpar ^= 1;
               }
             }
           }
@@ -531,93 +599,106 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       }
     } else if (warp == WARP_MMA) {
       // -------------------------------------------------------- MMA issuer --
+      // One thread issues both products, the scores of step n + 2 right behind the O product of step n, whose
+      // P and T they overwrite: that keeps the groups half a period apart.  With a warp for each product the
+      // O products of two steps came one behind the other, the scores of the next two behind those, and both
+      // groups waited at the same time (2 pairs of 29,140 tokens: 3.24 ms).
       if (elect_one()) {
         // Q [K | dK]^T -> S | dS and P [V | dV] -> O | dO are one product each (operands adjacent in
-        // shared memory, accumulators adjacent in TMEM); then dS += dQ K^T, dO += T V.
+        // shared memory, accumulators in TMEM): an SM reads 128 B of operands per clock, just what
+        // M = N = 128 from shared memory asks for
         constexpr uint32_t idesc_qk = idesc_bf16(TM, 2 * BN, 0, 0);
         constexpr uint32_t idesc_dqk = idesc_bf16(TM, BN, 0, 0);
         constexpr uint32_t idesc_pv = idesc_bf16(TM, 2 * VD, 0, 1);
         constexpr uint32_t idesc_tv = idesc_bf16(TM, VD, 0, 1);
-        const uint64_t q_desc = sdesc_kmajor(smem_u32(s.q[0])), dq_desc = sdesc_kmajor(smem_u32(s.q[1]));
-        const uint64_t k_desc = sdesc_kmajor(smem_u32(s.k[0][0]));
+        const uint64_t q_desc = sdesc_kmajor(smem_u32(s.q[0][0])), k_desc = sdesc_kmajor(smem_u32(s.k[0][0]));
         const uint64_t v_desc = sdesc_mnmajor(smem_u32(s.v[0][0]), KPANEL);
-        auto issue_qk = [&](int buf, int st) {
-          const uint64_t kd = k_desc + (uint32_t)(st * (2 * KPANEL >> 4));
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks)
-            mma_ss(tmem + t_col_s(buf), q_desc + ks * 2, kd + ks * 2, idesc_qk, ks != 0);
-#pragma unroll
-          for (int ks = 0; ks < HD / 16; ++ks)
-            mma_ss(tmem + t_col_ds(buf), dq_desc + ks * 2, kd + ks * 2, idesc_dqk, 1);
-          tc_commit(&s.s_full[buf]);
-          tc_commit(&s.k_empty[st]);
-        };
-        auto issue_pv = [&](int buf, int st, bool first, bool last) {
-          const uint64_t vd = v_desc + (uint32_t)(st * (4 * KPANEL >> 4));
-#pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks)
-            mma_ts(tmem + T_COL_O, tmem + t_col_s(buf) + ks * 8, vd + 128 * ks, idesc_pv, !(first && ks == 0));
-#pragma unroll
-          for (int ks = 0; ks < BN / 16; ++ks)
-            mma_ts(tmem + T_COL_DO, tmem + t_col_ds(buf) + ks * 8, vd + 128 * ks, idesc_tv, 1);
-          tc_commit(&s.o_done);
-          if (last) tc_commit(&s.o_final);
-        };
-        unsigned it = 0;          // K/V tiles so far: stage it % T_STAGES, buffer it & 1
-        int walk = 0;
+        int kst = 0, kbuf = 0, vst = 0, vbuf = 0, walk = 0;
+        uint32_t kpar = 0, vpar = 0, ppar = 0;
         Segment sg;
         bool ok = true;
         for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
           const int n_j = sg.j1 - sg.j0;
           for (int m = 0; m < 2 && ok; ++m, ++walk) {
-            ok = mbar_wait(&s.q_full, walk & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA) &&
-                 mbar_wait(&s.k_full[it % T_STAGES], (uint32_t)((it / T_STAGES) & 1), abort_flag, p.status,
-                           STATUS_TIMEOUT_TMA);
-            if (!ok) break;
-            tc_fence_after();
-            // Q K^T of the next tile is issued before waiting for the softmax of this one
-            issue_qk((int)(it & 1), (int)(it % T_STAGES));
-            if (n_j == 1) tc_commit(&s.q_empty);
-            for (int jj = 0; jj < n_j && ok; ++jj, ++it) {
-              const int st = (int)(it % T_STAGES);
-              if (jj + 1 < n_j) {
-                const int st1 = (int)((it + 1) % T_STAGES);
-                ok = mbar_wait(&s.k_full[st1], (uint32_t)(((it + 1) / T_STAGES) & 1), abort_flag, p.status,
-                               STATUS_TIMEOUT_TMA);
-                if (!ok) break;
-                tc_fence_after();
-                issue_qk((int)((it + 1) & 1), st1);
-                if (jj + 2 == n_j) tc_commit(&s.q_empty);
+            const int qs = walk & 1;
+            ok = UNIT ? mbar_wait(&s.q_ready, walk & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX)
+                      : mbar_wait(&s.q_full[qs], (uint32_t)((walk >> 1) & 1), abort_flag, p.status, STATUS_TIMEOUT_TMA);
+            const uint64_t qd = q_desc + (uint32_t)(qs * (2 * QPANEL >> 4)), dqd = qd + (QPANEL >> 4);
+            // scores of step jj of the walk
+            auto scores = [&](int jj) {
+              if (!mbar_wait(&s.k_full[kst], kpar, abort_flag, p.status, STATUS_TIMEOUT_TMA)) return false;
+              tc_fence_after();
+              const uint64_t kd = k_desc + (uint32_t)(kst * (2 * KPANEL >> 4));
+              const uint32_t sc = tmem + t_col_s(kbuf);
+#pragma unroll
+              for (int ks = 0; ks < HD / 16; ++ks) mma_ss(sc, qd + 2 * ks, kd + 2 * ks, idesc_qk, ks != 0);
+#pragma unroll
+              for (int ks = 0; ks < HD / 16; ++ks) mma_ss(sc + BN, dqd + 2 * ks, kd + 2 * ks, idesc_dqk, 1);
+              tc_commit(&s.s_full[kbuf]);
+              tc_commit(&s.k_empty[kst]);
+              if (jj + 1 == n_j) tc_commit(&s.q_empty[qs]);
+              if (++kst == T_KSTAGES) {
+                kst = 0;
+                kpar ^= 1;
               }
-              ok = mbar_wait(&s.p_full[it & 1], (uint32_t)((it >> 1) & 1), abort_flag, p.status,
-                             STATUS_TIMEOUT_SOFTMAX) &&
-                   mbar_wait(&s.v_full[st], (uint32_t)((it / T_STAGES) & 1), abort_flag, p.status,
-                             STATUS_TIMEOUT_TMA);
-              if (ok && jj == 0 && walk > 0)
-                ok = mbar_wait(&s.o_free, (uint32_t)((walk - 1) & 1), abort_flag, p.status,
-                               STATUS_TIMEOUT_SOFTMAX);
+              kbuf ^= 1;
+              return true;
+            };
+            ok = ok && scores(0) && (n_j == 1 || scores(1));
+            if (ok && walk > 0)      // epilogue of the previous walk has drained O
+              ok = mbar_wait(&s.o_free, (uint32_t)((walk - 1) & 1), abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
+            for (int jj = 0; jj < n_j && ok; ++jj) {
+              ok = mbar_wait(&s.v_full[vst], vpar, abort_flag, p.status, STATUS_TIMEOUT_TMA) &&
+                   mbar_wait(&s.p_full[vbuf], ppar, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
               if (!ok) break;
               tc_fence_after();
-              issue_pv((int)(it & 1), st, jj == 0, jj + 1 == n_j);
-              tc_commit(&s.v_empty[st]);
+              const uint64_t vd = v_desc + (uint32_t)(vst * (4 * KPANEL >> 4));
+              const uint32_t pc = tmem + t_col_s(vbuf);
+#pragma unroll
+              for (int ks = 0; ks < BN / 16; ++ks)
+                mma_ts(tmem + T_COL_O, pc + ks * 8, vd + 128 * ks, idesc_pv, !(jj == 0 && ks == 0));
+#pragma unroll
+              for (int ks = 0; ks < BN / 16; ++ks)
+                mma_ts(tmem + T_COL_DO, pc + BN / 2 + ks * 8, vd + 128 * ks, idesc_tv, 1);
+              tc_commit(&s.o_done[vbuf]);
+              tc_commit(&s.v_empty[vst]);
+              if (jj + 1 == n_j) tc_commit(&s.o_final);
+              if (++vst == T_VSTAGES) {
+                vst = 0;
+                vpar ^= 1;
+              }
+              vbuf ^= 1;
+              if (vbuf == 0) ppar ^= 1;
+              if (jj + 2 < n_j) ok = scores(jj + 2);
             }
           }
         }
       }
     }
   } else {
-    // --------------------------------------- softmax / correction / epilogue --
+    // ------------------------------------- softmax / correction / epilogue --
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFT));
-    const int half = warp >> 2, wl = warp & 3;      // column half; lane quadrant
-    const int c0 = half * NC;                       // first score column of this thread
+    // Group g takes the steps (K/V tiles) of parity g, with buffer g.  Either warp of a row pair needs
+    // the row's reference maximum as the step before left it: it is handed from one to the other,
+    // before the exponentials.
+    const int g = warp >> 2, wl = warp & 3;
     const int row = wl * 32 + lane;
     const uint32_t tb = tmem_addr(tmem, wl * 32, 0);
-    const float scale_log2 = p.scale * LOG2E;
-    // 64 columns of o, then of do, of this thread's half: [column][row]
-    float* const hold = p.hold + (size_t)cta * HOLD + (size_t)half * VD * TM + row;
-    unsigned it = 0;
-    uint32_t xn = 0;                                // exchanges done so far (phase of xbar)
+    const uint32_t sc = tb + t_col_s(g);
+    const float scale_log2 = (UNIT ? 1.f : p.scale) * LOG2E;
+    // 64 columns of o, then of do, of this thread's head: [column][row]
+    float* const hold = p.hold + (size_t)cta * HOLD + (size_t)g * VD * TM + row;
+    uint32_t par = 0;                               // phase of this group's buffer
+    int n0 = 0;                                     // number of the walk's first step
     int walk = 0;
+    auto scale_for = [&](int w) {                   // UNIT: the queries of walk w
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.q_full[w & 1], (uint32_t)((w >> 1) & 1), abort_flag, p.status,
+                                             STATUS_TIMEOUT_TMA)))
+        return false;
+      scale_queries(s.q[w & 1], p.scale);
+      if (lane == 0) mbar_arrive(&s.q_ready);
+      return true;
+    };
     Segment sg;
     bool ok = true;
     for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
@@ -628,121 +709,137 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll 1
       for (int m = 0; m < 2 && ok; ++m, ++walk) {
         float m_used = -INFINITY, l_sum = 0.f, l_sum2 = 0.f, mu_sum = 0.f, mu_sum2 = 0.f;
-        for (int j = sg.j0; j < sg.j1 && ok; ++j, ++it) {
-          const int buf = (int)(it & 1);
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[buf], (uint32_t)((it >> 1) & 1), abort_flag, p.status,
-                                                 STATUS_TIMEOUT_MMA));
+        const int j_own = sg.j0 + ((n0 ^ g) & 1);     // this group's first step of the walk
+        if (UNIT && walk == 0) ok = scale_for(0);
+        for (int j = j_own; j < sg.j1 && ok; j += 2) {
+          const int n = n0 + j - sg.j0;
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[g], par, abort_flag, p.status, STATUS_TIMEOUT_MMA));
           if (!ok) break;
           tc_fence_after();
-          uint32_t sv[NC], dsv[NC];
-          tmem_ld32(tb + t_col_s(buf) + c0, sv);
-          tmem_ld32(tb + t_col_ds(buf) + c0, dsv);
-          tc_wait_ld();
-          const int kv_rem = p.L - j * BN - c0;
-          if (kv_rem < NC) {
-#pragma unroll
-            for (int i = 0; i < NC; ++i)
-              if (i >= kv_rem) sv[i] = 0xff800000u;  // -inf
-          }
-          const bool first = j == sg.j0;
-          float alpha = 1.f;
-          // The exponentials are taken against the reference maximum that the rows already have
-          // while the new maximum is formed alongside; only when a row has outgrown its reference
-          // by more than 2^8 (or has none yet) is the reference moved, O and dO rescaled and the tile
-          // done again from the scores, which are still in registers.
-          uint32_t pk[NC / 2];
-          uint32_t tk[NC / 2];
-          f32x2 l_new, mu_new;
-          for (bool redo = false;; redo = true) {
-            const f32x2 neg_m2 = dup2(-m_used * scale_log2);
-            l_new = mu_new = dup2(0.f);
-            float mx0 = -INFINITY, mx1 = -INFINITY;
-#pragma unroll
-            for (int i = 0; i < NC; i += 2) {
-              float& mxi = (i & 2) ? mx1 : mx0;
-              asm("max.f32 %0, %0, %1, %2;" : "+f"(mxi) : "f"(__uint_as_float(sv[i])), "f"(__uint_as_float(sv[i + 1])));
-              const f32x2 e = fma2(pair2(sv[i], sv[i + 1]), dup2(scale_log2), neg_m2);
-              const float p0 = ex2(lo2(e)), p1 = ex2(hi2(e));
-              const f32x2 pp = pair2(__float_as_uint(p0), __float_as_uint(p1));
-              pk[i / 2] = pack_bf16(p0, p1);
-              l_new = add2(l_new, pp);
-              const f32x2 tt = mul2(mul2(pp, pair2(dsv[i], dsv[i + 1])), dup2(p.scale));
-              mu_new = add2(mu_new, tt);
-              tk[i / 2] = pack_bf16(lo2(tt), hi2(tt));
-            }
-            if (redo) break;
-            float mx = fmaxf(mx0, mx1);
-            // both column halves of a row must use the same maximum.  The exchange is also the
-            // point after which every S / dS column of this buffer has been read, so the bf16
-            // P / T written below may overlap the partner's score columns.
-            s.xmx[it & 1][half][row] = mx;
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.xbar);
-            ok = __all_sync(0xffffffffu, mbar_wait(&s.xbar, xn & 1, abort_flag, p.status,
-                                                   STATUS_TIMEOUT_SOFTMAX));
-            ++xn;
-            if (!ok) break;
-            mx = fmaxf(mx, s.xmx[it & 1][half ^ 1][row]);
-            const bool need = first || (mx - m_used) * scale_log2 > 8.0f;
-            if (!__any_sync(0xffffffffu, need)) break;
-            if (need) {
-              if (!first) alpha = ex2((m_used - mx) * scale_log2);
-              m_used = mx;
-            }
-            if (first) continue;               // nothing in O yet
-            // half 0 rescales O, half 1 dO, once P V of the step before has run
-            ok = __all_sync(0xffffffffu, mbar_wait(&s.o_done, (uint32_t)((it - 1) & 1), abort_flag, p.status,
-                                                   STATUS_TIMEOUT_MMA));
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t rb = tb + (half ? T_COL_DO : T_COL_O);
+          const int kv_rem = p.L - j * BN;
+          if (kv_rem < BN) {                          // scores of keys past the end: -inf
+            int c = kv_rem;
+            for (; c & 7; ++c) tmem_st1(sc + c, 0xff800000u);
 #pragma unroll 1
-            for (int c = 0; c < VD; c += 32) {
-              uint32_t ov[32];
-              tmem_ld32(rb + c, ov);
-              tc_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-              tmem_st32(rb + c, ov);
-            }
+            for (; c < BN; c += 8) tmem_fill8(sc + c, 0xff800000u);
             tc_wait_st();
           }
+          uint32_t sv[BN];
+          tmem_ld32(sc, sv);
+          tmem_ld32(sc + 32, sv + 32);
+          tc_wait_ld();
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int i = 0; i < BN; i += 2)
+            asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[(i / 2) & 3]) : "f"(__uint_as_float(sv[i])), "f"(__uint_as_float(sv[i + 1])));
+          mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+          // The reference is moved only when a row has outgrown it by more than 2^8 (or has none yet).
+          // The scores of step n follow the O product of step n - 2, so whoever has the reference of step n
+          // and asks o_done for the O product of step n finds the barrier in that phase or one further.
+          float m_prev;
+          ok = ref_of_step(&s.m_ref[row], n - 1, m_prev, abort_flag, p.status);
           if (!ok) break;
-          l_sum = fmaf(l_sum, alpha, lo2(l_new));
-          l_sum2 = fmaf(l_sum2, alpha, hi2(l_new));
-          mu_sum = fmaf(mu_sum, alpha, lo2(mu_new));
-          mu_sum2 = fmaf(mu_sum2, alpha, hi2(mu_new));
-          tmem_st16(tb + t_col_s(buf) + c0 / 2, pk);
-          tmem_st16(tb + t_col_ds(buf) + c0 / 2, tk);
+          if (j == sg.j0) m_prev = mx[0];
+          const bool need = (mx[0] - m_prev) * scale_log2 > 8.0f;
+          const float m_new = need ? mx[0] : m_prev;
+          publish_ref(&s.m_ref[row], m_new, n);
+          if (__any_sync(0xffffffffu, m_new != m_used)) {
+            if (__any_sync(0xffffffffu, need)) {      // O, as of the step before, to the new reference
+              ok = __all_sync(0xffffffffu, mbar_wait(&s.o_done[g ^ 1], g == 0 ? par ^ 1 : par, abort_flag,
+                                                     p.status, STATUS_TIMEOUT_MMA));
+              if (!ok) break;
+              tc_fence_after();
+              const float alpha = ex2((m_prev - m_new) * scale_log2);
+#pragma unroll 1
+              for (int c = 0; c < 2 * VD; c += 16) {
+                uint32_t ov[16];
+                tmem_ld16(tb + T_COL_O + c, ov);
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+                tmem_st16(tb + T_COL_O + c, ov);
+              }
+            }
+            if (j != j_own) {                         // the sums so far to the new reference
+              const float alpha = ex2((m_used - m_new) * scale_log2);
+              l_sum *= alpha;
+              l_sum2 *= alpha;
+              mu_sum *= alpha;
+              mu_sum2 *= alpha;
+            }
+            m_used = m_new;
+          }
+          const f32x2 neg_m2 = dup2(-m_used * scale_log2);
+          f32x2 l_new = dup2(0.f), mu_new = dup2(0.f);
+          uint32_t dsv[2][32];
+          tmem_ld32(sc + BN, dsv[0]);
+          tmem_ld32(sc + BN + 32, dsv[1]);
+          tc_wait_ld();
+#pragma unroll
+          for (int c = 0; c < BN; c += 32) {
+            uint32_t pk[16], tk[16];
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) {
+              const int i = c + e;
+              const f32x2 x = fma2(pair2(sv[i], sv[i + 1]), dup2(scale_log2), neg_m2);
+              const float p0 = ex2(lo2(x)), p1 = ex2(hi2(x));
+              const f32x2 pp = pair2(__float_as_uint(p0), __float_as_uint(p1));
+              pk[e / 2] = pack_bf16(p0, p1);
+              l_new = add2(l_new, pp);
+              f32x2 tt = mul2(pp, pair2(dsv[i >> 5][i & 31], dsv[i >> 5][(i & 31) + 1]));
+              if (!UNIT) tt = mul2(tt, dup2(p.scale));
+              mu_new = add2(mu_new, tt);
+              tk[e / 2] = pack_bf16(lo2(tt), hi2(tt));
+            }
+            tmem_st16(sc + c / 2, pk);
+            tmem_st16(sc + BN / 2 + c / 2, tk);
+          }
+          l_sum += lo2(l_new);
+          l_sum2 += hi2(l_new);
+          mu_sum += lo2(mu_new);
+          mu_sum2 += hi2(mu_new);
           tc_wait_st();
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) mbar_arrive(&s.p_full[buf]);
+          if (lane == 0) mbar_arrive(&s.p_full[g]);
+          par ^= 1;
         }
+        // the next walk's scores are made during this one's epilogue
+        Segment next;
+        if (UNIT && ok && (m == 0 || get_segment(p.sh, cta, G, si + 1, next))) ok = scale_for(walk + 1);
         // ---- epilogue of this walk ----
-        float l_tot = l_sum + l_sum2, mu_tot = mu_sum + mu_sum2;
-        s.xlm[half][0][row] = l_tot;
-        s.xlm[half][1][row] = mu_tot;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.xbar);
-        if (ok)
-          ok = mbar_wait(&s.xbar, xn & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX) &&
-               mbar_wait(&s.o_final, (uint32_t)(walk & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA);
-        ++xn;
+        if (ok) ok = mbar_wait(&s.o_final, (uint32_t)(walk & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        l_tot += s.xlm[half ^ 1][0][row];
-        mu_tot += s.xlm[half ^ 1][1][row];
+        s.xst[g][0][row] = l_sum + l_sum2;
+        s.xst[g][1][row] = mu_sum + mu_sum2;
+        s.xst[g][2][row] = m_used;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s.sums);
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.sums, (uint32_t)(walk & 1), abort_flag, p.status,
+                                               STATUS_TIMEOUT_SOFTMAX));
+        if (!ok) break;
+        // the group of the last step has the final reference
+        const int n_j = sg.j1 - sg.j0, gl = (n0 + n_j - 1) & 1;
+        const float m_fin = s.xst[gl][2][row];
+        float l_tot = s.xst[gl][0][row], mu_tot = s.xst[gl][1][row];
+        if (n_j > 1) {
+          const float alpha = ex2((s.xst[gl ^ 1][2][row] - m_fin) * scale_log2);
+          l_tot += alpha * s.xst[gl ^ 1][0][row];
+          mu_tot += alpha * s.xst[gl ^ 1][1][row];
+        }
+        n0 += n_j;
+        const float m_score = UNIT ? m_fin : m_fin * p.scale;      // of the scaled scores
         if (sg.rec < 0) {
-          // this thread takes the 64 channels of head 2h + half, of o and of do
+          // this thread takes the 64 channels of head 2h + g, of o and of do
           const float inv_l = 1.f / l_tot, mul = mu_tot * inv_l, lam = p.lam.at(h);
-          const int64_t off = (int64_t)b * p.o_sb + (int64_t)q_row * p.o_sl + (int64_t)(2 * h + half) * p.o_sh;
+          const int64_t off = (int64_t)b * p.o_sb + (int64_t)q_row * p.o_sl + (int64_t)(2 * h + g) * p.o_sh;
 #pragma unroll 1
           for (int c = 0; c < VD / 2; c += 32) {
             uint32_t ov[32], dv_[32];
-            tmem_ld32(tb + T_COL_O + half * (VD / 2) + c, ov);
-            tmem_ld32(tb + T_COL_DO + half * (VD / 2) + c, dv_);
+            tmem_ld32(tb + T_COL_O + g * (VD / 2) + c, ov);
+            tmem_ld32(tb + T_COL_DO + g * (VD / 2) + c, dv_);
             tc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 32; ++i) {
@@ -777,23 +874,22 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
               }
             }
           }
-          if (live && p.lse && half == 0)
-            p.lse[((int64_t)b * 2 * p.H + 2 * h + m) * p.L + q_row] = m_used * p.scale + __logf(l_tot);
+          if (live && p.lse && g == 0)
+            p.lse[((int64_t)b * 2 * p.H + 2 * h + m) * p.L + q_row] = m_score + __logf(l_tot);
         } else {
-          // half 0 stores the O accumulators (columns 0-127), half 1 those of dO (128-255)
+          // group 0 stores the O accumulators (columns 0-127), group 1 those of dO (128-255)
           float* part = p.scratch + (size_t)sg.rec * Rec<true>::ALL + m * Rec<true>::MAP;
-          const uint32_t rb = tb + (half ? T_COL_DO : T_COL_O);
           for (int c = 0; c < VD; c += 32) {
             uint32_t ov[32];
-            tmem_ld32(rb + c, ov);
+            tmem_ld32(tb + T_COL_O + g * VD + c, ov);
             tc_wait_ld();
-            float* acc = part + (size_t)(c + half * VD) * TM + row;
+            float* acc = part + (size_t)(c + g * VD) * TM + row;
 #pragma unroll
             for (int i = 0; i < 32; ++i) acc[i * TM] = __uint_as_float(ov[i]);
           }
-          if (half == 0) {
+          if (g == 0) {
             float* stats = part + Rec<true>::STATS;
-            stats[row] = m_used;
+            stats[row] = m_score;
             stats[TM + row] = l_tot;
             stats[2 * TM + row] = mu_tot;
           }
@@ -824,7 +920,7 @@ __global__ void __launch_bounds__(32 * VD / COMBINE_COLS) attn_diff_combine_kern
   if (!split_item(p.sh, c, G, item, parts)) return;
   int q0, h, b;
   item_coords(p, item, q0, h, b);
-  const float scale_log2 = p.scale * LOG2E, lam = p.lam.at(h);
+  const float lam = p.lam.at(h);
   const int r = blockIdx.y * COMBINE_ROWS + (threadIdx.x & 31);
   const int col = (threadIdx.x >> 5) * COMBINE_COLS;
   const int q_row = q0 + r;
@@ -841,7 +937,7 @@ __global__ void __launch_bounds__(32 * VD / COMBINE_COLS) attn_diff_combine_kern
 #pragma unroll 2
     for (int k = 0; k < parts; ++k, x += k == 1 ? R::ALL : 2 * R::ALL) {
       const float mk = x[R::STATS], mn = fmaxf(m, mk);
-      const float w0 = ex2((m - mn) * scale_log2), w1 = ex2((mk - mn) * scale_log2);
+      const float w0 = ex2((m - mn) * LOG2E), w1 = ex2((mk - mn) * LOG2E);
       m = mn;
       l = l * w0 + x[R::STATS + TM] * w1;
       mu = mu * w0 + x[R::STATS + 2 * TM] * w1;
@@ -861,7 +957,7 @@ __global__ void __launch_bounds__(32 * VD / COMBINE_COLS) attn_diff_combine_kern
     }
     if (map == 1 && p.o2) store_out8(p, 1, off, o);
     if (p.lse && col == 0)
-      p.lse[((int64_t)b * 2 * p.H + 2 * h + map) * p.L + q_row] = m * p.scale + __logf(l);
+      p.lse[((int64_t)b * 2 * p.H + 2 * h + map) * p.L + q_row] = m + __logf(l);
   }
   store_out8(p, 0, off, y);
   if (TANGENT)
@@ -956,14 +1052,18 @@ extern "C" int imf_attn_diff_fwd(const void* q, const void* k, const void* v, co
   if ((rc = make_map(&mk, k, B, L, 2 * H, strides + 3, BN))) return rc;
   if ((rc = make_map(&mv, v, B, L, 2 * H, strides + 6, BN))) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  static bool smem_set[2][HOST_MAX_DEVICES] = {{false}};
+  static bool smem_set[3][HOST_MAX_DEVICES] = {{false}};
   if (tangent) {
     if ((rc = make_map(&mdq, dq, B, L, 2 * H, strides + 9, TM))) return rc;
     if ((rc = make_map(&mdk, dk, B, L, 2 * H, strides + 12, BN))) return rc;
     if ((rc = make_map(&mdv, dv, B, L, 2 * H, strides + 15, BN))) return rc;
     const size_t smem = sizeof(TSmem) + 1024;
-    if (!allow_smem((const void*)attn_diff_jvp_kernel, smem, smem_set[1])) return IMF_ERR_LAUNCH;
-    attn_diff_jvp_kernel<<<G, THREADS, smem, st>>>(mq, mk, mv, mdq, mdk, mdv, prm);
+    int e;
+    // (a power of two so far below one that queries times it might leave bf16's normal numbers is not taken)
+    const bool unit = scale > 0x1p-9f && scale <= 1.f && frexpf(scale, &e) == 0.5f;
+    auto kern = unit ? attn_diff_jvp_kernel<true> : attn_diff_jvp_kernel<false>;
+    if (!allow_smem((const void*)kern, smem, smem_set[unit ? 2 : 1])) return IMF_ERR_LAUNCH;
+    kern<<<G, THREADS, smem, st>>>(mq, mk, mv, mdq, mdk, mdv, prm);
   } else {
     const size_t smem = sizeof(PSmem) + 1024;
     if (!allow_smem((const void*)attn_diff_fwd_kernel, smem, smem_set[0])) return IMF_ERR_LAUNCH;
