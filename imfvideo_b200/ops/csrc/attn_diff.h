@@ -13,6 +13,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "common.cuh"
+
 namespace imf {
 
 // The pairs' weights: bf16 or fp32, `stride` elements apart (0: one weight for all pairs).
@@ -25,6 +27,28 @@ struct DiffWeights {
                    : static_cast<const float*>(p)[pair * stride];
   }
 };
+
+// 2^x of two values, x up to 127, on the FMA units, for part of a tile's exponentials: the exponential unit takes four
+// values a clock and scheduler and would set the pace alone.  2^x = 2^n 2^f, n the nearest whole number (from the
+// low bits of x + 1.5 2^23) and f in [-1/2, 1/2], where a polynomial of degree 4 with p(0) = 1, fitted to the
+// smallest relative error, is off by at most 2.9e-6.  Below -126: 2^-126, which rounds away beside anything.  NaN
+// stays NaN (in every step: the factor 2^n is multiplied, not added to the exponent).
+__device__ __forceinline__ f32x2 ex2_fma2(f32x2 x) {
+  float lo = lo2(x), hi = hi2(x);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(lo) : "f"(-126.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(hi) : "f"(-126.f));
+  x = pair2(__float_as_uint(lo), __float_as_uint(hi));
+  const f32x2 t = add2(x, dup2(12582912.f));
+  const f32x2 f = fma2(add2(t, dup2(-12582912.f)), dup2(-1.f), x);
+  f32x2 p = fma2(f, dup2(0x1.39f372p-7f), dup2(0x1.c9fb4ep-5f));
+  p = fma2(p, f, dup2(0x1.ec03b6p-3f));
+  p = fma2(p, f, dup2(0x1.62e132p-1f));
+  p = fma2(p, f, dup2(1.f));
+  return mul2(p, pair2(((uint32_t)t << 23) + 0x3f800000u, ((uint32_t)(t >> 32) << 23) + 0x3f800000u));
+}
+__device__ __forceinline__ f32x2 ex2_mufu2(f32x2 x) {
+  return pair2(__float_as_uint(ex2(lo2(x))), __float_as_uint(ex2(hi2(x))));
+}
 
 // Eight values as bf16 and what that dropped, and back.
 __device__ __forceinline__ void diff_split8(const float* x, uint4& hi, uint2& low) {

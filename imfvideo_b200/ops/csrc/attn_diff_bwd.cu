@@ -17,9 +17,13 @@
 // the dP^T that it is made from, and S^T of the next step follows dV of this one.  The tensor core then
 // works in two stretches, dV and the next S^T (768 clocks) while the math warps are at dS^T, dK, dQ and the
 // next dP^T (1,280) while they take exponentials.  Both maps at once would share dP^T but take 64 columns
-// more.  Shared memory: both K, V, two stages each of Q and dO, dS^T and the dQ tile fill 226 of 227 KB;
-// the constants of a row (lse2, delta) are 32-bit numbers that the math warps read, the operand bands of
-// attn_bwd.cu have no room.
+// more.
+//
+// The constants of a query row ride on the tensor core: a band of 16 columns a row holds -lse / scale and
+// -delta as three bf16 parts each (24 bits), and one more K-step against a tile of ones in the columns
+// that are meant makes S^T - lse / scale and dP^T - delta.  Reading them from shared memory instead costs the
+// math warps 1,024 clocks of its 128 B a clock per step, every lane of a warp the same 16 bytes.
+// Shared memory: both K, V, two stages each of Q and dO, dS^T, half a dQ tile, bands and ones: 225 of 227 KB.
 #include "attn_bwd_split.h"
 #include "attn_diff.h"
 #include "common.cuh"
@@ -48,11 +52,9 @@ struct Smem {
   uint8_t q[STAGES][PANEL];
   uint8_t d_o[STAGES][2][PANEL];
   uint8_t ds[2][PANEL];              // dS^T: [kv 128][q 128] as two 64-column panels
-  uint8_t dq_stage[2][PANEL];        // dQ tile [q 128][64] fp32 as two 32-column panels
-  // the last row is infinity, for the rows behind the last key: their score is zero, and P = exp(-lse) would
-  // be infinite from lse = -89 on, dQ infinity times a key of zeros
-  alignas(16) float lse2[STAGES + 1][T];
-  alignas(16) float delta[STAGES][T];
+  uint8_t dq_stage[4][PANEL / 4];    // by warp: 32 rows of 32 columns of a dQ tile [q 128][64] fp32
+  uint8_t band[STAGES][T * 32];      // [q 128][16] bf16: -lse / scale, -delta in three parts each, zeros
+  uint8_t ones[2][T * 32];           // [kv 128][16] bf16: ones in columns 0-2, in columns 3-5
   uint64_t kv_full;
   uint64_t q_full[STAGES], q_empty[STAGES], do_full[STAGES], do_empty[STAGES];
   uint64_t s_full, p_ready, dp_full, ds_ready, dq_full, dq_free, dk_free, final_bar;
@@ -62,8 +64,6 @@ struct Smem {
 static_assert(sizeof(Smem) <= 232448, "shared memory of an SM");
 
 struct Params {
-  const float* lse2;      // (B, 2H, Lp) log2-domain LSE, +inf on padding rows
-  const float* delta;     // (B, 2H, Lp), 0 on padding rows
   DiffWeights lam;
   __nv_bfloat16* dk;
   __nv_bfloat16* dv;
@@ -77,18 +77,15 @@ struct Params {
   // [dK_1 | dK_2 | dV] ([128][64], [128][64], [128][128], dK unscaled) and a second kernel adds them up
   int n_whole, parts;
   float* part;
-  // fixed-order dQ (null = arrival order): one counter per (batch, head, query tile), zeroed before the
+  // fixed-order dQ (null = arrival order): one counter per (batch, head, 32 query rows), zeroed before the
   // launch; the CTA of K/V tile j adds when the counter shows j
   int* turn;
 };
 constexpr size_t PART = (size_t)T * (2 * HD + VD);       // floats of a partial result
 
-IMF_DEVICE void bulk_load_1d(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-      ::"r"(smem_u32(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
-      : "memory");
-}
+// which of a row's pairs of columns take their exponentials on the FMA units
+__device__ __forceinline__ constexpr bool fma_pair(int i) { return (i & 7) == 1 || (i & 7) == 4 || (i & 7) == 6; }
+
 IMF_DEVICE void tma_reduce_add_4d(const CUtensorMap* m, const void* src, int c0, int c1, int c2, int c3) {
   asm volatile(
       "cp.reduce.async.bulk.tensor.4d.global.shared::cta.add.tile.bulk_group"
@@ -100,7 +97,8 @@ IMF_DEVICE void tma_reduce_add_4d(const CUtensorMap* m, const void* src, int c0,
 __global__ void __launch_bounds__(THREADS, 1)
 attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ CUtensorMap tm_do,
-                     const __grid_constant__ CUtensorMap tm_dq, const Params p) {
+                     const __grid_constant__ CUtensorMap tm_dq, const __grid_constant__ CUtensorMap tm_band,
+                     const Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   auto& s = *reinterpret_cast<Smem*>(smem_raw);
   if (smem_u32(smem_raw) & 1023u) {      // the swizzled tiles need it; there is no room to align here
@@ -121,7 +119,7 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const int n = (int)((long)(qpart + 1) * 2 * n_qt / parts) - first;
   auto map_of = [&](int i) { return first + i >= n_qt ? 1 : 0; };
   auto tile_of = [&](int i) { return first + i >= n_qt ? first + i - n_qt : first + i; };
-  int* turn = p.turn ? p.turn + ((size_t)b * p.H + h) * 2 * n_qt : nullptr;     // by step of the tile
+  int* turn = p.turn ? p.turn + ((size_t)b * p.H + h) * 2 * n_qt * 4 : nullptr;     // by step of the tile and warp
 
   if (threadIdx.x == 0) {
     mbar_init(&s.kv_full, 1);
@@ -142,7 +140,15 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     s.abort_flag = 0;
     fence_barrier_init();
   }
-  if (threadIdx.x < T) s.lse2[STAGES][threadIdx.x] = INFINITY;
+  // rows of 16 bf16, 32 bytes, whose two halves SWIZZLE_32B exchanges in every other group of four rows
+  for (int i = threadIdx.x; i < 2 * T * 2; i += THREADS) {
+    const int which = i / (2 * T), r = i / 2 % T, half = i & 1;
+    const uint4 w = half ? make_uint4(0u, 0u, 0u, 0u)
+                         : which == 0 ? make_uint4(0x3f803f80u, 0x00003f80u, 0u, 0u)
+                                      : make_uint4(0u, 0x3f800000u, 0x3f803f80u, 0u);
+    *reinterpret_cast<uint4*>(s.ones[which] + r * 32 + ((half ^ ((r >> 2) & 1)) << 4)) = w;
+  }
+  fence_proxy_async_smem();
   if (warp == 12) {
     tmem_alloc(&s.tmem_base, 512);
     tmem_relinquish();
@@ -170,16 +176,14 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         for (int i = 0; i < n; ++i) {
           const int st = i & 1, m = map_of(i), qt = tile_of(i);
           const uint32_t par = (uint32_t)((i >> 1) & 1) ^ 1;
-          const size_t row = ((size_t)b * 2 * p.H + 2 * h + m) * p.Lp + (size_t)qt * T;
           // (the dO of a step has its last reader well before its Q has)
           if (i >= STAGES && !mbar_wait(&s.do_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) break;
           mbar_arrive_expect_tx(&s.do_full[st], 2 * PANEL);
           for (int c = 0; c < 2; ++c) tma_load_4d(s.d_o[st][c], &tm_do, &s.do_full[st], 0, 2 * h + c, qt * T, b);
           if (i >= STAGES && !mbar_wait(&s.q_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY)) break;
-          mbar_arrive_expect_tx(&s.q_full[st], PANEL + 2 * T * 4);
+          mbar_arrive_expect_tx(&s.q_full[st], PANEL + T * 32);
           tma_load_4d(s.q[st], &tm_q, &s.q_full[st], 0, 2 * h + m, qt * T, b);
-          bulk_load_1d(s.lse2[st], p.lse2 + row, T * 4, &s.q_full[st]);
-          bulk_load_1d(s.delta[st], p.delta + row, T * 4, &s.q_full[st]);
+          tma_load_3d(s.band[st], &tm_band, &s.q_full[st], 0, qt * T, b * 2 * p.H + 2 * h + m);
         }
       }
     } else if (warp == 12) {
@@ -195,6 +199,7 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
           for (int ks = 0; ks < HD / 16; ++ks)
             mma_ss(tmem + C_S, sdesc_kmajor(a + ks * 32), sdesc_kmajor(qa + ks * 32), id_st, ks != 0);
+          mma_ss(tmem + C_S, sdesc_kmajor_sw32(smem_u32(s.ones[0])), sdesc_kmajor_sw32(smem_u32(s.band[i & 1])), id_st, 1);
           tc_commit(&s.s_full);
         };
         auto issue_dp = [&](int i) {
@@ -203,6 +208,7 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           for (int ks = 0; ks < VD / 16; ++ks)
             mma_ss(tmem + C_DP, sdesc_kmajor(va + (ks / 4) * PANEL + (ks % 4) * 32),
                    sdesc_kmajor(doa + (ks / 4) * PANEL + (ks % 4) * 32), id_st, ks != 0);
+          mma_ss(tmem + C_DP, sdesc_kmajor_sw32(smem_u32(s.ones[1])), sdesc_kmajor_sw32(smem_u32(s.band[i & 1])), id_st, 1);
           tc_commit(&s.dp_full);
         };
         bool ok = n > 0 && mbar_wait(&s.kv_full, 0, abort_flag, p.status, STATUS_TIMEOUT_TMA) &&
@@ -316,36 +322,39 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.dq_free);
-      // stage the tile in shared memory and let TMA add it to the fp32 accumulator: rows >= L clipped
-      if (i > 0) {
-        if (threadIdx.x == 8 * 32) {
-          if (turn && turn_live) {
-            // the previous add has been performed: pass its query tile on
-            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-            turn_pass(turn + first + i - 1, kvb + 1);
-          } else {
-            asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+      // Each warp adds its 32 rows for itself, 32 columns at a time, by TMA from shared memory to the fp32
+      // accumulator (rows >= L clipped; a box that begins behind them is left out)
+      const int r0 = tile_of(i) * T + wl * 32;
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        if (i > 0 || hf > 0) {
+          if (lane == 0) {
+            if (turn && turn_live && hf == 0) {
+              // the previous tile's adds have been performed: pass its query rows on
+              asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+              turn_pass(turn + (first + i - 1) * 4 + wl, kvb + 1);
+            } else {
+              asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+            }
           }
+          __syncwarp();
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-      }
 #pragma unroll
-      for (int c = 0; c < 16; ++c) {
-        uint8_t* dst = s.dq_stage[c / 8] + row * 128 + (((c & 7) ^ (row & 7)) << 4);
-        *reinterpret_cast<uint4*>(dst) = make_uint4(r[4 * c], r[4 * c + 1], r[4 * c + 2], r[4 * c + 3]);
-      }
-      fence_proxy_async_smem();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
-      if (threadIdx.x == 8 * 32) {
-        if (turn && turn_live) turn_live = turn_wait(turn + first + i, kvb, abort_flag, p.status);
-        if (!turn || turn_live) {
-#pragma unroll
-          for (int c = 0; c < 2; ++c)
-            tma_reduce_add_4d(&tm_dq, s.dq_stage[c], c * 32, 2 * h + map_of(i), tile_of(i) * T, b);
+        for (int c = 0; c < 8; ++c) {
+          const int x = hf * 32 + 4 * c;
+          *reinterpret_cast<uint4*>(s.dq_stage[wl] + lane * 128 + ((c ^ (lane & 7)) << 4)) =
+              make_uint4(r[x], r[x + 1], r[x + 2], r[x + 3]);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          if (turn && turn_live && hf == 0) turn_live = turn_wait(turn + (first + i) * 4 + wl, kvb, abort_flag, p.status);
+          if ((!turn || turn_live) && r0 < p.L)
+            tma_reduce_add_4d(&tm_dq, s.dq_stage[wl], hf * 32, 2 * h + map_of(i), r0, b);
           asm volatile("cp.async.bulk.commit_group;" ::: "memory");
         }
+        __syncwarp();
       }
-      __syncwarp();
       // dQ of a map's last step is behind its last dK
       if (i + 1 == n || map_of(i + 1) != map_of(i)) {
         store_dk(map_of(i), false);
@@ -354,9 +363,9 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         if (lane == 0) mbar_arrive(&s.dk_free);
       }
     }
-    if (threadIdx.x == 8 * 32) {
+    if (lane == 0) {
       asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-      if (turn && turn_live && ok && n > 0) turn_pass(turn + first + n - 1, kvb + 1);
+      if (turn && turn_live && ok && n > 0) turn_pass(turn + (first + n - 1) * 4 + wl, kvb + 1);
     }
     __syncwarp();
     if (part && ok) {
@@ -371,41 +380,34 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     const int wl = warp & 3;
     const int row = wl * 32 + lane;     // kv row of this thread (TMEM lane)
     const uint32_t tb = tmem_addr(tmem, wl * 32, 0);
-    const float scale_log2 = p.scale * LOG2E;
     const int kv_row = kvb * T + row;
-    const float neg_lam = -p.lam.at(h);
+    // rows behind the last key take no part: their score is zero, and exp(-lse) would be infinite from lse = -89
+    // on, dQ infinity times a key of zeros
+    const bool key = kv_row < p.L;
+    const f32x2 to_exp = dup2(key ? p.scale * LOG2E : 0.f);
+    const float w1 = key ? 1.f : 0.f, w2 = key ? -p.lam.at(h) : 0.f;
     bool ok = true;
     for (int i = 0; i < n && ok; ++i) {
-      const int st = i & 1;
       const uint32_t par = (uint32_t)(i & 1);
-      ok = mbar_wait(&s.s_full, par, abort_flag, p.status, STATUS_TIMEOUT_MMA) &&
-           mbar_wait(&s.q_full[st], (uint32_t)((i >> 1) & 1), abort_flag, p.status, STATUS_TIMEOUT_TMA);
-      ok = __all_sync(0xffffffffu, ok);
+      ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full, par, abort_flag, p.status, STATUS_TIMEOUT_MMA));
       if (!ok) break;
       tc_fence_after();
-      uint32_t sv[64];                  // the scores, then P^T
+      uint32_t sv[64];                  // S - lse / scale, then P^T
       tmem_ld32(tb + C_S + wg * 64, sv);
       tmem_ld32(tb + C_S + wg * 64 + 32, sv + 32);
       tc_wait_ld();
-      const float4* lse4 = reinterpret_cast<const float4*>(s.lse2[kv_row < p.L ? st : STAGES] + wg * 64);
-      const f32x2 w = dup2(map_of(i) ? neg_lam : 1.f);
+      const f32x2 w = dup2(map_of(i) ? w2 : w1);
 #pragma unroll
       for (int hh = 0; hh < 2; ++hh) {
         uint32_t pk[16];
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
+        for (int c = 0; c < 32; c += 2) {
           const int cg = hh * 32 + c;
-          const float4 l4 = lse4[cg / 4];
-          const f32x2 p01 = mul2(w, pair2(__float_as_uint(ex2(fmaf(__uint_as_float(sv[cg]), scale_log2, -l4.x))),
-                                          __float_as_uint(ex2(fmaf(__uint_as_float(sv[cg + 1]), scale_log2, -l4.y)))));
-          const f32x2 p23 = mul2(w, pair2(__float_as_uint(ex2(fmaf(__uint_as_float(sv[cg + 2]), scale_log2, -l4.z))),
-                                          __float_as_uint(ex2(fmaf(__uint_as_float(sv[cg + 3]), scale_log2, -l4.w)))));
-          sv[cg] = __float_as_uint(lo2(p01));
-          sv[cg + 1] = __float_as_uint(hi2(p01));
-          sv[cg + 2] = __float_as_uint(lo2(p23));
-          sv[cg + 3] = __float_as_uint(hi2(p23));
-          pk[c / 2] = pack_bf16(lo2(p01), hi2(p01));
-          pk[c / 2 + 1] = pack_bf16(lo2(p23), hi2(p23));
+          const f32x2 x = mul2(pair2(sv[cg], sv[cg + 1]), to_exp);
+          const f32x2 e = mul2(w, fma_pair(c / 2) ? ex2_fma2(x) : ex2_mufu2(x));
+          sv[cg] = __float_as_uint(lo2(e));
+          sv[cg + 1] = __float_as_uint(hi2(e));
+          pk[c / 2] = pack_bf16(lo2(e), hi2(e));
         }
         tmem_st16(tb + C_S + wg * 64 + hh * 16, pk);
       }
@@ -413,12 +415,11 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.p_ready);
-      // dS^T = P^T .* (dP^T - delta): to TMEM for dK and to shared memory for dQ (dP^T was issued behind
+      // dS^T = P^T .* (dP^T - delta), the bracket straight from the tensor core: to TMEM for dK and to shared memory for dQ (dP^T was issued behind
       // the dQ product of the previous step)
       ok = __all_sync(0xffffffffu, mbar_wait(&s.dp_full, par, abort_flag, p.status, STATUS_TIMEOUT_MMA));
       if (!ok) break;
       tc_fence_after();
-      const float4* dl4 = reinterpret_cast<const float4*>(s.delta[st] + wg * 64);
       uint8_t* dsb = s.ds[wg] + row * 128;
       uint32_t dp[2][32];
       tmem_ld32(tb + C_DP + wg * 64, dp[0]);
@@ -429,15 +430,10 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         uint32_t dk_[16];
         if (hh == 1) tc_wait_ld();
 #pragma unroll
-        for (int c = 0; c < 32; c += 4) {
+        for (int c = 0; c < 32; c += 2) {
           const int cg = hh * 32 + c;
-          const float4 d4 = dl4[cg / 4];
-          const f32x2 a = mul2(pair2(sv[cg], sv[cg + 1]),
-                               add2(pair2(dp[hh][c], dp[hh][c + 1]), pair2(__float_as_uint(-d4.x), __float_as_uint(-d4.y))));
-          const f32x2 e = mul2(pair2(sv[cg + 2], sv[cg + 3]),
-                               add2(pair2(dp[hh][c + 2], dp[hh][c + 3]), pair2(__float_as_uint(-d4.z), __float_as_uint(-d4.w))));
-          dk_[c / 2] = pack_bf16(lo2(a), hi2(a));
-          dk_[c / 2 + 1] = pack_bf16(lo2(e), hi2(e));
+          const f32x2 d = mul2(pair2(sv[cg], sv[cg + 1]), pair2(dp[hh][c], dp[hh][c + 1]));
+          dk_[c / 2] = pack_bf16(lo2(d), hi2(d));
         }
         tmem_st16(tb + C_DP + wg * 64 + hh * 16, dk_);     // (columns that hh = 0 has read)
 #pragma unroll
@@ -493,15 +489,16 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   }
 }
 
-// Per (b, l, pair), 16 lanes of 8 channels: delta of both maps, lse2 = lse * log2(e) (padding rows:
-// infinity, so P = 0), and zeros for the dQ additions.
+// Per (b, l, pair), 16 lanes of 8 channels: the bands of both maps (padding rows: the exponent -30000, so
+// P = 0), delta_2 for dlam, and zeros for the dQ additions.
 __global__ void attn_diff_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o2,
                                           const uint8_t* __restrict__ low, int64_t plane,
                                           const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse,
-                                          const DiffWeights lam, float* __restrict__ lse2, float* __restrict__ delta,
+                                          const DiffWeights lam, uint4* __restrict__ band, float* __restrict__ delta2,
                                           float* __restrict__ dq_acc, int B, int L, int H, int Lp, int64_t o_sb,
                                           int64_t o_sl, int64_t o_sh, 
-                                          int64_t g_sb, int64_t g_sl, int64_t g_sh) {
+                                          int64_t g_sb, int64_t g_sl, int64_t g_sh,
+                                          float inv_exp_scale) {
   const int lane = threadIdx.x & 31, part = lane & 15, c = (part & 7) * 8;
   const long u = (((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5) * 2 + (lane >> 4);
   const bool in = u < (long)B * H * Lp;          // no early exit: the shuffles below need every lane
@@ -537,14 +534,21 @@ __global__ void attn_diff_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, c
   }
   if (!in || part >= 2) return;
   const long row = ((long)b * 2 * H + 2 * h + part) * Lp + l;
-  lse2[row] = live ? lse[((long)b * 2 * H + 2 * h + part) * L + l] * LOG2E : INFINITY;
-  delta[row] = part ? d2 : live ? fmaf(lam.at(h), d2, d) : 0.f;
+  float x = live ? lse[((long)b * 2 * H + 2 * h + part) * L + l] * LOG2E : 0.f;
+  // (infinities become what is still finite over the smallest scale, 1e-30)
+  x = -(live ? fminf(fmaxf(x, -1e8f), 1e8f) : 30000.f) * inv_exp_scale;
+  const float y = live ? -(part ? d2 : fmaf(lam.at(h), d2, d)) : 0.f;
+  const float x1 = bf16_lo(pack_bf16(x, 0.f)), x2 = bf16_lo(pack_bf16(x - x1, 0.f));
+  const float y1 = bf16_lo(pack_bf16(y, 0.f)), y2 = bf16_lo(pack_bf16(y - y1, 0.f));
+  band[2 * row] = make_uint4(pack_bf16(x1, x2), pack_bf16(x - x1 - x2, y1), pack_bf16(y2, y - y1 - y2), 0u);
+  band[2 * row + 1] = make_uint4(0u, 0u, 0u, 0u);
+  if (part) delta2[((long)b * H + h) * Lp + l] = d2;
 }
 
 // dq = bf16(acc * scale); the last H blocks: dlam = -sum of delta_2, in a fixed order.
 __global__ void __launch_bounds__(256)
 attn_diff_bwd_post_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, long n4, float scale,
-                          const float* __restrict__ delta, void* dlam, int dlam_bf16, int B, int H, int L, int Lp,
+                          const float* __restrict__ delta2, void* dlam, int dlam_bf16, int B, int H, int L, int Lp,
                           unsigned n_conv) {
   if (blockIdx.x < n_conv) {
     const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
@@ -557,7 +561,7 @@ attn_diff_bwd_post_kernel(const float* __restrict__ acc, __nv_bfloat16* __restri
   __shared__ double sum[256];
   double t = 0.0;
   for (int b = 0; b < B; ++b) {
-    const float* d = delta + ((long)b * 2 * H + 2 * h + 1) * Lp;
+    const float* d = delta2 + ((long)b * H + h) * Lp;
 #pragma unroll 8
     for (int l = threadIdx.x; l < L; l += 256) t += d[l];
   }
@@ -613,17 +617,17 @@ static int make_map(CUtensorMap* m, const void* ptr, int B, int L, int heads, co
 
 // Where the parts of the scratch begin, in bytes, and its whole size.
 struct Layout {
-  size_t turn, turn_bytes, lse2, delta, part, all;
+  size_t turn, turn_bytes, band, delta2, part, all;
 };
 static Layout layout(int B, int L, int H, const BwdSplit& sp) {
   const size_t Lp = (size_t)(L + T - 1) / T * T;
   auto up = [](size_t x) { return (x + 255) & ~size_t(255); };
   Layout y;
   y.turn = up((size_t)B * L * 2 * H * HD * 4);                // fp32 dQ first
-  y.turn_bytes = up((size_t)B * 2 * H * (Lp / T) * 4);
-  y.lse2 = y.turn + y.turn_bytes;
-  y.delta = y.lse2 + up((size_t)B * 2 * H * Lp * 4);
-  y.part = y.delta + up((size_t)B * 2 * H * Lp * 4);
+  y.turn_bytes = up((size_t)B * 2 * H * (Lp / 32) * 4);
+  y.band = y.turn + y.turn_bytes;
+  y.delta2 = y.band + up((size_t)B * 2 * H * Lp * 32);
+  y.part = y.delta2 + up((size_t)B * H * Lp * 4);
   y.all = y.part + (size_t)sp.n_split * sp.parts * PART * 4;
   return y;
 }
@@ -669,19 +673,19 @@ extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, co
   uint8_t* base = static_cast<uint8_t*>(scratch);
   const int Lp = (L + T - 1) / T * T;
   float* dq_acc = reinterpret_cast<float*>(base);
-  float* lse2 = reinterpret_cast<float*>(base + y.lse2);
-  float* delta = reinterpret_cast<float*>(base + y.delta);
+  uint4* band = reinterpret_cast<uint4*>(base + y.band);
+  float* delta2 = reinterpret_cast<float*>(base + y.delta2);
   const bool ordered = fixed_order && status != nullptr;
   if (ordered && cudaMemsetAsync(base + y.turn, 0, y.turn_bytes, st) != cudaSuccess) return IMF_ERR_LAUNCH;
   const DiffWeights w{lam, lam_stride, lam_bf16};
   typedef const __nv_bfloat16 cbf;
   const long threads = (long)B * H * Lp * 16;
   attn_diff_bwd_prep_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(
-      static_cast<cbf*>(o), static_cast<cbf*>(o2), static_cast<const uint8_t*>(low), plane, static_cast<cbf*>(d_o), lse, w, lse2, delta, dq_acc, B, L, H, Lp,
+      static_cast<cbf*>(o), static_cast<cbf*>(o2), static_cast<const uint8_t*>(low), plane, static_cast<cbf*>(d_o), lse, w, band, delta2, dq_acc, B, L, H, Lp,
       o_strides[0], o_strides[1], o_strides[2], strides[9], strides[10],
-      strides[11]);
+      strides[11], 1.f / (scale * LOG2E));
   if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
-  CUtensorMap mq, mk, mv, mdo, mdq;
+  CUtensorMap mq, mk, mv, mdo, mdq, mb;
   int rc;
   if ((rc = make_map(&mq, q, B, L, 2 * H, strides))) return rc;
   if ((rc = make_map(&mk, k, B, L, 2 * H, strides + 3))) return rc;
@@ -691,12 +695,17 @@ extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, co
     const uint64_t row = (uint64_t)2 * H * HD * 4;
     uint64_t dims[4] = {(uint64_t)HD, (uint64_t)2 * H, (uint64_t)L, (uint64_t)B};
     uint64_t str[4] = {4, (uint64_t)HD * 4, row, row * L};
-    uint32_t box[4] = {32, 1, (uint32_t)T, 1};
+    uint32_t box[4] = {32, 1, 32, 1};
     if ((rc = make_tmap(&mdq, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, dq_acc, dims, str, box))) return rc;
   }
+  {
+    uint64_t dims[3] = {16, (uint64_t)Lp, (uint64_t)B * 2 * H};
+    uint64_t str[3] = {2, 32, (uint64_t)Lp * 32};
+    uint32_t box[3] = {16, (uint32_t)T, 1};
+    if ((rc = make_tmap(&mb, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, band, dims, str, box, CU_TENSOR_MAP_SWIZZLE_32B)))
+      return rc;
+  }
   Params prm;
-  prm.lse2 = lse2;
-  prm.delta = delta;
   prm.lam = w;
   prm.dk = static_cast<__nv_bfloat16*>(dk);
   prm.dv = static_cast<__nv_bfloat16*>(dv);
@@ -714,7 +723,7 @@ extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, co
   prm.turn = ordered ? reinterpret_cast<int*>(base + y.turn) : nullptr;
   static bool smem_set[HOST_MAX_DEVICES] = {false};
   if (!allow_smem((const void*)attn_diff_bwd_kernel, sizeof(Smem), smem_set)) return IMF_ERR_LAUNCH;
-  attn_diff_bwd_kernel<<<sp.ctas(), THREADS, sizeof(Smem), st>>>(mq, mk, mv, mdo, mdq, prm);
+  attn_diff_bwd_kernel<<<sp.ctas(), THREADS, sizeof(Smem), st>>>(mq, mk, mv, mdo, mdq, mb, prm);
   if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
   if (sp.n_split) {
     const long n = (long)sp.n_split * (long)(PART / 4);
@@ -723,7 +732,7 @@ extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, co
   }
   const long n4 = (long)B * L * 2 * H * HD / 4;
   const unsigned n_conv = (unsigned)((n4 + 255) / 256);
-  attn_diff_bwd_post_kernel<<<n_conv + H, 256, 0, st>>>(dq_acc, static_cast<__nv_bfloat16*>(dq), n4, scale, delta, dlam,
+  attn_diff_bwd_post_kernel<<<n_conv + H, 256, 0, st>>>(dq_acc, static_cast<__nv_bfloat16*>(dq), n4, scale, delta2, dlam,
                                                         lam_bf16, B, H, L, Lp, n_conv);
   return cudaGetLastError() == cudaSuccess ? IMF_OK : IMF_ERR_LAUNCH;
 }
