@@ -84,7 +84,7 @@ struct Params {
 constexpr size_t PART = (size_t)T * (2 * HD + VD);       // floats of a partial result
 
 // which of a row's pairs of columns take their exponentials on the FMA units
-__device__ __forceinline__ constexpr bool fma_pair(int i) { return (i & 7) == 1 || (i & 7) == 4 || (i & 7) == 6; }
+__device__ __forceinline__ constexpr bool fma_pair(int i) { return (i & 3) == 1; }
 
 IMF_DEVICE void tma_reduce_add_4d(const CUtensorMap* m, const void* src, int c0, int c1, int c2, int c3) {
   asm volatile(

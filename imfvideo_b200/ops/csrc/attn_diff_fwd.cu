@@ -9,13 +9,12 @@
 // and sum; what they share is V.  O_1 and O_2 are divided and subtracted in 32 bits and rounded once.
 //
 // TMEM (512 columns of fp32 per SM) decides the shapes:
-//   primal  : an item is 128 query rows of a pair.  Each map has a slot of its own: S (64), O (128),
-//             P (bf16, 32) and four softmax warps, so K_1, K_2 and V are read once for both maps, and
-//             the epilogue reads both O (the warps of a lane quadrant see its lanes in every column).
+//   primal  : an item is 128 query rows of a pair.  Each map has O (128) and two buffers of S (64) with P
+//             over it, so K_1, K_2 and V are read once for both maps, and the epilogue reads both O (the
+//             warps of a lane quadrant see its lanes in every column).
 //   tangent : O | dO of one map (256) and two S | dS buffers leave no room for the other map.  A segment
 //             runs map 1, then map 2, over the same K/V tiles; map 1's finished rows wait in global
 //             memory (128 KB a CTA, in L2) and come back to the thread that wrote them.
-// Q K^T and P V of the primal are issued by two warps, so that neither waits for the other's barriers.
 // Scheduling, shares and records of split items are those of attn_fwd_split.h, with a record for each
 // map; the kernel that merges the parts also subtracts.
 #include "attn_diff.h"
@@ -35,7 +34,7 @@ constexpr int BN = 64;               // K/V rows per tile
 constexpr int QPANEL = TM * 128;     // bytes of a query tile (64 columns)
 constexpr int KPANEL = BN * 128;     // bytes of 64 columns of a K/V tile
 constexpr int SOFT_WARPS = 8;
-constexpr int WARP_MMA = 8, WARP_TMA = 9, WARP_PV = 10;   // primal: WARP_MMA issues Q K^T only
+constexpr int WARP_MMA = 8, WARP_TMA = 9;
 constexpr int THREADS = 12 * 32;
 constexpr int REG_SOFT = 216, REG_OTHER = 72, REG_LAUNCH = 168;
 static_assert(SOFT_WARPS * 32 * REG_SOFT + (THREADS - SOFT_WARPS * 32) * REG_OTHER <= THREADS * REG_LAUNCH,
@@ -114,28 +113,37 @@ IMF_DEVICE bool ref_of_step(const uint64_t* addr, int n, float& m, volatile int*
 
 // ------------------------------------------------------------------ primal ---
 constexpr int P_STAGES = 4;
-constexpr int P_SLOT = 256, P_COL_S = 0, P_COL_O = BN, P_COL_P = BN + VD;    // TMEM columns of a map
-static_assert(P_COL_P + BN / 2 <= P_SLOT, "TMEM budget");
+constexpr int P_SOFT_WARPS = 16;       // by map and parity of the step, four each
+constexpr int P_WARP_MMA = 16, P_WARP_TMA = 18;        // a warp that issues products for either map; loads
+constexpr int P_THREADS = 20 * 32;
+// setmaxnreg.inc draws from what the CTA was launched with; a request beyond that pool blocks for ever
+constexpr int P_REG_SOFT = 104, P_REG_OTHER = 64, P_REG_LAUNCH = 96;
+static_assert(P_SOFT_WARPS * 32 * P_REG_SOFT + (P_THREADS - P_SOFT_WARPS * 32) * P_REG_OTHER <= P_THREADS * P_REG_LAUNCH,
+              "register pool exceeded");
+// TMEM columns of a map: O, then S of even and of odd steps, P over the S that it is made from
+constexpr int P_MAP = 256, P_COL_O = 0;
+__host__ __device__ constexpr int p_col_s(int g) { return VD + g * BN; }
+static_assert(p_col_s(2) <= P_MAP, "TMEM budget");
 
 struct PSmem {
-  alignas(1024) uint8_t q[2][QPANEL];
+  alignas(1024) uint8_t q[2][2][QPANEL];             // of two segments: Q_1, Q_2
   alignas(1024) uint8_t k[P_STAGES][2][KPANEL];      // K_1, K_2
   alignas(1024) uint8_t v[P_STAGES][2][KPANEL];      // the two halves of V
-  float inv_l[2][TM];                                // 1 / l of either map
-  uint64_t q_full, q_empty;
+  uint64_t m_ref[2][TM];       // by map: reference maximum of the row as of the last step decided | that step's number
+  // of two segments (a group without a step in the next one may be there already), by map and group: l and
+  // reference maximum at the segment's end
+  float xst[2][2][2][2][TM];
+  uint64_t q_full[2], q_empty[2];
   uint64_t k_full[P_STAGES], k_empty[P_STAGES];
   uint64_t v_full[P_STAGES], v_empty[P_STAGES];
-  uint64_t s_full[2], s_taken[2], p_full[2];
-  uint64_t o_done[2];      // every P V
-  uint64_t o_final[2];     // last P V of a segment (one phase per segment, never skipped)
-  uint64_t o_free;
-  uint64_t xbar;
-  uint64_t turn[2][4];     // whose exponentials are next, for each pair of warps of a scheduler
+  uint64_t s_full[2][2], p_full[2][2], o_done[2][2];   // by map and group
+  uint64_t o_final[2];         // the last P V of a segment (one phase per segment, never skipped)
+  uint64_t o_free, sums;
   uint32_t tmem_base;
   int abort_flag;
 };
 
-__global__ void __launch_bounds__(THREADS, 1)
+__global__ void __launch_bounds__(P_THREADS, 1)
 attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ CUtensorMap tm_k,
                      const __grid_constant__ CUtensorMap tm_v, const Params p) {
   extern __shared__ uint8_t smem_raw[];
@@ -144,28 +152,29 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const int cta = blockIdx.x, G = gridDim.x;
 
   if (threadIdx.x == 0) {
-    mbar_init(&s.q_full, 1);
-    mbar_init(&s.q_empty, 1);
     for (int i = 0; i < P_STAGES; ++i) {
       mbar_init(&s.k_full[i], 1);
-      mbar_init(&s.k_empty[i], 1);
+      mbar_init(&s.k_empty[i], 2);         // read for either map
       mbar_init(&s.v_full[i], 1);
-      mbar_init(&s.v_empty[i], 1);
+      mbar_init(&s.v_empty[i], 2);
     }
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&s.s_full[t], 1);
-      mbar_init(&s.s_taken[t], 4);
-      mbar_init(&s.p_full[t], 4);
-      mbar_init(&s.o_done[t], 1);
+      mbar_init(&s.q_full[t], 1);
+      mbar_init(&s.q_empty[t], 2);
+      for (int g = 0; g < 2; ++g) {
+        mbar_init(&s.s_full[t][g], 1);
+        mbar_init(&s.p_full[t][g], 4);
+        mbar_init(&s.o_done[t][g], 1);
+      }
       mbar_init(&s.o_final[t], 1);
-      for (int w = 0; w < 4; ++w) mbar_init(&s.turn[t][w], 1);
     }
-    mbar_init(&s.o_free, SOFT_WARPS);
-    mbar_init(&s.xbar, SOFT_WARPS);
+    mbar_init(&s.o_free, P_SOFT_WARPS);
+    mbar_init(&s.sums, P_SOFT_WARPS);
     s.abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == WARP_MMA) {
+  if (threadIdx.x < 2 * TM) s.m_ref[threadIdx.x / TM][threadIdx.x % TM] = ref_word(0.f, -1);
+  if (warp == P_WARP_MMA) {
     tmem_alloc(&s.tmem_base, 512);
     tmem_relinquish();
   }
@@ -175,189 +184,172 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
   const uint32_t tmem = s.tmem_base;
   volatile int* abort_flag = &s.abort_flag;
 
-  if (warp >= SOFT_WARPS) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REG_OTHER));
-    if (warp == WARP_TMA) {
+  if (warp >= P_SOFT_WARPS) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(P_REG_OTHER));
+    if (warp == P_WARP_TMA) {
       // ------------------------------------------------------ TMA producer --
       if (elect_one()) {
         prefetch_tmap(&tm_q);
         prefetch_tmap(&tm_k);
         prefetch_tmap(&tm_v);
-        unsigned kv_it = 0;
+        int st = 0;
+        uint32_t par = 1;                    // an "empty" wait passes in the first round of a ring
         Segment sg;
         bool ok = true;
         for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
           int q0, h, b;
           item_coords(p, sg.item, q0, h, b);
-          if (si > 0) ok = mbar_wait(&s.q_empty, (si - 1) & 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+          const int qs = si & 1;
+          ok = mbar_wait(&s.q_empty[qs], (uint32_t)((si >> 1) & 1) ^ 1, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
           if (!ok) break;
-          mbar_arrive_expect_tx(&s.q_full, 2 * QPANEL);
-          for (int m = 0; m < 2; ++m) tma_load_4d(s.q[m], &tm_q, &s.q_full, 0, 2 * h + m, q0, b);
-          for (int j = sg.j0; j < sg.j1; ++j, ++kv_it) {
-            const int st = (int)(kv_it % P_STAGES);
-            const uint32_t par = (uint32_t)((kv_it / P_STAGES) & 1) ^ 1;
-            if (kv_it >= P_STAGES) {
-              ok = mbar_wait(&s.k_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
-              if (!ok) break;
-            }
+          mbar_arrive_expect_tx(&s.q_full[qs], 2 * QPANEL);
+          for (int m = 0; m < 2; ++m) tma_load_4d(s.q[qs][m], &tm_q, &s.q_full[qs], 0, 2 * h + m, q0, b);
+          for (int j = sg.j0; j < sg.j1; ++j) {
+            ok = mbar_wait(&s.k_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+            if (!ok) break;
             mbar_arrive_expect_tx(&s.k_full[st], 2 * KPANEL);
             for (int m = 0; m < 2; ++m) tma_load_4d(s.k[st][m], &tm_k, &s.k_full[st], 0, 2 * h + m, j * BN, b);
-            if (kv_it >= P_STAGES) {
-              ok = mbar_wait(&s.v_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
-              if (!ok) break;
-            }
+            ok = mbar_wait(&s.v_empty[st], par, abort_flag, p.status, STATUS_TIMEOUT_EMPTY);
+            if (!ok) break;
             mbar_arrive_expect_tx(&s.v_full[st], 2 * KPANEL);
             for (int m = 0; m < 2; ++m) tma_load_4d(s.v[st][m], &tm_v, &s.v_full[st], 0, 2 * h + m, j * BN, b);
+            if (++st == P_STAGES) {
+              st = 0;
+              par ^= 1;
+            }
           }
         }
       }
-    } else if (warp == WARP_MMA) {
-      // ---------------------------------------------------- Q K^T issuer --
+    } else if (warp < P_WARP_TMA) {
+      // ------------------------------------------- MMA issuer of a map --
+      // scores of step n + 2 right behind P V of step n, whose P they overwrite
+      const int t = warp - P_WARP_MMA;
       if (elect_one()) {
         constexpr uint32_t idesc_qk = idesc_bf16(TM, BN, 0, 0);
-        const uint64_t q_desc = sdesc_kmajor(smem_u32(s.q[0])), k_desc = sdesc_kmajor(smem_u32(s.k[0][0]));
-        unsigned kv_it = 0;
-        Segment sg;
-        bool ok = true;
-        for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
-          ok = mbar_wait(&s.q_full, si & 1, abort_flag, p.status, STATUS_TIMEOUT_TMA);
-          for (int j = sg.j0; j < sg.j1 && ok; ++j, ++kv_it) {
-            const int st = (int)(kv_it % P_STAGES);
-            ok = mbar_wait(&s.k_full[st], (uint32_t)((kv_it / P_STAGES) & 1), abort_flag, p.status,
-                           STATUS_TIMEOUT_TMA);
-#pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              ok = ok && mbar_wait(&s.s_taken[t], (uint32_t)(kv_it & 1) ^ 1, abort_flag, p.status,
-                                   STATUS_TIMEOUT_SOFTMAX);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t qd = q_desc + (uint32_t)(t * (QPANEL >> 4));
-              const uint64_t kd = k_desc + (uint32_t)((2 * st + t) * (KPANEL >> 4));
-#pragma unroll
-              for (int ks = 0; ks < HD / 16; ++ks)
-                mma_ss(tmem + t * P_SLOT + P_COL_S, qd + ks * 2, kd + ks * 2, idesc_qk, ks != 0);
-              tc_commit(&s.s_full[t]);
-            }
-            if (!ok) break;
-            tc_commit(&s.k_empty[st]);
-            if (j + 1 == sg.j1) tc_commit(&s.q_empty);
-          }
-        }
-      }
-    } else if (warp == WARP_PV) {
-      // ------------------------------------------------------ P V issuer --
-      if (elect_one()) {
         constexpr uint32_t idesc_pv = idesc_bf16(TM, VD, 0, 1);
+        const uint64_t q_desc = sdesc_kmajor(smem_u32(s.q[0][t])), k_desc = sdesc_kmajor(smem_u32(s.k[0][t]));
         const uint64_t v_desc = sdesc_mnmajor(smem_u32(s.v[0][0]), KPANEL);
-        unsigned kv_it = 0;
+        const uint32_t tb = tmem + t * P_MAP;
+        int kst = 0, kg = 0, vst = 0, vg = 0;
+        uint32_t kpar = 0, vpar = 0, ppar = 0;
         Segment sg;
         bool ok = true;
         for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
-          for (int j = sg.j0; j < sg.j1 && ok; ++j, ++kv_it) {
-            const int st = (int)(kv_it % P_STAGES);
-            ok = mbar_wait(&s.v_full[st], (uint32_t)((kv_it / P_STAGES) & 1), abort_flag, p.status,
-                           STATUS_TIMEOUT_TMA);
-            const uint64_t vd = v_desc + (uint32_t)(st * (2 * KPANEL >> 4));
-            if (j == sg.j0 && si > 0)        // epilogue of the previous segment has drained both O
-              ok = ok && mbar_wait(&s.o_free, (uint32_t)((si - 1) & 1), abort_flag, p.status,
-                                   STATUS_TIMEOUT_SOFTMAX);
+          const int n_j = sg.j1 - sg.j0, qs = si & 1;
+          ok = mbar_wait(&s.q_full[qs], (uint32_t)((si >> 1) & 1), abort_flag, p.status, STATUS_TIMEOUT_TMA);
+          const uint64_t qd = q_desc + (uint32_t)(qs * (2 * QPANEL >> 4));
+          auto scores = [&](int jj) {
+            if (!mbar_wait(&s.k_full[kst], kpar, abort_flag, p.status, STATUS_TIMEOUT_TMA)) return false;
+            tc_fence_after();
+            const uint64_t kd = k_desc + (uint32_t)(kst * (2 * KPANEL >> 4));
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              ok = ok && mbar_wait(&s.p_full[t], (uint32_t)(kv_it & 1), abort_flag, p.status,
-                                   STATUS_TIMEOUT_SOFTMAX);
-              if (!ok) break;
-              tc_fence_after();
-              const uint32_t tb = tmem + t * P_SLOT;
-#pragma unroll
-              for (int ks = 0; ks < BN / 16; ++ks)
-                mma_ts(tb + P_COL_O, tb + P_COL_P + ks * 8, vd + 128 * ks, idesc_pv, !(j == sg.j0 && ks == 0));
-              tc_commit(&s.o_done[t]);
-              if (j + 1 == sg.j1) tc_commit(&s.o_final[t]);
+            for (int ks = 0; ks < HD / 16; ++ks)
+              mma_ss(tb + p_col_s(kg), qd + ks * 2, kd + ks * 2, idesc_qk, ks != 0);
+            tc_commit(&s.s_full[t][kg]);
+            tc_commit(&s.k_empty[kst]);
+            if (jj + 1 == n_j) tc_commit(&s.q_empty[qs]);
+            if (++kst == P_STAGES) {
+              kst = 0;
+              kpar ^= 1;
             }
-            if (ok) tc_commit(&s.v_empty[st]);
+            kg ^= 1;
+            return true;
+          };
+          ok = ok && scores(0) && (n_j == 1 || scores(1));
+          if (ok && si > 0)        // epilogue of the previous segment has drained both O
+            ok = mbar_wait(&s.o_free, (uint32_t)((si - 1) & 1), abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
+          for (int jj = 0; jj < n_j && ok; ++jj) {
+            ok = mbar_wait(&s.v_full[vst], vpar, abort_flag, p.status, STATUS_TIMEOUT_TMA) &&
+                 mbar_wait(&s.p_full[t][vg], ppar, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t vd = v_desc + (uint32_t)(vst * (2 * KPANEL >> 4));
+#pragma unroll
+            for (int ks = 0; ks < BN / 16; ++ks)
+              mma_ts(tb + P_COL_O, tb + p_col_s(vg) + ks * 8, vd + 128 * ks, idesc_pv, !(jj == 0 && ks == 0));
+            tc_commit(&s.o_done[t][vg]);
+            tc_commit(&s.v_empty[vst]);
+            if (jj + 1 == n_j) tc_commit(&s.o_final[t]);
+            if (++vst == P_STAGES) {
+              vst = 0;
+              vpar ^= 1;
+            }
+            vg ^= 1;
+            if (vg == 0) ppar ^= 1;
+            if (jj + 2 < n_j) ok = scores(jj + 2);
           }
         }
       }
     }
   } else {
     // --------------------------------------- softmax / correction / epilogue --
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REG_SOFT));
-    const int t = warp >> 2, wl = warp & 3;         // map; lane quadrant
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(P_REG_SOFT));
+    // Group g of map t takes the steps (K/V tiles) of parity g.  The row's reference maximum goes from one
+    // group of a map to the other before the exponentials, as in the tangent kernel below.
+    const int t = warp >> 3, g = (warp >> 2) & 1, wl = warp & 3;
     const int row = wl * 32 + lane;
-    const uint32_t tq = tmem_addr(tmem, wl * 32, 0), tb = tq + t * P_SLOT;
+    const uint32_t tq = tmem_addr(tmem, wl * 32, 0), tb = tq + t * P_MAP, sc = tb + p_col_s(g);
     const float scale_log2 = p.scale * LOG2E;
-    unsigned it = 0;
-    uint32_t xn = 0;                                // exchanges done so far (phase of xbar)
+    uint32_t par = 0;                               // phase of this group's buffer
+    int n0 = 0;                                     // number of the segment's first step
     Segment sg;
     bool ok = true;
     for (int si = 0; ok && get_segment(p.sh, cta, G, si, sg); ++si) {
-      int q0, h, b;
-      item_coords(p, sg.item, q0, h, b);
-      const int q_row = q0 + row;
       float m_used = -INFINITY, l_sum = 0.f, l_sum2 = 0.f;
-      for (int j = sg.j0; j < sg.j1 && ok; ++j, ++it) {
-        ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[t], (uint32_t)(it & 1), abort_flag, p.status,
-                                               STATUS_TIMEOUT_MMA));
+      const int j_own = sg.j0 + ((n0 ^ g) & 1);     // this group's first step of the segment
+      for (int j = j_own; j < sg.j1 && ok; j += 2) {
+        const int n = n0 + j - sg.j0;
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[t][g], par, abort_flag, p.status, STATUS_TIMEOUT_MMA));
         if (!ok) break;
         tc_fence_after();
-        uint32_t sv[BN];
-#pragma unroll
-        for (int c = 0; c < BN; c += 32) tmem_ld32(tb + P_COL_S + c, sv + c);
-        // P of the step before has been read, probed here
-        const bool p_ok = it == 0 || mbar_test(&s.o_done[t], (uint32_t)((it - 1) & 1));
-        tc_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.s_taken[t]);
         const int kv_rem = p.L - j * BN;
-        if (kv_rem < BN) {
-#pragma unroll
-          for (int i = 0; i < BN; ++i)
-            if (i >= kv_rem) sv[i] = 0xff800000u;  // -inf
+        if (kv_rem < BN) {                          // scores of keys past the end: -inf
+          int c = kv_rem;
+          for (; c & 7; ++c) tmem_st1(sc + c, 0xff800000u);
+#pragma unroll 1
+          for (; c < BN; c += 8) tmem_fill8(sc + c, 0xff800000u);
+          tc_wait_st();
         }
-        const bool first = j == sg.j0;
-        float alpha = 1.f;
-        // Maximum first, so that P can be stored as it is made.  The reference moves only when a row
-        // has outgrown it by more than 2^8.
+        uint32_t sv[BN];
+        tmem_ld32(sc, sv);
+        tmem_ld32(sc + 32, sv + 32);
+        tc_wait_ld();
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
         for (int i = 0; i < BN; i += 2)
           asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[(i / 2) & 3]) : "f"(__uint_as_float(sv[i])), "f"(__uint_as_float(sv[i + 1])));
         mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-        const bool need = first || (mx[0] - m_used) * scale_log2 > 8.0f;
-        if (__any_sync(0xffffffffu, need)) {
-          if (need) {
-            if (!first) alpha = ex2((m_used - mx[0]) * scale_log2);
-            m_used = mx[0];
-          }
-          if (!first) {
-            // O, once P V of the step before has run, to the reference that the rows have now
-            ok = __all_sync(0xffffffffu, mbar_wait(&s.o_done[t], (uint32_t)((it - 1) & 1), abort_flag,
-                                                   p.status, STATUS_TIMEOUT_MMA));
+        // The reference moves only when a row has outgrown it by more than 2^8 (or has none yet).
+        float m_prev;
+        ok = ref_of_step(&s.m_ref[t][row], n - 1, m_prev, abort_flag, p.status);
+        if (!ok) break;
+        if (j == sg.j0) m_prev = mx[0];
+        const bool need = (mx[0] - m_prev) * scale_log2 > 8.0f;
+        const float m_new = need ? mx[0] : m_prev;
+        publish_ref(&s.m_ref[t][row], m_new, n);
+        if (__any_sync(0xffffffffu, m_new != m_used)) {
+          if (__any_sync(0xffffffffu, need)) {      // O, as of the step before, to the new reference
+            ok = __all_sync(0xffffffffu, mbar_wait(&s.o_done[t][g ^ 1], g == 0 ? par ^ 1 : par, abort_flag, p.status,
+                                                   STATUS_TIMEOUT_MMA));
             if (!ok) break;
             tc_fence_after();
+            const float alpha = ex2((m_prev - m_new) * scale_log2);
 #pragma unroll 1
-            for (int c = 0; c < VD; c += 32) {
-              uint32_t ov[32];
-              tmem_ld32(tb + P_COL_O + c, ov);
+            for (int c = 0; c < VD; c += 8) {
+              uint32_t ov[8];
+              tmem_ld8(tb + P_COL_O + c, ov);
               tc_wait_ld();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
-              tmem_st32(tb + P_COL_O + c, ov);
+              for (int i = 0; i < 8; ++i) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * alpha);
+              tmem_st8(tb + P_COL_O + c, ov);
             }
-            tc_wait_st();
           }
-        }
-        if (!__all_sync(0xffffffffu, p_ok)) {      // P of the step before is still being read
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.o_done[t], (uint32_t)((it - 1) & 1), abort_flag,
-                                                 p.status, STATUS_TIMEOUT_MMA));
-          if (!ok) break;
-        }
-        tc_fence_after();
-        if (t == 1 || it > 0) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.turn[t][wl], (uint32_t)((it - (t ^ 1)) & 1), abort_flag,
-                                                 p.status, STATUS_TIMEOUT_SOFTMAX));
-          if (!ok) break;
+          if (j != j_own) {                         // the sums so far to the new reference
+            const float alpha = ex2((m_used - m_new) * scale_log2);
+            l_sum *= alpha;
+            l_sum2 *= alpha;
+          }
+          m_used = m_new;
         }
         const f32x2 neg_m2 = dup2(-m_used * scale_log2);
         f32x2 l_new = dup2(0.f);
@@ -367,85 +359,91 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
             const f32x2 e = fma2(pair2(sv[c + i], sv[c + i + 1]), dup2(scale_log2), neg_m2);
-            const float p0 = ex2(lo2(e)), p1 = ex2(hi2(e));
-            pk[i / 2] = pack_bf16(p0, p1);
-            l_new = add2(l_new, pair2(__float_as_uint(p0), __float_as_uint(p1)));
+            const f32x2 pp = ex2_mufu2(e);
+            pk[i / 2] = pack_bf16(lo2(pp), hi2(pp));
+            l_new = add2(l_new, pp);
           }
-          if (c + 32 == BN) {
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&s.turn[t ^ 1][wl]);
-          }
-          tmem_st16(tb + P_COL_P + c / 2, pk);
+          tmem_st16(sc + c / 2, pk);
         }
-        l_sum = fmaf(l_sum, alpha, lo2(l_new));
-        l_sum2 = fmaf(l_sum2, alpha, hi2(l_new));
+        l_sum += lo2(l_new);
+        l_sum2 += hi2(l_new);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&s.p_full[t]);
+        if (lane == 0) mbar_arrive(&s.p_full[t][g]);
+        par ^= 1;
       }
       // ---- epilogue of this segment ----
-      const float l_tot = l_sum + l_sum2;
+      auto& xst = s.xst[si & 1];
+      xst[t][g][0][row] = l_sum + l_sum2;
+      xst[t][g][1][row] = m_used;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s.sums);
+      if (ok)
+        ok = mbar_wait(&s.sums, (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX) &&
+             mbar_wait(&s.o_final[0], (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA) &&
+             mbar_wait(&s.o_final[1], (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      tc_fence_after();
+      // the group of the last step has the final reference
+      const int n_j = sg.j1 - sg.j0, gl = (n0 + n_j - 1) & 1;
+      n0 += n_j;
+      float m_fin[2], l_tot[2];
+#pragma unroll
+      for (int m = 0; m < 2; ++m) {
+        m_fin[m] = xst[m][gl][1][row];
+        l_tot[m] = xst[m][gl][0][row];
+        if (n_j > 1) l_tot[m] += ex2((xst[m][gl ^ 1][1][row] - m_fin[m]) * scale_log2) * xst[m][gl ^ 1][0][row];
+      }
+      int q0, h, b;
+      item_coords(p, sg.item, q0, h, b);
+      const int q_row = q0 + row;
       const bool live = q_row < p.L;
+      const float m_score = (t ? m_fin[1] : m_fin[0]) * p.scale, l_own = t ? l_tot[1] : l_tot[0];
       if (sg.rec < 0) {
-        // Both maps have finished; this warp takes the rows of its quadrant and the channels of head
-        // 2h + t, from both O.
-        const float lam = p.lam.at(h);
-        s.inv_l[t][row] = 1.f / l_tot;
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.xbar);
-        if (ok)
-          ok = mbar_wait(&s.o_final[0], (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA) &&
-               mbar_wait(&s.o_final[1], (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA) &&
-               mbar_wait(&s.xbar, xn & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX);
-        ++xn;
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
-        const float w1 = s.inv_l[0][row], inv_l2 = s.inv_l[1][row], w2 = lam * inv_l2;
-        const int64_t off = (int64_t)b * p.o_sb + (int64_t)q_row * p.o_sl + (int64_t)(2 * h + t) * p.o_sh;
+        // this thread takes 32 channels of the pair, of both O: half g of head 2h + t
+        const float w1 = 1.f / l_tot[0], inv_l2 = 1.f / l_tot[1], w2 = p.lam.at(h) * inv_l2;
+        const int64_t off = (int64_t)b * p.o_sb + (int64_t)q_row * p.o_sl + (int64_t)(2 * h + t) * p.o_sh + g * 32;
 #pragma unroll 1
-        for (int c = 0; c < VD / 2; c += 32) {
-          uint32_t a[32], e[32];
-          tmem_ld32(tq + P_COL_O + t * (VD / 2) + c, a);
-          tmem_ld32(tq + P_SLOT + P_COL_O + t * (VD / 2) + c, e);
+        for (int c = 0; c < 32; c += 8) {
+          uint32_t a[8], e[8];
+          tmem_ld8(tq + P_COL_O + t * HD + g * 32 + c, a);
+          tmem_ld8(tq + P_MAP + P_COL_O + t * HD + g * 32 + c, e);
           tc_wait_ld();
           if (live) {
+            float r[8];
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              float r[8];
+            for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(a[u]) * w1 - __uint_as_float(e[u]) * w2;
+            store_out8(p, 0, off + c, r);
+            if (p.o2) {
 #pragma unroll
-              for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(a[i + u]) * w1 - __uint_as_float(e[i + u]) * w2;
-              store_out8(p, 0, off + c + i, r);
-              if (!p.o2) continue;
-#pragma unroll
-              for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(e[i + u]) * inv_l2;
-              store_out8(p, 1, off + c + i, r);
+              for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(e[u]) * inv_l2;
+              store_out8(p, 1, off + c, r);
             }
           }
         }
-        if (live && p.lse)
-          p.lse[((int64_t)b * 2 * p.H + 2 * h + t) * p.L + q_row] = m_used * p.scale + __logf(l_tot);
+        if (live && p.lse && g == 0)
+          p.lse[((int64_t)b * 2 * p.H + 2 * h + t) * p.L + q_row] = m_score + __logf(l_own);
       } else {
-        if (ok) ok = mbar_wait(&s.o_final[t], (uint32_t)(si & 1), abort_flag, p.status, STATUS_TIMEOUT_MMA);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        tc_fence_after();
         // partial result of a split item: raw accumulators, [column][row] so that a warp stores 128
-        // consecutive bytes, + (m, l, mu)
+        // consecutive bytes, + (m, l, mu); a group stores half the columns of its map
         float* part = p.scratch + (size_t)sg.rec * Rec<false>::ALL + t * Rec<false>::MAP;
-        for (int c = 0; c < VD; c += 32) {
-          uint32_t ov[32];
-          tmem_ld32(tb + P_COL_O + c, ov);
+#pragma unroll 1
+        for (int c = g * HD; c < (g + 1) * HD; c += 16) {
+          uint32_t ov[16];
+          tmem_ld16(tb + P_COL_O + c, ov);
           tc_wait_ld();
           float* acc = part + (size_t)c * TM + row;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) acc[i * TM] = __uint_as_float(ov[i]);
+          for (int i = 0; i < 16; ++i) acc[i * TM] = __uint_as_float(ov[i]);
         }
-        float* stats = part + Rec<false>::STATS;
-        stats[row] = m_used * p.scale;
-        stats[TM + row] = l_tot;
-        stats[2 * TM + row] = 0.f;
+        if (g == 0) {
+          float* stats = part + Rec<false>::STATS;
+          stats[row] = m_score;
+          stats[TM + row] = l_own;
+          stats[2 * TM + row] = 0.f;
+        }
       }
       tc_fence_before();
       __syncwarp();
@@ -454,7 +452,7 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     tc_fence_before();
   }
   __syncthreads();
-  if (warp == WARP_MMA) {
+  if (warp == P_WARP_MMA) {
     __syncwarp();
     tc_fence_after();
     tmem_dealloc(tmem, 512);
@@ -1067,7 +1065,7 @@ extern "C" int imf_attn_diff_fwd(const void* q, const void* k, const void* v, co
   } else {
     const size_t smem = sizeof(PSmem) + 1024;
     if (!allow_smem((const void*)attn_diff_fwd_kernel, smem, smem_set[0])) return IMF_ERR_LAUNCH;
-    attn_diff_fwd_kernel<<<G, THREADS, smem, st>>>(mq, mk, mv, prm);
+    attn_diff_fwd_kernel<<<G, P_THREADS, smem, st>>>(mq, mk, mv, prm);
   }
   if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
   if (split) {
