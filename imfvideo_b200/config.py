@@ -32,7 +32,7 @@ class ModelConfig:
     patch_size: tuple = (1, 2, 2)
     in_channels: int = 16
     num_classes: int = 1000
-    # "flash_jvp" | "sla2_jvp" | "sla2_cube_qat" | "sdpa_flash" | "sdpa"
+    # "flash_jvp" | "sla2_jvp" | "sla2_cube_qat" | "diff_jvp" | "sdpa_flash" | "sdpa"
     attn_impl: str = "flash_jvp"
     mla_use_output_gate: bool = True
     # SLA2 sparse-linear attention
@@ -41,6 +41,12 @@ class ModelConfig:
     sla2_bk: int = 64
     sla2_alpha_init: float = 0.9
     sla2_tile: tuple = (4, 4, 4)
+    # not in the reference: differential attention ("diff_jvp"), the pairs' weights to begin with
+    diff_lam_init: float = 0.5
+    # not in the reference: norm what a branch returns before its gate, and scale the residual it is added to by
+    # a learned vector
+    post_norm: bool = False
+    residual_scale: bool = False
     mlp_ratio: float = 8 / 3
     situ_beta: float = 4.0
     situ_linear_beta: Optional[float] = 25.0

@@ -286,8 +286,10 @@ class TransformerBlock(nn.Module):
                  qk_nope_head_dim, qk_rope_head_dim, v_head_dim, mlp_ratio=8 / 3,
                  weight_init_constant=1.0, norm_eps=1e-6, attn_impl=sdpa_math_attention,
                  use_attn_res=False, situ_beta=4.0, situ_linear_beta=25.0,
-                 mla_use_output_gate=True, act_store="bf16"):
+                 mla_use_output_gate=True, act_store="bf16", post_norm=False, residual_scale=False):
         super().__init__()
+        if residual_scale and not post_norm:
+            raise ValueError("residual_scale belongs to post_norm: without it the residual is not scaled")
         if act_store not in ("bf16", "int8"):
             raise ValueError(f"act_store is 'bf16' or 'int8', not {act_store!r}")
         self.act_store = act_store        # how the fused path keeps activations for the backward pass
@@ -301,6 +303,11 @@ class TransformerBlock(nn.Module):
                              weight_init_constant, situ_beta, situ_linear_beta)
         self.attn_scale = nn.Parameter(torch.zeros(hidden_size))
         self.mlp_scale = nn.Parameter(torch.zeros(hidden_size))
+        # norms of what a branch returns, before its gate, and learned scales of the residual it is added to
+        self.attn_post_norm = RMSNorm(hidden_size, eps=norm_eps) if post_norm else None
+        self.mlp_post_norm = RMSNorm(hidden_size, eps=norm_eps) if post_norm else None
+        self.attn_keep = nn.Parameter(torch.ones(hidden_size)) if residual_scale else None
+        self.mlp_keep = nn.Parameter(torch.ones(hidden_size)) if residual_scale else None
         if use_attn_res:
             self.attn_res_norm = RMSNorm(hidden_size, eps=norm_eps)
             self.mlp_res_norm = RMSNorm(hidden_size, eps=norm_eps)
@@ -394,7 +401,23 @@ class TransformerBlock(nn.Module):
             w1 = w2 = None
         return (w1, w2, self.norm1.weight, self.norm2.weight, a.q_a_layernorm.weight,
                 a.kv_a_layernorm.weight, a.q_norm.weight, a.k_norm.weight, self.attn_scale,
-                self.mlp_scale) + mats
+                self.mlp_scale) + tuple(self.post_params().values()) + mats
+
+    def post_params(self):
+        """The learned vectors around the branches by their role in ``ops.block`` (None: not there)."""
+        w = lambda m: None if m is None else m.weight
+        return {"post_a": w(self.attn_post_norm), "keep_a": self.attn_keep, "post_m": w(self.mlp_post_norm),
+                "keep_m": self.mlp_keep}
+
+    def post_add(self, res: Optional[Dual], y: Dual, branch: str, pre: Optional[Tensor] = None):
+        """res + gate * y, y normed first in a block with post norms; ("attn" or "mlp").  With ``pre`` also
+        the norm with that gain, in y's type: (x, n), else x."""
+        gate, norm, keep = (getattr(self, branch + s) for s in ("_scale", "_post_norm", "_keep"))
+        if norm is None:
+            assert pre is None
+            return D.scale_add(res, y, gate)
+        x, n = D.norm_add_norm(res, y, norm.weight, gate, norm.eps, res_scale=None if res is None else keep, pre=pre)
+        return x if pre is None else (x, n)
 
     def fused_sinks(self):
         """Which parameter each row band of the six fused bf16 matrices comes from (same
@@ -422,7 +445,8 @@ class TransformerBlock(nn.Module):
                 small={"g_n1": self.norm1.weight, "g_n2": self.norm2.weight,
                        "g_qa": a.q_a_layernorm.weight, "g_kva": a.kv_a_layernorm.weight,
                        "g_qn": a.q_norm.weight, "g_kn": a.k_norm.weight,
-                       "a_scale": self.attn_scale, "m_scale": self.mlp_scale})
+                       "a_scale": self.attn_scale, "m_scale": self.mlp_scale,
+                       **{k: v for k, v in self.post_params().items() if v is not None}})
         return sk
 
     def fused_forward(self, prefix: Dual, snaps, fresh: bool, use_res: bool, rope_cos, rope_sin,
@@ -447,9 +471,12 @@ class TransformerBlock(nn.Module):
             out = self.fused_forward(x, [], False, False, rope_cos, rope_sin, self.norm1.eps)
             return out.p if plain else out
         a = self.attn(self.norm1(x, compute_dtype), rope_cos, rope_sin)
-        x = D.scale_add(x, a, self.attn_scale)
-        m = self.mlp(self.norm2(x, compute_dtype))
-        x = D.scale_add(x, m, self.mlp_scale)
+        if self.attn_post_norm is not None:
+            x, h = self.post_add(x, a, "attn", pre=self.norm2.weight)
+        else:
+            x = self.post_add(x, a, "attn")
+            h = self.norm2(x, compute_dtype)
+        x = self.post_add(x, self.mlp(h), "mlp")
         return x.p if plain else x
 
 
@@ -550,7 +577,7 @@ class IMFDiTVideo(nn.Module):
                  attn_impl=sdpa_math_attention, eval_mode=False, attn_res_block_size=0,
                  situ_beta=4.0, situ_linear_beta=25.0, mla_use_output_gate=True,
                  grad_checkpoint=False, compute_dtype: Optional[torch.dtype] = None,
-                 act_store="bf16"):
+                 act_store="bf16", post_norm=False, residual_scale=False):
         super().__init__()
         self.head_dim = hidden_size // num_heads
         self.attn_res_block_size = attn_res_block_size
@@ -628,7 +655,7 @@ class IMFDiTVideo(nn.Module):
                   norm_eps=rmsnorm_eps, attn_impl=attn_impl,
                   use_attn_res=attn_res_block_size > 0, situ_beta=situ_beta,
                   situ_linear_beta=situ_linear_beta, mla_use_output_gate=mla_use_output_gate,
-                  act_store=act_store)
+                  act_store=act_store, post_norm=post_norm, residual_scale=residual_scale)
         shared_depth = depth - aux_head_depth
         self.shared_blocks = nn.ModuleList(TransformerBlock(**kw) for _ in range(shared_depth))
         self.u_heads = nn.ModuleList(TransformerBlock(**kw) for _ in range(aux_head_depth))
@@ -697,13 +724,13 @@ class IMFDiTVideo(nn.Module):
               if snaps else prefix)
         a = blk.attn(blk.norm1(h1, cd), self.rope_cos, self.rope_sin)
         if fresh:
-            snaps2, p2 = snaps + [prefix], D.scale_add(None, a, blk.attn_scale)
+            snaps2, p2 = snaps + [prefix], blk.post_add(None, a, "attn")
             p2 = Dual(p2.p.to(prefix.p.dtype), None if p2.t is None else p2.t.to(prefix.p.dtype))
         else:
-            snaps2, p2 = snaps, D.scale_add(prefix, a, blk.attn_scale)
+            snaps2, p2 = snaps, blk.post_add(prefix, a, "attn")
         h2 = D.attn_res(p2, snaps2, blk.mlp_res_norm.weight, blk.mlp_res_proj.weight, eps)
         m = blk.mlp(blk.norm2(h2, cd))
-        return D.scale_add(p2, m, blk.mlp_scale)
+        return blk.post_add(p2, m, "mlp")
 
     def _run_attn_res_blocks(self, prefix: Dual, snaps: List[Dual], blocks, start_idx: int):
         """Attention-residual schedule with a global block index: every

@@ -16,6 +16,9 @@ Block structure (reference ``models/imf_dit_video.py:909-972``, ``:422-467``):
     n2  = norm2(remix(p2, snaps2; w2))
     m   = situ(n2 [w1 | w3]^T) w2^T ;  out = p2 + m * mlp_scale
 
+With post norms (no counterpart in the reference; ``ops/postnorm.py``) the two residual updates are
+    p2  = keep_a * prefix + norm(a; post_a) * attn_scale ;  out = keep_m * p2 + norm(m; post_m) * mlp_scale
+
 With ``BlockGeom.act8`` the node keeps its activations in 8 bits (``ops/act8.py``): one launch at
 the end of the forward packs them, the backward reads n1, n2 and the latents in 8 bits as they
 are (weight gradients), [gate | up] as well (gated activation, which is recomputed there), q and k
@@ -31,6 +34,7 @@ import torch
 
 from . import act8 as A8
 from . import kernels as K
+from . import postnorm as PN
 from . import rowops as R
 
 _lib, c_int = K._lib, ctypes.c_int
@@ -38,8 +42,7 @@ if K._has("imf_block_pre"):
     _lib.imf_block_pre.restype = c_int
     _lib.imf_block_pre.argtypes = [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p]
     _lib.imf_block_post.restype = c_int
-    _lib.imf_block_post.argtypes = [ctypes.c_void_p, ctypes.c_void_p] + [ctypes.c_float] * 3 + \
-        [ctypes.c_void_p]
+    _lib.imf_block_post.argtypes = [ctypes.c_void_p] * 3 + [ctypes.c_float] * 3 + [ctypes.c_void_p]
 
 BF16, F32 = torch.bfloat16, torch.float32
 
@@ -78,6 +81,7 @@ class GradSinks:
 
     ORDER = ("W_a", "W_qb", "W_kvb", "W_out", "W13", "W2")
     SMALL = ("g_n1", "g_n2", "g_qa", "g_kva", "g_qn", "g_kn", "a_scale", "m_scale")
+    POST = ("post_a", "keep_a", "post_m", "keep_m")       # of blocks with post norms
 
     def __init__(self, pieces, small=None):
         self.pieces = pieces
@@ -93,7 +97,7 @@ class GradSinks:
         return p.grad.view(-1)
 
     def direct(self) -> bool:
-        if any(self.small_dst(nm) is None for nm in self.SMALL):
+        if any(self.small_dst(nm) is None for nm in self.SMALL + tuple(n for n in self.POST if n in self.small)):
             return False
         for name in self.ORDER:
             for p, r0, _n, _c in self.pieces[name]:
@@ -139,6 +143,7 @@ class _BlockFn(torch.autograd.Function):
     """inputs: geom, core, flags, eps, beta, lbeta, cos, sin, nsnap,
     prefix, dprefix, *snaps, *dsnaps,
     w1, w2, g_norm1, g_norm2, g_qa, g_kva, g_qn, g_kn, attn_scale, mlp_scale,
+    post_a, keep_a, post_m, keep_m (None without post norms / residual scales),
     W_a, W_qb, W_kvb, W_out, W13, W2
     outputs: new_prefix (fp32), new_dprefix (fp32 or empty)."""
 
@@ -149,7 +154,7 @@ class _BlockFn(torch.autograd.Function):
         core, sinks, grad_on = core
         snaps = list(rest[:nsnap])
         dsnaps = list(rest[nsnap:2 * nsnap])
-        (w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn, a_scale, m_scale,
+        (w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn, a_scale, m_scale, post_a, keep_a, post_m, keep_m,
          W_a, W_qb, W_kvb, W_out, W13, W2) = rest[2 * nsnap:]
         has_t = dprefix is not None
         need_bwd = any(ctx.needs_input_grad)
@@ -211,9 +216,10 @@ class _BlockFn(torch.autograd.Function):
                 ptr(w2) if use_res else 0, ptr(g_n2), ptr(W13), ptr(gu), ptr(act), ptr(W2), ptr(m),
                 ptr(m_scale), ptr(out), status]
         ptrs += [ptr(s) for s in sn2] + [ptr(s) for s in dsn2]
-        K._check(_lib.imf_block_post(R._ptr_array(ptrs), dims(len(sn2)), float(eps), float(beta),
+        post = None if post_a is None else R._ptr_array([ptr(post_a), 0 if fresh else ptr(keep_a), ptr(post_m), ptr(keep_m)])
+        K._check(_lib.imf_block_post(R._ptr_array(ptrs), dims(len(sn2)), post, float(eps), float(beta),
                                      float(lbeta or 0.0), stream), "imf_block_post")
-        K.LAUNCHES.count += 7 if g.gate else 6
+        K.LAUNCHES.count += (7 if g.gate else 6) + (post is not None and use_res)
         if need_bwd:
             if g.act8 and not grad_on:        # under no_grad: nothing to keep (parameters still ask for gradients)
                 kept = ()
@@ -229,9 +235,11 @@ class _BlockFn(torch.autograd.Function):
             else:
                 kept = (n1[0], a_[:rows], qlat[0], kvlat[0], qb[:rows], kvb[:rows], q[0], k[0], o, og[0],
                         a_out[:rows], n2[0], gu[:rows], act[:rows], m[:rows])
+            # the residual between the branches: without post norms it is made again where it is needed
+            p2 = p2[0] if post_a is not None and kept else None
             ctx.save_for_backward(prefix, *snaps, w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn,
-                                  a_scale, m_scale, W_a, W_qb, W_kvb, W_out, W13, W2, cos, sin,
-                                  *core_saved, *kept)
+                                  a_scale, m_scale, post_a, keep_a, post_m, keep_m, p2, W_a, W_qb, W_kvb, W_out, W13, W2,
+                                  cos, sin, *core_saved, *kept)
             ctx.meta = (g, core, fresh, use_res, eps, beta, lbeta, nsnap, B, L, len(core_saved))
             ctx.sinks = sinks
             ctx.mats_cached = bool(getattr(sinks, "mats_cached", False))
@@ -246,9 +254,9 @@ class _BlockFn(torch.autograd.Function):
         sv = ctx.saved_tensors
         prefix = sv[0]
         snaps = list(sv[1:1 + nsnap])
-        (w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn, a_scale, m_scale, W_a, W_qb, W_kvb, W_out,
-         W13, W2, cos, sin) = sv[1 + nsnap:1 + nsnap + 18]
-        core_saved, kept = sv[1 + nsnap + 18:1 + nsnap + 18 + ncore], sv[1 + nsnap + 18 + ncore:]
+        (w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn, a_scale, m_scale, post_a, keep_a, post_m, keep_m, p2,
+         W_a, W_qb, W_kvb, W_out, W13, W2, cos, sin) = sv[1 + nsnap:1 + nsnap + 23]
+        core_saved, kept = sv[1 + nsnap + 23:1 + nsnap + 23 + ncore], sv[1 + nsnap + 23 + ncore:]
         rows, d = B * L, g.d
         if g.act8:
             n1, a_, qlat, kvlat, qb, kvb, a_out, n2, gu, m, *qko = A8.in_buffer(kept[0], ctx.packed)
@@ -286,9 +294,16 @@ class _BlockFn(torch.autograd.Function):
         small = (lambda name, part, col, D: (cs.add(part, col, D, sinks.small_dst(name)), None)[1]) \
             if direct else (lambda name, part, col, D: cs.add(part, col, D, None))
 
-        # 11'. out = p2 + m * mlp_scale
-        g_m, part_ms = R.scale_add_bwd(m, m_scale, g_out, rows, d, raw=True)
-        g_mscale = small("m_scale", part_ms, 0, d)
+        # 11'. out = p2 + m * mlp_scale; g_p2: what reaches p2 this way
+        g_posta = g_keepa = g_postm = g_keepm = None
+        if post_m is not None:
+            g_p2, g_m, part_ms = PN.norm_add_norm_bwd(p2, m, post_m, m_scale, eps, keep_m, None, g_out, None, raw=True)
+            g_mscale, g_postm = small("m_scale", part_ms, 2, d), small("post_m", part_ms, 3, d)
+            g_keepm = None if keep_m is None else small("keep_m", part_ms, 1, d)
+        else:
+            g_p2 = g_out
+            g_m, part_ms = R.scale_add_bwd(m, m_scale, g_out, rows, d, raw=True)
+            g_mscale = small("m_scale", part_ms, 0, d)
         # 10'. MLP
         g_act = K.gemm(g_m, W2, b_mn=True)                          # [rows, fp]
         if g.act8:
@@ -301,12 +316,25 @@ class _BlockFn(torch.autograd.Function):
         gW13 = wgrad("W13", g_gu, n2)
         # 9'. residual + remix + norm2
         sn2 = sn + [pfx] if fresh else sn
-        g_res2, g_aout, g_sn2, part2 = R.resnorm_bwd(
-            None if fresh else pfx, a_out, a_scale, sn2, w2 if use_res else None, g_n2, eps,
-            g_n2v, g_out, want_g_res=not fresh, raw=True)
-        gg_n2 = small("g_n2", part2, 0, d)
-        g_w2 = cs.add(part2, 1, d, None) if use_res else None       # product of two parameters
-        g_ascale = small("a_scale", part2, 2, d)
+        if post_a is not None:
+            g_sn2, pre, keep = [], g_n2, None if fresh else keep_a
+            if use_res:          # remix and norm2 first, from p2
+                g_p2, _, g_sn2, part2 = R.resnorm_bwd(p2, None, None, sn2, w2, g_n2, eps, g_n2v, g_p2, raw=True)
+                gg_n2, pre, g_n2v = small("g_n2", part2, 0, d), None, None
+            g_w2 = cs.add(part2, 1, d, None) if use_res else None
+            g_res2, g_aout, part_as = PN.norm_add_norm_bwd(None if fresh else pfx, a_out, post_a, a_scale, eps, keep, pre,
+                                                           g_p2, g_n2v, want_g_res=not fresh, raw=True)
+            if pre is not None:
+                gg_n2 = small("g_n2", part_as, 0, d)
+            g_keepa = None if keep is None else small("keep_a", part_as, 1, d)
+            g_ascale, g_posta = small("a_scale", part_as, 2, d), small("post_a", part_as, 3, d)
+        else:
+            g_res2, g_aout, g_sn2, part2 = R.resnorm_bwd(
+                None if fresh else pfx, a_out, a_scale, sn2, w2 if use_res else None, g_n2, eps,
+                g_n2v, g_p2, want_g_res=not fresh, raw=True)
+            gg_n2 = small("g_n2", part2, 0, d)
+            g_w2 = cs.add(part2, 1, d, None) if use_res else None       # product of two parameters
+            g_ascale = small("a_scale", part2, 2, d)
         # 8'. output projection
         g_og = K.gemm(g_aout, W_out, b_mn=True)                     # [rows, hv]
         o2 = o.view(rows, hv)
@@ -374,7 +402,7 @@ class _BlockFn(torch.autograd.Function):
             g_w2 = torch.zeros_like(w2) if w2 is not None else None
         grads = (None,) * 10 + (g_pfx.view(B, L, d), None) + tuple(g_snaps) + (None,) * nsnap + (
             g_w1, g_w2, gg_n1, gg_n2, gg_qa, gg_kva, gg_qn, gg_kn, g_ascale, g_mscale,
-            gW_a, gW_qb, gW_kvb, gW_out, gW13, gW2)
+            g_posta, g_keepa, g_postm, g_keepm, gW_a, gW_qb, gW_kvb, gW_out, gW13, gW2)
         return grads
 
 
@@ -382,7 +410,7 @@ def run_block(geom: BlockGeom, core, fresh: bool, use_res: bool, eps: float, bet
               lbeta: Optional[float], cos, sin, prefix, dprefix, snaps, dsnaps, params,
               sinks: Optional[GradSinks] = None):
     """params: (w1, w2, g_norm1, g_norm2, g_qa, g_kva, g_qn, g_kn, attn_scale, mlp_scale,
-    W_a, W_qb, W_kvb, W_out, W13, W2) with bf16 weight matrices; ``sinks`` says which
+    post_a, keep_a, post_m, keep_m, W_a, W_qb, W_kvb, W_out, W13, W2) with bf16 weight matrices; ``sinks`` says which
     parameters those matrices were built from (see ``GradSinks``)."""
     nsnap = len(snaps)
     core = (core, sinks, torch.is_grad_enabled())

@@ -18,6 +18,7 @@ int imf_qkprep(void** p, int rows, int L, int H, int dn, int dr, int dv, int ld_
                float eps, int has_t, int bwd, void* stream);
 int imf_elementwise(int op, void** p, const int* dims, float beta, float lbeta, int has_lbeta,
                     int has_t, int bwd, void* stream);
+int imf_norm_add_norm(void** p, int rows, int D, float eps, int y_fp32, int mode, int* status, void* stream);
 int imf_gemm_bf16(const void* A, const void* B, void* C, const float* bias, int M, int N, int K,
                   int64_t lda, int64_t ldb, int64_t ldc, int a_mn, int b_mn, int out_fp32,
                   int bias_rows, float alpha, int accumulate_out, int* status, void* stream);
@@ -98,8 +99,9 @@ extern "C" int imf_block_pre(void** p, const int* dims, float eps, void* stream)
 // instead of computed when the block has no output gate), 4 W_out, 5 a_out, 6 attn_scale, 7 prefix
 // and 8 dprefix (null when the residual restarts here), 9 p2, 10 n2, 11 remix weight, 12 norm2 gain,
 // 13 W13, 14 gu, 15 act, 16 W2, 17 m, 18 mlp_scale, 19 out, 20 status word, 21.. snaps, then their
-// tangents.
-extern "C" int imf_block_post(void** p, const int* dims, float eps, float beta, float lbeta,
+// tangents.  post: null, or gains of the norms of a and m and scales of the residuals they are added to (0 post_a,
+// 1 keep_a or null, 2 post_m, 3 keep_m or null): p2 = keep_a prefix + norm(a) attn_scale, out likewise.
+extern "C" int imf_block_post(void** p, const int* dims, void** post, float eps, float beta, float lbeta,
                               void* stream) {
   using namespace imf;
   const BlockDims& g = *reinterpret_cast<const BlockDims*>(dims);
@@ -115,8 +117,20 @@ extern "C" int imf_block_post(void** p, const int* dims, float eps, float beta, 
   }
   IMF_STEP(linear(p[3], p[4], p[5], m, d, hv, g.ld_wout, p[20], stream));
   void* dp2 = t ? at(p[9], r * d * 4) : nullptr;
-  IMF_STEP(resnorm(p[7], p[8], p[5], t ? at(p[5], r * d * 2) : nullptr, p[6], p[11], p[12], p[9], dp2,
-                   p[10], t ? at(p[10], r * d * 2) : nullptr, p + 21, g.nsnap, t, rows, d, eps, stream));
+  void *da = t ? at(p[5], r * d * 2) : nullptr, *dn2 = t ? at(p[10], r * d * 2) : nullptr;
+  if (post) {
+    // without a remix in between, norm2 is part of the same launch
+    const bool pre = p[11] == nullptr && g.nsnap == 0;
+    void* q[18] = {p[7], p[8], p[5], da, post[0], p[6], post[1], pre ? p[12] : nullptr, p[9], dp2,
+                   pre ? p[10] : nullptr, pre ? dn2 : nullptr};
+    IMF_STEP(imf_norm_add_norm(q, rows, d, eps, 0, t, static_cast<int*>(p[20]), stream));
+    if (!pre)
+      IMF_STEP(resnorm(p[9], dp2, nullptr, nullptr, nullptr, p[11], p[12], nullptr, nullptr, p[10], dn2, p + 21,
+                       g.nsnap, t, rows, d, eps, stream));
+  } else {
+    IMF_STEP(resnorm(p[7], p[8], p[5], da, p[6], p[11], p[12], p[9], dp2, p[10], dn2, p + 21, g.nsnap, t, rows, d, eps,
+                     stream));
+  }
   IMF_STEP(linear(p[10], p[13], p[14], m, 2 * g.fp, d, g.ld_w13, p[20], stream));
   {
     void* gu1 = t ? at(p[14], r * 2 * g.fp * 2) : nullptr;
@@ -126,6 +140,11 @@ extern "C" int imf_block_post(void** p, const int* dims, float eps, float beta, 
     IMF_STEP(imf_elementwise(1, e, ed, beta, lbeta, g.has_lbeta, t, 0, stream));
   }
   IMF_STEP(linear(p[15], p[16], p[17], m, d, g.fp, g.ld_w2, p[20], stream));
+  if (post) {
+    void* q[18] = {p[9], dp2, p[17], t ? at(p[17], r * d * 2) : nullptr, post[2], p[18], post[3], nullptr,
+                   p[19], t ? at(p[19], r * d * 4) : nullptr};
+    return imf_norm_add_norm(q, rows, d, eps, 0, t, static_cast<int*>(p[20]), stream);
+  }
   void* e[16] = {p[17], t ? at(p[17], r * d * 2) : nullptr, nullptr, nullptr, p[9], dp2, p[18], nullptr,
                  nullptr, p[19], t ? at(p[19], r * d * 4) : nullptr};
   const int ed[7] = {rows, d, d, d, d, 0, 0};

@@ -56,9 +56,9 @@ def _check(what: str, shape, lam: Tensor, scale: Optional[float], **tensors) -> 
     if len(shape) != 4 or shape[3] != HEAD_DIM or shape[2] % 2:
         raise ValueError(f"{what} takes (B, L, an even number of heads, {HEAD_DIM}), not {tuple(shape)}")
     for name, t in tensors.items():
-        if t is not None and (t.shape != shape or t.dtype != BF16):
+        if t is not None and (t.dtype is not BF16 or t.shape != shape):
             raise ValueError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, bf16 {tuple(shape)} expected")
-    if lam.dtype not in (BF16, F32) or tuple(lam.shape) != (shape[2] // 2,):
+    if (lam.dtype is not F32 and lam.dtype is not BF16) or lam.dim() != 1 or lam.shape[0] != shape[2] // 2:
         raise ValueError(f"{what}: lam is {lam.dtype} {tuple(lam.shape)}, fp32 or bf16 ({shape[2] // 2},) expected")
     scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
     if not 1e-30 <= scale <= 1e30:
@@ -71,12 +71,15 @@ def _operand(t: Tensor):
     single dimensions are replaced, no address depends on them."""
     B, L, H, D = t.shape
     row = (L * H * D, H * D, D)
-    if not t.is_contiguous():
+    if t.is_contiguous():
+        if t.data_ptr() % 16 == 0:
+            return t, row
+    else:
         s = [s_ if n > 1 else r for n, s_, r in zip(t.shape, t.stride(), row)]
         if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(x % 8 or x == 0 for x in s):
             return t, tuple(s)
         t = t.contiguous()                 # a broadcast, transposed or unaligned tensor
-    return (t, row) if t.data_ptr() % 16 == 0 else (t.clone(), row)
+    return (t if t.data_ptr() % 16 == 0 else t.clone()), row
 
 
 def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Tensor] = None,
@@ -194,6 +197,8 @@ def diff_attention_dual(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[
     """``ops.dual.diff_attention`` on CUDA tensors; lam (H,)."""
     t = (q.t, k.t, v.t)
     if any(x is not None for x in t):
-        t = tuple(torch.zeros_like(p.p) if x is None else x.detach() for p, x in zip((q, k, v), t))
-        return Dual(*_DiffAttnFn.apply(q.p, k.p, v.p, lam, *t, scale))
-    return Dual(_DiffAttnFn.apply(q.p, k.p, v.p, lam, None, None, None, scale)[0], None)
+        t = tuple(torch.zeros_like(p.p) if x is None else x for p, x in zip((q, k, v), t))
+    if torch.is_grad_enabled() and (q.p.requires_grad or k.p.requires_grad or v.p.requires_grad or lam.requires_grad):
+        o, do = _DiffAttnFn.apply(q.p, k.p, v.p, lam, *t, scale)
+        return Dual(o, None if t[0] is None else do)
+    return Dual(*diff_attn_fwd(q.p, k.p, v.p, lam, *t, scale, need_bwd=False)[:2])

@@ -202,11 +202,12 @@ def diff_attention(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[float
         raise ValueError("diff_attention takes q, k, v of one shape (b, l, an even number of heads, d), not "
                          f"{tuple(q.p.shape)}, {tuple(k.p.shape)}, {tuple(v.p.shape)}")
     H = q.p.shape[2] // 2
-    if lam.numel() != 1 and tuple(lam.shape) != (H,):
-        raise ValueError(f"diff_attention: lam is {tuple(lam.shape)}, one weight or ({H},) expected")
-    lam = lam.reshape(-1).expand(H)
+    if lam.dim() != 1 or lam.shape[0] != H:
+        if lam.numel() != 1:
+            raise ValueError(f"diff_attention: lam is {tuple(lam.shape)}, one weight or ({H},) expected")
+        lam = lam.reshape(1).expand(H)
     cu = _cuda_ops(q.p)
-    if impl == "auto" and cu is not None:
+    if impl == "auto" and cu is not None and not torch._C._are_functorch_transforms_active():
         from . import diffattn
 
         return diffattn.diff_attention_dual(q, k, v, lam, scale)
@@ -236,14 +237,14 @@ def norm_add_norm(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor, eps:
         raise ValueError("norm_add_norm: res_scale without res")
     D = y.p.shape[-1]
     for name, w in (("post", post), ("gate", gate), ("res_scale", res_scale), ("pre", pre)):
-        if w is not None and tuple(w.shape) != (D,):
+        if w is not None and (w.dim() != 1 or w.shape[0] != D):
             raise ValueError(f"norm_add_norm: {name} is {tuple(w.shape)}, ({D},) expected")
     if res is not None and res.p.shape != y.p.shape:
         raise ValueError(f"norm_add_norm: res is {tuple(res.p.shape)}, y {tuple(y.p.shape)}")
     xd = res.p.dtype if res is not None else torch.promote_types(y.p.dtype, torch.float32)
     nd = out_dtype or y.p.dtype
     cu = _cuda_ops(y.p)
-    if cu is not None:
+    if cu is not None and not torch._C._are_functorch_transforms_active():
         from . import postnorm
 
         if postnorm.supported(y.p, xd, nd, post, gate, res_scale, pre):

@@ -24,7 +24,7 @@ from .dual import Dual
 Tensor = torch.Tensor
 BF16, F32 = torch.bfloat16, torch.float32
 MAX_WIDTH = 8192
-_PTRS = ctypes.c_void_p * 17
+_PTRS = ctypes.c_void_p * 18
 _KERNELS = None
 
 
@@ -40,7 +40,7 @@ def _kernels():
         K._lib.imf_norm_add_norm_grid.restype = ci
         K._lib.imf_norm_add_norm_grid.argtypes = [ci, ci]
         K._lib.imf_norm_add_norm.restype = ci
-        K._lib.imf_norm_add_norm.argtypes = [vp, ci, ci, ctypes.c_float, ci, ci, vp]
+        K._lib.imf_norm_add_norm.argtypes = [vp, ci, ci, ctypes.c_float, ci, ci, vp, vp]
         _KERNELS = K
     return _KERNELS
 
@@ -52,25 +52,31 @@ def supported(y: Tensor, x_dtype: torch.dtype, n_dtype: torch.dtype, *vectors: O
             and y.numel() // D < 1 << 31 and all(w is None or w.dtype == F32 for w in vectors))
 
 
-def _rows(what: str, shape, dtype: torch.dtype, t: Optional[Tensor]) -> Optional[Tensor]:
+def _rows(what: str, name: str, shape, dtype: torch.dtype, t: Optional[Tensor]) -> Optional[Tensor]:
     """Contiguous, 16-byte aligned rows of a tensor (the tensor itself where it has them)."""
     if t is None:
         return None
-    if t.shape != shape or t.dtype != dtype:
-        raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} where {dtype} {tuple(shape)} is expected")
+    if t.shape != shape or t.dtype is not dtype:
+        raise ValueError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, {dtype} {tuple(shape)} expected")
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _prepare(what: str, res, y, post, gate, res_scale, pre):
-    D = y.shape[-1] if y.dim() else 0
-    if not supported(y, F32, y.dtype, post, gate, res_scale, pre):
-        raise ValueError(f"{what}: y bf16 or fp32 with a multiple of 8 up to {MAX_WIDTH} channels and fp32 vectors, "
-                         f"not {y.dtype} {tuple(y.shape)}")
+def _prepare(what: str, res, y, post, gate, res_scale, pre, more):
+    """The operands as the kernels take them; ``more``: (name, dtype, tensor) of further tensors of y's shape."""
+    shape = y.shape
+    D = shape[-1] if shape else 0
+    if not supported(y, F32, y.dtype):
+        raise ValueError(f"{what}: y bf16 or fp32 with a multiple of 8 up to {MAX_WIDTH} channels, not {y.dtype} {tuple(shape)}")
     if res_scale is not None and res is None:
         raise ValueError(f"{what}: res_scale without res")
-    vec = [_rows(f"{what}: a vector", (D,), F32, w) for w in (post, gate, res_scale, pre)]
-    return _rows(f"{what}: res", y.shape, F32, res), _rows(f"{what}: y", y.shape, y.dtype, y), vec
+    _same_device(what, y, res, post, gate, res_scale, pre, *[t for _, _, t in more])
+    vec = (D,)
+    return (_rows(what, "res", shape, F32, res), _rows(what, "y", shape, y.dtype, y), _rows(what, "post", vec, F32, post),
+            _rows(what, "gate", vec, F32, gate), _rows(what, "res_scale", vec, F32, res_scale),
+            _rows(what, "pre", vec, F32, pre), *[_rows(what, n, shape, d, t) for n, d, t in more])
 
 
 def norm_add_norm_fwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tensor, eps: float,
@@ -80,28 +86,29 @@ def norm_add_norm_fwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tens
     """(x, n | None, dx | None, dn | None) of CUDA tensors; with ``dy`` the tangents too (``dres`` None: the
     residual stands still)."""
     what = "norm_add_norm_fwd"
-    dev = _same_device(what, y, res, post, gate, res_scale, pre, dres, dy)
     if dres is not None and (dy is None or res is None):
         raise ValueError(f"{what}: dres without dy or res")
-    res, y, (post, gate, res_scale, pre) = _prepare(what, res, y, post, gate, res_scale, pre)
-    dres, dy = _rows(f"{what}: dres", y.shape, F32, dres), _rows(f"{what}: dy", y.shape, y.dtype, dy)
+    yt = y.dtype
+    res, y, post, gate, res_scale, pre, dres, dy = _prepare(what, res, y, post, gate, res_scale, pre,
+                                                           (("dres", F32, dres), ("dy", yt, dy)))
+    dev, shape = y.device, y.shape
     if dev.type != "cuda":
         raise ValueError(f"{what} launches on a GPU; dual.norm_add_norm also takes CPU tensors")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return norm_add_norm_fwd(res, y, post, gate, eps, res_scale, pre, dres, dy)
-    shape, D = y.shape, y.shape[-1]
     x = _new(shape, F32, dev)
-    n = None if pre is None else _new(shape, y.dtype, dev)
+    n = None if pre is None else _new(shape, yt, dev)
     dx = None if dy is None else _new(shape, F32, dev)
-    dn = None if dy is None or pre is None else _new(shape, y.dtype, dev)
+    dn = None if dy is None or pre is None else _new(shape, yt, dev)
+    D = shape[-1]
     rows = y.numel() // D
     if rows:
         K = _kernels()
         p = K._ptr
         ptrs = _PTRS(p(res), p(dres), p(y), p(dy), p(post), p(gate), p(res_scale), p(pre), p(x), p(dx), p(n), p(dn))
-        K._check(K._lib.imf_norm_add_norm(ptrs, rows, D, float(eps), int(y.dtype == F32), int(dy is not None),
-                                          K._stream()), "imf_norm_add_norm")
+        K._check(K._lib.imf_norm_add_norm(ptrs, rows, D, eps, yt is F32, dy is not None,
+                                          K.status_word(dev).data_ptr(), K._stream()), "imf_norm_add_norm")
         K.LAUNCHES.count += 1
     return x, n, dx, dn
 
@@ -112,45 +119,43 @@ def norm_add_norm_bwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tens
     """(g_res | None, g_y, g_pre | None, g_r | None, g_gate, g_post) from the gradients of x and n (None: zero;
     ``gn`` together with ``pre``).  With ``raw`` the last four are replaced by the [g, 4, D] buffer of their
     partial sums (columns pre, r, gate, post) for a later ``rowops.ColSums`` reduction; columns of vectors that
-    are not there are not written."""
+    are not there are not written.  g_res may be ``gx`` itself."""
     what = "norm_add_norm_bwd"
-    dev = _same_device(what, y, res, post, gate, res_scale, pre, gx, gn)
     if (gn is None) != (pre is None):
         raise ValueError(f"{what}: gn and pre come together")
-    res, y, (post, gate, res_scale, pre) = _prepare(what, res, y, post, gate, res_scale, pre)
-    gx, gn = _rows(f"{what}: gx", y.shape, F32, gx), _rows(f"{what}: gn", y.shape, y.dtype, gn)
+    yt = y.dtype
+    res, y, post, gate, res_scale, pre, gx, gn = _prepare(what, res, y, post, gate, res_scale, pre,
+                                                         (("gx", F32, gx), ("gn", yt, gn)))
+    dev, shape = y.device, y.shape
     if dev.type != "cuda":
         raise ValueError(f"{what} launches on a GPU; dual.norm_add_norm also takes CPU tensors")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return norm_add_norm_bwd(res, y, post, gate, eps, res_scale, pre, gx, gn, want_g_res, raw)
-    shape, D = y.shape, y.shape[-1]
+    D = shape[-1]
     rows = y.numel() // D
     want_g_res = want_g_res and res is not None
     # without a second norm and a scale the residual's gradient is x's
     passed = want_g_res and pre is None and res_scale is None and gx is not None
     g_res = gx if passed else _new(shape, F32, dev) if want_g_res else None
-    g_y = _new(shape, y.dtype, dev)
-    if rows == 0:
-        zero = lambda w: None if w is None else torch.zeros_like(w)
-        part = torch.zeros(1, 4, D, dtype=F32, device=dev)
-        return (g_res, g_y, part) if raw else (g_res, g_y, zero(pre), zero(res_scale), zero(gate), zero(post))
-    K = _kernels()
-    part = _new((K._lib.imf_norm_add_norm_grid(rows, D), 4, D), F32, dev)
-    p = K._ptr
-    ptrs = _PTRS(p(res), None, p(y), None, p(post), p(gate), p(res_scale), p(pre), None, None, None, None, p(gx), p(gn),
-                 None if passed else p(g_res), p(g_y), p(part))
-    K._check(K._lib.imf_norm_add_norm(ptrs, rows, D, float(eps), int(y.dtype == F32), 2, K._stream()),
-             "imf_norm_add_norm")
-    K.LAUNCHES.count += 1
+    g_y = _new(shape, yt, dev)
+    part = sums = None
+    if rows:
+        K = _kernels()
+        p = K._ptr
+        part = _new((K._lib.imf_norm_add_norm_grid(rows, D), 4, D), F32, dev)
+        sums = None if raw else _new((4, D), F32, dev)
+        ptrs = _PTRS(p(res), None, p(y), None, p(post), p(gate), p(res_scale), p(pre), None, None, None, None, p(gx),
+                     p(gn), None if passed else p(g_res), p(g_y), p(part), p(sums))
+        K._check(K._lib.imf_norm_add_norm(ptrs, rows, D, eps, yt is F32, 2, K.status_word(dev).data_ptr(), K._stream()),
+                 "imf_norm_add_norm")
+        K.LAUNCHES.count += 1 if raw else 2
+    else:
+        part, sums = torch.zeros(1, 4, D, dtype=F32, device=dev), torch.zeros(4, D, dtype=F32, device=dev)
     if raw:
         return g_res, g_y, part
-    from .rowops import ColSums
-
-    cs = ColSums()
-    sums = [None if w is None else cs.add(part, i, D, None) for i, w in enumerate((pre, res_scale, gate, post))]
-    cs.flush()
-    return (g_res, g_y, *sums)
+    g_pre, g_r, g_gate, g_post = sums.unbind(0)
+    return g_res, g_y, None if pre is None else g_pre, None if res_scale is None else g_r, g_gate, g_post
 
 
 class _NormAddNormFn(torch.autograd.Function):
@@ -186,6 +191,8 @@ def norm_add_norm_dual(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor,
     dy = y.t
     if dy is None and rt is not None:
         dy = torch.zeros_like(y.p)
-    x, n, dx, dn = _NormAddNormFn.apply(rp, y.p, post, gate, res_scale, pre, None if rt is None else rt.detach(),
-                                        None if dy is None else dy.detach(), eps)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rp, y.p, post, gate, res_scale, pre)):
+        x, n, dx, dn = _NormAddNormFn.apply(rp, y.p, post, gate, res_scale, pre, rt, dy, eps)
+    else:
+        x, n, dx, dn = norm_add_norm_fwd(rp, y.p, post, gate, eps, res_scale, pre, rt, dy)
     return Dual(x, dx), None if n is None else Dual(n, dn)

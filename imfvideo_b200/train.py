@@ -66,6 +66,10 @@ def build_attn_impl(cfg: Config):
         return partial(SLA2CubeQATAttentionImpl,
                        grid=(cfg.data.latent_frames // pt, lh // ph, lw // pw),
                        tile=tuple(m.sla2_tile), topk=m.sla2_topk, alpha_init=m.sla2_alpha_init)
+    if name == "diff_jvp":
+        from .models.diff_attn import DiffAttentionImpl
+
+        return partial(DiffAttentionImpl, lam_init=m.diff_lam_init)
     raise ValueError(f"unknown attn_impl {name!r}")
 
 
@@ -90,7 +94,8 @@ def build_model(cfg: Optional[Config] = None) -> Tuple[M.IMFDiTVideo, int, str]:
         rope_theta=m.rope_theta, eval_mode=m.eval_mode, attn_impl=attn,
         attn_res_block_size=m.attn_res_block_size, situ_beta=m.situ_beta,
         situ_linear_beta=m.situ_linear_beta, mla_use_output_gate=m.mla_use_output_gate,
-        grad_checkpoint=m.grad_checkpoint, act_store=m.act_store)
+        grad_checkpoint=m.grad_checkpoint, act_store=m.act_store, post_norm=m.post_norm,
+        residual_scale=m.residual_scale)
     n = sum(p.numel() for p in net.parameters())
     assert n <= m.max_params, f"model has {n / 1e6:.1f}M params, cap {m.max_params / 1e6:.0f}M"
     return net, n, getattr(attn, "__name__", str(attn))
