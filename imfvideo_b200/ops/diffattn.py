@@ -15,6 +15,7 @@ stream of the tensors' device; workspaces belong to the call.  The reference has
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -52,34 +53,55 @@ def _kernels():
     return _KERNELS
 
 
-def _check(what: str, shape, lam: Tensor, scale: Optional[float], **tensors) -> Tuple[torch.device, float]:
+def _check(what: str, shape, lam: Tensor, scale: Optional[float], names: str, *tensors) -> Tuple[torch.device, float]:
     if len(shape) != 4 or shape[3] != HEAD_DIM or shape[2] % 2:
         raise ValueError(f"{what} takes (B, L, an even number of heads, {HEAD_DIM}), not {tuple(shape)}")
-    for name, t in tensors.items():
-        if t is not None and (t.dtype is not BF16 or t.shape != shape):
-            raise ValueError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, bf16 {tuple(shape)} expected")
+    dev = lam.device
+    for i, t in enumerate(tensors):
+        if t is not None and (t.dtype is not BF16 or t.shape != shape or t.device != dev):
+            raise ValueError(f"{what}: {names.split()[i]} is {t.dtype} {tuple(t.shape)} on {t.device}, bf16 {tuple(shape)} on "
+                             f"{dev} (where lam is) expected")
     if (lam.dtype is not F32 and lam.dtype is not BF16) or lam.dim() != 1 or lam.shape[0] != shape[2] // 2:
         raise ValueError(f"{what}: lam is {lam.dtype} {tuple(lam.shape)}, fp32 or bf16 ({shape[2] // 2},) expected")
     scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
     if not 1e-30 <= scale <= 1e30:
         raise ValueError(f"{what}: scale {scale} is not a positive number between 1e-30 and 1e30")
-    return _same_device(what, *tensors.values(), lam), scale
+    return dev, scale
 
 
-def _operand(t: Tensor):
-    """(the tensor or a copy with 16-byte aligned rows, its (batch, row, head) strides); strides of
-    single dimensions are replaced, no address depends on them."""
-    B, L, H, D = t.shape
+@lru_cache(maxsize=64)
+def _rows(shape: Tuple[int, ...]):
+    """(batch, row, head) strides of a contiguous tensor, as a tuple and for one and for six tensors as the
+    launchers take them."""
+    B, L, H, D = shape
     row = (L * H * D, H * D, D)
-    if t.is_contiguous():
-        if t.data_ptr() % 16 == 0:
-            return t, row
-    else:
-        s = [s_ if n > 1 else r for n, s_, r in zip(t.shape, t.stride(), row)]
-        if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(x % 8 or x == 0 for x in s):
-            return t, tuple(s)
-        t = t.contiguous()                 # a broadcast, transposed or unaligned tensor
-    return (t if t.data_ptr() % 16 == 0 else t.clone()), row
+    return row, (ctypes.c_int64 * 3)(*row), (ctypes.c_int64 * 18)(*row * 6)
+
+
+def _operands(tensors, row, six):
+    """(the tensors, or copies of those without 16-byte aligned rows; their strides as the launchers take
+    them).  Strides of single dimensions are replaced: no address depends on them."""
+    out, strides = [], None
+    for i, t in enumerate(tensors):
+        st = row
+        if not t.is_contiguous():
+            s = [x if n > 1 else r for n, x, r in zip(t.shape, t.stride(), row)]
+            if t.stride(3) == 1 and t.data_ptr() % 16 == 0 and not any(x % 8 or x == 0 for x in s):
+                st = s
+            else:
+                t = t.contiguous()             # a broadcast, transposed or unaligned tensor
+        if t.data_ptr() % 16:
+            t = t.clone()
+        out.append(t)
+        if st is not row:
+            strides = strides or list(row) * 6
+            strides[3 * i:3 * i + 3] = st
+    return out, six if strides is None else (ctypes.c_int64 * 18)(*strides)
+
+
+def _like(t: Tensor) -> Tensor:
+    """An uninitialised contiguous tensor of the same shape and type."""
+    return torch.empty_like(t) if t.is_contiguous() else _new(t.shape, t.dtype, t.device)
 
 
 def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Tensor] = None,
@@ -92,30 +114,30 @@ def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Ten
     shape, tang = q.shape, dq is not None
     if (dk is None) == tang or (dv is None) == tang:
         raise ValueError("diff_attn_fwd: tangents of q, k and v come together")
-    dev, scale = _check("diff_attn_fwd", shape, lam, scale, q=q, k=k, v=v, dq=dq, dk=dk, dv=dv)
+    dev, scale = _check("diff_attn_fwd", shape, lam, scale, "q k v dq dk dv", q, k, v, dq, dk, dv)
     if dev.type != "cuda":
         raise ValueError("diff_attn_fwd launches on a GPU; dual.diff_attention also takes CPU tensors")
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return diff_attn_fwd(q, k, v, lam, dq, dk, dv, scale, need_bwd)
     B, L, H2, D = shape
-    o = _new(shape, BF16, dev)
-    do = _new(shape, BF16, dev) if tang else None
-    o2, low, lse = saved = (_new(shape, BF16, dev), _new((2, *shape), torch.int8, dev),
-                            _new((B, H2, L), F32, dev)) if need_bwd else (None,) * 3
+    o = _like(q)
+    do = _like(q) if tang else None
+    o2, low, lse = saved = (_like(q), _new((2, *shape), torch.int8, dev), _new((B, H2, L), F32, dev)) if need_bwd else (None,) * 3
     saved = saved if need_bwd else ()
     if 0 in shape:
         return o, do, saved
     K = _kernels()
-    ops = [_operand(t) for t in ((q, k, v, dq, dk, dv) if tang else (q, k, v))]
-    ptrs = [t.data_ptr() for t, _ in ops] + ([] if tang else [None] * 3)
-    strides = [s for _, st in ops for s in st]
-    nscr = K._lib.imf_attn_diff_fwd_scratch_bytes(B, L, H2 // 2, int(tang))
+    row, row3, row18 = _rows(shape)
+    ts, strides = _operands((q, k, v, dq, dk, dv) if tang else (q, k, v), row, row18)
+    ptr = [t.data_ptr() for t in ts]
+    nscr = K._lib.imf_attn_diff_fwd_scratch_bytes(B, L, H2 // 2, tang)
     scr = _new(nscr, torch.uint8, dev) if nscr else None
+    p = K._ptr
     K._check(K._lib.imf_attn_diff_fwd(
-        *ptrs, lam.data_ptr(), lam.stride(0), int(lam.dtype == BF16), o.data_ptr(), K._ptr(do), K._ptr(o2),
-        K._ptr(low), o.numel(), K._ptr(lse), B, L, H2 // 2, (ctypes.c_int64 * 18)(*strides), (ctypes.c_int64 * 3)(L * H2 * D, H2 * D, D),
-        scale, K._ptr(scr), nscr, K.status_word(dev).data_ptr(), K._stream()), "imf_attn_diff_fwd")
+        *(ptr if tang else (*ptr, None, None, None)), lam.data_ptr(), lam.stride(0), lam.dtype is BF16, o.data_ptr(), p(do),
+        p(o2), p(low), o.numel(), p(lse), B, L, H2 // 2, strides, row3, scale, p(scr), nscr,
+        K.status_word(dev).data_ptr(), K._stream()), "imf_attn_diff_fwd")
     K.LAUNCHES.count += 1
     return o, do, saved
 
@@ -128,20 +150,21 @@ def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved
     ``kernels.attn_bwd``, whose fixed-order mode holds here too."""
     shape = q.shape
     o2, low, lse = saved
-    dev, scale = _check("diff_attn_bwd", shape, lam, scale, q=q, k=k, v=v, o=o, o2=o2, go=go, gv_out=gv_out)
+    dev, scale = _check("diff_attn_bwd", shape, lam, scale, "q k v o o2 go gv_out", q, k, v, o, o2, go, gv_out)
     _same_device("diff_attn_bwd", q, low, lse)
     if dev.type != "cuda":
         raise ValueError("diff_attn_bwd launches on a GPU; dual.diff_attention also takes CPU tensors")
     B, L, H2, D = shape
-    if lse.dtype != F32 or tuple(lse.shape) != (B, H2, L) or not lse.is_contiguous():
+    if lse.dtype is not F32 or lse.shape != (B, H2, L) or not lse.is_contiguous():
         raise ValueError(f"diff_attn_bwd: lse has to be contiguous fp32 {(B, H2, L)}")
-    if low.dtype != torch.int8 or low.shape != (2, *shape) or not (low.is_contiguous() and o2.is_contiguous()):
+    if low.dtype is not torch.int8 or low.shape != (2, *shape) or not (low.is_contiguous() and o2.is_contiguous()):
         raise ValueError("diff_attn_bwd: saved has to be what diff_attn_fwd returned")
-    row = (L * H2 * D, H2 * D, D)
-    dv_strides = row
+    row, row3, row18 = _rows(shape)
+    dv_strides = row3
     if gv_out is not None and 0 not in shape:
-        dv_strides = [s if n > 1 else r for n, s, r in zip(shape, gv_out.stride(), row)]
-        if gv_out.stride(3) != 1 or gv_out.data_ptr() % 16 or any(s % 8 for s in dv_strides):
+        st = [s if n > 1 else r for n, s, r in zip(shape, gv_out.stride(), row)]
+        dv_strides = (ctypes.c_int64 * 3)(*st)
+        if gv_out.stride(3) != 1 or gv_out.data_ptr() % 16 or any(s % 8 for s in st):
             raise ValueError("diff_attn_bwd: the dv output needs 16-byte aligned rows")
         if not _apart(*_places(gv_out)):
             raise ValueError("diff_attn_bwd: no two elements of the dv output in one place")
@@ -150,23 +173,21 @@ def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return diff_attn_bwd(q, k, v, lam, o, saved, go, scale, gv_out)
-    dq, dk = _new(shape, BF16, dev), _new(shape, BF16, dev)
-    dv = _new(shape, BF16, dev) if gv_out is None else gv_out
+    dq, dk = _like(o2), _like(o2)
+    dv = _like(o2) if gv_out is None else gv_out
     dlam = _new((H2 // 2,), lam.dtype, dev)
     if 0 in shape:
         return dq, dk, dv, dlam.zero_()
     K = _kernels()
-    (q_, sq), (k_, sk), (v_, sv), (g_, sg) = (_operand(t) for t in (q, k, v, go))
-    o_ = o.contiguous()
+    (q_, k_, v_, g_), strides = _operands((q, k, v, go), row, row18)
+    o = o.contiguous()
     nscr = K._lib.imf_attn_diff_bwd_scratch_bytes(B, L, H2 // 2)
     scr = _new(nscr, torch.uint8, dev)
-    i64 = ctypes.c_int64
     K._check(K._lib.imf_attn_diff_bwd(
-        q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), o_.data_ptr(), o2.data_ptr(), low.data_ptr(), o.numel(),
-        g_.data_ptr(), lse.data_ptr(), lam.data_ptr(), lam.stride(0), int(lam.dtype == BF16), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-        dlam.data_ptr(), B, L, H2 // 2, (i64 * 12)(*sq, *sk, *sv, *sg), (i64 * 3)(*row), (i64 * 3)(*row),
-        (i64 * 3)(*dv_strides), scale, scr.data_ptr(), nscr, int(K.DETERMINISTIC), K.status_word(dev).data_ptr(),
-        K._stream()), "imf_attn_diff_bwd")
+        q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), o.data_ptr(), o2.data_ptr(), low.data_ptr(), o.numel(), g_.data_ptr(),
+        lse.data_ptr(), lam.data_ptr(), lam.stride(0), lam.dtype is BF16, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+        dlam.data_ptr(), B, L, H2 // 2, strides, row3, row3, dv_strides, scale, scr.data_ptr(), nscr,
+        bool(K.DETERMINISTIC), K.status_word(dev).data_ptr(), K._stream()), "imf_attn_diff_bwd")
     K.LAUNCHES.count += 3
     return dq, dk, dv, dlam
 

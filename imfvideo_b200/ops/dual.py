@@ -51,6 +51,21 @@ def _cuda_ops(x: Tensor):
     return None
 
 
+_modules: dict = {}
+
+
+def _kernel_module(name: str, x: Tensor):
+    """The module of kernels ``name`` for a CUDA tensor, None where the formulas run."""
+    if not x.is_cuda or torch._C._are_functorch_transforms_active():
+        return None
+    mod = _modules.get(name)
+    if mod is None:
+        import importlib
+
+        mod = _modules[name] = (importlib.import_module(f".{name}", __package__), importlib.import_module(".cuda", __package__))
+    return mod[0] if mod[1].available() else None
+
+
 # ---------------------------------------------------------------- linear ---
 def linear(x: Dual, weight: Tensor, bias: Optional[Tensor] = None) -> Dual:
     """y = x W^T + b ; dy = dx W^T.  On CUDA the primal and tangent rows are
@@ -206,11 +221,9 @@ def diff_attention(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[float
         if lam.numel() != 1:
             raise ValueError(f"diff_attention: lam is {tuple(lam.shape)}, one weight or ({H},) expected")
         lam = lam.reshape(1).expand(H)
-    cu = _cuda_ops(q.p)
-    if impl == "auto" and cu is not None and not torch._C._are_functorch_transforms_active():
-        from . import diffattn
-
-        return diffattn.diff_attention_dual(q, k, v, lam, scale)
+    mod = _kernel_module("diffattn", q.p) if impl == "auto" else None
+    if mod is not None:
+        return mod.diff_attention_dual(q, k, v, lam, scale)
     p = ref.diff_attention(q.p, k.p, v.p, lam, scale)
     t = None
     if any(x.t is not None for x in (q, k, v)):
@@ -233,6 +246,10 @@ def norm_add_norm(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor, eps:
     this branch; ``res_scale`` None: 1.  x has the type of ``res`` (without one, 32 bits or y's), n
     ``out_dtype`` or y's.  CUDA: y bf16 or fp32 and res fp32 take one kernel a direction
     (``ops/postnorm.py``)."""
+    mod = _kernel_module("postnorm", y.p)
+    if mod is not None and mod.supported(y.p, torch.float32 if res is None else res.p.dtype, out_dtype, post, gate,
+                                         res_scale, pre):
+        return mod.norm_add_norm_dual(res, y, post, gate, eps, res_scale, pre)
     if res_scale is not None and res is None:
         raise ValueError("norm_add_norm: res_scale without res")
     D = y.p.shape[-1]
@@ -243,12 +260,6 @@ def norm_add_norm(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor, eps:
         raise ValueError(f"norm_add_norm: res is {tuple(res.p.shape)}, y {tuple(y.p.shape)}")
     xd = res.p.dtype if res is not None else torch.promote_types(y.p.dtype, torch.float32)
     nd = out_dtype or y.p.dtype
-    cu = _cuda_ops(y.p)
-    if cu is not None and not torch._C._are_functorch_transforms_active():
-        from . import postnorm
-
-        if postnorm.supported(y.p, xd, nd, post, gate, res_scale, pre):
-            return postnorm.norm_add_norm_dual(res, y, post, gate, eps, res_scale, pre)
     rp, rt = (None, None) if res is None else res
     x, n = ref.norm_add_norm(rp, y.p, post, gate, eps, res_scale, pre)
     dx = dn = None

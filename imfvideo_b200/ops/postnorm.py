@@ -18,7 +18,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import cuda as _cuda
-from .act8 import _elsewhere, _new, _same_device
+from .act8 import _elsewhere, _new
 from .dual import Dual
 
 Tensor = torch.Tensor
@@ -45,38 +45,42 @@ def _kernels():
     return _KERNELS
 
 
-def supported(y: Tensor, x_dtype: torch.dtype, n_dtype: torch.dtype, *vectors: Optional[Tensor]) -> bool:
+def supported(y: Tensor, x_dtype: torch.dtype, n_dtype: Optional[torch.dtype], post: Tensor, gate: Tensor,
+              res_scale: Optional[Tensor], pre: Optional[Tensor]) -> bool:
     """Whether the kernels take these types and this width."""
-    D = y.shape[-1]
-    return (y.dtype in (BF16, F32) and n_dtype == y.dtype and x_dtype == F32 and D % 8 == 0 and 0 < D <= MAX_WIDTH
-            and y.numel() // D < 1 << 31 and all(w is None or w.dtype == F32 for w in vectors))
+    yt, D = y.dtype, y.shape[-1] if y.dim() else 0
+    return ((yt is BF16 or yt is F32) and x_dtype is F32 and (n_dtype is None or n_dtype is yt) and D % 8 == 0
+            and 0 < D <= MAX_WIDTH and post.dtype is F32 and gate.dtype is F32
+            and (res_scale is None or res_scale.dtype is F32) and (pre is None or pre.dtype is F32))
 
 
-def _rows(what: str, name: str, shape, dtype: torch.dtype, t: Optional[Tensor]) -> Optional[Tensor]:
+def _aligned(t: Optional[Tensor]) -> Optional[Tensor]:
     """Contiguous, 16-byte aligned rows of a tensor (the tensor itself where it has them)."""
-    if t is None:
-        return None
-    if t.shape != shape or t.dtype is not dtype:
-        raise ValueError(f"{what}: {name} is {t.dtype} {tuple(t.shape)}, {dtype} {tuple(shape)} expected")
-    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+    if t is None or (t.is_contiguous() and t.data_ptr() % 16 == 0):
         return t
     t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _prepare(what: str, res, y, post, gate, res_scale, pre, more):
-    """The operands as the kernels take them; ``more``: (name, dtype, tensor) of further tensors of y's shape."""
-    shape = y.shape
-    D = shape[-1] if shape else 0
-    if not supported(y, F32, y.dtype):
-        raise ValueError(f"{what}: y bf16 or fp32 with a multiple of 8 up to {MAX_WIDTH} channels, not {y.dtype} {tuple(shape)}")
-    if res_scale is not None and res is None:
-        raise ValueError(f"{what}: res_scale without res")
-    _same_device(what, y, res, post, gate, res_scale, pre, *[t for _, _, t in more])
-    vec = (D,)
-    return (_rows(what, "res", shape, F32, res), _rows(what, "y", shape, y.dtype, y), _rows(what, "post", vec, F32, post),
-            _rows(what, "gate", vec, F32, gate), _rows(what, "res_scale", vec, F32, res_scale),
-            _rows(what, "pre", vec, F32, pre), *[_rows(what, n, shape, d, t) for n, d, t in more])
+def _prepare(what: str, y, vectors, streams, likes):
+    """Checks and aligns the operands: learned ``vectors`` and fp32 ``streams`` and others of y's type (``likes``),
+    of y's shape."""
+    shape, yt, dev = y.shape, y.dtype, y.device
+    if (yt is not BF16 and yt is not F32) or not shape or shape[-1] % 8 or not 0 < shape[-1] <= MAX_WIDTH or \
+            y.numel() // shape[-1] >= 1 << 31:
+        raise ValueError(f"{what}: y bf16 or fp32 with a multiple of 8 up to {MAX_WIDTH} channels, not {yt} {tuple(shape)}")
+    for want, dtype, ts in ((shape[-1:], F32, vectors), (shape, F32, streams), (shape, yt, likes)):
+        for t in ts:
+            if t is not None and (t.dtype is not dtype or t.shape != want or t.device != dev):
+                raise ValueError(f"{what}: {t.dtype} {tuple(t.shape)} on {t.device} where {dtype} {tuple(want)} on {dev} is expected")
+    if dev.type != "cuda":
+        raise ValueError(f"{what} launches on a GPU; dual.norm_add_norm also takes CPU tensors")
+    return [_aligned(t) for t in (y, *vectors, *streams, *likes)]
+
+
+def _like(y: Tensor, dtype: torch.dtype) -> Tensor:
+    """An uninitialised tensor of a contiguous one's shape."""
+    return torch.empty_like(y) if y.dtype is dtype else torch.empty_like(y, dtype=dtype)
 
 
 def norm_add_norm_fwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tensor, eps: float,
@@ -86,22 +90,18 @@ def norm_add_norm_fwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tens
     """(x, n | None, dx | None, dn | None) of CUDA tensors; with ``dy`` the tangents too (``dres`` None: the
     residual stands still)."""
     what = "norm_add_norm_fwd"
-    if dres is not None and (dy is None or res is None):
-        raise ValueError(f"{what}: dres without dy or res")
-    yt = y.dtype
-    res, y, post, gate, res_scale, pre, dres, dy = _prepare(what, res, y, post, gate, res_scale, pre,
-                                                           (("dres", F32, dres), ("dy", yt, dy)))
-    dev, shape = y.device, y.shape
-    if dev.type != "cuda":
-        raise ValueError(f"{what} launches on a GPU; dual.norm_add_norm also takes CPU tensors")
+    if (dres is not None and (dy is None or res is None)) or (res_scale is not None and res is None):
+        raise ValueError(f"{what}: dres without dy or res, or res_scale without res")
+    y, post, gate, res_scale, pre, res, dres, dy = _prepare(what, y, (post, gate, res_scale, pre), (res, dres), (dy,))
+    dev, yt = y.device, y.dtype
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return norm_add_norm_fwd(res, y, post, gate, eps, res_scale, pre, dres, dy)
-    x = _new(shape, F32, dev)
-    n = None if pre is None else _new(shape, yt, dev)
-    dx = None if dy is None else _new(shape, F32, dev)
-    dn = None if dy is None or pre is None else _new(shape, yt, dev)
-    D = shape[-1]
+    x = _like(y, F32)
+    n = None if pre is None else torch.empty_like(y)
+    dx = None if dy is None else _like(y, F32)
+    dn = None if dy is None or pre is None else torch.empty_like(y)
+    D = y.shape[-1]
     rows = y.numel() // D
     if rows:
         K = _kernels()
@@ -121,24 +121,20 @@ def norm_add_norm_bwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tens
     partial sums (columns pre, r, gate, post) for a later ``rowops.ColSums`` reduction; columns of vectors that
     are not there are not written.  g_res may be ``gx`` itself."""
     what = "norm_add_norm_bwd"
-    if (gn is None) != (pre is None):
-        raise ValueError(f"{what}: gn and pre come together")
-    yt = y.dtype
-    res, y, post, gate, res_scale, pre, gx, gn = _prepare(what, res, y, post, gate, res_scale, pre,
-                                                         (("gx", F32, gx), ("gn", yt, gn)))
-    dev, shape = y.device, y.shape
-    if dev.type != "cuda":
-        raise ValueError(f"{what} launches on a GPU; dual.norm_add_norm also takes CPU tensors")
+    if (gn is None) != (pre is None) or (res_scale is not None and res is None):
+        raise ValueError(f"{what}: gn and pre come together, res_scale with res")
+    y, post, gate, res_scale, pre, res, gx, gn = _prepare(what, y, (post, gate, res_scale, pre), (res, gx), (gn,))
+    dev, yt = y.device, y.dtype
     if _elsewhere(dev):
         with torch.cuda.device(dev):
             return norm_add_norm_bwd(res, y, post, gate, eps, res_scale, pre, gx, gn, want_g_res, raw)
-    D = shape[-1]
+    D = y.shape[-1]
     rows = y.numel() // D
     want_g_res = want_g_res and res is not None
     # without a second norm and a scale the residual's gradient is x's
     passed = want_g_res and pre is None and res_scale is None and gx is not None
-    g_res = gx if passed else _new(shape, F32, dev) if want_g_res else None
-    g_y = _new(shape, yt, dev)
+    g_res = gx if passed else _like(y, F32) if want_g_res else None
+    g_y = torch.empty_like(y)
     part = sums = None
     if rows:
         K = _kernels()
@@ -168,7 +164,8 @@ class _NormAddNormFn(torch.autograd.Function):
         if any(ctx.needs_input_grad[:6]):
             ctx.save_for_backward(res, y, post, gate, res_scale, pre)
             ctx.eps = eps
-        ctx.mark_non_differentiable(*[t for t in (dx, dn) if t is not None])
+        if dx is not None:
+            ctx.mark_non_differentiable(*((dx,) if dn is None else (dx, dn)))
         return x, n, dx, dn
 
     @staticmethod
@@ -191,7 +188,8 @@ def norm_add_norm_dual(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor,
     dy = y.t
     if dy is None and rt is not None:
         dy = torch.zeros_like(y.p)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (rp, y.p, post, gate, res_scale, pre)):
+    if torch.is_grad_enabled() and (y.p.requires_grad or post.requires_grad or gate.requires_grad or
+                                    any(t is not None and t.requires_grad for t in (rp, res_scale, pre))):
         x, n, dx, dn = _NormAddNormFn.apply(rp, y.p, post, gate, res_scale, pre, rt, dy, eps)
     else:
         x, n, dx, dn = norm_add_norm_fwd(rp, y.p, post, gate, eps, res_scale, pre, rt, dy)
