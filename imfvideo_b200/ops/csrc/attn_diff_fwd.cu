@@ -48,7 +48,6 @@ struct Rec {
   static constexpr int ACC = TANGENT ? 2 * VD : VD;
   static constexpr int STATS = ACC * TM;
   static constexpr size_t MAP = (size_t)TM * (ACC + 3), ALL = 2 * MAP;
-  static constexpr float PART_COST = TANGENT ? 0.9f : 0.6f;  // see fwd_share_cost
 };
 constexpr size_t HOLD = (size_t)TM * 2 * VD;      // floats a CTA holds of map 1 (tangent)
 
@@ -924,39 +923,60 @@ __global__ void __launch_bounds__(32 * VD / COMBINE_COLS) attn_diff_combine_kern
   const int q_row = q0 + r;
   if (q_row >= p.L) return;
   const int64_t off = (int64_t)b * p.o_sb + (int64_t)q_row * p.o_sl + (int64_t)(2 * h + col / HD) * p.o_sh + col % HD;
-  float y[COMBINE_COLS], dy[COMBINE_COLS];
+  const float* x = p.scratch + (size_t)(2 * c + 1) * R::ALL + r;   // then records 2c + 2, 2c + 4, ...
+  float m[2] = {x[R::STATS], x[R::MAP + R::STATS]}, l[2] = {0.f, 0.f}, mu[2] = {0.f, 0.f};
+  float o[2][COMBINE_COLS], d[2][COMBINE_COLS];
 #pragma unroll
-  for (int map = 0; map < 2; ++map) {
-    const float* x = p.scratch + (size_t)(2 * c + 1) * R::ALL + map * R::MAP + r;   // then records 2c + 2, 2c + 4, ...
-    float m = x[R::STATS], l = 0.f, mu = 0.f;
-    float o[COMBINE_COLS], d[COMBINE_COLS];
-#pragma unroll
-    for (int i = 0; i < COMBINE_COLS; ++i) o[i] = d[i] = 0.f;
+  for (int i = 0; i < COMBINE_COLS; ++i) o[0][i] = o[1][i] = d[0][i] = d[1][i] = 0.f;
+  // All of it is latency: with a tangent both maps' loads at once (1 x 1,100 rows, 2 pairs 41 -> 33 us in all), without
+  // one map after the other (24, at once 28).
+  if constexpr (TANGENT) {
 #pragma unroll 2
     for (int k = 0; k < parts; ++k, x += k == 1 ? R::ALL : 2 * R::ALL) {
-      const float mk = x[R::STATS], mn = fmaxf(m, mk);
-      const float w0 = ex2((m - mn) * LOG2E), w1 = ex2((mk - mn) * LOG2E);
-      m = mn;
-      l = l * w0 + x[R::STATS + TM] * w1;
-      mu = mu * w0 + x[R::STATS + 2 * TM] * w1;
 #pragma unroll
-      for (int i = 0; i < COMBINE_COLS; ++i) {
-        o[i] = o[i] * w0 + x[(col + i) * TM] * w1;
-        if (TANGENT) d[i] = d[i] * w0 + x[(VD + col + i) * TM] * w1;
+      for (int t = 0; t < 2; ++t) {
+        const float* z = x + t * R::MAP;
+        const float mk = z[R::STATS], mn = fmaxf(m[t], mk);
+        const float w0 = ex2((m[t] - mn) * LOG2E), w1 = ex2((mk - mn) * LOG2E);
+        m[t] = mn;
+        l[t] = l[t] * w0 + z[R::STATS + TM] * w1;
+        mu[t] = mu[t] * w0 + z[R::STATS + 2 * TM] * w1;
+#pragma unroll
+        for (int i = 0; i < COMBINE_COLS; ++i) {
+          o[t][i] = o[t][i] * w0 + z[(col + i) * TM] * w1;
+          d[t][i] = d[t][i] * w0 + z[(VD + col + i) * TM] * w1;
+        }
       }
     }
-    const float inv_l = 1.f / l, mul = mu * inv_l;
+  } else {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const float* z = x + t * R::MAP;
+#pragma unroll 2
+      for (int k = 0; k < parts; ++k, z += k == 1 ? R::ALL : 2 * R::ALL) {
+        const float mk = z[R::STATS], mn = fmaxf(m[t], mk);
+        const float w0 = ex2((m[t] - mn) * LOG2E), w1 = ex2((mk - mn) * LOG2E);
+        m[t] = mn;
+        l[t] = l[t] * w0 + z[R::STATS + TM] * w1;
+#pragma unroll
+        for (int i = 0; i < COMBINE_COLS; ++i) o[t][i] = o[t][i] * w0 + z[(col + i) * TM] * w1;
+      }
+    }
+  }
+  float y[COMBINE_COLS], dy[COMBINE_COLS];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const float inv_l = 1.f / l[t], mul = mu[t] * inv_l;
 #pragma unroll
     for (int i = 0; i < COMBINE_COLS; ++i) {
-      o[i] *= inv_l;
-      d[i] = d[i] * inv_l - mul * o[i];
-      y[i] = map == 0 ? o[i] : y[i] - lam * o[i];
-      dy[i] = map == 0 ? d[i] : dy[i] - lam * d[i];
+      o[t][i] *= inv_l;
+      d[t][i] = d[t][i] * inv_l - mul * o[t][i];
+      y[i] = t == 0 ? o[t][i] : y[i] - lam * o[t][i];
+      dy[i] = t == 0 ? d[t][i] : dy[i] - lam * d[t][i];
     }
-    if (map == 1 && p.o2) store_out8(p, 1, off, o);
-    if (p.lse && col == 0)
-      p.lse[((int64_t)b * 2 * p.H + 2 * h + map) * p.L + q_row] = m + __logf(l);
+    if (p.lse && col == 0) p.lse[((int64_t)b * 2 * p.H + 2 * h + t) * p.L + q_row] = m[t] + __logf(l[t]);
   }
+  if (p.o2) store_out8(p, 1, off, o[1]);
   store_out8(p, 0, off, y);
   if (TANGENT)
     *reinterpret_cast<uint4*>(p.dout + off) =
@@ -985,9 +1005,19 @@ static size_t scratch_floats(int G, bool split) {
   return (TANGENT ? (size_t)G * HOLD : 0) + (split ? (size_t)G * 2 * Rec<TANGENT>::ALL : 0);
 }
 
+// CTAs.  Fewer items than SMs: shares of at least two K/V tiles, if that shortens a CTA's walk by more than the
+// second kernel, the partial results and the second segment cost: 12 us at 148 CTAs (16 tiles of 0.74 us) or 16
+// (11 of 1.54) with a tangent, less with fewer records.  Measured whole / in shares, us, pairs of one batch
+// entry: 532 rows, 2 pairs 14.8 / 18.5 and 31.1 / 29.2; 1,100 rows, 2 pairs 21.7 / 23.7 and 45 / 34; 1,500
+// rows, 3 pairs 27.1 / 25.8 and 55 / 42; 4,116 rows, 1 pair 56 / 33 and 117 / 56.
 template <bool TANGENT>
 static int grid(const FwdShares& sh) {
-  return fwd_grid(sh.n_items, sh.n_kv, Rec<TANGENT>::PART_COST);
+  const int sms = fwd_sm_count();
+  if (sh.n_items >= sms) return sms;
+  const long g = sh.total / 2 < sms ? sh.total / 2 : sms;
+  if (g <= sh.n_items) return sh.n_items;
+  const float saved = (float)(sh.n_kv - (sh.total + g - 1) / g);
+  return saved < (TANGENT ? 5.f : 10.5f) + 0.04f * (float)g ? sh.n_items : (int)g;
 }
 
 }  // namespace diff
