@@ -415,8 +415,8 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&s.p_ready);
-      // dS^T = P^T .* (dP^T - delta), the bracket straight from the tensor core: to TMEM for dK and to shared memory for dQ (dP^T was issued behind
-      // the dQ product of the previous step)
+      // dS^T = P^T .* (dP^T - delta), the bracket straight from the tensor core: to TMEM for dK and to shared
+      // memory for dQ (dP^T was issued behind the dQ product of the previous step)
       ok = __all_sync(0xffffffffu, mbar_wait(&s.dp_full, par, abort_flag, p.status, STATUS_TIMEOUT_MMA));
       if (!ok) break;
       tc_fence_after();
@@ -496,8 +496,7 @@ __global__ void attn_diff_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, c
                                           const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse,
                                           const DiffWeights lam, uint4* __restrict__ band, float* __restrict__ delta2,
                                           float* __restrict__ dq_acc, int B, int L, int H, int Lp, int64_t o_sb,
-                                          int64_t o_sl, int64_t o_sh, 
-                                          int64_t g_sb, int64_t g_sl, int64_t g_sh,
+                                          int64_t o_sl, int64_t o_sh, int64_t g_sb, int64_t g_sl, int64_t g_sh,
                                           float inv_exp_scale) {
   const int lane = threadIdx.x & 31, part = lane & 15, c = (part & 7) * 8;
   const long u = (((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5) * 2 + (lane >> 4);
@@ -535,8 +534,9 @@ __global__ void attn_diff_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, c
   if (!in || part >= 2) return;
   const long row = ((long)b * 2 * H + 2 * h + part) * Lp + l;
   float x = live ? lse[((long)b * 2 * H + 2 * h + part) * L + l] * LOG2E : 0.f;
-  // (infinities become what is still finite over the smallest scale, 1e-30)
-  x = -(live ? fminf(fmaxf(x, -1e8f), 1e8f) : 30000.f) * inv_exp_scale;
+  // (infinities become what is still finite over the smallest scale, 1e-30; NaN stays)
+  if (x == x) x = fminf(fmaxf(x, -1e8f), 1e8f);
+  x = -(live ? x : 30000.f) * inv_exp_scale;
   const float y = live ? -(part ? d2 : fmaf(lam.at(h), d2, d)) : 0.f;
   const float x1 = bf16_lo(pack_bf16(x, 0.f)), x2 = bf16_lo(pack_bf16(x - x1, 0.f));
   const float y1 = bf16_lo(pack_bf16(y, 0.f)), y2 = bf16_lo(pack_bf16(y - y1, 0.f));
@@ -651,14 +651,17 @@ extern "C" long imf_attn_diff_bwd_scratch_bytes(int B, int L, int H) {
 // bytes (`plane` apart) and lse as imf_attn_diff_fwd wrote them; dq contiguous, dk and dv with strides of their own;
 // dlam: H values, in the type of lam.  All with 16-byte aligned rows.
 extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, const void* o, const void* o2,
-                                 const void* low, int64_t plane, const void* d_o, const float* lse, const void* lam, int64_t lam_stride, int lam_bf16,
-                                 void* dq, void* dk, void* dv, void* dlam, int B, int L, int H, const int64_t* strides,
+                                 const void* low, int64_t plane, const void* d_o, const float* lse, const void* lam,
+                                 int64_t lam_stride, int lam_bf16, void* dq, void* dk, void* dv, void* dlam, int B, int L, int H, const int64_t* strides,
                                  const int64_t* o_strides, const int64_t* dk_strides, const int64_t* dv_strides,
                                  float scale, void* scratch, long scratch_bytes, int fixed_order, int* status,
                                  void* stream) {
   using namespace imf;
   using namespace imf::diffb;
-  if (!q || !k || !v || !o || !o2 || !low || (reinterpret_cast<uintptr_t>(low) & 7) || (plane & 7) || !d_o || !lse || !lam || !dq || !dk || !dv || !dlam) return IMF_ERR_ARG;
+  for (const void* x : {q, k, v, o, o2, low, d_o, (const void*)lse, lam, (const void*)dq, (const void*)dk, (const void*)dv,
+                        (const void*)dlam})
+    if (!x) return IMF_ERR_ARG;
+  if ((reinterpret_cast<uintptr_t>(low) & 7) || (plane & 7)) return IMF_ERR_ARG;
   if (B <= 0 || L <= 0 || H <= 0 || !(scale > 0.f) || scale > 1e30f) return IMF_ERR_ARG;
   if ((long)B * H * ((L + T - 1) / T) > 0x3fffffffL) return IMF_ERR_TOO_LARGE;
   const BwdSplit sp = split_for(B, L, H);
@@ -681,9 +684,9 @@ extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, co
   typedef const __nv_bfloat16 cbf;
   const long threads = (long)B * H * Lp * 16;
   attn_diff_bwd_prep_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(
-      static_cast<cbf*>(o), static_cast<cbf*>(o2), static_cast<const uint8_t*>(low), plane, static_cast<cbf*>(d_o), lse, w, band, delta2, dq_acc, B, L, H, Lp,
-      o_strides[0], o_strides[1], o_strides[2], strides[9], strides[10],
-      strides[11], 1.f / (scale * LOG2E));
+      static_cast<cbf*>(o), static_cast<cbf*>(o2), static_cast<const uint8_t*>(low), plane, static_cast<cbf*>(d_o), lse, w,
+      band, delta2, dq_acc, B, L, H, Lp, o_strides[0], o_strides[1], o_strides[2], strides[9], strides[10], strides[11],
+      1.f / (scale * LOG2E));
   if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
   CUtensorMap mq, mk, mv, mdo, mdq, mb;
   int rc;

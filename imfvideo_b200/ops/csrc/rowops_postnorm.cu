@@ -139,6 +139,7 @@ struct Ring {
   __device__ __forceinline__ const uint8_t* row() const { return buf + (size_t)st * row_bytes; }
   // every warp of the group has the row in registers: its place goes to the row `stages` further
   __device__ __forceinline__ void pass() {
+    if (W == 1) __syncwarp();            // (a row's sum over several warps has a barrier)
     ask(st);
     if (++st == stages) {
       st = 0;
@@ -469,7 +470,8 @@ extern "C" int imf_colsum(const void* entries, int n, void* stream);
 // addresses 16-byte aligned; y, dy, n, dn, gn, g_y bf16 or (y_fp32) fp32, the rest fp32.
 extern "C" int imf_norm_add_norm(void** p, int rows, int D, float eps, int y_fp32, int mode, int* status, void* stream) {
   using namespace imf;
-  if (rows <= 0 || D <= 0 || D % 8 || D > 8192 || mode < 0 || mode > 2) return IMF_ERR_ARG;
+  // (a row's number, and that of a row some steps further, in 32 bits)
+  if (rows <= 0 || rows >= 1 << 30 || D <= 0 || D % 8 || D > 8192 || mode < 0 || mode > 2) return IMF_ERR_ARG;
   for (int i = 0; i < 18; ++i)
     if (reinterpret_cast<uintptr_t>(p[i]) & 15) return IMF_ERR_ARG;
   if (!p[2] || !p[4] || !p[5] || (p[6] && !p[0])) return IMF_ERR_ARG;

@@ -22,7 +22,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import cuda as _cuda
-from .act8 import _apart, _elsewhere, _in_one_place, _new, _places, _same_device
+from .act8 import _apart, _elsewhere, _in_one_place, _new, _places, _same_device, _span
 from .dual import Dual
 
 Tensor = torch.Tensor
@@ -104,6 +104,12 @@ def _like(t: Tensor) -> Tensor:
     return torch.empty_like(t) if t.is_contiguous() else _new(t.shape, t.dtype, t.device)
 
 
+def _meet(a: Tensor, b: Tensor) -> bool:
+    """Whether the stretches of memory from the first to the last byte of two tensors meet."""
+    (a0, a1), (b0, b1) = _span(a), _span(b)
+    return a0 < b1 and b0 < a1
+
+
 def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Tensor] = None,
                   dk: Optional[Tensor] = None, dv: Optional[Tensor] = None, scale: Optional[float] = None,
                   need_bwd: bool = True) -> Tuple[Tensor, Optional[Tensor], tuple]:
@@ -168,7 +174,7 @@ def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved
             raise ValueError("diff_attn_bwd: the dv output needs 16-byte aligned rows")
         if not _apart(*_places(gv_out)):
             raise ValueError("diff_attn_bwd: no two elements of the dv output in one place")
-        if any(_apart(*_places(t)) and _in_one_place(gv_out, t) for t in (q, k, v, go)):
+        if any(_in_one_place(gv_out, t) if _apart(*_places(t)) else _meet(gv_out, t) for t in (q, k, v, go)):
             raise ValueError("diff_attn_bwd: the dv output lies over an input")
     if _elsewhere(dev):
         with torch.cuda.device(dev):

@@ -3,8 +3,8 @@
     x = res_scale * res + gate * post * y / rms(y),    n = pre * x / rms(x)
 
 ``ops.dual.norm_add_norm`` is the entry point for models (dual numbers, any device);
-``norm_add_norm_fwd`` / ``norm_add_norm_bwd`` are the launches.  Rows are all leading dimensions; D a
-multiple of 8 up to 8,192; y and n bf16 or fp32 (one type), the residual stream and the learned vectors
+``norm_add_norm_fwd`` / ``norm_add_norm_bwd`` are the launches.  Rows are all leading dimensions, fewer than
+2^30; D a multiple of 8 up to 8,192; y and n bf16 or fp32 (one type), the residual stream and the learned vectors
 fp32.  Launches go to the current stream of the tensors' device; workspaces belong to the call.  The
 reference norms a branch's input only (reference ``models/imf_dit_video.py:909-972``).
 """
@@ -23,7 +23,7 @@ from .dual import Dual
 
 Tensor = torch.Tensor
 BF16, F32 = torch.bfloat16, torch.float32
-MAX_WIDTH = 8192
+MAX_WIDTH, MAX_ROWS = 8192, 1 << 30
 _PTRS = ctypes.c_void_p * 18
 _KERNELS = None
 
@@ -67,8 +67,9 @@ def _prepare(what: str, y, vectors, streams, likes):
     of y's shape."""
     shape, yt, dev = y.shape, y.dtype, y.device
     if (yt is not BF16 and yt is not F32) or not shape or shape[-1] % 8 or not 0 < shape[-1] <= MAX_WIDTH or \
-            y.numel() // shape[-1] >= 1 << 31:
-        raise ValueError(f"{what}: y bf16 or fp32 with a multiple of 8 up to {MAX_WIDTH} channels, not {yt} {tuple(shape)}")
+            y.numel() // shape[-1] >= MAX_ROWS:
+        raise ValueError(f"{what}: y bf16 or fp32 with a multiple of 8 up to {MAX_WIDTH} channels and fewer than 2^30 "
+                         f"rows, not {yt} {tuple(shape)}")
     for want, dtype, ts in ((shape[-1:], F32, vectors), (shape, F32, streams), (shape, yt, likes)):
         for t in ts:
             if t is not None and (t.dtype is not dtype or t.shape != want or t.device != dev):

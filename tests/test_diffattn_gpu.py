@@ -104,13 +104,9 @@ def test_forward(B, L, H):
     assert torch.equal(o_only[0], o) and o_only[1:] == (None, ())
 
 
-@pytest.mark.parametrize("B,L,H", SHAPES)
-def test_tangent(B, L, H):
-    q, k, v, lam, tan = _inputs(B, L, H, seed=L, tangent=True)
-    o, do, saved = _own(q, k, v, lam, tan)
-    A, O, want, e, e2 = _forward64(q, k, v, lam)
-    _within(_wide(o), want, e, "o")
-    _within(_wide(saved[0]), O[:, :, 1], e2, "o2")
+def _tangent64(q, k, v, lam, tan):
+    """do and its bound."""
+    A, O, *_ = _forward64(q, k, v, lam)
     dq, dk, dv = tan
     dS = (_pairs(dq) @ _pairs(k).transpose(-1, -2) + _pairs(q) @ _pairs(dk).transpose(-1, -2)) * 0.125
     V, dV = _wide(v)[:, :, None], _wide(dv)[:, :, None]
@@ -120,7 +116,17 @@ def test_tangent(B, L, H):
     b = T.abs() @ V.abs() + A @ dV.abs() + mu.abs() * (A @ V.abs())
     w = lam.double()[None, :, None, None]
     dwant = dO[:, :, 0] - w * dO[:, :, 1]
-    _within(_wide(do), dwant, SLACK * U * (b[:, :, 0] + w.abs() * b[:, :, 1]) + U * dwant.abs() + 1e-6, "do")
+    return dwant, SLACK * U * (b[:, :, 0] + w.abs() * b[:, :, 1]) + U * dwant.abs() + 1e-6
+
+
+@pytest.mark.parametrize("B,L,H", SHAPES)
+def test_tangent(B, L, H):
+    q, k, v, lam, tan = _inputs(B, L, H, seed=L, tangent=True)
+    o, do, saved = _own(q, k, v, lam, tan)
+    A, O, want, e, e2 = _forward64(q, k, v, lam)
+    _within(_wide(o), want, e, "o")
+    _within(_wide(saved[0]), O[:, :, 1], e2, "o2")
+    _within(_wide(do), *_tangent64(q, k, v, lam, tan), "do")
 
 
 def _backward64(q, k, v, lam, go, scale=0.125):
@@ -253,6 +259,97 @@ def test_infinite_and_nan_values_stay_in_their_row():
     assert torch.equal(o[0, rows], clean[0, rows]) and o[0, 17].isnan().all()
 
 
+def test_nan_keys_give_nan_gradients_to_their_pair_alone():
+    from imfvideo_b200.ops import diffattn as DA
+
+    q, k, v, lam, go = _inputs(1, 100, 2, seed=2)            # one K/V tile: dq has one order
+    clean = DA.diff_attn_bwd(q, k, v, lam, *_own(q, k, v, lam)[::2], go)
+    bad = k.clone()
+    bad[0, 17, 0, 5] = float("nan")
+    got = DA.diff_attn_bwd(q, bad, v, lam, *_own(q, bad, v, lam)[::2], go)
+    for a, b in zip(got[:3], clean[:3]):
+        assert a[:, :, 0].isnan().all() and torch.equal(a[:, :, 2:], b[:, :, 2:])
+    assert got[3][1] == clean[3][1]
+
+
+def _room(gb):
+    free = torch.cuda.mem_get_info()[0] + torch.cuda.memory_reserved() - torch.cuda.memory_allocated()
+    if free < gb * 1e9:
+        pytest.skip(f"{gb} GB of device memory")
+
+
+@pytest.mark.parametrize("dim", [0, 1])
+def test_strides_past_32_bits(dim):
+    """Bands of one buffer whose batches (or rows) are so far apart that offsets need 64 bits."""
+    from imfvideo_b200.ops import diffattn as DA
+
+    B, L, H = 2, 70, 1
+    ins = _inputs(B, L, H, seed=3)
+    n = (B, L)[dim] - 1
+    far = (2 ** 31 + 640) // n // 8 * 8 + 8                  # n strides of it pass 2^31 elements
+    _room(6 * far * n / 2 ** 31)
+    near = 640                                               # 2H heads of five tensors
+    buf = torch.empty(n * far + near * max(B, L) + 640, device="cuda", dtype=BF16)
+    st = (far, near) if dim == 0 else (near, far)
+    bands = [buf[i * 128:].as_strided((B, L, 2 * H, 64), (*st, 64, 1)) for i in range(5)]
+    q, k, v, go = (b.copy_(t) for b, t in zip(bands, (*ins[:3], ins[4])))
+    lam = ins[3]
+    o, _, saved = _own(q, k, v, lam)
+    want, _, want_saved = _own(*ins[:4])
+    assert torch.equal(o, want) and all(torch.equal(a, b) for a, b in zip(saved, want_saved))
+    got = DA.diff_attn_bwd(q, k, v, lam, o, saved, go, gv_out=bands[4])
+    assert got[2].data_ptr() == bands[4].data_ptr()
+    for a, b in zip(got, DA.diff_attn_bwd(*ins[:4], want, want_saved, ins[4])):
+        assert torch.equal(a, b)                             # (one K/V tile)
+
+
+def test_tensors_past_32_bits():
+    """More than 2^31 elements: the last batches agree with the formulas."""
+    from imfvideo_b200.ops import diffattn as DA
+
+    B, L, H = 65540, 128, 2
+    _room(70)
+    g = _gen(5)
+    q, k, v, go = (torch.randn(B, L, 2 * H, 64, device="cuda", dtype=BF16, generator=g) for _ in range(4))
+    lam = torch.tensor([0.4, 0.7], device="cuda")
+    tail = [t[-3:].clone() for t in (q, k, v)]
+    o, do, _ = _own(q, k, v, lam, (go, go, go), need_bwd=False)
+    _within(_wide(o[-3:]), *_forward64(*tail, lam)[2:4], "o")
+    _within(_wide(do[-3:]), *_tangent64(*tail, lam, (go[-3:],) * 3), "do")
+    del do
+    o, _, saved = _own(q, k, v, lam)
+    dq, dk, dv, _ = DA.diff_attn_bwd(q, k, v, lam, o, saved, go)
+    dlam = DA.diff_attn_bwd(*tail, lam, o[-3:], (saved[0][-3:], saved[1][:, -3:].contiguous(), saved[2][-3:]), go[-3:])[3]
+    _check_grads(*tail, lam, go[-3:], (dq[-3:], dk[-3:], dv[-3:], dlam))
+
+
+def test_two_graphs_at_once():
+    """Two captured calls of different sizes, with tangents, split items and gradients, replayed on two streams."""
+    from imfvideo_b200.ops import diffattn as DA
+
+    calls, graphs = [], []
+    for L, H in ((1100, 2), (1500, 1)):
+        q, k, v, lam, tan = _inputs(1, L, H, seed=L, tangent=True)
+        o, _, saved = _own(q, k, v, lam)
+
+        def call(q=q, k=k, v=v, lam=lam, tan=tan, o=o, saved=saved):
+            return (*_own(q, k, v, lam, tan, need_bwd=False)[:2], *DA.diff_attn_bwd(q, k, v, lam, o, saved, tan[0])[1:])
+        want = call()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            out = call()
+        calls.append((call, want, out))              # (call keeps its inputs alive)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for gr, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                gr.replay()
+    torch.cuda.synchronize()
+    for _, want, got in calls:
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_far_negative_scores():
     """lse of -400: the rows behind the last key must not turn infinite in the backward pass."""
     from imfvideo_b200.ops import diffattn as DA
@@ -360,6 +457,15 @@ def test_empty():
         assert dq.shape == z.shape and (dlam == 0).all() and dlam.shape == lam.shape
 
 
+def _dv_over_sliding_rows(lam, o, saved, go):
+    """q's rows lie over one another, and dv over them"""
+    from imfvideo_b200.ops import diffattn as DA
+
+    buf = torch.zeros(1, 100, 4, 64, device="cuda", dtype=BF16)
+    q = buf.as_strided(go.shape, (100 * 256, 64, 64, 1))
+    return DA.diff_attn_bwd(q, go, go, lam, o, saved, go, gv_out=buf[:, :40])
+
+
 def test_refusals():
     from imfvideo_b200.ops import diffattn as DA
 
@@ -377,6 +483,7 @@ def test_refusals():
            lambda: DA.diff_attn_bwd(q, k, v, lam, o, (o2.float(), low, lse), go),
            lambda: DA.diff_attn_bwd(q, k, v, lam, o, saved, go, gv_out=q[:, :1].expand_as(q)),
            lambda: DA.diff_attn_bwd(q, k, v, lam, o, saved, go, gv_out=v),
+           lambda: _dv_over_sliding_rows(lam, o, saved, go),
            lambda: DA.diff_attn_bwd(q, k, v, lam, o, saved, go, gv_out=torch.empty(
                1, 40, 4, 66, device="cuda", dtype=BF16)[..., :64])]
     for f in bad:

@@ -80,3 +80,11 @@ def test_refusals():
                 dict(res=v["res"][:1]), dict(res_scale=torch.ones((), dtype=F64))):
         with pytest.raises(ValueError):
             _call({**v, **bad})
+
+
+def test_row_numbers_have_32_bits():
+    from imfvideo_b200.ops import postnorm as PN
+
+    w = torch.empty(8, device="meta")
+    with pytest.raises(ValueError, match="2\\^30"):
+        PN.norm_add_norm_fwd(None, torch.empty(1 << 30, 8, device="meta"), w, w, 1e-5)

@@ -235,6 +235,54 @@ def test_streams_and_graph_replay():
     assert all(torch.equal(a, b) for a, b in zip(out, want[1]))
 
 
+def test_tensors_past_32_bits():
+    """More than 2^31 elements: the last rows agree with the formulas."""
+    from imfvideo_b200.ops import postnorm as PN
+
+    R, D = 262160, 8192
+    if torch.cuda.mem_get_info()[0] + torch.cuda.memory_reserved() - torch.cuda.memory_allocated() < 60e9:
+        pytest.skip("60 GB of device memory")
+    v, t, go = _inputs(20, D, True, True, True, seed=3)
+    big = lambda z: torch.zeros(R, D, device="cuda", dtype=z.dtype)
+    res, y, gx, gn = (big(z) for z in (v["res"], v["y"], go["gx"], go["gn"]))
+    for b, z in zip((res, y, gx, gn), (v["res"], v["y"], go["gx"], go["gn"])):
+        b[-20:] = z
+    args = (res, y, v["post"], v["gate"], EPS, v["r"], v["pre"])
+    x, n, _, _ = PN.norm_add_norm_fwd(*args)
+    _check_forward(v, None, (x[-20:], n[-20:], None, None))
+    assert not x[:-20].any() and not n[:-20].any()
+    del x, n
+    got = PN.norm_add_norm_bwd(*args, gx, gn)
+    _check_backward(v, go, (got[0][-20:], got[1][-20:], *got[2:]))
+
+
+def test_two_graphs_at_once():
+    """Two captured calls of different widths replayed on two streams."""
+    from imfvideo_b200.ops import postnorm as PN
+
+    calls, graphs = [], []
+    for R, D in ((700, 256), (300, 1536)):
+        v, t, go = _inputs(R, D, True, True, True, seed=D)
+        args = (v["res"], v["y"], v["post"], v["gate"], EPS, v["r"], v["pre"])
+
+        def call(args=args, t=t, go=go):
+            return (*PN.norm_add_norm_fwd(*args, t["dres"], t["dy"]), *PN.norm_add_norm_bwd(*args, go["gx"], go["gn"]))
+        want = call()
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            out = call()
+        calls.append((call, want, out))              # (call keeps its inputs alive)
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(5):
+        for gr, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                gr.replay()
+    torch.cuda.synchronize()
+    for _, want, got in calls:
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
 def test_types_that_have_no_kernel_take_the_formulas():
     from imfvideo_b200.ops import dual as D
 
