@@ -28,8 +28,8 @@ struct DiffWeights {
   }
 };
 
-// 2^x of two values, x up to 127, on the FMA units, for part of a tile's exponentials: the exponential unit takes four
-// values a clock and scheduler and would set the pace alone.  2^x = 2^n 2^f, n the nearest whole number (from the
+// 2^x of two values, x up to 127, on the FMA units, for part of a tile's exponentials (backward pass): the exponential
+// unit takes four values a clock and scheduler.  2^x = 2^n 2^f, n the nearest whole number (from the
 // low bits of x + 1.5 2^23) and f in [-1/2, 1/2], where a polynomial of degree 4 with p(0) = 1, fitted to the
 // smallest relative error, is off by at most 2.9e-6.  Below -126: 2^-126, which rounds away beside anything.  NaN
 // stays NaN (in every step: the factor 2^n is multiplied, not added to the exponent).

@@ -24,6 +24,17 @@
 // that are meant makes S^T - lse / scale and dP^T - delta.  Reading them from shared memory instead costs the
 // math warps 1,024 clocks of its 128 B a clock per step, every lane of a warp the same 16 bytes.
 // Shared memory: both K, V, two stages each of Q and dO, dS^T, half a dQ tile, bands and ones: 225 of 227 KB.
+//
+// Roundings: P^T and dS^T go to the tensor core in bf16 (each off by at most 2^-8 of its value); dP, delta,
+// the exponents and all sums are in 32 bits (delta and the log-sum-exp as three bf16 parts, 24 bits).
+//
+// What bounds it: shared memory moves 361 KB a step, 2,820 clocks at 128 B a clock, and a step takes some
+// 2,800 to 2,900; the tensor pipe is 69 % busy.  Measured, 1 x 7,820 rows, 8 pairs: 745 us (cold) to 817 in a loop,
+// with preparation and conversion 897; 1 x 29,140 rows, 2 pairs: 2.8 ms.  Before: row constants from shared
+// memory, all exponentials on their unit and whole dQ tiles behind a barrier of four warps 926 us; a quarter of the
+// exponentials on the FMA units 838 -> 817.  Slower: P^T and dS^T both over dP^T, with S^T a step ahead (1,130), dQ
+// added from registers (1,135).  Both maps at once on 64-row steps would need one dP^T and one dV, but each map has a delta
+// of its own, to be read from shared memory again: 346 KB for what are 361 now.
 #include "attn_bwd_split.h"
 #include "attn_diff.h"
 #include "common.cuh"
@@ -652,7 +663,8 @@ extern "C" long imf_attn_diff_bwd_scratch_bytes(int B, int L, int H) {
 // dlam: H values, in the type of lam.  All with 16-byte aligned rows.
 extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, const void* o, const void* o2,
                                  const void* low, int64_t plane, const void* d_o, const float* lse, const void* lam,
-                                 int64_t lam_stride, int lam_bf16, void* dq, void* dk, void* dv, void* dlam, int B, int L, int H, const int64_t* strides,
+                                 int64_t lam_stride, int lam_bf16, void* dq, void* dk, void* dv, void* dlam, int B,
+                                 int L, int H, const int64_t* strides,
                                  const int64_t* o_strides, const int64_t* dk_strides, const int64_t* dv_strides,
                                  float scale, void* scratch, long scratch_bytes, int fixed_order, int* status,
                                  void* stream) {

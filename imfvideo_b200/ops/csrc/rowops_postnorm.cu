@@ -15,6 +15,10 @@
 // 174 with one).  The backward pass makes x again from res and y, of which it needs both anyway, instead of
 // reading it.  Row sums add in a fixed order; column sums go through one partial row a CTA, added up in a fixed
 // order by imf_colsum.
+//
+// Measured, 32,780 x 1,024, bf16 branch, cold: forward 66 us (342 of 402 MB reach DRAM by the end: 5.2 TB/s, copy
+// 6.55), with tangent 138 (746 of 806 MB, 5.4 TB/s), gradients 103 (563 of 604 MB, 5.5 TB/s).  Fewer rows pay for
+// the chain of two or three row sums of each: 7,820 x 1,536 gradients 60 us, column sums included, for 216 MB.
 #include "common.cuh"
 #include "host_util.h"
 #include "rowops_common.cuh"
