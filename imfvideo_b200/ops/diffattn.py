@@ -165,8 +165,8 @@ def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved
         raise ValueError(f"diff_attn_bwd: lse has to be contiguous fp32 {(B, H2, L)}")
     if low.dtype is not torch.int8 or low.shape != (2, *shape) or not (low.is_contiguous() and o2.is_contiguous()):
         raise ValueError("diff_attn_bwd: saved has to be what diff_attn_fwd returned")
-    row, row3, row18 = _rows(shape)
-    dv_strides = row3
+    row = _rows(shape)[0]
+    dv_strides = None
     if gv_out is not None and 0 not in shape:
         st = [s if n > 1 else r for n, s, r in zip(shape, gv_out.stride(), row)]
         dv_strides = (ctypes.c_int64 * 3)(*st)
@@ -176,26 +176,40 @@ def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved
             raise ValueError("diff_attn_bwd: no two elements of the dv output in one place")
         if any(_in_one_place(gv_out, t) if _apart(*_places(t)) else _meet(gv_out, t) for t in (q, k, v, go)):
             raise ValueError("diff_attn_bwd: the dv output lies over an input")
+    return _backward(q, k, v, lam, o, saved, go, scale, gv_out, dv_strides)
+
+
+def _backward(q, k, v, lam, o, saved, go, scale, gv_out, dv_strides):
+    """``diff_attn_bwd`` of checked tensors; dv_strides None: those of a contiguous one."""
+    shape, dev = q.shape, q.device
     if _elsewhere(dev):
         with torch.cuda.device(dev):
-            return diff_attn_bwd(q, k, v, lam, o, saved, go, scale, gv_out)
+            return _backward(q, k, v, lam, o, saved, go, scale, gv_out, dv_strides)
+    B, L, H2, D = shape
+    o2, low, lse = saved
     dq, dk = _like(o2), _like(o2)
     dv = _like(o2) if gv_out is None else gv_out
     dlam = _new((H2 // 2,), lam.dtype, dev)
     if 0 in shape:
         return dq, dk, dv, dlam.zero_()
     K = _kernels()
+    row, row3, row18 = _rows(shape)
     (q_, k_, v_, g_), strides = _operands((q, k, v, go), row, row18)
     o = o.contiguous()
-    nscr = K._lib.imf_attn_diff_bwd_scratch_bytes(B, L, H2 // 2)
+    nscr = _scratch_bytes(B, L, H2 // 2)
     scr = _new(nscr, torch.uint8, dev)
     K._check(K._lib.imf_attn_diff_bwd(
         q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), o.data_ptr(), o2.data_ptr(), low.data_ptr(), o.numel(), g_.data_ptr(),
         lse.data_ptr(), lam.data_ptr(), lam.stride(0), lam.dtype is BF16, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-        dlam.data_ptr(), B, L, H2 // 2, strides, row3, row3, dv_strides, scale, scr.data_ptr(), nscr,
+        dlam.data_ptr(), B, L, H2 // 2, strides, row3, row3, dv_strides or row3, scale, scr.data_ptr(), nscr,
         bool(K.DETERMINISTIC), K.status_word(dev).data_ptr(), K._stream()), "imf_attn_diff_bwd")
     K.LAUNCHES.count += 3
     return dq, dk, dv, dlam
+
+
+@lru_cache(maxsize=64)
+def _scratch_bytes(B: int, L: int, H: int) -> int:
+    return _kernels()._lib.imf_attn_diff_bwd_scratch_bytes(B, L, H)
 
 
 class _DiffAttnFn(torch.autograd.Function):
@@ -207,17 +221,20 @@ class _DiffAttnFn(torch.autograd.Function):
         o, do, saved = diff_attn_fwd(q, k, v, lam, dq, dk, dv, scale, need_bwd)
         if need_bwd:
             ctx.save_for_backward(q, k, v, lam, o, *saved)
-            ctx.scale = scale
-        if do is None:
-            do = o.new_empty(0)
-        ctx.mark_non_differentiable(do)
+            ctx.scale = HEAD_DIM ** -0.5 if scale is None else float(scale)
+            ctx.set_materialize_grads(False)
+        if do is not None:
+            ctx.mark_non_differentiable(do)
         return o, do
 
     @staticmethod
     @once_differentiable
     def backward(ctx, go, _gdo):
+        if go is None:
+            return (None,) * 8
+        # (the forward pass has checked these, autograd gives a gradient of o's shape and type)
         q, k, v, lam, o, *saved = ctx.saved_tensors
-        return (*diff_attn_bwd(q, k, v, lam, o, saved, go, ctx.scale), None, None, None, None)
+        return (*_backward(q, k, v, lam, o, saved, go, ctx.scale, None, None), None, None, None, None)
 
 
 def diff_attention_dual(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[float] = None) -> Dual:
@@ -227,5 +244,5 @@ def diff_attention_dual(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[
         t = tuple(torch.zeros_like(p.p) if x is None else x for p, x in zip((q, k, v), t))
     if torch.is_grad_enabled() and (q.p.requires_grad or k.p.requires_grad or v.p.requires_grad or lam.requires_grad):
         o, do = _DiffAttnFn.apply(q.p, k.p, v.p, lam, *t, scale)
-        return Dual(o, None if t[0] is None else do)
+        return Dual(o, do)
     return Dual(*diff_attn_fwd(q.p, k.p, v.p, lam, *t, scale, need_bwd=False)[:2])

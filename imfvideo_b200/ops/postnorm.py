@@ -12,6 +12,7 @@ reference norms a branch's input only (reference ``models/imf_dit_video.py:909-9
 from __future__ import annotations
 
 import ctypes
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -106,8 +107,7 @@ def norm_add_norm_fwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tens
     rows = y.numel() // D
     if rows:
         K = _kernels()
-        p = K._ptr
-        ptrs = _PTRS(p(res), p(dres), p(y), p(dy), p(post), p(gate), p(res_scale), p(pre), p(x), p(dx), p(n), p(dn))
+        ptrs = _PTRS(*[0 if t is None else t.data_ptr() for t in (res, dres, y, dy, post, gate, res_scale, pre, x, dx, n, dn)])
         K._check(K._lib.imf_norm_add_norm(ptrs, rows, D, eps, yt is F32, dy is not None,
                                           K.status_word(dev).data_ptr(), K._stream()), "imf_norm_add_norm")
         K.LAUNCHES.count += 1
@@ -125,25 +125,28 @@ def norm_add_norm_bwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tens
     if (gn is None) != (pre is None) or (res_scale is not None and res is None):
         raise ValueError(f"{what}: gn and pre come together, res_scale with res")
     y, post, gate, res_scale, pre, res, gx, gn = _prepare(what, y, (post, gate, res_scale, pre), (res, gx), (gn,))
-    dev, yt = y.device, y.dtype
+    return _backward(res, y, post, gate, eps, res_scale, pre, gx, gn, want_g_res, raw)
+
+
+def _backward(res, y, post, gate, eps, res_scale, pre, gx, gn, want_g_res, raw):
+    """``norm_add_norm_bwd`` of checked and aligned tensors."""
+    dev, yt, D = y.device, y.dtype, y.shape[-1]
     if _elsewhere(dev):
         with torch.cuda.device(dev):
-            return norm_add_norm_bwd(res, y, post, gate, eps, res_scale, pre, gx, gn, want_g_res, raw)
-    D = y.shape[-1]
+            return _backward(res, y, post, gate, eps, res_scale, pre, gx, gn, want_g_res, raw)
     rows = y.numel() // D
     want_g_res = want_g_res and res is not None
     # without a second norm and a scale the residual's gradient is x's
     passed = want_g_res and pre is None and res_scale is None and gx is not None
     g_res = gx if passed else _like(y, F32) if want_g_res else None
     g_y = torch.empty_like(y)
-    part = sums = None
     if rows:
         K = _kernels()
-        p = K._ptr
-        part = _new((K._lib.imf_norm_add_norm_grid(rows, D), 4, D), F32, dev)
+        part = _new((_partial_rows(rows, D), 4, D), F32, dev)
         sums = None if raw else _new((4, D), F32, dev)
-        ptrs = _PTRS(p(res), None, p(y), None, p(post), p(gate), p(res_scale), p(pre), None, None, None, None, p(gx),
-                     p(gn), None if passed else p(g_res), p(g_y), p(part), p(sums))
+        ptrs = _PTRS(*[0 if t is None else t.data_ptr() for t in (
+            res, None, y, None, post, gate, res_scale, pre, None, None, None, None, gx, gn, None if passed else g_res, g_y,
+            part, sums)])
         K._check(K._lib.imf_norm_add_norm(ptrs, rows, D, eps, yt is F32, 2, K.status_word(dev).data_ptr(), K._stream()),
                  "imf_norm_add_norm")
         K.LAUNCHES.count += 1 if raw else 2
@@ -153,6 +156,11 @@ def norm_add_norm_bwd(res: Optional[Tensor], y: Tensor, post: Tensor, gate: Tens
         return g_res, g_y, part
     g_pre, g_r, g_gate, g_post = sums.unbind(0)
     return g_res, g_y, None if pre is None else g_pre, None if res_scale is None else g_r, g_gate, g_post
+
+
+@lru_cache(maxsize=64)
+def _partial_rows(rows: int, D: int) -> int:
+    return _kernels()._lib.imf_norm_add_norm_grid(rows, D)
 
 
 class _NormAddNormFn(torch.autograd.Function):
@@ -172,13 +180,13 @@ class _NormAddNormFn(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, gx, gn, _gdx, _gdn):
-        res, y, post, gate, res_scale, pre = ctx.saved_tensors
         if gx is None and gn is None:
             return (None,) * 9
-        if pre is not None and gn is None:
-            gn = torch.zeros_like(y)
-        g_res, g_y, g_pre, g_r, g_gate, g_post = norm_add_norm_bwd(
-            res, y, post, gate, ctx.eps, res_scale, pre, gx, gn, want_g_res=ctx.needs_input_grad[0])
+        # (the forward pass has checked these, autograd gives gradients of the outputs' shapes and types)
+        res, y, post, gate, res_scale, pre = map(_aligned, ctx.saved_tensors)
+        gn = None if pre is None else torch.zeros_like(y) if gn is None else _aligned(gn)
+        g_res, g_y, g_pre, g_r, g_gate, g_post = _backward(
+            res, y, post, gate, ctx.eps, res_scale, pre, _aligned(gx), gn, ctx.needs_input_grad[0], False)
         return g_res, g_y, g_post, g_gate, g_r, g_pre, None, None, None
 
 
