@@ -85,7 +85,7 @@ struct Params {
   int n_t, group;         // K/V tiles of a chain; chains that are worked on at a time (bwd_item)
   // the steps of each K/V tile from n_whole on are split over `parts` CTAs to even out the last wave
   // (attn_bwd_split.h); each writes fp32 partials to part[(tile - n_whole) * parts + r] =
-  // [dK_1 | dK_2 | dV] ([128][64], [128][64], [128][128], dK unscaled) and a second kernel adds them up
+  // [dK_1 | dK_2 | dV] ([128][64], [128][64], [128][128], dK unscaled) and the last kernel adds them up
   int n_whole, parts;
   float* part;
   // fixed-order dQ (null = arrival order): one counter per (batch, head, 32 query rows), zeroed before the
@@ -93,6 +93,7 @@ struct Params {
   int* turn;
 };
 constexpr size_t PART = (size_t)T * (2 * HD + VD);       // floats of a partial result
+static_assert(PART % (4 * 256) == 0, "blocks of the merge lie within a tile");
 
 // which of a row's pairs of columns take their exponentials on the FMA units
 __device__ __forceinline__ constexpr bool fma_pair(int i) { return (i & 3) == 1; }
@@ -556,45 +557,10 @@ __global__ void attn_diff_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, c
   if (part) delta2[((long)b * H + h) * Lp + l] = d2;
 }
 
-// dq = bf16(acc * scale); the last H blocks: dlam = -sum of delta_2, in a fixed order.
-__global__ void __launch_bounds__(256)
-attn_diff_bwd_post_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, long n4, float scale,
-                          const float* __restrict__ delta2, void* dlam, int dlam_bf16, int B, int H, int L, int Lp,
-                          unsigned n_conv) {
-  if (blockIdx.x < n_conv) {
-    const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= n4) return;
-    const float4 v = reinterpret_cast<const float4*>(acc)[i];
-    reinterpret_cast<uint2*>(dq)[i] = make_uint2(pack_bf16(v.x * scale, v.y * scale), pack_bf16(v.z * scale, v.w * scale));
-    return;
-  }
-  const int h = (int)(blockIdx.x - n_conv);
-  __shared__ double sum[256];
-  double t = 0.0;
-  for (int b = 0; b < B; ++b) {
-    const float* d = delta2 + ((long)b * H + h) * Lp;
-#pragma unroll 8
-    for (int l = threadIdx.x; l < L; l += 256) t += d[l];
-  }
-  sum[threadIdx.x] = t;
-  for (int k = 128; k > 0; k >>= 1) {
-    __syncthreads();
-    if (threadIdx.x < k) sum[threadIdx.x] += sum[threadIdx.x + k];
-  }
-  if (threadIdx.x == 0) {
-    if (dlam_bf16)
-      static_cast<__nv_bfloat16*>(dlam)[h] = __double2bfloat16(-sum[0]);
-    else
-      static_cast<float*>(dlam)[h] = (float)-sum[0];
-  }
-}
-
 // dK_m = scale * sum_r part[r].dK_m, dV = sum_r part[r].dV (fixed order) of the split K/V tiles.  One
-// thread per 4 channels of a row.
-__global__ void attn_diff_bwd_combine_kernel(const Params p, int n_split) {
+// thread (i) per 4 channels of a row.
+IMF_DEVICE void combine4(const Params& p, int i) {
   constexpr int TILE4 = (int)(PART / 4);
-  const int i = (int)(blockIdx.x * blockDim.x + threadIdx.x);
-  if (i >= n_split * TILE4) return;
   const int t = i / TILE4, e = (i % TILE4) * 4;           // e: first float of the thread in a partial result
   const bool is_dk = e < 2 * T * HD;
   const int e2 = is_dk ? e : e - 2 * T * HD;
@@ -617,6 +583,44 @@ __global__ void attn_diff_bwd_combine_kernel(const Params p, int n_split) {
   __nv_bfloat16* dst = is_dk ? p.dk + (int64_t)b * p.dk_sb + (int64_t)kv_row * p.dk_sl + (int64_t)head * p.dk_sh
                              : p.dv + (int64_t)b * p.dv_sb + (int64_t)kv_row * p.dv_sl + (int64_t)head * p.dv_sh;
   *reinterpret_cast<uint2*>(dst + c % HD) = make_uint2(pack_bf16(a.x * mul, a.y * mul), pack_bf16(a.z * mul, a.w * mul));
+}
+
+// What is left when the sums are there, in one launch, longest first: in H blocks dlam = -sum of delta_2, in a fixed
+// order; in n_merge the split K/V tiles; then dq = bf16(acc * scale).
+__global__ void __launch_bounds__(256)
+attn_diff_bwd_post_kernel(const float* __restrict__ acc, __nv_bfloat16* __restrict__ dq, long n4, float scale,
+                          const float* __restrict__ delta2, void* dlam, int dlam_bf16, int B, int H, int L, int Lp,
+                          int n_merge, const Params p) {
+  const int h = (int)blockIdx.x;
+  if (h >= H) {
+    if (h < H + n_merge) {
+      combine4(p, (h - H) * 256 + threadIdx.x);
+      return;
+    }
+    const long i = (long)(h - H - n_merge) * 256 + threadIdx.x;
+    if (i >= n4) return;
+    const float4 v = reinterpret_cast<const float4*>(acc)[i];
+    reinterpret_cast<uint2*>(dq)[i] = make_uint2(pack_bf16(v.x * scale, v.y * scale), pack_bf16(v.z * scale, v.w * scale));
+    return;
+  }
+  __shared__ double sum[256];
+  double t = 0.0;
+  for (int b = 0; b < B; ++b) {
+    const float* d = delta2 + ((long)b * H + h) * Lp;
+#pragma unroll 8
+    for (int l = threadIdx.x; l < L; l += 256) t += d[l];
+  }
+  sum[threadIdx.x] = t;
+  for (int k = 128; k > 0; k >>= 1) {
+    __syncthreads();
+    if (threadIdx.x < k) sum[threadIdx.x] += sum[threadIdx.x + k];
+  }
+  if (threadIdx.x == 0) {
+    if (dlam_bf16)
+      static_cast<__nv_bfloat16*>(dlam)[h] = __double2bfloat16(-sum[0]);
+    else
+      static_cast<float*>(dlam)[h] = (float)-sum[0];
+  }
 }
 
 static int make_map(CUtensorMap* m, const void* ptr, int B, int L, int heads, const int64_t* st) {
@@ -740,14 +744,9 @@ extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, co
   if (!allow_smem((const void*)attn_diff_bwd_kernel, sizeof(Smem), smem_set)) return IMF_ERR_LAUNCH;
   attn_diff_bwd_kernel<<<sp.ctas(), THREADS, sizeof(Smem), st>>>(mq, mk, mv, mdo, mdq, mb, prm);
   if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
-  if (sp.n_split) {
-    const long n = (long)sp.n_split * (long)(PART / 4);
-    attn_diff_bwd_combine_kernel<<<(unsigned)((n + 255) / 256), 256, 0, st>>>(prm, sp.n_split);
-    if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;
-  }
   const long n4 = (long)B * L * 2 * H * HD / 4;
-  const unsigned n_conv = (unsigned)((n4 + 255) / 256);
-  attn_diff_bwd_post_kernel<<<n_conv + H, 256, 0, st>>>(dq_acc, static_cast<__nv_bfloat16*>(dq), n4, scale, delta2, dlam,
-                                                        lam_bf16, B, H, L, Lp, n_conv);
+  const int n_merge = (int)(sp.n_split * (PART / 4 / 256));
+  attn_diff_bwd_post_kernel<<<(unsigned)(H + n_merge + (n4 + 255) / 256), 256, 0, st>>>(
+      dq_acc, static_cast<__nv_bfloat16*>(dq), n4, scale, delta2, dlam, lam_bf16, B, H, L, Lp, n_merge, prm);
   return cudaGetLastError() == cudaSuccess ? IMF_OK : IMF_ERR_LAUNCH;
 }
