@@ -17,8 +17,10 @@
 // order by imf_colsum.
 //
 // Measured, 32,780 x 1,024, bf16 branch, cold: forward 66 us (342 of 402 MB reach DRAM by the end: 5.2 TB/s, copy
-// 6.55), with tangent 138 (746 of 806 MB, 5.4 TB/s), gradients 103 (563 of 604 MB, 5.5 TB/s).  Fewer rows pay for
-// the chain of two or three row sums of each: 7,820 x 1,536 gradients 60 us, column sums included, for 216 MB.
+// 6.55), with tangent 138 (746 of 806 MB, 5.4 TB/s), gradients 103 (563 of 604 MB, 5.5 TB/s).  From 1,025
+// channels on an SM has two rows at a time, and a row of gradients takes 1.8 us whatever its width: 7,820 x 1,032 49 us,
+// 7,820 x 1,536 52 us, 20,000 x 2,048 130 us (5.7 TB/s); one exchange less between a row's warps, the next row's sum over y
+// going with this row's last, changes nothing there and costs the tangent 11 % at 2,048.  Column sums 4 to 6 us.
 #include "common.cuh"
 #include "host_util.h"
 #include "rowops_common.cuh"
