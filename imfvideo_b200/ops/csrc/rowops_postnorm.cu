@@ -18,12 +18,15 @@
 //
 // Measured, 32,780 x 1,024, bf16 branch, cold: forward 66 us (342 of 402 MB reach DRAM by the end: 5.2 TB/s, copy
 // 6.55), with tangent 138 (746 of 806 MB, 5.4 TB/s), gradients 103 (563 of 604 MB, 5.5 TB/s).  From 1,025
-// channels on an SM has two rows at a time, and a row of gradients takes 1.8 us whatever its width: 7,820 x 1,032 49 us,
-// 7,820 x 1,536 52 us, 20,000 x 2,048 130 us (5.7 TB/s); one exchange less between a row's warps, the next row's sum over y
-// going with this row's last, changes nothing there and costs the tangent 11 % at 2,048.  Column sums 4 to 6 us.
+// channels on a CTA has one row at a time, some 1.8 us each for gradients whatever its width, and fewer bytes on their way: 7,820
+// x 1,536 gradients 49 us, 4.4 TB/s; 20,000 x 2,048 130 us, 5.7 TB/s.  One exchange less between a row's warps, the
+// next row's sum over y going with this row's last, changes nothing there and costs the tangent 10 % at 2,048.
+// Column sums take 4 to 6 us more.
 #include "common.cuh"
 #include "host_util.h"
 #include "rowops_common.cuh"
+
+#include <type_traits>
 
 namespace imf {
 namespace pn {
@@ -75,7 +78,14 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const V8& a) {
 }
 __device__ __forceinline__ float sum2(f32x2 v) { return lo2(v) + hi2(v); }
 
-// Sums over a row, which W warps hold (group `g` of the CTA's ROW_WARPS / W; `slot` alternates, so that a
+// Warps of a CTA and CTAs of an SM.  From 1,025 channels on a CTA has one row at a time and as many warps as that takes;
+// where registers leave room (five warps, or six without column sums), three such CTAs share an SM.  7,820 rows forward
+// and gradients, against eight warps and two CTAs: 1,032 channels 33 -> 25 and 53 -> 39 us, 1,280 33 -> 29 and 53 -> 39,
+// 1,536 35 -> 31 and 56 -> 49, 1,792 the same.
+constexpr int cta_warps(int W) { return W > 4 ? W : ROW_WARPS; }
+constexpr int ctas(int NV, int W, bool bwd) { return NV > 1 ? 1 : W == 5 || (W == 6 && !bwd) ? 3 : 2; }
+
+// Sums over a row, which W warps hold (group `g` of the CTA's cta_warps(W) / W; `slot` alternates, so that a
 // sum's values are read before the one after the next is written).
 template <int W>
 struct RowSum {
@@ -158,7 +168,7 @@ struct Ring {
 constexpr int HEAD = ROW_WARPS * MAX_STAGES * 8 + 64;
 template <int W>
 __device__ __forceinline__ Ring<W> make_ring(uint8_t* smem, const Args& a, const Source& src) {
-  constexpr int GROUPS = ROW_WARPS / W;
+  constexpr int GROUPS = cta_warps(W) / W;
   const int warp = threadIdx.x >> 5, grp = warp / W;
   Ring<W> r;
   r.full = reinterpret_cast<uint64_t*>(smem) + grp * MAX_STAGES;
@@ -186,10 +196,10 @@ __device__ __forceinline__ Ring<W> make_ring(uint8_t* smem, const Args& a, const
 }
 
 template <typename TY, int NV, int W, bool T>
-__global__ void __launch_bounds__(ROW_THREADS, NV == 1 ? 2 : 1) fwd_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * cta_warps(W), ctas(NV, W, false)) fwd_kernel(const Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 red[2][ROW_WARPS];
-  constexpr int GROUPS = ROW_WARPS / W;
+  constexpr int GROUPS = cta_warps(W) / W;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float inv_d = 1.f / a.D;
   const uint32_t by = a.D * (uint32_t)sizeof(TY), bf = a.D * 4u;
@@ -275,10 +285,10 @@ __global__ void __launch_bounds__(ROW_THREADS, NV == 1 ? 2 : 1) fwd_kernel(const
 }
 
 template <typename TY, int NV, int W>
-__global__ void __launch_bounds__(ROW_THREADS, NV == 1 ? 2 : 1) bwd_kernel(const Args a) {
+__global__ void __launch_bounds__(32 * cta_warps(W), ctas(NV, W, true)) bwd_kernel(const Args a) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float2 red[2][ROW_WARPS];
-  constexpr int GROUPS = ROW_WARPS / W, COLS = NV * W * 256;
+  constexpr int GROUPS = cta_warps(W) / W, COLS = NV * W * 256;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, grp = warp / W;
   const float inv_d = 1.f / a.D;
   const bool need_res = a.res && (a.pre || a.r);
@@ -398,7 +408,7 @@ __global__ void __launch_bounds__(ROW_THREADS, NV == 1 ? 2 : 1) bwd_kernel(const
 #pragma unroll
       for (int e = 0; e < 4; ++e) reinterpret_cast<f32x2*>(flush + grp * COLS + col[i])[e] = acc[i].v[e];
     __syncthreads();
-    for (int c = threadIdx.x; c < a.D; c += ROW_THREADS) {
+    for (int c = threadIdx.x; c < a.D; c += 32 * cta_warps(W)) {
       float t = 0.f;
 #pragma unroll
       for (int k = 0; k < GROUPS; ++k) t += flush[k * COLS + c];
@@ -415,20 +425,17 @@ __global__ void __launch_bounds__(ROW_THREADS, NV == 1 ? 2 : 1) bwd_kernel(const
   write(c_s, 2);
 }
 
-// CTAs: every one of them works on rows from its start on, and the partial rows stay few.
-template <int W>
-static int grid(int rows, int ctas_per_sm) {
-  const int groups = ROW_WARPS / W, most = 148 * ctas_per_sm, want = (rows + groups - 1) / groups;
+// CTAs: every one of them works on rows from its start on, and the partial rows stay few.  (With four CTAs an SM of the
+// forward pass and three with tangent, fewer rows each on their way, 32,780 x 1,024 takes 89 and 161 us instead of 82
+// and 150.)
+static int grid(int rows, int groups, int ctas_per_sm) {
+  const int most = 148 * ctas_per_sm, want = (rows + groups - 1) / groups;
   return want < most ? want : most;
 }
 
-// CTAs per SM (from 2,049 channels on one: registers).  With four of the forward pass and three with tangent,
-// fewer rows each on their way, 32,780 x 1,024 takes 89 and 161 us instead of 82 and 150.
-static int ctas(int D) { return D <= 2048 ? 2 : 1; }
-
 template <typename TY, int NV, int W>
 static int launch(Args a, int mode, cudaStream_t st) {
-  const int per_sm = ctas(a.D), groups = ROW_WARPS / W;
+  const int per_sm = ctas(NV, W, mode == 2), groups = cta_warps(W) / W;
   const size_t ty = sizeof(TY);
   const size_t row = a.D * (mode == 0 ? ty + (a.res ? 4 : 0)
                             : mode == 1 ? 2 * ty + (a.res ? 4 : 0) + (a.dres ? 4 : 0)
@@ -442,18 +449,31 @@ static int launch(Args a, int mode, cudaStream_t st) {
   auto kern = mode == 0 ? fwd_kernel<TY, NV, W, false> : mode == 1 ? fwd_kernel<TY, NV, W, true> : bwd_kernel<TY, NV, W>;
   static bool smem_set[3][HOST_MAX_DEVICES] = {{false}};
   if (!allow_smem((const void*)kern, 225 * 1024, smem_set[mode])) return IMF_ERR_LAUNCH;
-  kern<<<grid<W>(a.rows, per_sm), ROW_THREADS, smem, st>>>(a);
+  kern<<<grid(a.rows, groups, per_sm), 32 * cta_warps(W), smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? IMF_OK : IMF_ERR_LAUNCH;
 }
 
+// f(chunks a lane, warps a row) for rows of D channels
+template <typename F>
+static int by_width(int D, F f) {
+  using std::integral_constant;
+  #define IMF_WIDTH(NV, W) \
+  if (D <= NV * W * 256) return f(integral_constant<int, NV>(), integral_constant<int, W>())
+  IMF_WIDTH(1, 1);
+  IMF_WIDTH(1, 2);
+  IMF_WIDTH(1, 4);
+  IMF_WIDTH(1, 5);
+  IMF_WIDTH(1, 6);
+  IMF_WIDTH(1, 7);
+  IMF_WIDTH(1, 8);
+  IMF_WIDTH(2, 8);
+  return f(integral_constant<int, 4>(), integral_constant<int, 8>());
+#undef IMF_WIDTH
+}
+
 template <typename TY>
-static int by_width(const Args& a, int mode, cudaStream_t st) {
-  if (a.D <= 256) return launch<TY, 1, 1>(a, mode, st);
-  if (a.D <= 512) return launch<TY, 1, 2>(a, mode, st);
-  if (a.D <= 1024) return launch<TY, 1, 4>(a, mode, st);
-  if (a.D <= 2048) return launch<TY, 1, 8>(a, mode, st);
-  if (a.D <= 4096) return launch<TY, 2, 8>(a, mode, st);
-  return launch<TY, 4, 8>(a, mode, st);
+static int run(const Args& a, int mode, cudaStream_t st) {
+  return by_width(a.D, [&](auto nv, auto w) { return launch<TY, nv.value, w.value>(a, mode, st); });
 }
 
 }  // namespace pn
@@ -462,10 +482,9 @@ static int by_width(const Args& a, int mode, cudaStream_t st) {
 // Partial rows of column sums that mode 2 of imf_norm_add_norm writes.
 extern "C" int imf_norm_add_norm_grid(int rows, int D) {
   using namespace imf::pn;
-  if (D <= 256) return grid<1>(rows, ctas(D));
-  if (D <= 512) return grid<2>(rows, ctas(D));
-  if (D <= 1024) return grid<4>(rows, ctas(D));
-  return grid<8>(rows, ctas(D));
+  return by_width(D, [&](auto nv, auto w) {
+    return grid(rows, cta_warps(w.value) / w.value, ctas(nv.value, w.value, true));
+  });
 }
 
 extern "C" int imf_colsum(const void* entries, int n, void* stream);
@@ -492,7 +511,7 @@ extern "C" int imf_norm_add_norm(void** p, int rows, int D, float eps, int y_fp3
   a.rows = rows; a.D = D; a.eps = eps;
   a.stages = 0; a.status = status;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int rc = y_fp32 ? pn::by_width<float>(a, mode, st) : pn::by_width<__nv_bfloat16>(a, mode, st);
+  const int rc = y_fp32 ? pn::run<float>(a, mode, st) : pn::run<__nv_bfloat16>(a, mode, st);
   if (rc != IMF_OK || mode != 2 || !p[17]) return rc;
   struct {
     const float* part;

@@ -15,7 +15,8 @@ U = {BF16: torch.finfo(BF16).eps / 2, F32: torch.finfo(F32).eps / 2}
 EPS, REL = 1e-5, 1e-5
 FORMS = [f for f in itertools.product([True, False], [True, False], [True, False]) if f[0] or not f[1]]
 SIZES = [(1, 8), (3, 64), (7, 256), (532, 256), (33, 264), (300, 512), (257, 520), (129, 1000), (64, 1024), (65, 1536),
-         (20, 2048), (9, 2056), (5, 4096), (5, 8192), (2500, 768)]
+         (20, 2048), (9, 2056), (5, 4096), (5, 8192), (2500, 768),
+         (450, 1032), (300, 1280), (450, 1288), (299, 1792), (20, 1800)]
 
 
 def _inputs(R, D, has_res, has_scale, has_pre, dtype=BF16, seed=0):
