@@ -50,33 +50,31 @@ __device__ __forceinline__ f32x2 ex2_mufu2(f32x2 x) {
   return pair2(__float_as_uint(ex2(lo2(x))), __float_as_uint(ex2(hi2(x))));
 }
 
-// Eight values as bf16 and what that dropped, and back.
+// Eight values as bf16 and what that dropped, and back.  The 32-bit patterns of a value and of its rounding differ by at
+// most 2^15 whatever the exponent: the byte is that difference over 2^8, rounded (2^7 at the largest: one less).
+// Infinities differ by nothing; whatever the byte of a NaN, the sum of both is one.
 __device__ __forceinline__ void diff_split8(const float* x, uint4& hi, uint2& low) {
-  uint32_t w[4], c[2] = {0u, 0u};
+  uint32_t w[4], c[2];
+  int t[8];
 #pragma unroll
   for (int i = 0; i < 8; i += 2) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(w[i / 2]) : "f"(x[i + 1]), "f"(x[i]));
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const uint32_t bits = u ? w[i / 2] & 0xffff0000u : w[i / 2] << 16;
-      // last place 2^(e - 134), e the exponent's field; below 2^-112 the codes are zero
-      const int e = max((int)((bits >> 23) & 255u), 15);
-      const int code = __float2int_rn((x[i + u] - __uint_as_float(bits)) * __uint_as_float((uint32_t)(269 - e) << 23));
-      c[(i + u) / 4] |= (uint32_t)(max(-127, min(127, code)) & 255) << (8 * ((i + u) & 3));
-    }
+    for (int u = 0; u < 2; ++u)
+      t[i + u] = min((int)(__float_as_uint(x[i + u]) - (u ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) + 128u), 0x7fff);
   }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)            // the second bytes of four
+    c[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0051), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0051), 0x5410);
   hi = make_uint4(w[0], w[1], w[2], w[3]);
   low = make_uint2(c[0], c[1]);
 }
 __device__ __forceinline__ void diff_join8(const uint4& hi, const uint2& low, float* x) {
   const uint32_t w[4] = {hi.x, hi.y, hi.z, hi.w}, c[2] = {low.x, low.y};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t bits = (i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16;
-    const int e = (int)((bits >> 23) & 255u), code = (int)(c[i / 4] << (24 - 8 * (i & 3))) >> 24;
-    const float step = e > 15 ? __uint_as_float((uint32_t)(e - 15) << 23) : 0.f;
-    x[i] = fmaf((float)code, step, __uint_as_float(bits));
-  }
+  for (int i = 0; i < 8; ++i)
+    x[i] = __uint_as_float(((i & 1) ? w[i / 2] & 0xffff0000u : w[i / 2] << 16) +
+                           (uint32_t)((int)(c[i / 4] << (24 - 8 * (i & 3))) >> 24 << 8));
 }
 
 }  // namespace imf
