@@ -504,7 +504,7 @@ attn_diff_bwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
 // Per (b, l, pair), 16 lanes of 8 channels: the bands of both maps (padding rows: the exponent -30000, so
 // P = 0), delta_2 for dlam, and zeros for the dQ additions.
 __global__ void attn_diff_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, const __nv_bfloat16* __restrict__ o2,
-                                          const uint8_t* __restrict__ low, int64_t plane,
+                                          const uint8_t* __restrict__ low,
                                           const __nv_bfloat16* __restrict__ d_o, const float* __restrict__ lse,
                                           const DiffWeights lam, uint4* __restrict__ band, float* __restrict__ delta2,
                                           float* __restrict__ dq_acc, int B, int L, int H, int Lp, int64_t o_sb,
@@ -527,8 +527,9 @@ __global__ void attn_diff_bwd_prep_kernel(const __nv_bfloat16* __restrict__ o, c
     const uint4 g = *reinterpret_cast<const uint4*>(d_o + b * g_sb + l * g_sl + head * g_sh + c);
     const uint32_t gw[4] = {g.x, g.y, g.z, g.w};
     float x[8], y[8];
-    diff_join8(*reinterpret_cast<const uint4*>(o + at), *reinterpret_cast<const uint2*>(low + at), x);
-    diff_join8(*reinterpret_cast<const uint4*>(o2 + at), *reinterpret_cast<const uint2*>(low + plane + at), y);
+    const uint4 lo = *reinterpret_cast<const uint4*>(low + 2 * at);
+    diff_join8(*reinterpret_cast<const uint4*>(o + at), make_uint2(lo.x, lo.y), x);
+    diff_join8(*reinterpret_cast<const uint4*>(o2 + at), make_uint2(lo.z, lo.w), y);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float ge = (i & 1) ? bf16_hi(gw[i / 2]) : bf16_lo(gw[i / 2]);
@@ -663,10 +664,10 @@ extern "C" long imf_attn_diff_bwd_scratch_bytes(int B, int L, int H) {
 }
 
 // q, k, v, d_o: (B, L, 2H, 64) bf16, (batch, row, head) element strides in strides[0..11]; o, o2 and their low
-// bytes (`plane` apart) and lse as imf_attn_diff_fwd wrote them; dq contiguous, dk and dv with strides of their own;
+// bytes and lse as imf_attn_diff_fwd wrote them; dq contiguous, dk and dv with strides of their own;
 // dlam: H values, in the type of lam.  All with 16-byte aligned rows.
 extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, const void* o, const void* o2,
-                                 const void* low, int64_t plane, const void* d_o, const float* lse, const void* lam,
+                                 const void* low, const void* d_o, const float* lse, const void* lam,
                                  int64_t lam_stride, int lam_bf16, void* dq, void* dk, void* dv, void* dlam, int B,
                                  int L, int H, const int64_t* strides,
                                  const int64_t* o_strides, const int64_t* dk_strides, const int64_t* dv_strides,
@@ -677,13 +678,12 @@ extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, co
   for (const void* x : {q, k, v, o, o2, low, d_o, (const void*)lse, lam, (const void*)dq, (const void*)dk, (const void*)dv,
                         (const void*)dlam})
     if (!x) return IMF_ERR_ARG;
-  if ((reinterpret_cast<uintptr_t>(low) & 7) || (plane & 7)) return IMF_ERR_ARG;
   if (B <= 0 || L <= 0 || H <= 0 || !(scale > 0.f) || scale > 1e30f) return IMF_ERR_ARG;
   if ((long)B * H * ((L + T - 1) / T) > 0x3fffffffL) return IMF_ERR_TOO_LARGE;
   const BwdSplit sp = split_for(B, L, H);
   const Layout y = layout(B, L, H, sp);
   if (scratch == nullptr || scratch_bytes < (long)y.all || (reinterpret_cast<uintptr_t>(scratch) & 255)) return IMF_ERR_ARG;
-  for (const void* x : {q, k, v, o, o2, d_o, (const void*)dq, (const void*)dk, (const void*)dv})
+  for (const void* x : {q, k, v, o, o2, low, d_o, (const void*)dq, (const void*)dk, (const void*)dv})
     if (reinterpret_cast<uintptr_t>(x) & 15) return IMF_ERR_ARG;
   for (int i = 0; i < 3; ++i)
     if ((dk_strides[i] & 7) || (dv_strides[i] & 7) || (o_strides[i] & 7) || (strides[9 + i] & 7))
@@ -700,7 +700,7 @@ extern "C" int imf_attn_diff_bwd(const void* q, const void* k, const void* v, co
   typedef const __nv_bfloat16 cbf;
   const long threads = (long)B * H * Lp * 16;
   attn_diff_bwd_prep_kernel<<<(unsigned)((threads + 255) / 256), 256, 0, st>>>(
-      static_cast<cbf*>(o), static_cast<cbf*>(o2), static_cast<const uint8_t*>(low), plane, static_cast<cbf*>(d_o), lse, w,
+      static_cast<cbf*>(o), static_cast<cbf*>(o2), static_cast<const uint8_t*>(low), static_cast<cbf*>(d_o), lse, w,
       band, delta2, dq_acc, B, L, H, Lp, o_strides[0], o_strides[1], o_strides[2], strides[9], strides[10], strides[11],
       1.f / (scale * LOG2E));
   if (cudaGetLastError() != cudaSuccess) return IMF_ERR_LAUNCH;

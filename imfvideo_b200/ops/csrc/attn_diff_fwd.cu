@@ -63,8 +63,7 @@ constexpr size_t HOLD = (size_t)TM * 2 * VD;      // floats a CTA holds of map 1
 
 struct Params {
   __nv_bfloat16 *o, *dout, *o2;      // o2: O_2 for the backward pass, or null
-  int8_t* low;                       // what bf16 dropped of o, then (plane elements on) of o2; null with o2
-  int64_t plane;
+  int8_t* low;                       // what bf16 dropped of eight channels of o, then of the same of o2; null with o2
   float* lse;                        // (B, 2H, L) or null
   float* scratch;                    // records of split items
   float* hold;                       // tangent: the held rows of map 1, HOLD a CTA
@@ -83,13 +82,16 @@ IMF_DEVICE void item_coords(const Params& p, int item, int& q0, int& h, int& b) 
   b = item / (p.n_qblk * p.H);
 }
 
-// Eight channels of o or (which = 1) O_2 at element `at`.
-IMF_DEVICE void store_out8(const Params& p, int which, int64_t at, const float* x) {
+// Eight channels of o and, where they are kept, of O_2 (z) at element `at`, with the bytes that both lost.
+IMF_DEVICE void store_out8(const Params& p, int64_t at, const float* y, const float* z) {
   uint4 hi;
-  uint2 low;
-  diff_split8(x, hi, low);
-  *reinterpret_cast<uint4*>((which ? p.o2 : p.o) + at) = hi;
-  if (p.low) *reinterpret_cast<uint2*>(p.low + which * p.plane + at) = low;
+  uint2 ly, lz;
+  diff_split8(y, hi, ly);
+  *reinterpret_cast<uint4*>(p.o + at) = hi;
+  if (!p.o2) return;
+  diff_split8(z, hi, lz);
+  *reinterpret_cast<uint4*>(p.o2 + at) = hi;
+  *reinterpret_cast<uint4*>(p.low + 2 * at) = make_uint4(ly.x, ly.y, lz.x, lz.y);
 }
 
 // The row's reference maximum as step `n` of its map left it goes to the warp of the other group in one
@@ -421,15 +423,13 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           tmem_ld8(tq + P_MAP + P_COL_O + t * HD + g * 32 + c, e);
           tc_wait_ld();
           if (live) {
-            float r[8];
+            float y[8], z[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(a[u]) * w1 - __uint_as_float(e[u]) * w2;
-            store_out8(p, 0, off + c, r);
-            if (p.o2) {
-#pragma unroll
-              for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(e[u]) * inv_l2;
-              store_out8(p, 1, off + c, r);
+            for (int u = 0; u < 8; ++u) {
+              y[u] = __uint_as_float(a[u]) * w1 - __uint_as_float(e[u]) * w2;
+              z[u] = __uint_as_float(e[u]) * inv_l2;
             }
+            store_out8(p, off + c, y, z);
           }
         }
         if (live && p.lse && g == 0)
@@ -865,15 +865,13 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             } else if (live) {
 #pragma unroll
               for (int i = 0; i < 32; i += 8) {
-                float r[8];
-                if (p.o2) {
+                float r[8], z[8];
 #pragma unroll
-                  for (int u = 0; u < 8; ++u) r[u] = __uint_as_float(ov[i + u]);
-                  store_out8(p, 1, off + c + i, r);
+                for (int u = 0; u < 8; ++u) {
+                  z[u] = __uint_as_float(ov[i + u]);
+                  r[u] = ho[(i + u) * TM] - lam * z[u];
                 }
-#pragma unroll
-                for (int u = 0; u < 8; ++u) r[u] = ho[(i + u) * TM] - lam * __uint_as_float(ov[i + u]);
-                store_out8(p, 0, off + c + i, r);
+                store_out8(p, off + c + i, r, z);
 #pragma unroll
                 for (int u = 0; u < 8; ++u) r[u] = hd[(i + u) * TM] - lam * __uint_as_float(dv_[i + u]);
                 *reinterpret_cast<uint4*>(p.dout + off + c + i) =
@@ -986,8 +984,7 @@ __global__ void __launch_bounds__(32 * VD / COMBINE_COLS) attn_diff_combine_kern
     }
     if (p.lse && col == 0) p.lse[((int64_t)b * 2 * p.H + 2 * h + t) * p.L + q_row] = m[t] + __logf(l[t]);
   }
-  if (p.o2) store_out8(p, 1, off, o[1]);
-  store_out8(p, 0, off, y);
+  store_out8(p, off, y, o[1]);
   if (TANGENT)
     *reinterpret_cast<uint4*>(p.dout + off) =
         make_uint4(pack_bf16(dy[0], dy[1]), pack_bf16(dy[2], dy[3]), pack_bf16(dy[4], dy[5]), pack_bf16(dy[6], dy[7]));
@@ -1045,10 +1042,11 @@ extern "C" long imf_attn_diff_fwd_scratch_bytes(int B, int L, int H, int tangent
 
 // q, k, v (, dq, dk, dv): (B, L, 2H, 64) bf16 with (batch, row, head) element strides in strides[0..17]; o, dout, o2
 // share (batch, row, head) strides o_strides; dout null without a tangent.  Where a backward pass follows: o2, lse
-// (B, 2H, L) and low, the bytes of o at o's strides and `plane` bytes on those of o2 (see attn_diff.h).  lam: H weights, lam_stride elements apart.
+// (B, 2H, L) and low, 16 bytes at twice o's offsets, of eight channels of o and then of o2 (see attn_diff.h).  lam: H
+// weights, lam_stride elements apart.
 extern "C" int imf_attn_diff_fwd(const void* q, const void* k, const void* v, const void* dq, const void* dk,
                                  const void* dv, const void* lam, int64_t lam_stride, int lam_bf16, void* o, void* dout,
-                                 void* o2, void* low, int64_t plane, float* lse, int B, int L, int H, const int64_t* strides,
+                                 void* o2, void* low, float* lse, int B, int L, int H, const int64_t* strides,
                                  const int64_t* o_strides, float scale, void* scratch, long scratch_bytes, int* status,
                                  void* stream) {
   using namespace imf;
@@ -1056,7 +1054,7 @@ extern "C" int imf_attn_diff_fwd(const void* q, const void* k, const void* v, co
   const bool tangent = dq != nullptr;
   if (!q || !k || !v || !lam || !o || B <= 0 || L <= 0 || H <= 0) return IMF_ERR_ARG;
   if (tangent != (dk != nullptr) || tangent != (dv != nullptr) || tangent != (dout != nullptr)) return IMF_ERR_ARG;
-  if ((o2 != nullptr) != (low != nullptr) || (reinterpret_cast<uintptr_t>(low) & 7) || (plane & 7)) return IMF_ERR_ARG;
+  if ((o2 != nullptr) != (low != nullptr) || (reinterpret_cast<uintptr_t>(low) & 15)) return IMF_ERR_ARG;
   if (!(scale > 0.f) || scale > 1e30f) return IMF_ERR_ARG;
   if ((long)B * H * ((L + TM - 1) / TM) > 0x3fffffffL) return IMF_ERR_TOO_LARGE;
   for (const void* x : {(const void*)o, (const void*)dout, (const void*)o2})
@@ -1068,7 +1066,6 @@ extern "C" int imf_attn_diff_fwd(const void* q, const void* k, const void* v, co
   prm.dout = static_cast<__nv_bfloat16*>(dout);
   prm.o2 = static_cast<__nv_bfloat16*>(o2);
   prm.low = static_cast<int8_t*>(low);
-  prm.plane = plane;
   prm.lse = lse;
   prm.lam = {lam, lam_stride, lam_bf16};
   prm.B = B; prm.H = H; prm.L = L;

@@ -46,9 +46,9 @@ def _kernels():
             getattr(lib, name).restype = cl
             getattr(lib, name).argtypes = [ci] * n
         lib.imf_attn_diff_fwd.restype = ci
-        lib.imf_attn_diff_fwd.argtypes = [vp] * 7 + [i64, ci] + [vp] * 4 + [i64, vp] + [ci] * 3 + [vp, vp, cf, vp, cl, vp, vp]
+        lib.imf_attn_diff_fwd.argtypes = [vp] * 7 + [i64, ci] + [vp] * 5 + [ci] * 3 + [vp, vp, cf, vp, cl, vp, vp]
         lib.imf_attn_diff_bwd.restype = ci
-        lib.imf_attn_diff_bwd.argtypes = [vp] * 6 + [i64] + [vp] * 3 + [i64, ci] + [vp] * 4 + [ci] * 3 + [vp] * 4 + [cf, vp, cl, ci, vp, vp]
+        lib.imf_attn_diff_bwd.argtypes = [vp] * 9 + [i64, ci] + [vp] * 4 + [ci] * 3 + [vp] * 4 + [cf, vp, cl, ci, vp, vp]
         _KERNELS = K
     return _KERNELS
 
@@ -76,6 +76,11 @@ def _rows(shape: Tuple[int, ...]):
     B, L, H, D = shape
     row = (L * H * D, H * D, D)
     return row, (ctypes.c_int64 * 3)(*row), (ctypes.c_int64 * 18)(*row * 6)
+
+
+@lru_cache(maxsize=64)
+def _scratch_bytes(which: str, *sizes: int) -> int:
+    return getattr(_kernels()._lib, f"imf_attn_diff_{which}_scratch_bytes")(*sizes)
 
 
 def _operands(tensors, row, six):
@@ -115,7 +120,7 @@ def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Ten
                   need_bwd: bool = True) -> Tuple[Tensor, Optional[Tensor], tuple]:
     """(o, do | None, saved) of (B, L, 2H, 64) bf16 CUDA tensors at any strides; lam (H,).  With tangents
     dq, dk, dv (all or none) also do.  ``need_bwd``: saved is what ``diff_attn_bwd`` takes, O_2 in bf16, the
-    bytes that o and O_2 lost when they were rounded (int8, two planes of o's shape) and the log-sum-exp
+    bytes that o and O_2 lost when they were rounded (int8, o's shape with twice the channels) and the log-sum-exp
     (B, 2H, L) of both maps; otherwise it is empty."""
     shape, tang = q.shape, dq is not None
     if (dk is None) == tang or (dv is None) == tang:
@@ -129,7 +134,7 @@ def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Ten
     B, L, H2, D = shape
     o = _like(q)
     do = _like(q) if tang else None
-    o2, low, lse = saved = (_like(q), _new((2, *shape), torch.int8, dev), _new((B, H2, L), F32, dev)) if need_bwd else (None,) * 3
+    o2, low, lse = saved = (_like(q), _new((B, L, H2, 2 * D), torch.int8, dev), _new((B, H2, L), F32, dev)) if need_bwd else (None,) * 3
     saved = saved if need_bwd else ()
     if 0 in shape:
         return o, do, saved
@@ -137,12 +142,12 @@ def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Ten
     row, row3, row18 = _rows(shape)
     ts, strides = _operands((q, k, v, dq, dk, dv) if tang else (q, k, v), row, row18)
     ptr = [t.data_ptr() for t in ts]
-    nscr = K._lib.imf_attn_diff_fwd_scratch_bytes(B, L, H2 // 2, tang)
+    nscr = _scratch_bytes("fwd", B, L, H2 // 2, tang)
     scr = _new(nscr, torch.uint8, dev) if nscr else None
     p = K._ptr
     K._check(K._lib.imf_attn_diff_fwd(
         *(ptr if tang else (*ptr, None, None, None)), lam.data_ptr(), lam.stride(0), lam.dtype is BF16, o.data_ptr(), p(do),
-        p(o2), p(low), o.numel(), p(lse), B, L, H2 // 2, strides, row3, scale, p(scr), nscr,
+        p(o2), p(low), p(lse), B, L, H2 // 2, strides, row3, scale, p(scr), nscr,
         K.status_word(dev).data_ptr(), K._stream()), "imf_attn_diff_fwd")
     K.LAUNCHES.count += 1
     return o, do, saved
@@ -163,7 +168,7 @@ def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved
     B, L, H2, D = shape
     if lse.dtype is not F32 or lse.shape != (B, H2, L) or not lse.is_contiguous():
         raise ValueError(f"diff_attn_bwd: lse has to be contiguous fp32 {(B, H2, L)}")
-    if low.dtype is not torch.int8 or low.shape != (2, *shape) or not (low.is_contiguous() and o2.is_contiguous()):
+    if low.dtype is not torch.int8 or low.shape != (B, L, H2, 2 * D) or not (low.is_contiguous() and o2.is_contiguous()):
         raise ValueError("diff_attn_bwd: saved has to be what diff_attn_fwd returned")
     row = _rows(shape)[0]
     dv_strides = None
@@ -196,20 +201,15 @@ def _backward(q, k, v, lam, o, saved, go, scale, gv_out, dv_strides):
     row, row3, row18 = _rows(shape)
     (q_, k_, v_, g_), strides = _operands((q, k, v, go), row, row18)
     o = o.contiguous()
-    nscr = _scratch_bytes(B, L, H2 // 2)
+    nscr = _scratch_bytes("bwd", B, L, H2 // 2)
     scr = _new(nscr, torch.uint8, dev)
     K._check(K._lib.imf_attn_diff_bwd(
-        q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), o.data_ptr(), o2.data_ptr(), low.data_ptr(), o.numel(), g_.data_ptr(),
+        q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), o.data_ptr(), o2.data_ptr(), low.data_ptr(), g_.data_ptr(),
         lse.data_ptr(), lam.data_ptr(), lam.stride(0), lam.dtype is BF16, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
         dlam.data_ptr(), B, L, H2 // 2, strides, row3, row3, dv_strides or row3, scale, scr.data_ptr(), nscr,
         bool(K.DETERMINISTIC), K.status_word(dev).data_ptr(), K._stream()), "imf_attn_diff_bwd")
     K.LAUNCHES.count += 3
     return dq, dk, dv, dlam
-
-
-@lru_cache(maxsize=64)
-def _scratch_bytes(B: int, L: int, H: int) -> int:
-    return _kernels()._lib.imf_attn_diff_bwd_scratch_bytes(B, L, H)
 
 
 class _DiffAttnFn(torch.autograd.Function):
