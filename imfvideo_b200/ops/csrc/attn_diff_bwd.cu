@@ -29,12 +29,13 @@
 // the exponents and all sums are in 32 bits (delta and the log-sum-exp as three bf16 parts, 24 bits).
 //
 // What bounds it: shared memory moves 361 KB a step, 2,820 clocks at 128 B a clock, and a step takes some
-// 2,800 to 2,900; the tensor pipe is 69 % busy.  Measured, 1 x 7,820 rows, 8 pairs: 745 us (cold) to 817 in a loop,
-// with preparation and conversion 897; 1 x 29,140 rows, 2 pairs: 2.8 ms.  Before: row constants from shared
+// 2,800 to 2,900; the tensor pipe is 69 % busy.  Measured, 1 x 7,820 rows, 8 pairs: 730 to 745 us, with
+// preparation and conversion 780; 1 x 29,140 rows, 2 pairs: 2.5 to 2.7 ms.  Before: row constants from shared
 // memory, all exponentials on their unit and whole dQ tiles behind a barrier of four warps 926 us; a quarter of the
-// exponentials on the FMA units 838 -> 817.  Slower: P^T and dS^T both over dP^T, with S^T a step ahead (1,130), dQ
-// added from registers (1,135).  Both maps at once on 64-row steps would need one dP^T and one dV, but each map has a delta
-// of its own, to be read from shared memory again: 346 KB for what are 361 now.
+// exponentials on the FMA units 838 -> 817.  Slower: P^T and dS^T both over dP^T, with S^T a step ahead (1,130); dQ
+// added from registers (1,135); V as dP^T's operand in TMEM, 329 KB a step, for which dQ has to lie over dP^T (798
+// for 780).  Both maps at once on 64-row steps would need one dP^T and one dV, but each map has a delta of its own,
+// to be read from shared memory again: 346 KB for what are 361 now.
 #include "attn_bwd_split.h"
 #include "attn_diff.h"
 #include "common.cuh"
