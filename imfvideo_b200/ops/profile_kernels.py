@@ -5,6 +5,8 @@ under ``ncu`` (or for a quick CUDA-event timing without it).
     python -m imfvideo_b200.ops.profile_kernels attn_jvp  --L 9472
     python -m imfvideo_b200.ops.profile_kernels attn_bwd  --L 4736
     python -m imfvideo_b200.ops.profile_kernels attn_jvp  --L 32780 --H 12 --hd 128
+    python -m imfvideo_b200.ops.profile_kernels diff_bwd  --L 7820 --H 16    # differential attention (diff_fwd, diff_jvp)
+    python -m imfvideo_b200.ops.profile_kernels post_norm_bwd --rows 29140 --D 256    # norms around a branch (post_norm, post_norm_jvp)
     python -m imfvideo_b200.ops.profile_kernels gemm      --M 58280 --N 528 --K 256
     python -m imfvideo_b200.ops.profile_kernels gemm_fp8  --M 65560 --N 4096 --K 1024   # e4m3 operands
     python -m imfvideo_b200.ops.profile_kernels sparse    --L 9472
@@ -50,7 +52,8 @@ def main() -> None:
     ap = argparse.ArgumentParser()
     ap.add_argument("kernel", choices=["attn_fwd", "attn_jvp", "attn_bwd", "gemm", "gemm_fp8", "sparse",
                                        "sparse_jvp", "resnorm", "resnorm_bwd", "lin", "route", "ns",
-                                       "qkprep_bwd"])
+                                       "qkprep_bwd", "diff_fwd", "diff_jvp", "diff_bwd", "post_norm",
+                                       "post_norm_jvp", "post_norm_bwd"])
     ap.add_argument("--L", type=int, default=9472)
     ap.add_argument("--B", type=int, default=1)
     ap.add_argument("--H", type=int, default=4)
@@ -85,6 +88,33 @@ def main() -> None:
         else:
             o, _, lse = K.attn_fwd(q, k, v)
             fn, flops = (lambda: K.attn_bwd(q, k, v, o, lse, dq)), 2.5 * base
+    elif args.kernel in ("diff_fwd", "diff_jvp", "diff_bwd"):
+        from . import diffattn as DA
+
+        q, k, v, dq, dk, dv = (mk() for _ in range(6))
+        lam = torch.rand(H // 2, device=dev)
+        base = 384.0 * B * H * L * L                  # two maps of 64 channels, values of 128, a pair
+        if args.kernel == "diff_fwd":
+            fn, flops = (lambda: DA.diff_attn_fwd(q, k, v, lam, need_bwd=False)), base
+        elif args.kernel == "diff_jvp":
+            fn, flops = (lambda: DA.diff_attn_fwd(q, k, v, lam, dq, dk, dv, need_bwd=False)), 3 * base
+        else:
+            o, _, saved = DA.diff_attn_fwd(q, k, v, lam)
+            fn, flops = (lambda: DA.diff_attn_bwd(q, k, v, lam, o, saved, dq)), base * 5 / 3
+    elif args.kernel.startswith("post_norm"):
+        from . import postnorm as PN
+
+        rows, D = args.rows, args.D
+        y, dy, gn = (torch.randn(rows, D, device=dev).bfloat16() for _ in range(3))
+        res, dres, gx = (torch.randn(rows, D, device=dev) for _ in range(3))
+        post, gate, keep, gain = (torch.randn(D, device=dev) for _ in range(4))
+        if args.kernel == "post_norm_bwd":
+            fn = lambda: PN.norm_add_norm_bwd(res, y, post, gate, 1e-5, keep, gain, gx, gn)
+            bytes_ = 18.0 * rows * D
+        else:
+            t = (dres, dy) if args.kernel == "post_norm_jvp" else ()
+            fn = lambda: PN.norm_add_norm_fwd(res, y, post, gate, 1e-5, keep, gain, *t)
+            bytes_ = 12.0 * rows * D * (2 if t else 1)
     elif args.kernel == "gemm":
         a = torch.randn(args.M, args.K, device=dev).bfloat16()
         b = torch.randn(args.N, args.K, device=dev).bfloat16()
