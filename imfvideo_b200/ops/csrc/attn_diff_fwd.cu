@@ -479,7 +479,10 @@ struct TSmem {
   alignas(1024) uint8_t v[T_VSTAGES][4][KPANEL];     // V, dV
   uint64_t m_ref[TM];       // reference maximum of the row as of the last step decided | that step's number
   float xst[2][3][TM];      // l, mu and reference maximum of either group, at a walk's end
-  uint64_t q_full[2], q_empty[2], q_ready;
+  uint64_t q_full[2], q_empty[2];
+  // Queries scaled, a barrier for each of the two walks: a group without a step in a walk of one tile scales the
+  // next walk's at once, and must not be counted for a warp that has not scaled its share of this one's.
+  uint64_t q_ready[2];
   uint64_t k_full[T_KSTAGES], k_empty[T_KSTAGES];
   uint64_t v_full[T_VSTAGES], v_empty[T_VSTAGES];
   uint64_t s_full[2], p_full[2];
@@ -531,11 +534,11 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
     for (int i = 0; i < 2; ++i) {
       mbar_init(&s.q_full[i], 1);
       mbar_init(&s.q_empty[i], 1);
+      mbar_init(&s.q_ready[i], SOFT_WARPS);
       mbar_init(&s.s_full[i], 1);
       mbar_init(&s.p_full[i], SOFT_WARPS / 2);
       mbar_init(&s.o_done[i], 1);
     }
-    mbar_init(&s.q_ready, SOFT_WARPS);
     mbar_init(&s.o_final, 1);
     mbar_init(&s.o_free, SOFT_WARPS);
     mbar_init(&s.sums, SOFT_WARPS);
@@ -628,7 +631,7 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
           const int n_j = sg.j1 - sg.j0;
           for (int m = 0; m < 2 && ok; ++m, ++walk) {
             const int qs = walk & 1;
-            ok = UNIT ? mbar_wait(&s.q_ready, walk & 1, abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX)
+            ok = UNIT ? mbar_wait(&s.q_ready[qs], (uint32_t)((walk >> 1) & 1), abort_flag, p.status, STATUS_TIMEOUT_SOFTMAX)
                       : mbar_wait(&s.q_full[qs], (uint32_t)((walk >> 1) & 1), abort_flag, p.status, STATUS_TIMEOUT_TMA);
             const uint64_t qd = q_desc + (uint32_t)(qs * (2 * QPANEL >> 4)), dqd = qd + (QPANEL >> 4);
             // scores of step jj of the walk
@@ -703,7 +706,7 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
                                              STATUS_TIMEOUT_TMA)))
         return false;
       scale_queries(s.q[w & 1], p.scale);
-      if (lane == 0) mbar_arrive(&s.q_ready);
+      if (lane == 0) mbar_arrive(&s.q_ready[w & 1]);
       return true;
     };
     Segment sg;
