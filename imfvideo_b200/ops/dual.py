@@ -19,6 +19,7 @@ from __future__ import annotations
 from typing import List, NamedTuple, Optional, Sequence
 
 import torch
+import torch.autograd.forward_ad as fwAD
 import torch.nn.functional as F
 
 from . import reference as ref
@@ -54,9 +55,13 @@ def _cuda_ops(x: Tensor):
 _modules: dict = {}
 
 
-def _kernel_module(name: str, x: Tensor):
-    """The module of kernels ``name`` for a CUDA tensor, None where the formulas run."""
-    if not x.is_cuda or torch._C._are_functorch_transforms_active():
+def _kernel_module(name: str, *operands: Optional[Tensor]):
+    """The module of kernels ``name`` where the first operand is a CUDA tensor, None where the formulas run: off the GPU,
+    and where torch differentiates forwards (a functorch transform, or an operand with a tangent of
+    ``torch.autograd.forward_ad``), which the launchers would not see."""
+    if not operands[0].is_cuda or torch._C._are_functorch_transforms_active():
+        return None
+    if fwAD._current_level >= 0 and any(t is not None and fwAD.unpack_dual(t).tangent is not None for t in operands):
         return None
     mod = _modules.get(name)
     if mod is None:
@@ -221,7 +226,7 @@ def diff_attention(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[float
         if lam.numel() != 1:
             raise ValueError(f"diff_attention: lam is {tuple(lam.shape)}, one weight or ({H},) expected")
         lam = lam.reshape(1).expand(H)
-    mod = _kernel_module("diffattn", q.p) if impl == "auto" else None
+    mod = _kernel_module("diffattn", q.p, k.p, v.p, lam) if impl == "auto" else None
     if mod is not None:
         return mod.diff_attention_dual(q, k, v, lam, scale)
     p = ref.diff_attention(q.p, k.p, v.p, lam, scale)
@@ -246,7 +251,7 @@ def norm_add_norm(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor, eps:
     this branch; ``res_scale`` None: 1.  x has the type of ``res`` (without one, 32 bits or y's), n
     ``out_dtype`` or y's.  CUDA: y bf16 or fp32 and res fp32 take one kernel a direction
     (``ops/postnorm.py``)."""
-    mod = _kernel_module("postnorm", y.p)
+    mod = _kernel_module("postnorm", y.p, post, gate, res_scale, pre, None if res is None else res.p)
     if mod is not None and mod.supported(y.p, torch.float32 if res is None else res.p.dtype, out_dtype, post, gate,
                                          res_scale, pre):
         return mod.norm_add_norm_dual(res, y, post, gate, eps, res_scale, pre)
