@@ -40,29 +40,24 @@ class DiffAttentionImpl(nn.Module):
 
 
 class DiffCore:
-    """Attention core for ``ops.block``: the forward and backward kernels.  The weights' gradient is added to
-    ``lam.grad`` (they are no input of the block's autograd node)."""
+    """Attention core for ``ops.block``: the forward and backward kernels, with the pairs' weights as an input of the
+    block's node."""
 
     def __init__(self, mod: DiffAttentionImpl):
-        self.mod = mod
+        self.params = (mod.lam,)
 
     def fwd(self, q, k, v, dq, dk, dv, need_bwd: bool):
         from ..ops import diffattn as DA
 
-        return DA.diff_attn_fwd(q, k, v, self.mod.lam.detach(), dq, dk, dv, need_bwd=need_bwd)
+        lam, = self.params
+        o, do, saved = DA.diff_attn_fwd(q, k, v, lam, dq, dk, dv, need_bwd=need_bwd)
+        return o, do, (lam, *saved)
 
     def bwd(self, q, k, v, o, saved, go, gv_out: Optional[Tensor] = None):
         from ..ops import diffattn as DA
 
-        lam = self.mod.lam
-        with torch.no_grad():
-            gq, gk, gv, glam = DA.diff_attn_bwd(q, k, v, lam.detach(), o, saved, go, gv_out=gv_out)
-            if lam.requires_grad:
-                if lam.grad is None:
-                    lam.grad = glam
-                else:
-                    lam.grad.add_(glam)
-        return gq, gk, gv
+        lam, *saved = saved
+        return DA.diff_attn_bwd(q, k, v, lam, o, saved, go, gv_out=gv_out)
 
 
 def _fused_core(self):

@@ -49,7 +49,9 @@ BF16, F32 = torch.bfloat16, torch.float32
 
 class DenseCore:
     """Dense softmax attention core: fused primal+tangent forward kernel and
-    reverse-mode kernel.  SLA2 cores implement the same two methods."""
+    reverse-mode kernel.  SLA2 cores implement the same two methods.  A core with learned tensors of
+    its own names them in ``params``: they become inputs of the block's node, and ``bwd`` returns their gradients
+    behind those of q, k and v."""
 
     def fwd(self, q, k, v, dq, dk, dv, need_bwd: bool):
         o, do, lse = K.attn_fwd(q, k, v, dq, dk, dv, need_lse=need_bwd)
@@ -144,7 +146,7 @@ class _BlockFn(torch.autograd.Function):
     prefix, dprefix, *snaps, *dsnaps,
     w1, w2, g_norm1, g_norm2, g_qa, g_kva, g_qn, g_kn, attn_scale, mlp_scale,
     post_a, keep_a, post_m, keep_m (None without post norms / residual scales),
-    W_a, W_qb, W_kvb, W_out, W13, W2
+    W_a, W_qb, W_kvb, W_out, W13, W2, *the core's params
     outputs: new_prefix (fp32), new_dprefix (fp32 or empty)."""
 
     @staticmethod
@@ -155,7 +157,7 @@ class _BlockFn(torch.autograd.Function):
         snaps = list(rest[:nsnap])
         dsnaps = list(rest[nsnap:2 * nsnap])
         (w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn, a_scale, m_scale, post_a, keep_a, post_m, keep_m,
-         W_a, W_qb, W_kvb, W_out, W13, W2) = rest[2 * nsnap:]
+         W_a, W_qb, W_kvb, W_out, W13, W2, *_core_params) = rest[2 * nsnap:]
         has_t = dprefix is not None
         need_bwd = any(ctx.needs_input_grad)
         B, L, d = prefix.shape
@@ -357,11 +359,11 @@ class _BlockFn(torch.autograd.Function):
         kv4 = kvb.view(B, L, g.H, g.dn + g.dv)
         gkv4 = g_kvb.view(B, L, g.H, g.dn + g.dv)
         if isinstance(q, A8.Packed8):
-            gq, gk, _gv = A8.attn_bwd8(q, k, kv4[..., g.dn:], o, core_saved[0], g_o.view(B, L, g.H, g.dv),
-                                       gv_out=gkv4[..., g.dn:])
+            gq, gk, _gv, *g_core = A8.attn_bwd8(q, k, kv4[..., g.dn:], o, core_saved[0], g_o.view(B, L, g.H, g.dv),
+                                                gv_out=gkv4[..., g.dn:])
         else:
-            gq, gk, _gv = core.bwd(q, k, kv4[..., g.dn:], o, core_saved, g_o.view(B, L, g.H, g.dv),
-                                   gv_out=gkv4[..., g.dn:])
+            gq, gk, _gv, *g_core = core.bwd(q, k, kv4[..., g.dn:], o, core_saved, g_o.view(B, L, g.H, g.dv),
+                                            gv_out=gkv4[..., g.dn:])
         # 5'. q / k preparation
         g_qb = new(rows, g.H * g.hd)
         part_qk = R.qkprep_bwd(qb, kvb, cos, sin, g_qn, g_kn, gq.contiguous(),
@@ -402,7 +404,7 @@ class _BlockFn(torch.autograd.Function):
             g_w2 = torch.zeros_like(w2) if w2 is not None else None
         grads = (None,) * 10 + (g_pfx.view(B, L, d), None) + tuple(g_snaps) + (None,) * nsnap + (
             g_w1, g_w2, gg_n1, gg_n2, gg_qa, gg_kva, gg_qn, gg_kn, g_ascale, g_mscale,
-            g_posta, g_keepa, g_postm, g_keepm, gW_a, gW_qb, gW_kvb, gW_out, gW13, gW2)
+            g_posta, g_keepa, g_postm, g_keepm, gW_a, gW_qb, gW_kvb, gW_out, gW13, gW2, *g_core)
         return grads
 
 
@@ -416,7 +418,7 @@ def run_block(geom: BlockGeom, core, fresh: bool, use_res: bool, eps: float, bet
     core = (core, sinks, torch.is_grad_enabled())
     args = list(snaps) + ([s for s in dsnaps] if dprefix is not None else [None] * nsnap)
     p, t = _BlockFn.apply(geom, core, fresh, use_res, eps, beta, lbeta, cos, sin, nsnap, prefix,
-                          dprefix, *args, *params)
+                          dprefix, *args, *params, *getattr(core[0], "params", ()))
     return p, (t if dprefix is not None else None)
 
 
