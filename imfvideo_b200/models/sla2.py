@@ -478,6 +478,7 @@ class SparseCore:
 
     def __init__(self, mod, qblk: int, bk: int, n_comp: Optional[int], int8: bool):
         self.mod, self.qblk, self.bk, self.n_comp, self.int8 = mod, qblk, bk, n_comp, int8
+        self.params = (self._alpha(),)
 
     def _select(self, qh, kh):
         m = self.mod
@@ -486,12 +487,12 @@ class SparseCore:
         with torch.no_grad():
             return m.sla2.router(qh, kh, m.sla2.topk, need_mask=False)[1]
 
-    def _a_rows(self, L):
+    def _a_rows(self, alpha, L):
         """(H, L) mixing ratio per row, differentiable."""
         m = self.mod
         if isinstance(m, SLA2CubeQATAttentionImpl):
-            return torch.sigmoid(m.alpha_logit)[:, m.a_index]
-        return torch.sigmoid(m.sla2.alpha_logit).repeat_interleave(m.bq, dim=-1)[:, :L]
+            return torch.sigmoid(alpha)[:, m.a_index]
+        return torch.sigmoid(alpha).repeat_interleave(m.bq, dim=-1)[:, :L]
 
     def _alpha(self):
         """The mixing logits, (H, query blocks): row r of both attention forms takes block
@@ -502,6 +503,7 @@ class SparseCore:
     def fwd(self, q, k, v, dq, dk, dv, need_bwd: bool):
         from ..ops import sparse as SP
 
+        alpha, = self.params
         qh, kh, vh = (x.permute(0, 2, 1, 3) for x in (q, k, v))
         sel = self._select(qh.detach(), kh.detach())
         lut, flags, cnt, fm = SP.route_tables(sel, self.qblk, q.shape[1])
@@ -520,12 +522,12 @@ class SparseCore:
         if LA.AVAILABLE:
             with torch.no_grad():
                 o, do, C = LA.forward(q, k, v, dq, dk, dv, o_s, do_s, sel, None, self.qblk, self.bk,
-                                      self.n_comp, alpha=self._alpha())
+                                      self.n_comp, alpha=alpha)
                 if need_bwd and isinstance(self.mod, SLA2CubeQATAttentionImpl):
                     self.mod.logit_max_log2 = (lse.amax(dim=(0, 2)) * 1.4426950408889634).float()
-            return o, do, (sel, lut, flags, o_s, lse, C if need_bwd else None) + fq
+            return o, do, (alpha, sel, lut, flags, o_s, lse, C if need_bwd else None) + fq
         f = lambda a, b, c: linear_branch(a, b, c, sel, self.qblk, self.bk, self.n_comp)
-        a_rows = self._a_rows(q.shape[1])
+        a_rows = self._a_rows(alpha, q.shape[1])
         with torch.no_grad():
             if dq is not None:
                 o_l, do_l = torch.func.jvp(f, (qh.float(), kh.float(), vh.float()),
@@ -541,7 +543,7 @@ class SparseCore:
                 do = (a * do_s.float() + (1 - a) * do_l.permute(0, 2, 1, 3)).to(q.dtype).contiguous()
             if need_bwd and isinstance(self.mod, SLA2CubeQATAttentionImpl):
                 self.mod.logit_max_log2 = (lse.amax(dim=(0, 2)) * 1.4426950408889634).float()
-        return o, do, (sel, lut, flags, o_s, lse, None) + fq
+        return o, do, (alpha, sel, lut, flags, o_s, lse, None) + fq
 
     def bwd(self, q, k, v, o, saved, go, gv_out=None):
         """o = a o_s + (1 - a) o_l: the sparse branch goes through the block-sparse
@@ -551,23 +553,20 @@ class SparseCore:
         from ..ops import kernels as K
         from ..ops import sparse as SP
 
-        sel, lut, flags, o_s, lse, C, *fq = saved
-        m = self.mod
-        cube = isinstance(m, SLA2CubeQATAttentionImpl)
-        alpha_param = m.alpha_logit if cube else m.sla2.alpha_logit
+        alpha, sel, lut, flags, o_s, lse, C, *fq = saved
         B, L, H, D = q.shape
         if C is not None:
-            return self._bwd_kernels(q, k, v, saved, go, gv_out, alpha_param, cube)
+            return self._bwd_kernels(q, k, v, saved, go, gv_out)
         with torch.enable_grad():
-            a_rows = self._a_rows(L)
+            alpha = alpha.detach().requires_grad_(True)
+            a_rows = self._a_rows(alpha, L)
             ql, kl, vl = (x.detach().permute(0, 2, 1, 3).float().requires_grad_(True)
                           for x in (q, k, v))
             o_l = linear_branch(ql, kl, vl, sel, self.qblk, self.bk, self.n_comp)
             a = a_rows.t().reshape(1, L, H, 1)
             gof = go.float()
             mix = (a * o_s.float().detach() + (1 - a) * o_l.permute(0, 2, 1, 3))
-            gq_l, gk_l, gv_l, ga = torch.autograd.grad(mix, (ql, kl, vl, alpha_param), gof)
-        alpha_param.grad = ga if alpha_param.grad is None else alpha_param.grad + ga
+            gq_l, gk_l, gv_l, ga = torch.autograd.grad(mix, (ql, kl, vl, alpha), gof)
         with torch.no_grad():
             g_os = (a.detach() * gof).to(q.dtype).contiguous()
             qq, kk, vv = fq if self.int8 else (q, k, v)
@@ -580,10 +579,10 @@ class SparseCore:
             if gv_out is not None:
                 gv_out.copy_(gv)
                 gv = gv_out
-        return gq, gk, gv
+        return gq, gk, gv, ga
 
 
-def _sparse_core_bwd_kernels(self, q, k, v, saved, go, gv_out, alpha_param, cube):
+def _sparse_core_bwd_kernels(self, q, k, v, saved, go, gv_out):
     """Reverse mode with the linear branch on this library's kernels: row side first
     (it produces the sparse branch's upstream gradient a*go), then the block-sparse
     backward kernel, then the key side, which adds both branches."""
@@ -591,23 +590,21 @@ def _sparse_core_bwd_kernels(self, q, k, v, saved, go, gv_out, alpha_param, cube
     from ..ops import linattn as LA
     from ..ops import sparse as SP
 
-    sel, lut, flags, o_s, lse, C, *fq = saved
-    m = self.mod
+    alpha, sel, lut, flags, o_s, lse, C, *fq = saved
     B, L, H, D = q.shape
     with torch.no_grad():
-        gq_l, gnum, gden, ga, g_os = LA.backward_rows(q, o_s, go, C, None, self.qblk, alpha=alpha_param)
+        gq_l, gnum, gden, ga, g_os = LA.backward_rows(q, o_s, go, C, None, self.qblk, alpha=alpha)
         ga = ga[0] if B == 1 else ga.sum(0)
-        if ga.shape[1] < alpha_param.shape[1]:
-            ga = F.pad(ga, (0, alpha_param.shape[1] - ga.shape[1]))
-        ga = ga.to(alpha_param.dtype)
-        alpha_param.grad = ga if alpha_param.grad is None else alpha_param.grad + ga
+        if ga.shape[1] < alpha.shape[1]:
+            ga = F.pad(ga, (0, alpha.shape[1] - ga.shape[1]))
+        ga = ga.to(alpha.dtype)
         qq, kk, vv = fq if self.int8 else (q, k, v)
         # the linear branch's query gradient rides into the block-sparse backward's dQ epilogue
         gq, gk_s, gv_s = K.attn_bwd(qq, kk, vv, o_s, lse, g_os, dq_add=gq_l,
                                     **SP.bwd_lists(flags))         # `flags`: the maps (see fwd)
         gk, gv = LA.backward_kv(q, k, v, gnum, gden, sel, gk_s, gv_s, self.qblk, self.bk,
                                 self.n_comp, gv_out=gv_out)
-    return gq, gk, gv
+    return gq, gk, gv, ga
 
 
 SparseCore._bwd_kernels = _sparse_core_bwd_kernels
