@@ -210,7 +210,9 @@ class _BlockFn(torch.autograd.Function):
         else:
             og = torch.stack([o.view(rows, hv), do.view(rows, hv)]) if has_t else o.view(1, rows, hv)
         a_out, m = new(T * rows, d), new(T * rows, d)
-        p2, n2 = new(T, rows, d, dt=F32), new(T, rows, d)
+        # with post norms p2 is kept for the backward pass, its tangent is not: apart
+        p2s = [new(rows, d, dt=F32) for _ in range(T)] if post_a is not None else new(T, rows, d, dt=F32)
+        p2, n2 = p2s[0], new(T, rows, d)
         gu, act = new(T * rows, 2 * g.fp), new(T * rows, g.fp)
         out = new(T, rows, d, dt=F32)
         ptrs = [ptr(o), ptr(do), ptr(a_), ptr(og), ptr(W_out), ptr(a_out), ptr(a_scale),
@@ -218,7 +220,8 @@ class _BlockFn(torch.autograd.Function):
                 ptr(w2) if use_res else 0, ptr(g_n2), ptr(W13), ptr(gu), ptr(act), ptr(W2), ptr(m),
                 ptr(m_scale), ptr(out), status]
         ptrs += [ptr(s) for s in sn2] + [ptr(s) for s in dsn2]
-        post = None if post_a is None else R._ptr_array([ptr(post_a), 0 if fresh else ptr(keep_a), ptr(post_m), ptr(keep_m)])
+        post = None if post_a is None else R._ptr_array([ptr(post_a), 0 if fresh else ptr(keep_a), ptr(post_m), ptr(keep_m),
+                                                         ptr(p2s[1]) if has_t else 0])
         K._check(_lib.imf_block_post(R._ptr_array(ptrs), dims(len(sn2)), post, float(eps), float(beta),
                                      float(lbeta or 0.0), stream), "imf_block_post")
         K.LAUNCHES.count += (7 if g.gate else 6) + (post is not None and use_res)
@@ -238,7 +241,7 @@ class _BlockFn(torch.autograd.Function):
                 kept = (n1[0], a_[:rows], qlat[0], kvlat[0], qb[:rows], kvb[:rows], q[0], k[0], o, og[0],
                         a_out[:rows], n2[0], gu[:rows], act[:rows], m[:rows])
             # the residual between the branches: without post norms it is made again where it is needed
-            p2 = p2[0] if post_a is not None and kept else None
+            p2 = p2 if post_a is not None and kept else None
             ctx.save_for_backward(prefix, *snaps, w1, w2, g_n1, g_n2, g_qa, g_kva, g_qn, g_kn,
                                   a_scale, m_scale, post_a, keep_a, post_m, keep_m, p2, W_a, W_qb, W_kvb, W_out, W13, W2,
                                   cos, sin, *core_saved, *kept)

@@ -100,7 +100,8 @@ extern "C" int imf_block_pre(void** p, const int* dims, float eps, void* stream)
 // and 8 dprefix (null when the residual restarts here), 9 p2, 10 n2, 11 remix weight, 12 norm2 gain,
 // 13 W13, 14 gu, 15 act, 16 W2, 17 m, 18 mlp_scale, 19 out, 20 status word, 21.. snaps, then their
 // tangents.  post: null, or gains of the norms of a and m and scales of the residuals they are added to (0 post_a,
-// 1 keep_a or null, 2 post_m, 3 keep_m or null): p2 = keep_a prefix + norm(a) attn_scale, out likewise.
+// 1 keep_a or null, 2 post_m, 3 keep_m or null), and 4 the tangent of p2, which is not behind p2 there, since p2 alone is
+// kept for the backward pass: p2 = keep_a prefix + norm(a) attn_scale, out likewise.
 extern "C" int imf_block_post(void** p, const int* dims, void** post, float eps, float beta, float lbeta,
                               void* stream) {
   using namespace imf;
@@ -116,7 +117,7 @@ extern "C" int imf_block_post(void** p, const int* dims, void** post, float eps,
     IMF_STEP(imf_elementwise(0, e, ed, 0.f, 0.f, 0, t, 0, stream));
   }
   IMF_STEP(linear(p[3], p[4], p[5], m, d, hv, g.ld_wout, p[20], stream));
-  void* dp2 = t ? at(p[9], r * d * 4) : nullptr;
+  void* dp2 = !t ? nullptr : post ? post[4] : at(p[9], r * d * 4);
   void *da = t ? at(p[5], r * d * 2) : nullptr, *dn2 = t ? at(p[10], r * d * 2) : nullptr;
   if (post) {
     // without a remix in between, norm2 is part of the same launch

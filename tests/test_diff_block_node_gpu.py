@@ -1,4 +1,5 @@
-"""GPU: the fused block node with differential attention -- the pairs' weights as inputs of the node."""
+"""GPU: the fused block node with differential attention and post norms -- the pairs' weights as inputs of the node,
+and what the node keeps."""
 import pytest
 import torch
 
@@ -63,3 +64,41 @@ def test_frozen_weights_get_no_gradient():
         p.requires_grad_(False)
     _, got = _run(net, ins)
     assert got and not any(n.endswith("attn_impl.lam") for n in got)
+
+
+def _kept(act_store, tangent):
+    """The storages that a block's node keeps besides its inputs, and the tensors in them."""
+    from imfvideo_b200.models.diff_attn import DiffAttentionImpl
+    from imfvideo_b200.models.imf_dit_video import TransformerBlock, precompute_axial_rope_3d
+    from imfvideo_b200.ops.dual import Dual
+    from functools import partial
+
+    torch.manual_seed(0)
+    cos, sin = (t.cuda() for t in precompute_axial_rope_3d(16, (3, 5, 9), 20))
+    L = cos.shape[0]
+    blk = TransformerBlock(256, 4, 128, 128, 48, 16, 64, norm_eps=1e-5,
+                           attn_impl=partial(DiffAttentionImpl, seq_len=L, num_heads=4), use_attn_res=True,
+                           act_store=act_store, post_norm=True, residual_scale=True).cuda()
+    mk = lambda: torch.randn(2, L, 256, device="cuda")
+    xs = [Dual(mk().requires_grad_(), mk() if tangent else None) for _ in range(2)]
+    saved = []
+
+    def pack(t):
+        saved.append(t)
+        return t
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        out = blk.fused_forward(xs[0], xs[1:], False, True, cos, sin, 1e-5)
+    assert out.p.grad_fn is not None
+    out.p.square().sum().backward()
+    inputs = {t.untyped_storage().data_ptr() for t in [x.p for x in xs] + list(blk.parameters()) + [cos, sin]}
+    kept = {}
+    for t in saved:
+        if t.untyped_storage().data_ptr() not in inputs:
+            kept.setdefault(t.untyped_storage().data_ptr(), (t.untyped_storage().nbytes(), []))[1].append(t)
+    return kept, 2 * L
+
+
+def test_the_kept_residual_holds_no_tangent():
+    kept, rows = _kept("bf16", True)
+    mid = [(n, t) for n, ts in kept.values() for t in ts if t.dtype is torch.float32 and t.shape == (rows, 256)]
+    assert len(mid) == 1 and mid[0][0] == rows * 256 * 4
