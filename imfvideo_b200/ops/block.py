@@ -188,10 +188,12 @@ class _BlockFn(torch.autograd.Function):
         n1, a_ = new(T, rows, d), new(T * rows, na)
         qlat, kvlat = new(T, rows, g.dq), new(T, rows, g.dc)
         qb, kvb = new(T * rows, nq), new(T * rows, nkv)
-        q, k = new(T, B, L, g.H, g.hd), new(T, B, L, g.H, g.hd)
+        # (q and k apart from their tangents, which are not kept for the backward pass)
+        q, k = ([new(B, L, g.H, g.hd) for _ in range(T)] for _ in range(2))
         ptrs = [ptr(pfx), ptr(dpfx), ptr(w1) if (use_res and nsnap) else 0, ptr(g_n1), ptr(W_a), ptr(g_qa),
                 ptr(g_kva), ptr(W_qb), ptr(W_kvb), ptr(cos), ptr(sin), ptr(g_qn), ptr(g_kn), ptr(n1),
-                ptr(a_), ptr(qlat), ptr(kvlat), ptr(qb), ptr(kvb), ptr(q), ptr(k), status]
+                ptr(a_), ptr(qlat), ptr(kvlat), ptr(qb), ptr(kvb), ptr(q[0]), ptr(k[0]), status,
+                ptr(q[1]) if has_t else 0, ptr(k[1]) if has_t else 0]
         ptrs += [ptr(s) for s in sn] + [ptr(s) for s in dsn]
         K._check(_lib.imf_block_pre(R._ptr_array(ptrs), dims(nsnap), float(eps), stream), "imf_block_pre")
         K.LAUNCHES.count += 6

@@ -63,8 +63,8 @@ static int resnorm(void* res, void* dres, void* y, void* dy, void* gate, void* w
 // n1 = norm1(remix(prefix, snaps)); a = n1 W_a^T; latent norms; q_b, kv_b; q / k preparation.
 // ptrs: 0 prefix, 1 dprefix, 2 remix weight, 3 norm1 gain, 4 W_a, 5 q latent gain, 6 kv latent gain,
 // 7 W_qb, 8 W_kvb, 9 cos, 10 sin, 11 q gain, 12 k gain, outputs 13 n1, 14 a, 15 q latent, 16 kv
-// latent, 17 qb, 18 kvb, 19 q, 20 k (tangent rows behind the primal rows), 21 status word,
-// 22.. snaps, then their tangents.
+// latent, 17 qb, 18 kvb (tangent rows behind the primal rows), 19 q, 20 k, 21 status word, 22 and 23 the tangents of
+// q and k (apart: q and k may be kept for the backward pass), 24.. snaps, then their tangents.
 extern "C" int imf_block_pre(void** p, const int* dims, float eps, void* stream) {
   using namespace imf;
   const BlockDims& g = *reinterpret_cast<const BlockDims*>(dims);
@@ -72,7 +72,7 @@ extern "C" int imf_block_pre(void** p, const int* dims, float eps, void* stream)
   const int rows = g.rows, m = g.T * rows;
   const int64_t r = rows;
   IMF_STEP(resnorm(p[0], p[1], nullptr, nullptr, nullptr, p[2], p[3], nullptr, nullptr, p[13],
-                   t ? at(p[13], r * g.d * 2) : nullptr, p + 22, g.nsnap, t, rows, g.d, eps, stream));
+                   t ? at(p[13], r * g.d * 2) : nullptr, p + 24, g.nsnap, t, rows, g.d, eps, stream));
   IMF_STEP(linear(p[13], p[4], p[14], m, g.na, g.d, g.ld_wa, p[21], stream));
   void* a0 = p[14];
   void* a1 = t ? at(a0, r * g.na * 2) : nullptr;
@@ -89,7 +89,7 @@ extern "C" int imf_block_pre(void** p, const int* dims, float eps, void* stream)
   const int64_t kr = (int64_t)(g.dq + g.dc) * 2;
   void* q[20] = {p[17], t ? at(p[17], r * nq * 2) : nullptr, p[18], t ? at(p[18], r * nkv * 2) : nullptr,
                  at(a0, kr), at(a1, kr), p[9], p[10], p[11], p[12],
-                 p[19], t ? at(p[19], r * nq * 2) : nullptr, p[20], t ? at(p[20], r * nq * 2) : nullptr};
+                 p[19], t ? p[22] : nullptr, p[20], t ? p[23] : nullptr};
   return imf_qkprep(q, rows, g.L, g.H, g.dn, g.dr, g.dv, g.na, 0, eps, t, 0, stream);
 }
 

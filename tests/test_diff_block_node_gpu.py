@@ -102,3 +102,8 @@ def test_the_kept_residual_holds_no_tangent():
     kept, rows = _kept("bf16", True)
     mid = [(n, t) for n, ts in kept.values() for t in ts if t.dtype is torch.float32 and t.shape == (rows, 256)]
     assert len(mid) == 1 and mid[0][0] == rows * 256 * 4
+
+
+def test_8_bit_activations_hold_no_tangents():
+    bytes_ = [sum(n for n, _ in _kept("int8", tangent)[0].values()) for tangent in (False, True)]
+    assert bytes_[0] == bytes_[1], bytes_
