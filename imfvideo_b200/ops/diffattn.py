@@ -79,7 +79,8 @@ def _rows(shape: Tuple[int, ...]):
 
 
 @lru_cache(maxsize=64)
-def _scratch_bytes(which: str, *sizes: int) -> int:
+def _scratch_bytes(which: str, device: int, *sizes: int) -> int:
+    """Of a launch on the current device, whose index is ``device``: they go by its SMs."""
     return getattr(_kernels()._lib, f"imf_attn_diff_{which}_scratch_bytes")(*sizes)
 
 
@@ -142,7 +143,7 @@ def diff_attn_fwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, dq: Optional[Ten
     row, row3, row18 = _rows(shape)
     ts, strides = _operands((q, k, v, dq, dk, dv) if tang else (q, k, v), row, row18)
     ptr = [t.data_ptr() for t in ts]
-    nscr = _scratch_bytes("fwd", B, L, H2 // 2, tang)
+    nscr = _scratch_bytes("fwd", dev.index, B, L, H2 // 2, tang)
     scr = _new(nscr, torch.uint8, dev) if nscr else None
     p = K._ptr
     K._check(K._lib.imf_attn_diff_fwd(
@@ -201,7 +202,7 @@ def _backward(q, k, v, lam, o, saved, go, scale, gv_out, dv_strides):
     row, row3, row18 = _rows(shape)
     (q_, k_, v_, g_), strides = _operands((q, k, v, go), row, row18)
     o = o.contiguous()
-    nscr = _scratch_bytes("bwd", B, L, H2 // 2)
+    nscr = _scratch_bytes("bwd", dev.index, B, L, H2 // 2)
     scr = _new(nscr, torch.uint8, dev)
     K._check(K._lib.imf_attn_diff_bwd(
         q_.data_ptr(), k_.data_ptr(), v_.data_ptr(), o.data_ptr(), o2.data_ptr(), low.data_ptr(), g_.data_ptr(),
