@@ -239,10 +239,11 @@ class _DiffAttnFn(torch.autograd.Function):
 
 
 def diff_attention_dual(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[float] = None) -> Dual:
-    """``ops.dual.diff_attention`` on CUDA tensors; lam (H,)."""
+    """``ops.dual.diff_attention`` on CUDA tensors; lam (H,).  Tangents of another type are rounded to their primal's:
+    the tensor core multiplies both with the same operands."""
     t = (q.t, k.t, v.t)
     if any(x is not None for x in t):
-        t = tuple(torch.zeros_like(p.p) if x is None else x for p, x in zip((q, k, v), t))
+        t = tuple(torch.zeros_like(p.p) if x is None else x.to(p.p.dtype) for p, x in zip((q, k, v), t))
     if torch.is_grad_enabled() and (q.p.requires_grad or k.p.requires_grad or v.p.requires_grad or lam.requires_grad):
         o, do = _DiffAttnFn.apply(q.p, k.p, v.p, lam, *t, scale)
         return Dual(o, do)

@@ -215,7 +215,8 @@ def diff_attention(q: Dual, k: Dual, v: Dual, lam: Tensor, scale: Optional[float
 
     with learned weights ``lam`` (H,), or one (a number's tensor) for all pairs; scale 1/sqrt(d) unless
     given.  The output's heads 2j and 2j + 1 are the two halves of pair j's channels.  lam carries no
-    tangent.  impl: "auto" (kernels for CUDA tensors: bf16, d = 64; formulas on CPU) or "math"."""
+    tangent.  impl: "auto" (kernels for CUDA tensors: bf16, d = 64, any other is refused, as in dense
+    attention; formulas on CPU) or "math" (the formulas, which hold 2H maps of l x l in 32 bits)."""
     if impl not in ("auto", "math"):
         raise ValueError(f"diff_attention: impl is 'auto' or 'math', not {impl!r}")
     if q.p.dim() != 4 or q.p.shape[2] % 2 or k.p.shape != q.p.shape or v.p.shape != q.p.shape:
@@ -249,11 +250,11 @@ def norm_add_norm(res: Optional[Dual], y: Dual, post: Tensor, gate: Tensor, eps:
     (rms(z) = sqrt(mean z^2 + eps); post, gate, res_scale and pre are learned, per channel, and carry no
     tangent).  Returns (x, n) as duals; n is None without ``pre``.  ``res`` None: the stream begins with
     this branch; ``res_scale`` None: 1.  x has the type of ``res`` (without one, 32 bits or y's), n
-    ``out_dtype`` or y's.  CUDA: y bf16 or fp32 and res fp32 take one kernel a direction
-    (``ops/postnorm.py``)."""
+    ``out_dtype`` or y's.  CUDA: y bf16 or fp32 and res fp32, tangents like their primals, take one kernel a direction
+    (``ops/postnorm.py``), other types the formulas."""
     mod = _kernel_module("postnorm", y.p, post, gate, res_scale, pre, None if res is None else res.p)
     if mod is not None and mod.supported(y.p, torch.float32 if res is None else res.p.dtype, out_dtype, post, gate,
-                                         res_scale, pre):
+                                         res_scale, pre, y.t, None if res is None else res.t):
         return mod.norm_add_norm_dual(res, y, post, gate, eps, res_scale, pre)
     if res_scale is not None and res is None:
         raise ValueError("norm_add_norm: res_scale without res")

@@ -47,12 +47,14 @@ def _kernels():
 
 
 def supported(y: Tensor, x_dtype: torch.dtype, n_dtype: Optional[torch.dtype], post: Tensor, gate: Tensor,
-              res_scale: Optional[Tensor], pre: Optional[Tensor]) -> bool:
+              res_scale: Optional[Tensor], pre: Optional[Tensor], dy: Optional[Tensor] = None,
+              dres: Optional[Tensor] = None) -> bool:
     """Whether the kernels take these types and this width."""
     yt, D = y.dtype, y.shape[-1] if y.dim() else 0
     return ((yt is BF16 or yt is F32) and x_dtype is F32 and (n_dtype is None or n_dtype is yt) and D % 8 == 0
             and 0 < D <= MAX_WIDTH and post.dtype is F32 and gate.dtype is F32
-            and (res_scale is None or res_scale.dtype is F32) and (pre is None or pre.dtype is F32))
+            and (res_scale is None or res_scale.dtype is F32) and (pre is None or pre.dtype is F32)
+            and (dy is None or dy.dtype is yt) and (dres is None or dres.dtype is F32))
 
 
 def _aligned(t: Optional[Tensor]) -> Optional[Tensor]:

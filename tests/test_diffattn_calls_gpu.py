@@ -1,0 +1,36 @@
+"""GPU: tangents of another type than their primal's."""
+import pytest
+import torch
+
+from test_diffattn_gpu import _inputs, _status  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def test_tangents_of_another_type_of_diff_attention():
+    from imfvideo_b200.ops import dual as D
+
+    q, k, v, lam, tan = _inputs(1, 90, 2, seed=8, tangent=True)
+    want = D.diff_attention(*(D.Dual(*z) for z in zip((q, k, v), tan)), lam)
+    for dt in (torch.float32, torch.float64):
+        got = D.diff_attention(*(D.Dual(a, b.to(dt)) for a, b in zip((q, k, v), tan)), lam)
+        assert torch.equal(got.p, want.p) and torch.equal(got.t, want.t)
+
+
+@pytest.mark.parametrize("dres,dy", [(torch.bfloat16, torch.bfloat16), (torch.float32, torch.float32)])
+def test_tangents_of_another_type_of_norm_add_norm(dres, dy):
+    """As on the CPU, where the formulas take them as they are."""
+    from imfvideo_b200.ops import dual as D
+
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(*s, device="cuda", generator=g)
+    res, y = D.Dual(rnd(5, 64), rnd(5, 64).to(dres)), D.Dual(rnd(5, 64).bfloat16(), rnd(5, 64).to(dy))
+    vec = [rnd(64) for _ in range(4)]
+    call = lambda r, y, w: D.norm_add_norm(r, y, w[0], w[1], 1e-5, w[2], w[3])
+    x, n = call(res, y, vec)
+    xc, nc = call(res.map(torch.Tensor.cpu), y.map(torch.Tensor.cpu), [w.cpu() for w in vec])
+    assert x.t.dtype == torch.float32 and n.t.dtype == torch.bfloat16
+    for a, b in ((x.p, xc.p), (x.t, xc.t)):
+        assert (a.cpu() - b).abs().max() < 1e-5 * (1 + b.abs().max())       # 32-bit sums of 64 terms
+    for a, b in ((n.p, nc.p), (n.t, nc.t)):                                 # one step of bf16 where those fall apart
+        assert (a.cpu().float() - b.float()).abs().max() <= 2.0 ** -7 * b.float().abs().max()
