@@ -9,6 +9,7 @@ attention; the module is a plug-in like its SLA2 family (reference ``models/sla2
 
 from __future__ import annotations
 
+import warnings
 from typing import Optional
 
 import torch
@@ -28,6 +29,10 @@ class DiffAttentionImpl(nn.Module):
         super().__init__()
         if num_heads % 2:
             raise ValueError(f"differential attention pairs heads: {num_heads} is odd")
+        maps = 4 * num_heads * seq_len ** 2                 # bytes of a batch entry's
+        if head_dim != 64 and maps > 1 << 30:
+            warnings.warn(f"differential attention has kernels for head_dim 64 only: with {head_dim} the formulas run, whose "
+                          f"softmax maps take {maps / 1e9:.1f} GB a batch entry and tensor", stacklevel=2)
         self.head_dim = head_dim
         self.lam = nn.Parameter(torch.full((num_heads // 2,), float(lam_init)))
 
