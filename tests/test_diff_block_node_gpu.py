@@ -107,3 +107,22 @@ def test_the_kept_residual_holds_no_tangent():
 def test_8_bit_activations_hold_no_tangents():
     bytes_ = [sum(n for n, _ in _kept("int8", tangent)[0].values()) for tangent in (False, True)]
     assert bytes_[0] == bytes_[1], bytes_
+
+
+def test_every_residual_scale_moves():
+    """Training steps without weight decay: the scales of all residuals but the one that restarts move."""
+    from imfvideo_b200.config import apply_overrides, preset
+    from imfvideo_b200.train import Trainer
+
+    cfg = apply_overrides(preset("d256"), {
+        "model.attn_impl": "diff_jvp", "model.post_norm": True, "model.residual_scale": True, "model.depth": 3,
+        "model.aux_head_depth": 1, "optim.warmup_steps": 0, "optim.weight_decay": 0.0})
+    cfg.data.latent_frames, cfg.data.latent_size = 4, (32, 32)
+    assert cfg.model.attn_res_block_size == 4                # of four blocks only the first begins a residual
+    tr = Trainer(cfg, device=torch.device("cuda", 0), verbose=False)
+    first = {n: p.detach().clone() for n, p in tr.net.named_parameters() if n.endswith("_keep")}
+    g = torch.Generator().manual_seed(7)
+    for _ in range(3):
+        tr.train_step(torch.randn(1, 16, 4, 32, 32, generator=g).pin_memory(), torch.randint(0, 1000, (1,), generator=g))
+    still = [n for n, p in tr.net.named_parameters() if n in first and torch.equal(p, first[n])]
+    assert len(first) == 4 * 2 and still == ["shared_blocks.0.attn_keep"], still
