@@ -158,8 +158,9 @@ def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved
                   scale: Optional[float] = None, gv_out: Optional[Tensor] = None
                   ) -> Tuple[Tensor, Tensor, Tensor, Tensor]:
     """(dq, dk, dv, dlam) from what ``diff_attn_fwd`` returned and the output gradient ``go``.  ``gv_out``
-    takes dv (16-byte aligned rows, no two elements in one place, apart from the inputs), as in
-    ``kernels.attn_bwd``, whose fixed-order mode holds here too."""
+    takes dv (16-byte aligned rows, no two elements in one place, apart from q, k, v, lam and go; what the forward
+    pass returned is read before dv is written), as in ``kernels.attn_bwd``, whose fixed-order mode holds here
+    too."""
     shape = q.shape
     o2, low, lse = saved
     dev, scale = _check("diff_attn_bwd", shape, lam, scale, "q k v o o2 go gv_out", q, k, v, o, o2, go, gv_out)
@@ -180,7 +181,7 @@ def diff_attn_bwd(q: Tensor, k: Tensor, v: Tensor, lam: Tensor, o: Tensor, saved
             raise ValueError("diff_attn_bwd: the dv output needs 16-byte aligned rows")
         if not _apart(*_places(gv_out)):
             raise ValueError("diff_attn_bwd: no two elements of the dv output in one place")
-        if any(_in_one_place(gv_out, t) if _apart(*_places(t)) else _meet(gv_out, t) for t in (q, k, v, go)):
+        if any(_in_one_place(gv_out, t) if _apart(*_places(t)) else _meet(gv_out, t) for t in (q, k, v, lam, go)):
             raise ValueError("diff_attn_bwd: the dv output lies over an input")
     return _backward(q, k, v, lam, o, saved, go, scale, gv_out, dv_strides)
 

@@ -1,4 +1,4 @@
-"""GPU: tangents of another type than their primal's."""
+"""GPU: tangents of another type than their primal's; outputs over inputs."""
 import pytest
 import torch
 
@@ -34,3 +34,23 @@ def test_tangents_of_another_type_of_norm_add_norm(dres, dy):
         assert (a.cpu() - b).abs().max() < 1e-5 * (1 + b.abs().max())       # 32-bit sums of 64 terms
     for a, b in ((n.p, nc.p), (n.t, nc.t)):                                 # one step of bf16 where those fall apart
         assert (a.cpu().float() - b.float()).abs().max() <= 2.0 ** -7 * b.float().abs().max()
+
+
+def test_dv_over_the_weights():
+    """The weights are read while dv is written: refused.  The forward pass's results are read before: the same gradients."""
+    from imfvideo_b200.ops import diffattn as DA
+
+    q, k, v, lam, go = _inputs(1, 40, 2)
+    o, _, saved = DA.diff_attn_fwd(q, k, v, lam)
+    want = DA.diff_attn_bwd(q, k, v, lam, o, saved, go)
+    out = torch.empty_like(q)
+    for inside in (out.view(-1)[640:642], out.view(torch.float32).view(-1)[100:102]):
+        inside.copy_(lam)
+        with pytest.raises(ValueError, match="over an input"):
+            DA.diff_attn_bwd(q, k, v, inside, o, saved, go, gv_out=out)
+    wide = torch.empty(1, 40, 4, 72, device="cuda", dtype=torch.bfloat16)
+    wide[0, 3, 1, 64:68] = lam.view(torch.bfloat16)          # between two rows of the output
+    got = DA.diff_attn_bwd(q, k, v, wide[0, 3, 1, 64:68].view(torch.float32), o, saved, go, gv_out=wide[..., :64])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for a, b in zip(DA.diff_attn_bwd(q, k, v, lam, o, saved, go, gv_out=o), want):
+        assert torch.equal(a, b)                             # (one K/V tile)
