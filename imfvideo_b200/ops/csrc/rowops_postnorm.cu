@@ -11,17 +11,18 @@
 // warps, a lane to 8 adjacent channels of each of NV chunks; NV is 1 up to 2,048 channels, so that the column
 // sums of the backward pass (24 registers a chunk) leave two CTAs of eight warps their place.  Rows come through
 // shared memory, each group of W warps keeping the next STAGES rows on their way by bulk copies: loads from
-// the warps themselves leave too few bytes in flight (32,780 x 1,024, gradients: 221 us with two chunks a lane,
-// 174 with one).  The backward pass makes x again from res and y, of which it needs both anyway, instead of
+// the warps themselves left too few bytes in flight (an earlier form, 32,780 x 1,024, gradients: 221 us with two chunks a
+// lane, 174 with one; 104 this way).  The backward pass makes x again from res and y, of which it needs both anyway, instead of
 // reading it.  Row sums add in a fixed order; column sums go through one partial row a CTA, added up in a fixed
 // order by imf_colsum.
 //
-// Measured, 32,780 x 1,024, bf16 branch, cold: forward 66 us (342 of 402 MB reach DRAM by the end: 5.2 TB/s, copy
-// 6.55), with tangent 138 (746 of 806 MB, 5.4 TB/s), gradients 103 (563 of 604 MB, 5.5 TB/s).  From 1,025
-// channels on a CTA has one row at a time, some 1.8 us each for gradients whatever its width, and fewer bytes on their way: 7,820
-// x 1,536 gradients 49 us, 4.4 TB/s; 20,000 x 2,048 130 us, 5.7 TB/s.  One exchange less between a row's warps, the
-// next row's sum over y going with this row's last, changes nothing there and costs the tangent 10 % at 2,048.
-// Column sums take 4 to 6 us more.
+// Measured, 32,780 x 1,024, bf16 branch, cold, on the device: forward 66 us (342 of 402 MB reach DRAM by the end: 5.2
+// TB/s, copy 6.55), with tangent 136 (746 of 806 MB, 5.5 TB/s), gradients 104 (563 of 604 MB, 5.4 TB/s).  From 1,025
+// channels on a CTA has one row at a time, some 1.8 us each for gradients whatever its width: two or three
+// exchanges between its warps, one behind the other, with two or three rows on an SM at a time (enough bytes
+// are on their way: 72 to 192 KB an SM).  7,820 x 1,536 gradients 50 us, 4.3 TB/s; 20,000 x 2,048 133 us, 5.5
+// TB/s.  One exchange less between a row's warps, the next row's sum over y going with this row's last, changes
+// nothing there and costs the tangent 10 % at 2,048.  Column sums take 4 to 6 us more.
 #include "common.cuh"
 #include "host_util.h"
 #include "rowops_common.cuh"
@@ -425,9 +426,9 @@ __global__ void __launch_bounds__(32 * cta_warps(W), ctas(NV, W, true)) bwd_kern
   write(c_s, 2);
 }
 
-// CTAs: every one of them works on rows from its start on, and the partial rows stay few.  (With four CTAs an SM of the
-// forward pass and three with tangent, fewer rows each on their way, 32,780 x 1,024 takes 89 and 161 us instead of 82
-// and 150.)
+// CTAs: every one of them works on rows from its start on, and the partial rows stay few.  (Three or four CTAs an SM of the
+// forward pass, with fewer rows each on their way, change nothing: 32,780 x 1,024 77 and 78 us instead of 77, with
+// tangent 147 and 148 to 152 instead of 147, launch included.)
 static int grid(int rows, int groups, int ctas_per_sm) {
   const int most = 148 * ctas_per_sm, want = (rows + groups - 1) / groups;
   return want < most ? want : most;
