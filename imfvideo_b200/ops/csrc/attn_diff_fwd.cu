@@ -310,7 +310,10 @@ attn_diff_fwd_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
       const int j_own = sg.j0 + ((n0 ^ g) & 1);     // this group's first step of the segment
       for (int j = j_own; j < sg.j1 && ok; j += 2) {
         const int n = n0 + j - sg.j0;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[t][g], par, abort_flag, p.status, STATUS_TIMEOUT_MMA));
+        // (the O product of this group's step before first, as in the tangent kernel below)
+        ok = mbar_wait(&s.o_done[t][g], par ^ 1, abort_flag, p.status, STATUS_TIMEOUT_MMA) &&
+             mbar_wait(&s.s_full[t][g], par, abort_flag, p.status, STATUS_TIMEOUT_MMA);
+        ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
         const int kv_rem = p.L - j * BN;
@@ -723,7 +726,14 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
         if (UNIT && walk == 0) ok = scale_for(0);
         for (int j = j_own; j < sg.j1 && ok; j += 2) {
           const int n = n0 + j - sg.j0;
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.s_full[g], par, abort_flag, p.status, STATUS_TIMEOUT_MMA));
+          // The O product of this group's step before, n - 2, is seen to be over before the reference of step n is
+          // published: whoever has that reference and asks o_done for the O product of step n then finds the
+          // barrier in that phase or one further.  (A wait by parity on a barrier still two phases back returns at
+          // once.  The scores of step n are made behind that product, but nothing says that arrivals on two
+          // barriers are seen in their order.)
+          ok = mbar_wait(&s.o_done[g], par ^ 1, abort_flag, p.status, STATUS_TIMEOUT_MMA) &&
+               mbar_wait(&s.s_full[g], par, abort_flag, p.status, STATUS_TIMEOUT_MMA);
+          ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           tc_fence_after();
           const int kv_rem = p.L - j * BN;
@@ -744,8 +754,6 @@ attn_diff_jvp_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_cons
             asm("max.f32 %0, %0, %1, %2;" : "+f"(mx[(i / 2) & 3]) : "f"(__uint_as_float(sv[i])), "f"(__uint_as_float(sv[i + 1])));
           mx[0] = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
           // The reference is moved only when a row has outgrown it by more than 2^8 (or has none yet).
-          // The scores of step n follow the O product of step n - 2, so whoever has the reference of step n
-          // and asks o_done for the O product of step n finds the barrier in that phase or one further.
           float m_prev;
           ok = ref_of_step(&s.m_ref[row], n - 1, m_prev, abort_flag, p.status);
           if (!ok) break;
