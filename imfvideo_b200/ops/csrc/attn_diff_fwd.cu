@@ -21,8 +21,9 @@
 // Roundings: P and P .* dS go to the tensor core in bf16 (each off by at most 2^-8 of its value,
 // independently from key to key), o and do are rounded once; scores, maxima, sums and both O are in 32 bits.
 //
-// Measured, 1 x 29,140 rows, 2 pairs: primal 1.21 to 1.30 ms, some 1,040 TFLOP/s; with tangent 2.74 ms alone and 2.85
-// to 3.04 in a loop under the power cap, 1,430 and 1,290 to 1,370.  1 x 7,820 rows, 8 pairs: 343 and 850 to 910 us.
+// Measured, 1 x 29,140 rows, 2 pairs: primal 1.13 to 1.30 ms, 1,000 to 1,150 TFLOP/s; with tangent 2.61 to 2.74 ms alone and
+// 2.85 to 3.09 in a loop under the power cap, 1,430 to 1,500 and 1,270 to 1,370.  1 x 7,820 rows, 8 pairs: 343 to 375
+// and 850 to 910 us.
 // Primal: the exponential unit sets the pace (72 % busy, the tensor pipe 53 %); a sixteenth of the
 // exponentials on the FMA units takes registers that are not there (371 -> 404 us).  Four groups of softmax warps, by
 // map and parity of the step, against two: 427 -> 371.  Tangent: the tensor pipe is 76 % busy, the rest the
